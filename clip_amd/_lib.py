@@ -21,6 +21,13 @@ class ClipConfig(C.Structure):
                [("layer_norm_eps", C.c_float), ("max_tokens", C.c_int32), ("max_seqs", C.c_int32)]
 
 
+class ClipLinear(C.Structure):
+    """clip_linear: hidden rows and a decoder (include/clip_amd.h)"""
+    _fields_ = [("operand", C.c_int32), ("n", C.c_int32), ("hidden_size", C.c_int32), ("vocab", C.c_int64),
+                ("dev_hidden", C.c_void_p), ("ld_hidden", C.c_int64), ("dev_weight", C.c_void_p), ("ld_weight", C.c_int64),
+                ("dev_bias", C.c_void_p)]
+
+
 class ClipError(RuntimeError):
     def __init__(self, code, msg):
         super().__init__(f"libclip_amd error {code}: {msg}")
@@ -44,6 +51,12 @@ SIGNATURES = {
     "clip_bce_loss": [_p, _p, _i32, _p, _p],
     "clip_mlm_head": [_p, _p, _p, _i32, _p, _p, _i32, _p],
     "clip_ce_loss": [_p, _p, _i32, _i32, _p, _p, _i32, _p],
+    "clip_linear_loss_workspace": [_p, _i32, _i32, _p],
+    "clip_linear_ce": [_p, _p, _i64, _i32, _p, _p, _p, _p, _p, _i64, _p],
+    "clip_linear_ce_grad": [_p, _p, _i64, _i32, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    "clip_linear_distill": [_p, _p, _p, _i32, _f, _i32, _p, _p, _p, _p, _p, _i64, _p],
+    "clip_linear_distill_grad": [_p, _p, _p, _i32, _f, _i32, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    "clip_topk_scores": [_i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p],
     "clip_gemm_bf16": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
     "clip_gemm_f16": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
     "clip_gemm_bf16_lnres": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],

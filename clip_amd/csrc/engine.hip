@@ -649,6 +649,87 @@ int mlm_head_impl(clip_engine* e, const int32_t* rows, const int32_t* labels, in
   return CLIP_OK;
 }
 
+// ---- losses of the vocabulary decoder (vocab.hip)
+enum { REDUCE_NONE = 0, REDUCE_MEAN = 1, REDUCE_SUM = 2 };
+
+int check_linear(const char* who, const clip_linear* d) {
+  if (!d) return fail(CLIP_ERR_ARG, "%s: null argument", who);
+  if (d->operand != CLIP_PRECISION_BF16 && d->operand != CLIP_PRECISION_F16)
+    return fail(CLIP_ERR_ARG, "%s: operand type %d (CLIP_PRECISION_BF16 or CLIP_PRECISION_F16)", who, d->operand);
+  if (d->n < 0 || d->n >= (1 << 24) || d->hidden_size < 64 || d->hidden_size > 8192 || d->hidden_size % 64 || d->vocab < 1 ||
+      d->vocab > (1ll << 30))
+    return fail(CLIP_ERR_ARG, "%s: unsupported sizes n %d, hidden %d, vocab %lld (n < 2^24; hidden a multiple of 64, <= 8192; vocab <= 2^30)",
+                who, d->n, d->hidden_size, (long long)d->vocab);
+  if (d->ld_weight < d->hidden_size || d->ld_weight % 8 || d->ld_weight > (1 << 22) || (d->n > 1 && d->ld_hidden < d->hidden_size))
+    return fail(CLIP_ERR_ARG, "%s: row strides %lld / %lld (weight: a multiple of 8, <= 2^22)", who, (long long)d->ld_hidden,
+                (long long)d->ld_weight);
+  return CLIP_OK;
+}
+
+// rows, decoder and workspace of one call; `k` 0 = labels
+int linear_args(const char* who, const clip_linear* d, int32_t k, const int64_t* labels, int64_t ignore, const float* t_values,
+                const int64_t* t_index, float temperature, int32_t reduction, bool grad, const void* work, int64_t work_bytes,
+                VocabRows* a, VocabPlan* p) {
+  int rc = check_linear(who, d);
+  if (rc) return rc;
+  if (!d->dev_weight || !work || reduction < REDUCE_NONE || reduction > REDUCE_SUM ||
+      (d->n > 0 && (!d->dev_hidden || (k ? !t_values || !t_index : !labels))))
+    return fail(CLIP_ERR_ARG, "%s: bad argument", who);
+  if (((uintptr_t)d->dev_weight & 15) || ((uintptr_t)work & 15))
+    return fail(CLIP_ERR_ARG, "%s: weight and workspace must be 16-byte aligned", who);
+  if (k < 0 || k > 1024) return fail(CLIP_ERR_ARG, "%s: k = %d (1 .. 1024)", who, k);
+  if (!(temperature > 0.f) || !std::isfinite(temperature)) return fail(CLIP_ERR_ARG, "%s: temperature must be positive", who);
+  *p = vocab_plan(d->n, d->vocab, d->hidden_size, d->ld_weight, k ? k : 1, k != 0, grad);
+  if (work_bytes < (int64_t)p->bytes)
+    return fail(CLIP_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed (clip_linear_loss_workspace)", who,
+                (long long)work_bytes, (long long)p->bytes);
+  VocabRows r = {};
+  r.n = d->n; r.hidden = d->hidden_size; r.k = k ? k : 1; r.vocab = d->vocab;
+  r.h = d->dev_hidden; r.ldh = d->ld_hidden;
+  r.h_aligned = ((uintptr_t)d->dev_hidden & 15) == 0 && (d->ld_hidden % 8 == 0 || d->n == 1);
+  r.w = d->dev_weight; r.ldw = d->ld_weight; r.bias = d->dev_bias;
+  r.labels = labels; r.ignore = ignore;
+  r.t_values = t_values; r.ld_t = k; r.t_index = t_index; r.ld_ti = k;
+  r.inv_t = 1.f / temperature; r.loss_factor = temperature * temperature; r.grad_factor = temperature;
+  r.mean = reduction == REDUCE_MEAN;
+  *a = r;
+  return CLIP_OK;
+}
+
+int linear_loss(const char* who, const clip_linear* d, int32_t k, const int64_t* labels, int64_t ignore, const float* t_values,
+                const int64_t* t_index, float temperature, int32_t reduction, float* row_loss, float* lse, float* target, float* loss,
+                void* work, int64_t work_bytes, void* stream) {
+  VocabRows a;
+  VocabPlan p;
+  const int rc = linear_args(who, d, k, labels, ignore, t_values, t_index, temperature, reduction, false, work, work_bytes, &a, &p);
+  if (rc) return rc;
+  if ((d->n > 0 && (!row_loss || !lse || !target)) || (reduction != REDUCE_NONE && !loss)) return fail(CLIP_ERR_ARG, "%s: null output", who);
+  a.row_loss = row_loss; a.lse_out = lse; a.target = target;
+  a.loss = reduction == REDUCE_NONE ? nullptr : loss;
+  HIP_TRY(d->operand == CLIP_PRECISION_F16 ? k_f16::launch_vocab_loss(a, p, work, (hipStream_t)stream)
+                                           : k_bf16::launch_vocab_loss(a, p, work, (hipStream_t)stream));
+  return CLIP_OK;
+}
+
+int linear_grad(const char* who, const clip_linear* d, int32_t k, const int64_t* labels, int64_t ignore, const float* t_values,
+                const int64_t* t_index, float temperature, int32_t reduction, const float* lse, const float* target, const float* grad,
+                uint16_t* dh, int64_t ld_dh, uint16_t* dw, int64_t ld_dw, float* dbias, void* work, int64_t work_bytes, void* stream) {
+  VocabRows a;
+  VocabPlan p;
+  const int rc = linear_args(who, d, k, labels, ignore, t_values, t_index, temperature, reduction, true, work, work_bytes, &a, &p);
+  if (rc) return rc;
+  if ((d->n > 0 && (!lse || !target || !grad)) || (!grad && reduction != REDUCE_NONE)) return fail(CLIP_ERR_ARG, "%s: null argument", who);
+  if (dh && d->n > 1 && ld_dh < d->hidden_size) return fail(CLIP_ERR_ARG, "%s: row stride of dhidden", who);
+  if (dw && (((uintptr_t)dw & 7) || ld_dw % 4 || ld_dw < d->hidden_size))
+    return fail(CLIP_ERR_ARG, "%s: dweight must be 8-byte aligned with a row stride that is a multiple of 4", who);
+  a.lse = lse; a.target_in = target; a.grad = grad;
+  a.grad_rows = reduction == REDUCE_NONE;
+  a.dh = dh; a.ld_dh = ld_dh; a.dbias = dbias;
+  HIP_TRY(d->operand == CLIP_PRECISION_F16 ? k_f16::launch_vocab_grad(a, p, dw, ld_dw, work, (hipStream_t)stream)
+                                           : k_bf16::launch_vocab_grad(a, p, dw, ld_dw, work, (hipStream_t)stream));
+  return CLIP_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -930,6 +1011,55 @@ int clip_ce_loss(const float* logits, const int32_t* labels, int32_t n, int32_t 
     return fail(CLIP_ERR_ARG, "clip_ce_loss: bad argument");
   HIP_TRY(launch_ce_rows(logits, n_classes, n_classes, labels, n, row_loss, nullptr, (hipStream_t)stream));
   HIP_TRY(launch_mean_loss(row_loss, n, loss, accumulate, (hipStream_t)stream));
+  return CLIP_OK;
+}
+
+int clip_linear_loss_workspace(const clip_linear* d, int32_t k, int32_t grad, int64_t* bytes) {
+  const int rc = check_linear("clip_linear_loss_workspace", d);
+  if (rc) return rc;
+  if (!bytes || k < 0 || k > 1024) return fail(CLIP_ERR_ARG, "clip_linear_loss_workspace: bad argument");
+  *bytes = (int64_t)vocab_plan(d->n, d->vocab, d->hidden_size, d->ld_weight, k ? k : 1, k != 0, grad != 0).bytes;
+  return CLIP_OK;
+}
+
+int clip_linear_ce(const clip_linear* d, const int64_t* labels, int64_t ignore_index, int32_t reduction, float* row_loss, float* lse,
+                   float* target, float* loss, void* work, int64_t work_bytes, void* stream) {
+  return linear_loss("clip_linear_ce", d, 0, labels, ignore_index, nullptr, nullptr, 1.f, reduction, row_loss, lse, target, loss, work,
+                     work_bytes, stream);
+}
+
+int clip_linear_ce_grad(const clip_linear* d, const int64_t* labels, int64_t ignore_index, int32_t reduction, const float* lse,
+                        const float* target, const float* grad, uint16_t* dhidden, int64_t ld_dhidden, uint16_t* dweight,
+                        int64_t ld_dweight, float* dbias, void* work, int64_t work_bytes, void* stream) {
+  return linear_grad("clip_linear_ce_grad", d, 0, labels, ignore_index, nullptr, nullptr, 1.f, reduction, lse, target, grad, dhidden,
+                     ld_dhidden, dweight, ld_dweight, dbias, work, work_bytes, stream);
+}
+
+int clip_linear_distill(const clip_linear* d, const float* teacher_values, const int64_t* teacher_index, int32_t k, float temperature,
+                        int32_t reduction, float* row_loss, float* lse, float* target, float* loss, void* work, int64_t work_bytes,
+                        void* stream) {
+  if (k < 1) return fail(CLIP_ERR_ARG, "clip_linear_distill: k = %d (1 .. 1024)", k);
+  return linear_loss("clip_linear_distill", d, k, nullptr, 0, teacher_values, teacher_index, temperature, reduction, row_loss, lse,
+                     target, loss, work, work_bytes, stream);
+}
+
+int clip_linear_distill_grad(const clip_linear* d, const float* teacher_values, const int64_t* teacher_index, int32_t k,
+                             float temperature, int32_t reduction, const float* lse, const float* target, const float* grad,
+                             uint16_t* dhidden, int64_t ld_dhidden, uint16_t* dweight, int64_t ld_dweight, float* dbias, void* work,
+                             int64_t work_bytes, void* stream) {
+  if (k < 1) return fail(CLIP_ERR_ARG, "clip_linear_distill_grad: k = %d (1 .. 1024)", k);
+  return linear_grad("clip_linear_distill_grad", d, k, nullptr, 0, teacher_values, teacher_index, temperature, reduction, lse, target,
+                     grad, dhidden, ld_dhidden, dweight, ld_dweight, dbias, work, work_bytes, stream);
+}
+
+int clip_topk_scores(int32_t type, const void* scores, int64_t ld, int32_t n, int32_t vocab, int32_t k, void* values, int64_t* index,
+                     void* stream) {
+  if (type != CLIP_PRECISION_BF16 && type != CLIP_PRECISION_FP32 && type != CLIP_PRECISION_F16)
+    return fail(CLIP_ERR_ARG, "clip_topk_scores: type %d", type);
+  if (n < 0 || vocab < 1 || k < 1 || k > vocab || k > 1024 || (n > 1 && ld < vocab) || (n > 0 && (!scores || !values || !index)))
+    return fail(CLIP_ERR_ARG, "clip_topk_scores: bad argument (1 <= k <= min(vocab, 1024))");
+  if ((uintptr_t)scores & (type == CLIP_PRECISION_FP32 ? 3 : 1)) return fail(CLIP_ERR_ARG, "clip_topk_scores: misaligned scores");
+  HIP_TRY(launch_topk_rows(scores, type, ld, n, vocab, k, values, index, (hipStream_t)stream));
   return CLIP_OK;
 }
 

@@ -96,6 +96,56 @@ hipError_t launch_ce_rows(const float* scores, int ld, int V, const int32_t* lab
                           float* row_loss, float* copy, hipStream_t st);
 hipError_t launch_mean_loss(const float* row_loss, int n, float* loss, int accumulate, hipStream_t st);
 
+// a row's k largest scores, ties to the lowest id (topk.hip); type 0 bf16, 1 fp32, 2 fp16
+hipError_t launch_topk_rows(const void* logits, int type, int64_t ld, int n, int vocab, int k, void* values, int64_t* index,
+                            hipStream_t st);
+
+// ---- losses of the vocabulary decoder (vocab.hip)
+struct VocabRows {          // rows, targets and results of one call; what is null is not asked for
+  int32_t n, hidden, k;     // k: targets per row (1 for labels)
+  int64_t vocab;
+  const bf16_t* h; int64_t ldh; bool h_aligned;   // hidden rows; rows start on 16 bytes
+  const bf16_t* w; int64_t ldw;                   // decoder weight [vocab, hidden], rows on 16 bytes
+  const float* bias;
+  const int64_t* labels; int64_t ignore;          // cross entropy
+  const float* t_values; int64_t ld_t;            // distillation: the teacher's scores [n, k] and
+  const int64_t* t_index; int64_t ld_ti;          // their vocabulary ids (negative: left out)
+  float inv_t, loss_factor, grad_factor;          // 1 / T, T^2, T
+  bool mean;                                      // the mean over live rows (else the sum, or the rows)
+  float *row_loss, *lse_out, *target, *loss;      // forward: [n], [n], [n, k] scores / T of the targets, [1]
+  const float *lse, *target_in;                   // backward: what the forward left
+  const float* grad; bool grad_rows;              // upstream gradient: [n] or [1]
+  bf16_t* dh; int64_t ld_dh;
+  float* dbias;
+  // workspace (VocabPlan)
+  int32_t *count, *row_map, *state;
+  float *t_p, *t_logp, *out_scale;
+  bf16_t* x;
+  float2* row_coef;
+  int64_t* fix;
+};
+struct VocabGemm {          // arguments of vocab_gemm_kernel
+  const bf16_t *x, *w;
+  const float* bias;
+  int64_t ldw, vocab, v0;   // v0: first vocabulary entry of the piece
+  int32_t hidden, tiles_n, ldg, slot0;
+  const int32_t* count;
+  float scale2;             // log2(e) / T
+  float2* part;
+  bf16_t* g;
+  const float2* row_coef;
+  float* colsum; int64_t ld_colsum;
+  float* out32; int64_t slot_stride;
+  bf16_t* out16; int64_t ldo;
+  const float* out_scale;
+};
+struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
+  size_t count, out_scale, row_map, state, t_p, t_logp, x, part, row_coef, fix, g, colsum, dh_part, bytes;
+  int64_t piece, pieces, ld_colsum, dh_slot;
+  int32_t splits;
+};
+VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad);
+
 // ---- launchers of the kernels that touch 16-bit operands: one set per operand type.  Every kernel
 // file is compiled twice (common.h: CLIP_OPERAND_F16) and defines KSET::launch_* ; the engine picks
 // the set by its precision (k_bf16 also holds the fp32 check-mode instantiations).
@@ -136,7 +186,12 @@ hipError_t launch_mean_loss(const float* row_loss, int n, float* loss, int accum
                                    float* logits, int32_t* err, hipStream_t st);                     \
   static hipError_t launch_classifier(const void* x, const int32_t* rows, const float* Wc,           \
                                       const float* bc, float* logits, int n, int H, int L,           \
-                                      hipStream_t st, bool f32 = false);
+                                      hipStream_t st, bool f32 = false);                             \
+  /* losses of the vocabulary decoder, workspace laid out by vocab_plan */                           \
+  static hipError_t launch_vocab_loss(const VocabRows& a, const VocabPlan& p, void* work,            \
+                                      hipStream_t st);                                               \
+  static hipError_t launch_vocab_grad(const VocabRows& a, const VocabPlan& p, bf16_t* dw,            \
+                                      int64_t ld_dw, void* work, hipStream_t st);
 struct k_bf16 { CLIP_KERNEL_SET_MEMBERS };
 struct k_f16 { CLIP_KERNEL_SET_MEMBERS };
 // err |= 4 unless cu_seqlens[0] == 0, every row has 1..max_seqlen tokens and cu_seqlens[n] == total_tokens

@@ -170,6 +170,69 @@ int clip_mlm_head(clip_engine* e, const int32_t* dev_rows, const int32_t* dev_la
 int clip_ce_loss(const float* dev_logits, const int32_t* dev_labels, int32_t n, int32_t n_classes,
                  float* dev_row_loss, float* dev_loss, int32_t accumulate, void* stream);
 
+/* ---- losses of the vocabulary decoder with their gradients, the scores never kept ----
+ * The reference trains BertContextMLMSwitch's LM head with CrossEntropyLoss over scores = decoder(hidden)
+ * (bert_model.py:165,175-179; its loop is pretrain_tasks.py:333-466); clip_mlm_head evaluates that loss and keeps
+ * [n_rows, vocab] fp32 scores.  The entry points below take any hidden rows and any decoder and give the loss AND the
+ * gradients with a workspace of n x hidden plus one bounded piece of 16-bit score gradients.  Stateless: no engine, all
+ * memory is the caller's, all work is queued on `stream` of the current device, nothing waits on the host, and calls can be
+ * captured into HIP graphs (after one eager call per device) and replayed; calls that run at the same time need workspaces
+ * of their own. */
+typedef struct clip_linear {
+  int32_t operand;               /* CLIP_PRECISION_BF16 or CLIP_PRECISION_F16: type of hidden, weight and their gradients */
+  int32_t n;                     /* hidden rows, 0 <= n < 2^24 */
+  int32_t hidden_size;           /* a multiple of 64, <= 8192 */
+  int64_t vocab;                 /* decoder rows, 1 .. 2^30 */
+  const uint16_t* dev_hidden;    /* [n, hidden_size], row stride ld_hidden (elements, >= hidden_size) */
+  int64_t ld_hidden;
+  const uint16_t* dev_weight;    /* [vocab, hidden_size], row stride ld_weight (a multiple of 8), 16-byte aligned */
+  int64_t ld_weight;
+  const float* dev_bias;         /* [vocab] fp32, or NULL; -inf leaves an entry out of the softmax */
+} clip_linear;
+
+/* Bytes of workspace (16-byte aligned) of the calls below for these sizes: k = 0 for the cross entropy, else the teacher's
+ * entries per row; grad = 0 for the loss, 1 for the gradients. */
+int clip_linear_loss_workspace(const clip_linear* d, int32_t k, int32_t grad, int64_t* bytes);
+
+/* z = hidden weight^T + bias;  row_loss[i] = logsumexp(z_i) - z_i[labels[i]] (CrossEntropyLoss, bert_model.py:175-179),
+ * 0 where labels[i] == ignore_index; NaN (with NaN gradients) where a label is neither that nor in [0, vocab).
+ *   reduction 0: rows only;  1: loss[0] = mean over the rows that are not ignored (NaN when there is none, as torch);
+ *   2: loss[0] = sum.   dev_loss may be NULL for 0.
+ * dev_lse [n] (the rows' logsumexp) and dev_target [n] (z_i[labels[i]]) are what the gradient call needs of the forward. */
+int clip_linear_ce(const clip_linear* d, const int64_t* dev_labels, int64_t ignore_index, int32_t reduction,
+                   float* dev_row_loss, float* dev_lse, float* dev_target, float* dev_loss, void* dev_work,
+                   int64_t work_bytes, void* stream);
+/* Gradients of the same loss: dz_i = g_i (softmax(z_i) - onehot(labels[i])), dhidden = dz weight, dweight = dz^T hidden,
+ * dbias = column sums of dz; g_i = dev_grad[i] for reduction 0, dev_grad[0] / count for 1, dev_grad[0] for 2 (fp32).  Ignored
+ * rows get zero dhidden rows and reach nothing else, whatever they hold.  Any of the three outputs may be NULL.  dz is rounded
+ * once to the operand type for the two products (relative, 2^-9 or 2^-12); dbias is summed from unrounded values.  dweight
+ * must be 8-byte aligned with a row stride that is a multiple of 4.  Same bits on every call. */
+int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t ignore_index, int32_t reduction,
+                        const float* dev_lse, const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden,
+                        int64_t ld_dhidden, uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,
+                        int64_t work_bytes, void* stream);
+/* Distillation from a teacher's top scores at `temperature` T > 0: row i lists k scores teacher_values[i, :] with their
+ * vocabulary ids teacher_index[i, :]; p_i = softmax of the listed values / T, q_i = softmax(z_i / T) over the vocabulary,
+ *   row_loss[i] = T^2 sum_j p_ij (log p_ij - log q_i[index_ij]).
+ * An entry with a negative id or the value -inf is left out; a row with none left contributes nothing (loss 0, no gradient,
+ * not counted by the mean).  Ids may repeat within a row.  An id >= vocab, a NaN or a +inf makes the row's loss NaN (and the
+ * gradients).  1 <= k <= 1024.  dev_target is [n, k].  No counterpart in the reference. */
+int clip_linear_distill(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index, int32_t k,
+                        float temperature, int32_t reduction, float* dev_row_loss, float* dev_lse, float* dev_target,
+                        float* dev_loss, void* dev_work, int64_t work_bytes, void* stream);
+/* Its gradients, dz_i = g_i T (q_i - p_i), as clip_linear_ce_grad. */
+int clip_linear_distill_grad(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index,
+                             int32_t k, float temperature, int32_t reduction, const float* dev_lse,
+                             const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden, int64_t ld_dhidden,
+                             uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,
+                             int64_t work_bytes, void* stream);
+/* The k largest scores of every row with their ids, largest first, ties to the lowest id, NaN above everything (torch.topk's
+ * order with its ties settled): what a teacher hands to clip_linear_distill.  `type` CLIP_PRECISION_BF16 / FP32 / F16 is that
+ * of dev_scores [n, vocab] (row stride ld) and dev_values [n, k]; 1 <= k <= min(vocab, 1024).  The last step before it in the
+ * reference's terms is the decoder's scores, bert_model.py:165 (clip_mlm_head's dev_scores_out). */
+int clip_topk_scores(int32_t type, const void* dev_scores, int64_t ld, int32_t n, int32_t vocab, int32_t k,
+                     void* dev_values, int64_t* dev_index, void* stream);
+
 /* ---- single-kernel entry points (parity tests drive each kernel through the ABI) ---- */
 /* out[M,N] = epi(A[M,K] W[N,K]^T + bias): epi 0 bias, 1 bias+erf-GELU, 2 bias+residual, 3 bias+tanh
  * (modeling_bert.py:175-177, 289-293, 334-337, 347-351, 457-463). A, W, res are bf16; out bf16 or

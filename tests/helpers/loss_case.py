@@ -1,0 +1,81 @@
+"""Plain 64-bit forms of the decoder losses and the error bounds of their 16-bit kernels (clip_amd.losses)."""
+import torch
+
+TINY = {torch.bfloat16: 2.0 ** -134, torch.float16: 2.0 ** -25}        # half a step of the smallest subnormal
+F32 = 2.0 ** -24
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def make(n, vocab, hidden, dtype, seed, bias=True, spread=0.1):
+    g = torch.Generator().manual_seed(seed)
+    h = torch.randn(n, hidden, generator=g).to(dtype)
+    w = (spread * torch.randn(vocab, hidden, generator=g)).to(dtype)
+    b = 0.5 * torch.randn(vocab, generator=g) if bias else None
+    return h.cuda(), w.cuda(), None if b is None else b.cuda()
+
+
+def targets_ce(labels, vocab, ignore):
+    live = labels != ignore
+    p = torch.zeros(len(labels), vocab, dtype=torch.float64, device=labels.device)
+    p[live.nonzero()[:, 0], labels[live]] = 1.0
+    return p, live
+
+
+def targets_distill(values, index, vocab, temperature):
+    there = (index >= 0) & (values > -float("inf"))
+    live = there.any(1)
+    t = (values.double() / temperature).masked_fill(~there, -float("inf"))
+    t[~live] = 0.0
+    each = torch.softmax(t, 1) * there * live[:, None]
+    p = torch.zeros(len(values), vocab, dtype=torch.float64, device=values.device)
+    p.scatter_add_(1, index.clamp(min=0), each)
+    # sum p log p over the listed entries, each for itself (an id may repeat)
+    entropy = (each * torch.where(each > 0, each, 1.0).log()).sum(1)
+    return p, live, entropy
+
+
+def reference(h, w, b, p, live, temperature, row_grad, entropy=None):
+    """Row losses, (dh, dw, db) for upstream row gradients, and bounds on the kernels' errors: every rounding counted
+    once at its half step, fp32 sums of m terms at m half steps of the sum of magnitudes."""
+    hd, wd = h.double(), w.double()
+    hd = torch.where(live[:, None], hd, 0.0)
+    zero = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device)
+    bd = zero if b is None else b.double()
+    z = (hd @ wd.t() + bd) / temperature
+    lse = torch.logsumexp(z, 1)
+    q = (z - lse[:, None]).exp()
+    cross = torch.where(p > 0, p * z, 0.0).sum(1)
+    loss = temperature ** 2 * (lse - cross + (0 if entropy is None else entropy)) * live
+    g = (row_grad.double() * live)[:, None] * temperature
+    dz = g * (q - p)
+    n, vocab, hidden = h.shape[0], w.shape[0], h.shape[1]
+    u = half_step(h.dtype)
+    finite_b = torch.where(bd.isfinite(), bd, 0.0)
+    # a score: hidden + bias terms; then a few roundings of numbers as large as z or lse (in units of log 2: * 1.45)
+    z_err = ((hidden + 2) * F32 * (hd.abs() @ wd.abs().t() + finite_b.abs()) / temperature).amax(1)
+    mag = torch.where(z.isfinite(), z, 0.0).abs().amax(1) + lse.abs()
+    z_err = z_err + 8 * F32 * mag
+    loss_err = temperature ** 2 * (2 * z_err + (16 + vocab / 64) * F32 * (1 + mag))
+    # q's relative error: its exponent's, exp2 (2 half steps), the sum of a row's exponentials (vocab terms, tree of 64s)
+    rel = 2 * z_err + (16 + vocab / 64) * F32
+    size = g.abs() * (q + p)
+    dz_err = u * dz.abs() + rel[:, None] * size + 2.0 ** -39 * g.abs().max().clamp(min=1e-300) * (q > 0)
+    dh, dw, db = dz @ wd, dz.t() @ hd, dz.sum(0)
+    dh_err = dz_err @ wd.abs() + vocab * F32 * (size @ wd.abs()) + u * dh.abs() * 1.01 + TINY[h.dtype]
+    dw_err = dz_err.t() @ hd.abs() + n * F32 * (size.t() @ hd.abs()) + u * dw.abs() * 1.01 + TINY[h.dtype]
+    db_err = (rel[:, None] * size).sum(0) + (n + 4) * F32 * size.sum(0) + n * 2.0 ** -38 * g.abs().max()
+    return (loss, dh, dw, db), (loss_err, dh_err, dw_err, db_err)
+
+
+def assert_within(name, got, want, err):
+    got = got.double()
+    assert got.shape == want.shape, (name, got.shape, want.shape)
+    assert torch.equal(got.isfinite(), want.isfinite()), f"{name}: finite where it should not be, or the other way round"
+    fin = want.isfinite()
+    over = ((got - want).abs() - err)[fin]
+    if over.numel():
+        i = int(over.argmax())
+        assert over[i] <= 0, f"{name}: off by {(got - want).abs()[fin][i]:.3e}, bound {err.expand_as(want)[fin][i]:.3e}"

@@ -1,0 +1,468 @@
+"""clip_amd.losses on the GPU: the decoder losses and their gradients against 64-bit forms, over the sizes, masks,
+strides and layouts where tiles end; a teacher's top scores bit for bit; refusals; streams and graphs."""
+import os
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "helpers"))
+import loss_case as R  # noqa: E402
+from clip_amd import _lib, losses  # noqa: E402
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+INF, NAN = float("inf"), float("nan")
+
+
+def _labels(n, vocab, seed, ignored=0.0, ignore=-100):
+    g = torch.Generator().manual_seed(seed + 1)
+    y = torch.randint(0, vocab, (n,), generator=g)
+    y[torch.rand(n, generator=g) < ignored] = ignore
+    return y.cuda()
+
+
+def _teacher(n, vocab, k, seed, dropped=0.0):
+    g = torch.Generator().manual_seed(seed + 2)
+    values = 3 * torch.randn(n, k, generator=g)
+    index = torch.stack([torch.randperm(vocab, generator=g)[:k] for _ in range(n)]) if n else torch.zeros(0, k, dtype=torch.int64)
+    index[torch.rand(n, k, generator=g) < dropped] = -1
+    return values.cuda(), index.cuda()
+
+
+def _check(h, w, b, run, p, live, temperature, reduction, seed, entropy=None):
+    """run(h, w, b) -> loss; compares loss and gradients"""
+    leaves = [t.detach().clone().requires_grad_() if t is not None else None for t in (h, w, b)]
+    n = h.shape[0]
+    loss = run(*leaves)
+    count = int(live.sum())
+    if reduction == "none":
+        up = torch.randn(n, generator=torch.Generator().manual_seed(seed)).cuda()
+        row_grad = up
+    else:
+        up = torch.tensor(0.7, device="cuda")
+        row_grad = (up / (max(count, 1) if reduction == "mean" else 1)).expand(n)
+    inputs = [t for t in leaves if t is not None]
+    grads = torch.autograd.grad(loss, inputs, up)
+    (ref, dh, dw, db), (e_loss, e_h, e_w, e_b) = R.reference(h, w, b, p, live, temperature, row_grad, entropy)
+    if reduction == "none":
+        R.assert_within("loss", loss.detach(), ref, e_loss)
+    else:
+        total, err = ref.sum(), e_loss.sum() + n * 2.0 ** -24 * ref.abs().sum()
+        if reduction == "mean":
+            total, err = total / count if count else ref.new_tensor(NAN), err / max(count, 1)
+        R.assert_within("loss", loss.detach(), total, err)
+    R.assert_within("dh", grads[0], dh, e_h)
+    R.assert_within("dw", grads[1], dw, e_w)
+    if b is not None:
+        R.assert_within("db", grads[2], db, e_b)
+    assert grads[0].dtype == h.dtype and grads[1].dtype == w.dtype
+    return loss.detach(), grads
+
+
+SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64, 128, 64), (65, 129, 192), (130, 777, 320),
+         (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,vocab,hidden", SIZES)
+def test_cross_entropy_sizes(n, vocab, hidden, dtype):
+    h, w, b = R.make(n, vocab, hidden, dtype, n + vocab)
+    y = _labels(n, vocab, n)
+    p, live = R.targets_ce(y, vocab, -100)
+    _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y), p, live, 1.0, "mean", 5)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("ignored", [0.0, 0.6, 0.97, 1.1])
+def test_cross_entropy_reductions_and_ignored_rows(dtype, reduction, ignored):
+    n, vocab, hidden = 401, 523, 128
+    h, w, b = R.make(n, vocab, hidden, dtype, 3)
+    y = _labels(n, vocab, 4, ignored, ignore=-7)
+    p, live = R.targets_ce(y, vocab, -7)
+    if ignored:                       # whatever an ignored row holds stays there
+        h[~live] = NAN
+        h[~live, 0] = INF
+    _, grads = _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y, ignore_index=-7, reduction=reduction), p, live,
+                      1.0, reduction, 6)
+    assert not grads[0][~live].any()
+    if ignored > 1:
+        assert not any(g.any() for g in grads)
+
+
+def test_mean_over_no_rows():
+    h, w, b = R.make(5, 70, 64, BF16, 1)
+    y = torch.full((5,), -100).cuda()
+    assert losses.linear_cross_entropy(h, w, b, y).isnan()
+    assert losses.linear_cross_entropy(h, w, b, y, reduction="sum") == 0
+    h, w, b = (t.requires_grad_() for t in (h[:0].clone(), w, b))
+    for red in ("mean", "sum", "none"):
+        loss = losses.linear_cross_entropy(h, w, b, y[:0], reduction=red)
+        assert loss.isnan() if red == "mean" else not loss.any()
+        grads = torch.autograd.grad(loss.sum(), (h, w, b))
+        assert grads[0].shape == (0, 64) and not grads[1].any() and not grads[2].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_without_bias_and_with_entries_left_out(dtype):
+    n, vocab, hidden = 90, 700, 64
+    h, w, b = R.make(n, vocab, hidden, dtype, 8)
+    y = _labels(n, vocab, 9)
+    p, live = R.targets_ce(y, vocab, -100)
+    _check(h, w, None, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y), p, live, 1.0, "mean", 5)
+    # a whole column tile and single entries at -inf, one at the type's lowest value
+    b[128:256] = -INF
+    b[[3, 699]] = -INF
+    b[400] = torch.finfo(F32).min
+    ok = torch.tensor([v for v in range(vocab) if b[v] > -1e30]).cuda()
+    y = ok[torch.randint(0, len(ok), (n,), generator=torch.Generator().manual_seed(1)).cuda()]
+    p, live = R.targets_ce(y, vocab, -100)
+    b2 = torch.where(b == torch.finfo(F32).min, -INF, b)      # the same softmax; the bounds are made from finite scores
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y, reduction="none")
+    grads = torch.autograd.grad(loss.sum(), leaves)
+    want, err = R.reference(h, w, b2, p, live, 1.0, torch.ones(n).cuda())
+    for name, got, a, e in zip(("loss", "dh", "dw", "db"), (loss.detach(), *grads), want, err):
+        R.assert_within(name, got, a, e)
+    assert not grads[1][128:256].any() and not grads[2][128:256].any() and grads[2][400] == 0
+    # a label whose entry is left out: an infinite loss, and -1 in its gradient
+    y[0] = 3
+    loss = losses.linear_cross_entropy(*leaves, y, reduction="none")
+    assert loss[0] == INF and loss[1:].isfinite().all()
+    assert torch.autograd.grad(loss[1:].sum() + loss[0], leaves)[2][3] == -1
+    # nothing left at all
+    assert losses.linear_cross_entropy(h, w, torch.full_like(b, -INF), y, reduction="none").isnan().all()
+
+
+def test_non_finite_rows_stay_in_their_rows():
+    n, vocab, hidden = 140, 300, 64
+    h, w, b = R.make(n, vocab, hidden, BF16, 12)
+    h[5], h[77, 3] = NAN, INF
+    y = _labels(n, vocab, 13)
+    y[9] = vocab                      # no such entry
+    y[11] = -1
+    bad = torch.zeros(n, dtype=torch.bool).cuda()
+    bad[[5, 77, 9, 11]] = True
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y, reduction="none")
+    assert torch.equal(loss.isnan(), bad)
+    dh, dw, db = torch.autograd.grad(loss.sum(), leaves)
+    assert torch.equal(dh.isnan().any(1), bad)
+    assert dw.isnan().all() and db.isnan().all()
+    assert losses.linear_cross_entropy(*leaves, y).isnan()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_strides_and_shapes(dtype):
+    n, vocab, hidden = 66, 333, 128
+    big_h = torch.randn(n, 3 * hidden + 5, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+    big_w = (0.1 * torch.randn(vocab, hidden + 24, generator=torch.Generator().manual_seed(2))).to(dtype).cuda()
+    b = torch.randn(2 * vocab, generator=torch.Generator().manual_seed(3)).cuda()[::2]
+    y = _labels(n, vocab, 3, 0.2)
+    p, live = R.targets_ce(y, vocab, -100)
+
+    def loss(h, w, b):
+        return losses.linear_cross_entropy(h, w, b, y)
+    base = loss(big_h[:, 7:7 + hidden].contiguous(), big_w[:, 8:8 + hidden].contiguous(), b.contiguous())
+    views_h = {"odd start": big_h[:, 7:7 + hidden], "transposed": big_h[:, 7:7 + hidden].t().contiguous().t()}
+    views_w = {"strided": big_w[:, 8:8 + hidden], "unaligned": big_w.reshape(-1)[8:].as_strided((vocab, hidden), (hidden + 24, 1)),
+               "transposed": big_w[:, 8:8 + hidden].t().contiguous().t()}
+    for hv in views_h.values():
+        for wv in views_w.values():
+            assert torch.equal(loss(hv, wv, b), base)
+    wide = big_h.detach().clone().requires_grad_()
+    wfull = big_w.detach().clone().requires_grad_()
+    got = torch.autograd.grad(loss(wide[:, 7:7 + hidden], wfull[:, 8:8 + hidden], b), (wide, wfull))
+    _, want = _check(big_h[:, 7:7 + hidden], big_w[:, 8:8 + hidden], b, loss, p, live, 1.0, "mean", 2)
+    assert not got[0][:, :7].any() and not got[1][:, :8].any()
+    # [batch, width, H] with [batch, width] labels, int32 labels, one broadcast row
+    h = big_h[:, 7:7 + hidden].contiguous()
+    assert torch.equal(losses.linear_cross_entropy(h.view(6, 11, hidden), big_w[:, 8:8 + hidden], b, y.view(6, 11).int()), base)
+    rows = losses.linear_cross_entropy(h[:1].expand(4, hidden), big_w[:, 8:8 + hidden], b, y[live][:1].expand(4), reduction="none")
+    assert (rows == rows[0]).all()
+    row3 = losses.linear_cross_entropy(h.view(6, 11, hidden), big_w[:, 8:8 + hidden], b, y.view(6, 11), reduction="none")
+    assert row3.shape == (6, 11)
+    # one row's loss has the same bits wherever it stands
+    alone = losses.linear_cross_entropy(h[live][20:21], big_w[:, 8:8 + hidden], b, y[live][20:21], reduction="none")
+    assert torch.equal(alone[0], row3.view(-1)[live][20])
+    # one hidden vector, one label
+    one = losses.linear_cross_entropy(h[live][0], big_w[:, 8:8 + hidden], b, y[live][0])
+    assert one.shape == () and torch.equal(one, row3.view(-1)[live][0])
+
+
+def test_gradients_of_some_inputs_only():
+    h, w, b = R.make(70, 200, 64, BF16, 4)
+    y = _labels(70, 200, 4)
+    full = [t.clone().requires_grad_() for t in (h, w, b)]
+    want = torch.autograd.grad(losses.linear_cross_entropy(*full, y), full)
+    for i in range(3):
+        args = [t.clone().requires_grad_(j == i) for j, t in enumerate((h, w, b))]
+        got, = torch.autograd.grad(losses.linear_cross_entropy(*args, y), args[i])
+        assert torch.equal(got, want[i])
+    # an in-place change of the loss before the backward pass
+    loss = losses.linear_cross_entropy(*full, y)
+    loss *= 2.0
+    assert torch.equal(torch.autograd.grad(loss, full)[2], 2 * want[2])
+    again = torch.autograd.grad(losses.linear_cross_entropy(*full, y), full)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))          # the same bits every time
+
+
+def test_large_scores_and_common_shift():
+    # scores of some hundred: the softmax is taken relative to the row's maximum; bounds grow with the scores
+    for dtype in (BF16, F16):
+        h, w, b = R.make(50, 400, 128, dtype, 21, spread=2.0)
+        b = b + 300.0
+        y = _labels(50, 400, 2)
+        p, live = R.targets_ce(y, 400, -100)
+        _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y, reduction="none"), p, live, 1.0, "none", 3)
+
+
+def test_loss_differences():
+    # central differences of the loss itself along +-1 directions; hidden values on a grid of 2^-5 that bf16 holds with the
+    # step added.  Third derivative of logsumexp along d: a third cumulant of d.w_v, at most 8 M^3, M = max |d.w_v|.
+    n, vocab, hidden = 40, 150, 64
+    h, w, b = R.make(n, vocab, hidden, BF16, 31, spread=0.02)
+    h = (h.float().clamp(-3, 3) * 32).round() / 32
+    h = h.to(BF16)
+    y = _labels(n, vocab, 3)
+    sign = torch.Generator().manual_seed(5)
+    dh_dir = (torch.randint(0, 2, h.shape, generator=sign) * 2 - 1).cuda().double()
+    db_dir = (torch.randint(0, 2, b.shape, generator=sign) * 2 - 1).cuda().double()
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y, reduction="sum")
+    gh, _, gb = torch.autograd.grad(loss, leaves)
+
+    def f(h, b):
+        return losses.linear_cross_entropy(h.to(BF16), w, b.float(), y, reduction="none").double().sum()
+    step = 2.0 ** -5
+    hp, hm = h.double() + step * dh_dir, h.double() - step * dh_dir
+    assert torch.equal(hp.to(BF16).double(), hp) and torch.equal(hm.to(BF16).double(), hm)
+    p, live = R.targets_ce(y, vocab, -100)
+    _, (e_loss, e_h, _, e_b) = R.reference(h, w, b, p, live, 1.0, torch.ones(n).cuda())
+    m = (dh_dir @ w.double().t()).abs().amax(1)
+    slope = (f(hp, b.double()) - f(hm, b.double())) / (2 * step)
+    assert abs(slope - (gh.double() * dh_dir).sum()) <= (step ** 2 / 6 * 8 * m ** 3).sum() + e_loss.sum() / step + e_h.sum()
+    step = 2.0 ** -4
+    slope = (f(h, b.double() + step * db_dir) - f(h, b.double() - step * db_dir)) / (2 * step)
+    assert abs(slope - (gb.double() * db_dir).sum()) <= n * step ** 2 / 6 * 8 + e_loss.sum() / step + e_b.sum()
+
+
+def test_vocabulary_in_several_pieces():
+    # 16-bit score gradients of 4500 x 65 536 are beyond one piece's bound: the products run piece by piece
+    n, vocab, hidden = 4500, 65537, 64
+    h, w, b = R.make(n, vocab, hidden, BF16, 77)
+    y = _labels(n, vocab, 78, 0.01)
+    y[0], y[1] = vocab - 1, 0
+    p, live = R.targets_ce(y, vocab, -100)
+    _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y), p, live, 1.0, "mean", 5)
+
+
+# ---------------------------------------------------------------- distillation
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,vocab,hidden,k,temperature", [
+    (1, 1, 64, 1, 1.0), (1, 30, 64, 30, 2.0), (3, 65, 128, 7, 0.5), (70, 1000, 128, 64, 2.0), (130, 777, 320, 65, 4.0),
+    (33, 2000, 64, 200, 1.0), (300, 3001, 256, 16, 1.5), (9, 1500, 64, 1024, 3.0), (19, 30522, 768, 8, 1.0)])
+def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
+    h, w, b = R.make(n, vocab, hidden, dtype, n + k)
+    values, index = _teacher(n, vocab, k, n)
+    p, live, entropy = R.targets_distill(values, index, vocab, temperature)
+    _check(h, w, b, lambda h, w, b: losses.linear_distillation(h, w, b, values, index, temperature=temperature), p, live, temperature,
+           "mean", 5, entropy)
+
+
+@pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_distillation_ragged_empty_and_repeated_entries(dtype, reduction):
+    n, vocab, hidden, k = 150, 400, 128, 12
+    h, w, b = R.make(n, vocab, hidden, dtype, 5)
+    values, index = _teacher(n, vocab, k, 6, dropped=0.4)
+    index[[0, 17, 149]] = -1              # nothing listed
+    index[40] = -5
+    values[41] = -INF
+    values[42, 3:] = -INF
+    values[43] = torch.finfo(F32).min     # the lowest finite value everywhere: a uniform teacher
+    index[44, :5] = index[44, 5].clamp(min=0)   # one id several times
+    index[45] = 399
+    p, live, entropy = R.targets_distill(values, index, vocab, 2.0)
+    assert not live[[0, 17, 149, 40, 41]].any()
+    h[~live] = NAN
+    _, grads = _check(h, w, b, lambda h, w, b: losses.linear_distillation(h, w, b, values, index, temperature=2.0, reduction=reduction),
+                      p, live, 2.0, reduction, 9, entropy)
+    assert not grads[0][~live].any()
+
+
+def test_distillation_of_bad_entries_is_nan():
+    n, vocab, k = 30, 100, 4
+    h, w, b = R.make(n, vocab, 64, BF16, 5)
+    values, index = _teacher(n, vocab, k, 6)
+    index[3, 1] = vocab
+    values[4, 2] = NAN
+    values[5, 0] = INF
+    bad = torch.zeros(n, dtype=torch.bool).cuda()
+    bad[3:6] = True
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_distillation(*leaves, values, index, reduction="none")
+    assert torch.equal(loss.isnan(), bad)
+    dh, dw, db = torch.autograd.grad(loss.sum(), leaves)
+    assert torch.equal(dh.isnan().any(1), bad) and dw.isnan().all() and db.isnan().all()
+
+
+def test_distillation_of_itself_is_zero():
+    # the teacher lists the whole vocabulary with the student's own scores: loss and gradient vanish up to rounding
+    n, vocab, hidden = 40, 60, 64
+    h, w, b = R.make(n, vocab, hidden, BF16, 14)
+    scores = h.float() @ w.float().t() + b
+    values, index = losses.topk_logits(scores, vocab)
+    p, live, entropy = R.targets_distill(values, index, vocab, 1.0)
+    loss, grads = _check(h, w, b, lambda h, w, b: losses.linear_distillation(h, w, b, values, index, reduction="none"), p, live, 1.0,
+                         "none", 3, entropy)
+    assert loss.abs().max() < 1e-5 and grads[0].abs().max() < 1e-5
+
+
+# ---------------------------------------------------------------- a teacher's top scores
+def _topk_plain(x, k):
+    """by a stable sort of 64-bit values, NaN first"""
+    y = x.double()
+    y = torch.where(y.isnan(), torch.inf, y)
+    order = torch.argsort(torch.where(x.isnan(), 1, 0), dim=-1, descending=True, stable=True)
+    first = torch.gather(y, -1, order).argsort(dim=-1, descending=True, stable=True)
+    index = torch.gather(order, -1, first)[..., :k]
+    return torch.gather(x, -1, index), index
+
+
+def _same_topk(x, k):
+    values, index = losses.topk_logits(x, k)
+    want_v, want_i = _topk_plain(x, k)
+    assert torch.equal(index, want_i)
+    as_int = {F32: torch.int32}.get(x.dtype, torch.int16)
+    assert torch.equal(values.contiguous().view(as_int), want_v.contiguous().view(as_int)), "values are the scores' own bits"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (2, 3, 3), (5, 17, 5), (7, 1000, 1000), (3, 255, 256 - 1), (4, 4097, 64), (9, 30522, 10),
+                                       (2, 30522, 257), (3, 50001, 1024), (1, 200003, 128), (70, 8192, 1)])
+def test_topk_sizes(n, vocab, k, dtype):
+    g = torch.Generator().manual_seed(vocab)
+    _same_topk((2.5 * torch.randn(n, vocab, generator=g)).to(dtype).cuda(), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("k", [1, 64, 300])
+def test_topk_orders_that_fill_the_list(dtype, k):
+    vocab = 20000
+    up = torch.linspace(-50, 50, vocab)
+    rows = [up, up.flip(0), torch.zeros(vocab), torch.full((vocab,), -INF), torch.full((vocab,), NAN), (torch.arange(vocab) % 7).float(),
+            torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0), torch.where(torch.arange(vocab) < 100, INF, -INF),
+            torch.where(torch.arange(vocab) % 97 == 5, NAN, torch.finfo(F16).min), torch.full((vocab,), torch.finfo(dtype).min)]
+    _same_topk(torch.stack(rows).to(dtype).cuda(), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_topk_strides_and_shapes(dtype):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(6, 5003, generator=g).to(dtype).cuda()
+    for lo in range(9):
+        _same_topk(x[:, lo:lo + 4990], 33)
+    _same_topk(x.t().contiguous().t(), 5)
+    _same_topk(x[::2, ::3], 5)
+    v, i = losses.topk_logits(x.view(2, 3, 5003), 4)
+    assert v.shape == i.shape == (2, 3, 4) and torch.equal(i.view(6, 4), _topk_plain(x, 4)[1])
+    v, i = losses.topk_logits(x[0], 4)
+    assert v.shape == (4,)
+    v, i = losses.topk_logits(x[:0], 4)
+    assert v.shape == i.shape == (0, 4)
+
+
+# ---------------------------------------------------------------- used together, streams, graphs
+def test_teacher_to_student_step():
+    """a teacher's scores -> its top entries -> the student's distillation and cross entropy on the same rows"""
+    n, vocab = 120, 3000
+    th, tw, tb = R.make(n, vocab, 256, BF16, 50)
+    h, w, b = R.make(n, vocab, 128, BF16, 51)
+    y = _labels(n, vocab, 52, 0.3)
+    values, index = losses.topk_logits(th.float() @ tw.float().t() + tb, 20)
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    total = losses.linear_distillation(*leaves, values, index, temperature=2.0) + 0.5 * losses.linear_cross_entropy(*leaves, y)
+    grads = torch.autograd.grad(total, leaves)
+    p1, l1, ent = R.targets_distill(values, index, vocab, 2.0)
+    p2, l2 = R.targets_ce(y, vocab, -100)
+    a, ea = R.reference(h.detach(), w.detach(), b.detach(), p1, l1, 2.0, torch.full((n,), 1 / n).cuda(), ent)
+    c, ec = R.reference(h.detach(), w.detach(), b.detach(), p2, l2, 1.0, torch.full((n,), 0.5 / int(l2.sum())).cuda())
+    u = R.half_step(BF16)
+    for name, got, x, y_, e, f in zip(("dh", "dw", "db"), grads, a[1:], c[1:], ea[1:], ec[1:]):
+        R.assert_within(name, got, x + y_, e + f + (u if name != "db" else R.F32) * 1.01 * (x + y_).abs())
+
+
+def test_other_stream():
+    h, w, b = R.make(500, 3000, 128, BF16, 60)
+    y = _labels(500, 3000, 61)
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    want = torch.autograd.grad(losses.linear_cross_entropy(*leaves, y), leaves)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for s in (s1, s2, s1, s2):      # calls side by side: each has its own workspace
+        with torch.cuda.stream(s):
+            got.append(torch.autograd.grad(losses.linear_cross_entropy(*leaves, y), leaves))
+    torch.cuda.synchronize()
+    for g in got:
+        assert all(torch.equal(a, b) for a, b in zip(g, want))
+
+
+def test_captured_step_replays():
+    n, vocab, hidden = 90, 1111, 128
+    h, w, b = R.make(n, vocab, hidden, BF16, 70)
+    y = _labels(n, vocab, 71, 0.3)
+    values, index = _teacher(n, vocab, 9, 72)
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+
+    def step():
+        loss = losses.linear_cross_entropy(*leaves, y)
+        kd = losses.linear_distillation(*leaves, values, index, temperature=2.0)
+        top = losses.topk_logits(b.detach().view(1, -1), 5)
+        return (loss.detach(), kd.detach(), *torch.autograd.grad(loss, leaves), *torch.autograd.grad(kd, leaves), *top)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in (80, 81, 82, 83):
+        h2, w2, b2 = R.make(n, vocab, hidden, BF16, seed)
+        with torch.no_grad():
+            h.copy_(h2), w.copy_(w2), b.copy_(b2)
+            y.copy_(_labels(n, vocab, seed, 0.5 if seed % 2 else 1.1))
+            index.copy_(_teacher(n, vocab, 9, seed, 0.3)[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in out]
+        for got, want in zip(kept, step()):
+            assert torch.equal(got, want) or (got.isnan().all() and want.isnan().all())
+
+
+# ---------------------------------------------------------------- refusals
+def test_refusals():
+    h, w, b = R.make(4, 10, 64, BF16, 1)
+    y = torch.zeros(4, dtype=torch.int64).cuda()
+    ce, kd, top = losses.linear_cross_entropy, losses.linear_distillation, losses.topk_logits
+    v, i = _teacher(4, 10, 3, 1)
+    for err, call in [
+            (TypeError, lambda: ce(h.float(), w.float(), b, y)), (TypeError, lambda: ce(h, w.half(), b, y)),
+            (TypeError, lambda: ce(h, w, b.bfloat16(), y)), (TypeError, lambda: ce(h, w, b[:9], y)),
+            (ValueError, lambda: ce(h[:, :32], w, b, y)), (ValueError, lambda: ce(h, w, b, y[:3])),
+            (ValueError, lambda: ce(h, w, b, y.float())), (ValueError, lambda: ce(h, w, b, y, reduction="batchmean")),
+            (RuntimeError, lambda: ce(h, w, b, y.cpu())), (RuntimeError, lambda: ce(h, w.cpu(), b, y)),
+            (_lib.ClipError, lambda: ce(h[:, :32].contiguous(), w[:, :32].contiguous(), b, y)),
+            (ValueError, lambda: kd(h, w, b, v, i, temperature=0.0)), (ValueError, lambda: kd(h, w, b, v, i, temperature=float("nan"))),
+            (ValueError, lambda: kd(h, w, b, v, i.int())), (ValueError, lambda: kd(h, w, b, v[:, :2], i)),
+            (ValueError, lambda: kd(h, w, b, v[:, :0], i[:, :0])), (ValueError, lambda: kd(h, w, b, v[:3], i[:3])),
+            (ValueError, lambda: top(w, 0)), (ValueError, lambda: top(w, 65)), (TypeError, lambda: top(i, 2))]:
+        with pytest.raises(err):
+            call()
+    leaf = h.requires_grad_()
+    g, = torch.autograd.grad(ce(leaf, w, b, y), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.float().sum(), leaf)
