@@ -119,30 +119,34 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   float* dbias;
   // workspace (VocabPlan)
   int32_t *count, *row_map, *state;
+  int32_t* splits;          // V_DH's splits: of every piece but the last, and of the last
+  int32_t split_tiles_n, split_pairs[2], split_cap, split_wgs;   // what they are chosen from (split_wgs 0: split_cap itself)
   float *t_p, *t_logp, *out_scale;
   bf16_t* x;
-  float2* row_coef;
+  float4* row_coef;
   int64_t* fix;
 };
 struct VocabGemm {          // arguments of vocab_gemm_kernel
   const bf16_t *x, *w;
   const float* bias;
   int64_t ldw, vocab, v0;   // v0: first vocabulary entry of the piece
-  int32_t hidden, tiles_n, ldg, slot0;
+  int32_t hidden, tiles_n, ldg;
   const int32_t* count;
   float scale2;             // log2(e) / T
-  float2* part;
+  float2* part; int32_t n_part;
   bf16_t* g;
-  const float2* row_coef;
+  const float4* row_coef;   // per live row (x, y, lse log2(e), c): G = y exp2(z log2(e) / T - x)
   float* colsum; int64_t ld_colsum;
-  float* out32; int64_t slot_stride;
+  float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: a slot is the live rows, padded, x hidden)
+  const int32_t* splits;
   bf16_t* out16; int64_t ldo;
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
   size_t count, out_scale, row_map, state, t_p, t_logp, x, part, row_coef, fix, g, colsum, dh_part, bytes;
-  int64_t piece, pieces, ld_colsum, dh_slot;
+  int64_t piece, pieces, ld_colsum, dh_slot, dh_piece;   // dh_piece: floats of one piece's partials
   int32_t splits;
+  bool large;             // 256 x 256 tiles (vocab8.hip)
 };
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad);
 
@@ -190,6 +194,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   /* losses of the vocabulary decoder, workspace laid out by vocab_plan */                           \
   static hipError_t launch_vocab_loss(const VocabRows& a, const VocabPlan& p, void* work,            \
                                       hipStream_t st);                                               \
+  static hipError_t launch_vocab8(int what, const VocabGemm& g, hipStream_t st);                     \
   static hipError_t launch_vocab_grad(const VocabRows& a, const VocabPlan& p, bf16_t* dw,            \
                                       int64_t ld_dw, void* work, hipStream_t st);
 struct k_bf16 { CLIP_KERNEL_SET_MEMBERS };

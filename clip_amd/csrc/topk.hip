@@ -70,28 +70,22 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
   // the list's k largest, sorted, to its front
   auto cut = [&]() {
     __syncthreads();
+    // (the list is rarely longer than one or two scores per thread: those keep their scores in registers)
     u64 mine[CAP / NT];
     int rank[CAP / NT];
 #pragma unroll
     for (int i = 0; i < CAP / NT; ++i) {
-      if (i * NT >= have) break;
       mine[i] = tid + i * NT < have ? cand[tid + i * NT] : 0;
       rank[i] = 0;
     }
-    for (int j = 0; j < have; ++j) {
-      const u64 c = cand[j];
 #pragma unroll
-      for (int i = 0; i < CAP / NT; ++i) {
-        if (i * NT >= have) break;
-        rank[i] += c > mine[i];
-      }
-    }
+    for (int i = 0; i < CAP / NT; ++i)
+      if (i * NT < have)
+        for (int j = 0; j < have; ++j) rank[i] += cand[j] > mine[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CAP / NT; ++i) {
-      if (i * NT >= have) break;
+    for (int i = 0; i < CAP / NT; ++i)
       if (tid + i * NT < have && rank[i] < k) cand[rank[i]] = mine[i];
-    }
     if (have > k) have = k;
     __syncthreads();
     if (have == k) {

@@ -12,63 +12,14 @@
 // the products are stored.
 // Rows that take no part (ignored label, empty teacher list) are dropped first: the live rows are copied side by side, so
 // their products cost nothing and whatever a dropped row holds (NaN included) reaches no gradient.
-#include "common.h"
-#include "kernels.h"
+#include "vocab.h"
 
 namespace {
-
-constexpr int BK = 64;               // K tile
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-#if CLIP_OPERAND_F16
-constexpr float G_SCALE = 32768.f;
-#else
-constexpr float G_SCALE = 1.f;       // bf16 has fp32's range
-#endif
-constexpr double FIX = 274877906944.0;   // 2^38: fixed-point unit of the target sums, |sum| <= 2^24 rows
-typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
-
-// ---- buffer descriptor of [p, p + bytes): loads past the end return zero, which is how ragged vocabulary tails are read
-__device__ __forceinline__ u32x4_t make_rsrc(const void* p, int64_t bytes) {
-  const uint64_t a = (uint64_t)p;
-  const int64_t b = bytes < 0 ? 0 : (bytes > 0xffffffffll ? 0xffffffffll : bytes);
-  u32x4_t r;
-  r[0] = __builtin_amdgcn_readfirstlane((uint32_t)a);
-  r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xffffu);
-  r[2] = __builtin_amdgcn_readfirstlane((uint32_t)b);
-  r[3] = 0x00020000u;
-  return r;
-}
-// one wave's 1-KiB LDS-DMA piece: lane l's 16 bytes at r + voff land at lds + 16 l
-__device__ __forceinline__ void dma16(const u32x4_t& r, uint32_t voff, uint32_t lds) {
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(r), "s"(lds) : "memory", "m0");
-#pragma clang diagnostic pop
-}
-
-// sum / max over the 16 lanes fr = lane & 15, and over the 4 lanes fq = lane >> 4
-__device__ __forceinline__ float fr_sum(float v) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
-}
-__device__ __forceinline__ float fq_sum(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
-}
-__device__ __forceinline__ float fq_max(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
-}
 
 // ---- LDS image of a K tile of one operand, R rows (of the output's M or N) by 64 k:
 //   K-major (the operand is [R, K] in memory): [R][128 B], 16-byte chunks swizzled by swz128, read by ds_read_b128
 //   R-major (the operand is [K, R] in memory): [64][2R B], 32-byte slots swizzled so that the 4 rows x 32 bytes that each
 //     16-lane group of ds_read_b64_tr_b16 takes, and those of its neighbour group 8 rows on, fall into different banks
-template <int R>
-__device__ __forceinline__ int tr_swz(int k) {
-  return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) : (((k >> 1) & 1) | ((k >> 3) & 1) << 1);
-}
 template <int R, bool TR, int NW>
 struct Operand {
   static constexpr int BYTES = R * BK * 2, PIECES = BYTES / 1024 / NW;   // per wave
@@ -111,13 +62,7 @@ struct Operand {
   }
 };
 
-enum { V_STATS = 0, V_GRAD = 1, V_DH = 2, V_DW = 3 };
-
-// One output tile of BM x BN per workgroup of WM x WN waves.
-//   V_STATS  rows x vocabulary: (max, sum) of every row's 16 NB columns per wave        A = live rows, B = W
-//   V_GRAD   the same product once more -> G and the column sums of G before rounding
-//   V_DH     rows x hidden over a range of the vocabulary piece -> fp32 partial         A = G, B = W (R-major)
-//   V_DW     vocabulary x hidden over the rows -> 16-bit dW                             A = G, B = live rows (both R-major)
+// One output tile of BM x BN per workgroup of WM x WN waves (few rows: many small tiles; vocab8.hip takes the large calls).
 template <int EPI, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
   constexpr int NW = WM * WN, MB = BM / WM / 16, NB = BN / WN / 16;
@@ -153,11 +98,21 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
     oa.init(a.g + (int64_t)tm * BM, ((int64_t)nt * BK * a.ldg - (int64_t)tm * BM) * 2, a.ldg, w, lane);
     ob.init(a.x + tn * BN, ((int64_t)nt * BK * a.hidden - tn * BN) * 2, a.hidden, w, lane);
   }
+  // acc[m][n][e]: row fr of the 16-row block m, column 4 fq + e of the 16-column block n
+  const int row0 = tm * BM + wm * (BM / WM) + fr, col0 = tn * BN + wn * (BN / WN) + fq * 4;
   f32x4_t acc[MB][NB];
 #pragma unroll
-  for (int m = 0; m < MB; ++m)
+  for (int n = 0; n < NB; ++n) {
+    f32x4_t start = {0.f, 0.f, 0.f, 0.f};
+    if (EPI == V_STATS || EPI == V_GRAD)   // the bias; -inf past the vocabulary
 #pragma unroll
-    for (int n = 0; n < NB; ++n) acc[m][n] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 4; ++e) {
+        const int64_t v = a.v0 + col0 + n * 16 + e;
+        start[e] = v < a.vocab ? (a.bias ? a.bias[v] : 0.f) : -INFINITY;
+      }
+#pragma unroll
+    for (int m = 0; m < MB; ++m) acc[m][n] = start;
+  }
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(smem);
   if (nt > 0) {
@@ -187,75 +142,56 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
     }
   }
 
-  // acc[m][n][e]: row fr of the 16-row block m, column 4 fq + e of the 16-column block n
-  const int row0 = tm * BM + wm * (BM / WM) + fr, col0 = tn * BN + wn * (BN / WN) + fq * 4;
-  if (EPI == V_STATS || EPI == V_GRAD) {
-    float bs[NB][4];   // bias in units of log2; columns past the vocabulary: exp2(-inf) = 0
+  if (EPI == V_STATS) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int64_t v = a.v0 + col0 + n * 16 + e;
-        bs[n][e] = v < a.vocab ? (a.bias ? a.bias[v] * a.scale2 : 0.f) : -INFINITY;
-      }
-    if (EPI == V_STATS) {
-#pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        float mx = -INFINITY, s = 0.f;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc[m][n][e] = fmaf(acc[m][n][e], a.scale2, bs[n][e]);
-            mx = fmaxf(mx, acc[m][n][e]);
-          }
-        mx = fq_max(mx);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s += __builtin_amdgcn_exp2f(acc[m][n][e] - ref);
-        s = fq_sum(s);
-        if (fq == 0)
-          a.part[(int64_t)(row0 + m * 16) * (a.tiles_n * WN) + tn * WN + wn] = make_float2(mx, s);
-      }
-    } else {
-      float cs[NB][4];
+    for (int m = 0; m < MB; ++m) {
+      float mx = -INFINITY, t = 0.f;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) cs[n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[m][n][e]);
+      mx = fq_max(mx) * a.scale2;
+      const float ref = mx == -INFINITY ? 0.f : mx;
 #pragma unroll
-      for (int m = 0; m < MB; ++m) {
-        const int r = row0 + m * 16;
-        const float2 rc = a.row_coef[r];   // (lse in log2 units, c)
-        const bool live = r < count;       // rows up to the tile's end: zeros, the products read them
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          float g[4];
+        for (int e = 0; e < 4; ++e) t += __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -ref));
+      t = fq_sum(t);
+      if (fq == 0) a.part[(int64_t)(row0 + m * 16) * a.n_part + tn * WN + wn] = make_float2(mx, t);
+    }
+  } else if (EPI == V_GRAD) {
+    float cs[NB][4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float q = __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, bs[n][e]) - rc.x);
-            g[e] = live ? q * rc.y : 0.f;
-            cs[n][e] += g[e];
-          }
-          *reinterpret_cast<uint2*>(a.g + (int64_t)r * a.ldg + col0 + n * 16) =
-              make_uint2(pack_op2(g[0] * G_SCALE, g[1] * G_SCALE), pack_op2(g[2] * G_SCALE, g[3] * G_SCALE));
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cs[n][e] = 0.f;
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int r = row0 + m * 16;
+      const float4 rc = a.row_coef[r];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        float g[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          g[e] = __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -rc.x)) * rc.y;
+          cs[n][e] += g[e];
         }
+        *reinterpret_cast<uint2*>(a.g + (int64_t)r * a.ldg + col0 + n * 16) = make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3]));
       }
-      if (a.colsum) {   // fp32 column sums of what was rounded above: db is not made of rounded values
+    }
+    if (a.colsum) {   // fp32 column sums of what was rounded above: db is not made of rounded values
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-          f32x4_t t;
+      for (int n = 0; n < NB; ++n) {
+        f32x4_t t;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = fr_sum(cs[n][e]);
-          if (fr == 0)
-            *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * WM + wm) * a.ld_colsum + a.v0 + col0 + n * 16) = t;
-        }
+        for (int e = 0; e < 4; ++e) t[e] = fr_sum(cs[n][e]);
+        if (fr == 0)
+          *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * WM + wm) * a.ld_colsum + a.v0 + col0 + n * 16) = t;
       }
     }
   } else if (EPI == V_DH) {
-    float* out = a.out32 + (int64_t)(a.slot0 + split) * a.slot_stride;
+    float* out = a.out32 + (int64_t)split * a.slot_stride;
 #pragma unroll
     for (int m = 0; m < MB; ++m)
 #pragma unroll
@@ -329,6 +265,23 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
 }
 
+// dh = G W over one piece has (rows / 256)(hidden / 256) tiles and a long k of `pairs` x 128: it is cut into the number of
+// splits that fills the persistent workgroups best, a round of them costing its k plus about 8 pairs' time for the fp32
+// partials (256 KiB a tile, written here and read by the last kernel).
+__device__ int choose_splits(const VocabRows& a, int total, int pairs) {
+  const int rows = (total + 255) & ~255, tiles = (rows >> 8) * a.split_tiles_n;
+  if (tiles == 0) return 1;
+  int64_t most = (int64_t)a.split_cap * 65536 / ((int64_t)rows * a.hidden);   // split_cap: 65536 floats of room each
+  if (most > 64) most = 64;
+  if (most > pairs) most = pairs;
+  int best = 1, best_cost = 0x7fffffff;
+  for (int s = 1; s <= (int)most; ++s) {
+    const int cost = ((tiles * s + a.split_wgs - 1) / a.split_wgs) * ((pairs + s - 1) / s + 8);
+    if (cost < best_cost) { best_cost = cost; best = s; }
+  }
+  return best;
+}
+
 // Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the next multiple of 256, count = how many.  One
 // workgroup per 64 rows; each counts all rows' states itself (8 bytes a row from L2), so there is no scan kernel.
 // Backward: also every live row's (lse, c), the common factor, zeroed gradients of the dropped rows and a zeroed table.
@@ -364,14 +317,12 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
   before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
   total = total_s[0] + total_s[1] + total_s[2] + total_s[3];
   // the factor common to all rows; c = what is left of a row's gradient, |c| <= 1
-  float common = 1.f, sign = 1.f;
+  float common = 1.f;
   if (GRAD) {
     if (a.grad_rows) {
       common = gm;
     } else {
-      const float g = a.grad[0];
-      common = fabsf(g);
-      sign = g < 0.f ? -1.f : 1.f;
+      common = a.grad[0];
     }
   }
   if (blockIdx.x == 0 && tid == 0) {
@@ -380,6 +331,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       const float f = common * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);   // no live row: zeros, not 0 / 0
       a.out_scale[0] = f / G_SCALE;
       a.out_scale[1] = f;
+      for (int i = 0; i < 2; ++i) a.splits[i] = a.split_wgs ? choose_splits(a, total, a.split_pairs[i]) : a.split_cap;
     }
   }
   if (w == 0) {
@@ -391,13 +343,15 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       rows[local] = r;
       a.row_map[rank] = st == 2 ? ~r : r;    // a row whose target is outside the vocabulary: NaN loss and gradients
       if (GRAD) {
-        float c = sign;
+        float c = 1.f;
         if (a.grad_rows) {
           const float g = a.grad[r];
           c = fabsf(g) < INFINITY ? (common > 0.f ? g / common : 0.f) : g;
         }
         if (st == 2) c = __builtin_nanf("");
-        a.row_coef[rank] = make_float2(a.lse[r] * LOG2E, c);
+        const float l2 = a.lse[r] * LOG2E;
+        // G = y exp2(z log2(e) / T - x): x takes |c| (and G's scale), y its sign
+        a.row_coef[rank] = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, l2, c);
       }
     } else if (r < a.n && !GRAD) {
       a.row_loss[r] = 0.f;
@@ -418,7 +372,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
   const int pad = (total + 255) & ~255;
   for (int r = total + blockIdx.x * 4 + w; r < pad; r += gridDim.x * 4) {
     for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)r * H + c) = make_uint4(0, 0, 0, 0);
-    if (GRAD && lane == 0) a.row_coef[r] = make_float2(0.f, 0.f);
+    if (GRAD && lane == 0) a.row_coef[r] = make_float4(INFINITY, 1.f, 0.f, 0.f);   // G = 0
   }
   if (GRAD) {
     if (a.dh)
@@ -509,7 +463,7 @@ __global__ __launch_bounds__(256) void vocab_targets_kernel(VocabRows a, bf16_t*
   if (r >= *a.count) return;
   const int row = a.row_map[r];
   if (row < 0) return;
-  const float2 rc = a.row_coef[r];
+  const float4 rc = a.row_coef[r];
   for (int j = lane; j < a.k; j += 64) {
     const int64_t v = a.state ? a.t_index[(int64_t)row * a.ld_ti + j] : a.labels[row];
     if (v < 0) continue;
@@ -519,29 +473,33 @@ __global__ __launch_bounds__(256) void vocab_targets_kernel(VocabRows a, bf16_t*
       p = 0.f;
       for (int i = 0; i < a.k; ++i)
         if (a.t_index[(int64_t)row * a.ld_ti + i] == v) p += a.t_p[(int64_t)row * a.k + i];
-      if (table && fabsf(rc.y * own) <= 1.f)
-        atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(rc.y * own) * FIX));
-    } else if (table && fabsf(rc.y) <= 1.f) {
-      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)rc.y * FIX));
+      if (table && fabsf(rc.w * own) <= 1.f)
+        atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(rc.w * own) * FIX));
+    } else if (table && fabsf(rc.w) <= 1.f) {
+      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)rc.w * FIX));
     }
     if (v < v0 || v >= v1) continue;
-    const float q = __builtin_amdgcn_exp2f(a.target_in[(int64_t)row * a.k + j] * LOG2E - rc.x);
-    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(rc.y * (q - p) * G_SCALE);
+    const float q = __builtin_amdgcn_exp2f(a.target_in[(int64_t)row * a.k + j] * LOG2E - rc.z);
+    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(rc.w * (q - p) * G_SCALE);
   }
 }
 
 // dh of the live rows from the fp32 partials (fixed order), and db from the column sums and the targets' table
-__global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, const float* __restrict__ part, int slots, int64_t slot_stride,
-                                                           const float* __restrict__ colsum, int n_colsum_rows, int64_t ld_colsum,
-                                                           int row_blocks, int rows_per_colsum) {
+__global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPlan p, const float* __restrict__ part,
+                                                           const float* __restrict__ colsum, int row_blocks) {
   const int count = *a.count;
   if ((int)blockIdx.x < row_blocks) {
     const int64_t total = (int64_t)count * (a.hidden / 4);
+    const int64_t slot = p.large ? (int64_t)((count + 255) & ~255) * a.hidden : p.dh_slot;
     const float s = a.out_scale[0];
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
       const int r = (int)(i / (a.hidden / 4)), c = (int)(i % (a.hidden / 4)) * 4;
       f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-      for (int k = 0; k < slots; ++k) v += *reinterpret_cast<const f32x4_t*>(part + k * slot_stride + (int64_t)r * a.hidden + c);
+      for (int64_t piece = 0; piece < p.pieces; ++piece) {
+        const int n = a.splits[piece == p.pieces - 1];
+        const float* q = part + piece * p.dh_piece + (int64_t)r * a.hidden + c;
+        for (int k = 0; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
+      }
       const int m = a.row_map[r];
       bf16_t* o = a.dh + (int64_t)(m < 0 ? ~m : m) * a.ld_dh + c;
 #pragma unroll
@@ -550,10 +508,11 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, const fl
   } else {
     const int64_t v = (int64_t)(blockIdx.x - row_blocks) * 256 + threadIdx.x;
     if (v >= a.vocab) return;
-    const int n_sums = min(n_colsum_rows, (count + rows_per_colsum - 1) / rows_per_colsum);
+    const int n_sums = p.large ? (count + 255) / 256 * 2 : (count + 127) / 128 * 2;
     float s = 0.f;
-    for (int k = 0; k < n_sums; ++k) s += colsum[(int64_t)k * ld_colsum + v];
-    a.dbias[v] = (float)((double)s - (double)a.fix[v] / FIX) * a.out_scale[1];
+    for (int k = 0; k < n_sums; ++k) s += colsum[(int64_t)k * p.ld_colsum + v];
+    // (s is in units of G, the table in units of c)
+    a.dbias[v] = (float)((double)s / G_SCALE - (double)a.fix[v] / FIX) * a.out_scale[1];
   }
 }
 
@@ -571,6 +530,9 @@ hipError_t launch_tiles(const VocabGemm& g, int tiles_m, int splits, hipStream_t
 // G of one piece of the vocabulary may take this much: the pieces are as few as that allows
 constexpr int64_t G_BYTES = 512ll << 20;
 
+// From here on the 256 x 256 tiles
+constexpr int LARGE_ROWS = 256;
+
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {
   VocabPlan p = {};
   size_t at = 0;
@@ -579,9 +541,10 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     at += (bytes + 255) & ~(size_t)255;
     return o;
   };
+  p.large = n > LARGE_ROWS && hidden % 128 == 0;
   const int64_t rows = ((int64_t)n + 255) / 256 * 256, vp = (vocab + 255) / 256 * 256;
   p.count = take(4);
-  p.out_scale = take(8);
+  p.out_scale = take(16);   // and V_DH's splits
   p.row_map = take(rows * 4);
   if (distill) {
     p.state = take(rows * 4);
@@ -592,7 +555,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   if (!grad) {
     p.part = take(rows * (vp / 64) * 8);
   } else {
-    p.row_coef = take(rows * 8);
+    p.row_coef = take(rows * 16);
     p.fix = take(vocab * 8);
     // a piece: whole 256-column tiles, G within its bound, 32-bit byte offsets into the piece of W
     int64_t piece = rows > 0 ? G_BYTES / (rows * 2) : vp;
@@ -612,7 +575,13 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     if (s > p.piece / 256) s = p.piece / 256;
     p.splits = (int32_t)(s < 1 ? 1 : s);
     p.dh_slot = rows * hidden;
-    p.dh_part = take((size_t)p.pieces * p.splits * p.dh_slot * 4);
+    p.dh_piece = p.splits * p.dh_slot;
+    if (p.large) {   // room for the splits that few live rows call for
+      const int64_t tiles8 = (rows / 256) * ((hidden + 255) / 256);
+      p.dh_piece = (tiles8 > 256 ? 2 * tiles8 : 512) * 65536;
+      if (p.dh_piece < p.dh_slot) p.dh_piece = p.dh_slot;
+    }
+    p.dh_part = take((size_t)p.pieces * p.dh_piece * 4);
   }
   p.bytes = at;
   return p;
@@ -648,9 +617,15 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
     g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
     g.scale2 = LOG2E * a.inv_t;
     g.part = part;
-    g.tiles_n = (int)((a.vocab + T_BN - 1) / T_BN);
-    TRY(launch_tiles<V_STATS>(g, (a.n + T_BM - 1) / T_BM, 1, st));
-    hipLaunchKernelGGL(vocab_loss_kernel, dim3(a.n), dim3(256), 0, st, a, part, g.tiles_n * 2);
+    g.n_part = (int)((a.vocab + 255) / 256 * 4);   // 64 columns each
+    if (p.large) {
+      g.tiles_n = (int)((a.vocab + 255) / 256);
+      TRY(launch_vocab8(V_STATS, g, st));
+    } else {
+      g.tiles_n = g.n_part / 2;
+      TRY(launch_tiles<V_STATS>(g, (a.n + T_BM - 1) / T_BM, 1, st));
+    }
+    hipLaunchKernelGGL(vocab_loss_kernel, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
     TRY(hipGetLastError());
   }
   if (a.loss) {
@@ -666,7 +641,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   a.count = reinterpret_cast<int32_t*>(base + p.count);
   a.out_scale = reinterpret_cast<float*>(base + p.out_scale);
   a.row_map = reinterpret_cast<int32_t*>(base + p.row_map);
-  a.row_coef = reinterpret_cast<float2*>(base + p.row_coef);
+  a.row_coef = reinterpret_cast<float4*>(base + p.row_coef);
   a.x = reinterpret_cast<bf16_t*>(base + p.x);
   a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
   if (a.t_index) {
@@ -677,6 +652,17 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
       TRY(hipGetLastError());
     }
   }
+  a.splits = reinterpret_cast<int32_t*>(base + p.out_scale + 8);
+  a.split_cap = p.splits;
+  if (p.large) {
+    static DeviceOnce once;
+    TRY(once.get([](int dev, int* val) { return hipDeviceGetAttribute(val, hipDeviceAttributeMultiprocessorCount, dev); }, &a.split_wgs));
+    a.split_wgs &= ~7;
+    a.split_tiles_n = (a.hidden + 255) / 256;
+    a.split_cap = (int32_t)(p.dh_piece / 65536);
+    a.split_pairs[0] = (int32_t)(p.piece / 128);
+    a.split_pairs[1] = (int32_t)((a.vocab - (p.pieces - 1) * p.piece + 255) / 256 * 2);
+  }
   hipLaunchKernelGGL(vocab_pack_kernel<true>, dim3(a.n > 0 ? (a.n + 63) / 64 : 1), dim3(256), 0, st, a);
   TRY(hipGetLastError());
   VocabGemm g = {};
@@ -686,34 +672,34 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.row_coef = a.row_coef;
   g.colsum = a.dbias ? reinterpret_cast<float*>(base + p.colsum) : nullptr;
   g.ld_colsum = p.ld_colsum;
-  g.out32 = reinterpret_cast<float*>(base + p.dh_part);
+  float* dh_part = reinterpret_cast<float*>(base + p.dh_part);
   g.slot_stride = p.dh_slot;
   g.out16 = dw; g.ldo = ld_dw;
   g.out_scale = a.out_scale;
-  const int tiles_r = (a.n + T_BM - 1) / T_BM, tiles_h = (a.hidden + T_BN - 1) / T_BN;
+  const int tiles_r = (a.n + T_BM - 1) / T_BM, tiles_h = (int)((a.hidden + (p.large ? 255 : T_BN - 1)) / (p.large ? 256 : T_BN));
   for (int64_t v0 = 0, piece = 0; v0 < a.vocab; v0 += p.piece, ++piece) {
     const int64_t v1 = v0 + p.piece < a.vocab ? v0 + p.piece : a.vocab;
     g.v0 = v0;
     g.ldg = (int)((v1 - v0 + 255) / 256 * 256);
     if (a.n > 0) {
-      g.tiles_n = g.ldg / T_BN;
-      TRY(launch_tiles<V_GRAD>(g, tiles_r, 1, st));
+      g.tiles_n = g.ldg / (p.large ? 256 : T_BN);
+      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_tiles<V_GRAD>(g, tiles_r, 1, st));
       hipLaunchKernelGGL(vocab_targets_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
                          (a.fix && piece == 0) ? 1 : 0);
       TRY(hipGetLastError());
     }
     g.tiles_n = tiles_h;
     if (a.dh && a.n > 0) {
-      g.slot0 = (int)(piece * p.splits);
-      TRY(launch_tiles<V_DH>(g, tiles_r, p.splits, st));
+      g.out32 = dh_part + piece * p.dh_piece;
+      g.splits = a.splits + (piece == p.pieces - 1);
+      TRY(p.large ? launch_vocab8(V_DH, g, st) : launch_tiles<V_DH>(g, tiles_r, p.splits, st));
     }
-    if (dw) TRY(launch_tiles<V_DW>(g, (g.ldg + T_BM - 1) / T_BM, 1, st));
+    if (dw) TRY(p.large ? launch_vocab8(V_DW, g, st) : launch_tiles<V_DW>(g, (g.ldg + T_BM - 1) / T_BM, 1, st));
   }
   const int row_blocks = a.dh && a.n > 0 ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
   const int b_blocks = a.dbias ? (int)((a.vocab + 255) / 256) : 0;
   if (row_blocks + b_blocks > 0) {
-    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks), dim3(256), 0, st, a, g.out32, (int)(p.pieces * p.splits),
-                       p.dh_slot, g.colsum, tiles_r * 2, p.ld_colsum, row_blocks, T_BM / 2);
+    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks), dim3(256), 0, st, a, p, dh_part, g.colsum, row_blocks);
     TRY(hipGetLastError());
   }
   return hipSuccess;

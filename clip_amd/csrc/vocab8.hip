@@ -1,0 +1,489 @@
+// The products of the decoder losses for large calls: 256 x 256 x 64 tiles on 8 waves, persistent workgroups, the ping-pong
+// schedule of gemm8.hip (a K tile = four 16-KiB half-tiles by LDS-DMA into an 8-slot ring, two phases of 32 MFMAs per K tile,
+// waves 4..7 one barrier behind waves 0..3, counted vmcnt waits) with what these products need beside it:
+//  * either operand may lie R-major in memory ([K, R]: W in dh = G W, both in dW = G^T h).  Its half-tile is the same 16 KiB,
+//    [64 k][128 x 2 B], read by ds_read_b64_tr_b16 in place of ds_read_b128: no transposed copy of W, h or G is ever made;
+//  * loads go through a buffer descriptor, so the vocabulary may end anywhere (rows past the end read as zero);
+//  * the number of live rows is read on the device: tiles past it are never visited;
+//  * epilogues: (max, sum of exp2) per row and 64 columns; the 16-bit score gradients with their column sums; fp32 partials;
+//    16-bit weight gradients.
+#include "vocab.h"
+
+namespace {
+
+constexpr int BM = 256, BN = 256;
+constexpr int HT = 16384;              // half-tile
+constexpr int RING = 8 * HT;           // 2 K tiles
+constexpr int SCR = 2048;              // epilogue scratch per wave
+constexpr int LDS8 = RING + 8 * SCR + 2 * 1024;   // + bias[2][256]
+
+__device__ __forceinline__ float xor16_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float xor32_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float xor16_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float xor32_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// where a staging cursor stands: the bytes from `at` on that may be read (saturated; every walk is shorter than 2^31)
+struct Cursor {
+  uint64_t at;
+  uint32_t left;
+  __device__ __forceinline__ void set(const void* p, int64_t bytes) {
+    at = (uint64_t)p;
+    left = bytes <= 0 ? 0u : (bytes > 0xfffffff0ll ? 0xfffffff0u : (uint32_t)bytes);
+  }
+  __device__ __forceinline__ void step(uint32_t by) {
+    at += by;
+    left = left > by ? left - by : 0u;
+  }
+  __device__ __forceinline__ u32x4_t rsrc(uint32_t ahead) const {
+    const uint64_t p = at + ahead;
+    u32x4_t r;
+    r[0] = __builtin_amdgcn_readfirstlane((uint32_t)p);
+    r[1] = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32) & 0xffffu);
+    r[2] = __builtin_amdgcn_readfirstlane(left > ahead ? left - ahead : 0u);
+    r[3] = 0x00020000u;
+    return r;
+  }
+};
+
+template <int EPI>
+__global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  constexpr bool A_TR = EPI == V_DW, B_TR = EPI == V_DH || EPI == V_DW, ROWS = EPI == V_STATS || EPI == V_GRAD;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = w >> 2, wc = w & 3;   // wr: barrier group AND 64-row block inside each A half
+  char* scr = smem + RING + w * SCR;
+  const float* bias_lds = reinterpret_cast<const float*>(smem + RING + 8 * SCR);
+  const int count = __builtin_amdgcn_readfirstlane(*a.count);
+  const int rows_pad = (count + 255) & ~255;
+
+  // ---- items: (row or vocabulary panel tm, column tile tn, K tiles kt0 .. kt0 + nt)
+  const int G = gridDim.x, per_x = G >> 3;
+  const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
+  const int tiles_m = EPI == V_DW ? a.ldg / BM : rows_pad / BM, tiles_n = a.tiles_n;
+  const int splits = EPI == V_DH ? __builtin_amdgcn_readfirstlane(*a.splits) : 1;
+  // the 8 XCDs take contiguous runs of the longer side: the vocabulary's tiles (each XCD its own part of W)
+  const int run_all = ROWS ? tiles_n : tiles_m, run = (run_all >> 3) + (xcd < (run_all & 7) ? 1 : 0);
+  const int run0 = xcd * (run_all >> 3) + min(xcd, run_all & 7);
+  int tm, tn, kt0, nt;
+  auto item = [&](int i, int& tm_o, int& tn_o, int& kt0_o, int& nt_o) -> bool {
+    if (ROWS) {
+      // column groups of 4 tiles (their slice of W stays in this XCD's L2), all row panels of one before the next
+      const int q = slot + per_x * i;
+      if (q >= run * tiles_m) return false;
+      const int per_group = 4 * tiles_m, g = q / per_group, r = q - g * per_group;
+      const int wide = min(4, run - g * 4), m = r / wide;
+      tm_o = m;
+      tn_o = run0 + g * 4 + (r - m * wide);
+      kt0_o = 0;
+      nt_o = a.hidden / BK;
+      return true;
+    }
+    if (EPI == V_DW) {
+      const int q = slot + per_x * i;
+      if (q >= run * tiles_n) return false;
+      tm_o = run0 + q / tiles_n;
+      tn_o = q % tiles_n;
+      kt0_o = 0;
+      nt_o = (count + 127) / 128 * 2;
+      return true;
+    }
+    const int q = xcd * per_x + slot + G * i, tiles = tiles_m * tiles_n;
+    if (q >= tiles * splits) return false;
+    const int s = q / tiles, t = q - s * tiles, all = a.ldg / 128;
+    tm_o = t / tiles_n;
+    tn_o = t - tm_o * tiles_n;
+    kt0_o = all * s / splits * 2;
+    nt_o = all * (s + 1) / splits * 2 - kt0_o;
+    return true;
+  };
+  if (!item(0, tm, tn, kt0, nt)) return;   // workgroup-uniform
+
+  // ---- LDS-DMA: this wave's two 1-KiB pieces of a half-tile.  K-major image [128 rows][128 B]: rows 8 w .. and 64 + 8 w ..;
+  // R-major image [64 k][256 B]: k 4 w .. and 32 + 4 w ..; the source chunk carries the swizzle
+  const uint32_t ld_a = (uint32_t)(ROWS ? a.hidden : a.ldg) * 2, ld_b = (uint32_t)((ROWS || EPI == V_DH) ? a.ldw : a.hidden) * 2;
+  auto lane_off = [&](bool tr, uint32_t ld) -> uint32_t {
+    if (!tr) {
+      const int r = w * 8 + (lane >> 3);
+      return r * ld + swz128(r, lane & 7) * 16;
+    }
+    const int k = w * 4 + (lane >> 4), c = lane & 15;
+    return k * ld + (((((c >> 1) ^ tr_swz<128>(k)) << 1) | (c & 1)) << 4);
+  };
+  const uint32_t a_off = lane_off(A_TR, ld_a), b_off = lane_off(B_TR, ld_b);
+  const uint32_t a_off2 = a_off + (A_TR ? 32 : 64) * ld_a, b_off2 = b_off + (B_TR ? 32 : 64) * ld_b;   // (same swizzle)
+  const uint32_t a_half = A_TR ? 256 : 128 * ld_a, b_half = B_TR ? 256 : 128 * ld_b;
+  const uint32_t a_step = A_TR ? BK * ld_a : BK * 2, b_step = B_TR ? BK * ld_b : BK * 2;
+  const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(smem);
+  auto stage_a = [&](const Cursor& c, int half, int slot_idx) {
+    const uint32_t dst = lds0 + slot_idx * HT + w * 1024;
+    const u32x4_t r = c.rsrc(half ? a_half : 0);
+    dma16(r, a_off, dst);
+    dma16(r, a_off2, dst + 8192);
+  };
+  auto stage_b = [&](const Cursor& c, int half, int slot_idx) {
+    const uint32_t dst = lds0 + slot_idx * HT + w * 1024;
+    const u32x4_t r = c.rsrc(half ? b_half : 0);
+    dma16(r, b_off, dst);
+    dma16(r, b_off2, dst + 8192);
+  };
+  auto stage_bias = [&](int tn_x, int buf) {   // every wave fetches the whole 1 KiB: uniform counts
+    const int64_t v0 = a.v0 + (int64_t)tn_x * BN;
+    dma16(make_rsrc(a.bias ? a.bias + v0 : nullptr, a.bias ? (a.vocab - v0) * 4 : 0), lane * 16, lds0 + RING + 8 * SCR + buf * 1024);
+  };
+  auto start_of = [&](int tm_x, int tn_x, int kt, Cursor& ca, Cursor& cb) {
+    if (ROWS) {
+      ca.set(a.x + (int64_t)tm_x * BM * a.hidden, (int64_t)BM * a.hidden * 2);
+      const int64_t v0 = a.v0 + (int64_t)tn_x * BN;
+      cb.set(a.w + v0 * a.ldw, ((a.vocab - 1 - v0) * a.ldw + a.hidden) * 2);
+    } else if (EPI == V_DH) {
+      ca.set(a.g + (int64_t)tm_x * BM * a.ldg + (int64_t)kt * BK, ((int64_t)BM * a.ldg - (int64_t)kt * BK) * 2);
+      const int64_t v0 = a.v0 + (int64_t)kt * BK;
+      cb.set(a.w + v0 * a.ldw + tn_x * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - tn_x * BN) * 2);
+    } else {
+      ca.set(a.g + (int64_t)tm_x * BM, ((int64_t)rows_pad * a.ldg - (int64_t)tm_x * BM) * 2);
+      cb.set(a.x + tn_x * BN, ((int64_t)rows_pad * a.hidden - tn_x * BN) * 2);
+    }
+  };
+
+  // staging cursors: K tile t + 1 (c1) and t + 2 (c2) of the flattened (item, k) stream
+  Cursor a1, b1, a2, b2;
+  bool v1, v2;
+  int s_it = 0, s_kt = 0, s_tm = tm, s_tn = tn, s_k0 = kt0, s_nt = nt;   // position of c2
+  auto advance = [&]() {
+    a1 = a2; b1 = b2; v1 = v2;
+    if (!v2) return;
+    if (++s_kt == s_nt) {
+      s_kt = 0;
+      ++s_it;
+      v2 = item(s_it, s_tm, s_tn, s_k0, s_nt);
+      if (!v2) return;
+      start_of(s_tm, s_tn, s_k0, a2, b2);
+    } else {
+      a2.step(a_step);
+      b2.step(b_step);
+    }
+  };
+  f32x4_t acc[2][2][4][2];
+  if (nt > 0) {   // (V_DW without a live row has no K tile; then no item has one)
+    start_of(tm, tn, kt0, a2, b2);
+    v2 = true;
+    stage_a(a2, 0, 0);
+    stage_b(b2, 0, 1);
+    stage_b(b2, 1, 2);
+    stage_a(a2, 1, 3);
+    if (ROWS) stage_bias(tn, 0);
+    advance();   // c2 = K tile 1
+    advance();   // c1 = K tile 1, c2 = K tile 2 (or the next item's first)
+    stage_a(a1, 0, 4);
+    stage_b(b1, 0, 5);
+    asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+  }
+
+  const int fr = lane & 15, fq = lane >> 4;
+  const int lsw = (fr >> 1) & 7, qq = fr >> 2, pp = fr & 3, trg = qq | (fq & 1) << 2;   // trg = tr_swz of k = 8 fq + qq
+  const int c0 = (fq ^ lsw) * 16, c1 = ((4 + fq) ^ lsw) * 16;   // K-major: chunk of k-step 0 / 1
+  const int tr_row = (fq * 8 + qq) * 256 + pp * 8;
+  int a_tr[4], b_tr[4];   // R-major: 16-column block of m / (nh, i)
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    a_tr[m] = tr_row + (((wr * 4 + m) ^ trg) << 5);
+    b_tr[m] = (1 + (wc >> 1)) * HT + tr_row + ((((wc & 1) * 4 + m) ^ trg) << 5);
+  }
+  const int a_rd = (wr * 64 + fr) * 128;                                  // within an A half-tile
+  const int b_rd = (1 + (wc >> 1)) * HT + ((wc & 1) * 64 + fr) * 128;     // B half slot + row
+  auto tr_frag = [&](const char* p) -> opx8_t {   // k and k + 4 rows of 256 B
+    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
+    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 1024));
+    const s16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    return *reinterpret_cast<const opx8_t*>(&v);
+  };
+  auto a_frag = [&](const char* half, int m, int ks) -> opx8_t {
+    if (A_TR) return tr_frag(half + a_tr[m] + ks * 8192);
+    return *reinterpret_cast<const opx8_t*>(half + a_rd + m * 2048 + (ks ? c1 : c0));
+  };
+  auto b_frag = [&](const char* buf, int nh, int i, int ks) -> opx8_t {
+    if (B_TR) return tr_frag(buf + b_tr[nh * 2 + i] + ks * 8192);
+    return *reinterpret_cast<const opx8_t*>(buf + b_rd + nh * 4096 + i * 2048 + (ks ? c1 : c0));
+  };
+
+  int it = 0;
+  while (true) {
+    int ntm = 0, ntn = 0, nkt0 = 0, nnt = 0;
+    const bool has_next = item(it + 1, ntm, ntn, nkt0, nnt);
+    // acc[mh][nh][m][i]: lane holds n = 4 fq .. +3 of 16-column block (nh, i), row fr of 16-row block (mh, m)
+#pragma unroll
+    for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x4_t start = {0.f, 0.f, 0.f, 0.f};
+        if (ROWS) start = *reinterpret_cast<const f32x4_t*>(bias_lds + (it & 1) * 256 + wc * 64 + fq * 4 + nh * 32 + i * 16);
+#pragma unroll
+        for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[mh][nh][m][i] = start;
+      }
+    if (wr == 1) __builtin_amdgcn_s_barrier();   // waves 4..7 run one barrier behind
+
+    opx8_t af[4][2], bf0[2][2], bf1[2][2];
+    for (int kk = 0; kk < nt; kk += 2) {
+      auto ktile = [&]<int B>() {
+        const char* buf = smem + B * 4 * HT;
+        // ---------------- phase A: A0, both B halves -> acc[0][*]; stage (t+1).B1, (t+1).A1
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          bf0[i][0] = b_frag(buf, 0, i, 0);
+          bf0[i][1] = b_frag(buf, 0, i, 1);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          af[m][0] = a_frag(buf, m, 0);
+          af[m][1] = a_frag(buf, m, 1);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          bf1[i][0] = b_frag(buf, 1, i, 0);
+          bf1[i][1] = b_frag(buf, 1, i, 1);
+        }
+        if (v1) {
+          stage_b(b1, 1, (B ^ 1) * 4 + 2);
+          stage_a(a1, 1, (B ^ 1) * 4 + 3);
+          // in flight behind this wait: (t+1).A0/B0 from the previous phase and the four just issued
+          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (ROWS && B == 1 && kk == 0 && has_next) stage_bias(ntn, (it + 1) & 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              acc[0][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[0][0][m][i]);
+              acc[0][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[0][1][m][i]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        // ---------------- phase B: A1 -> acc[1][*]; stage (t+2).A0, (t+2).B0; K tile t+1 retired
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          af[m][0] = a_frag(buf + 3 * HT, m, 0);
+          af[m][1] = a_frag(buf + 3 * HT, m, 1);
+        }
+        const bool staged2 = v2;
+        if (v2) {
+          stage_a(a2, 0, B * 4 + 0);
+          stage_b(b2, 0, B * 4 + 1);
+        }
+        advance();
+        if (staged2) {
+          asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              acc[1][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[1][1][m][i]);
+              acc[1][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[1][0][m][i]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+      };
+      ktile.template operator()<0>();
+      ktile.template operator()<1>();
+    }
+    if (wr == 0) __builtin_amdgcn_s_barrier();   // balances the extra barrier of waves 4..7
+
+    // ---- epilogue.  Lane's rows: mh * 128 + wr * 64 + m * 16 + fr; its columns: wc * 64 + nh * 32 + i * 16 + 4 fq + e
+    const int row0 = tm * BM + wr * 64 + fr, col0 = tn * BN + wc * 64 + fq * 4;
+    if (ROWS && a.v0 + (int64_t)(tn + 1) * BN > a.vocab) {   // the last tile: nothing past the vocabulary
+#pragma unroll
+      for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (a.v0 + col0 + nh * 32 + i * 16 + e >= a.vocab) {
+#pragma unroll
+              for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) acc[mh][nh][m][i][e] = -INFINITY;
+            }
+    }
+    if (EPI == V_STATS) {
+#pragma unroll
+      for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          float mx = -INFINITY, t = 0.f;
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[mh][nh][m][i][e]);
+          mx = xor32_max(xor16_max(mx)) * a.scale2;
+          const float ref = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) t += __builtin_amdgcn_exp2f(fmaf(acc[mh][nh][m][i][e], a.scale2, -ref));
+          t = xor32_sum(xor16_sum(t));
+          if (fq == 0) a.part[(int64_t)(row0 + mh * 128 + m * 16) * a.n_part + tn * 4 + wc] = make_float2(mx, t);
+        }
+    } else if (EPI == V_GRAD) {
+      float cs[2][2][4];
+#pragma unroll
+      for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) cs[nh][i][e] = 0.f;
+#pragma unroll
+      for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const int r = row0 + mh * 128 + m * 16;
+          const float4 rc = a.row_coef[r];
+          // image [16 rows][128 B] in this wave's scratch, whole 128-byte row segments out
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float g[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                g[e] = __builtin_amdgcn_exp2f(fmaf(acc[mh][nh][m][i][e], a.scale2, -rc.x)) * rc.y;
+                cs[nh][i][e] += g[e];
+              }
+              const int sl = ((nh * 2 + i) * 4 + fq) ^ ((fr & 7) << 1);
+              *reinterpret_cast<uint2*>(scr + fr * 128 + sl * 8) = make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3]));
+            }
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int row = p * 8 + (lane >> 3), c16 = lane & 7;
+            const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
+            *reinterpret_cast<u32x4_t*>(a.g + (int64_t)(tm * BM + mh * 128 + wr * 64 + m * 16 + row) * a.ldg + tn * BN + wc * 64 +
+                                        c16 * 8) = v;
+          }
+        }
+      if (a.colsum) {
+#pragma unroll
+        for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            f32x4_t t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = fr_sum(cs[nh][i][e]);
+            if (fr == 0)
+              *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + a.v0 + col0 + nh * 32 + i * 16) = t;
+          }
+      }
+    } else if (EPI == V_DH) {
+      const int split = (it * G + xcd * per_x + slot) / (tiles_m * tiles_n);
+      float* out = a.out32 + (int64_t)split * rows_pad * a.hidden;
+#pragma unroll
+      for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              if (col0 + nh * 32 + i * 16 < a.hidden)
+                *reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + mh * 128 + m * 16) * a.hidden + col0 + nh * 32 + i * 16) = acc[mh][nh][m][i];
+    } else {
+      const float s = a.out_scale[0];
+#pragma unroll
+      for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const f32x4_t v = acc[mh][nh][m][i];
+              const int sl = ((nh * 2 + i) * 4 + fq) ^ ((fr & 7) << 1);
+              *reinterpret_cast<uint2*>(scr + fr * 128 + sl * 8) = make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
+            }
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const int row = p * 8 + (lane >> 3), c16 = lane & 7;
+            const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
+            const int64_t vocab_row = a.v0 + tm * BM + mh * 128 + wr * 64 + m * 16 + row;
+            const int c = tn * BN + wc * 64 + c16 * 8;
+            if (vocab_row < a.vocab && c < a.hidden) {   // (8-byte stores: the row stride is a multiple of 4)
+              uint2* o = reinterpret_cast<uint2*>(a.out16 + vocab_row * a.ldo + c);
+              o[0] = make_uint2(v[0], v[1]);
+              o[1] = make_uint2(v[2], v[3]);
+            }
+          }
+        }
+    }
+    if (!has_next) break;
+    tm = ntm; tn = ntn; kt0 = nkt0; nt = nnt;
+    ++it;
+  }
+}
+
+template <int EPI>
+hipError_t launch_8(const VocabGemm& g, hipStream_t st) {
+  auto kfn = vocab8_kernel<EPI>;
+  static DeviceOnce once;
+  int n_cu = 0;
+  hipError_t e0 = once.get([&](int dev, int* val) {
+    hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kfn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS8);
+    if (e != hipSuccess) return e;
+    int cus = 0;
+    if ((e = hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev)) != hipSuccess) return e;
+    *val = cus & ~7;
+    return *val < 8 ? hipErrorInvalidValue : hipSuccess;
+  }, &n_cu);
+  if (e0 != hipSuccess) return e0;
+  hipLaunchKernelGGL(kfn, dim3(n_cu), dim3(512), LDS8, st, g);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t KSET::launch_vocab8(int what, const VocabGemm& g, hipStream_t st) {
+  if (g.hidden % 128 || g.ldg % 256) return hipErrorInvalidValue;
+  switch (what) {
+    case V_STATS: return launch_8<V_STATS>(g, st);
+    case V_GRAD: return launch_8<V_GRAD>(g, st);
+    case V_DH: return launch_8<V_DH>(g, st);
+    case V_DW: return launch_8<V_DW>(g, st);
+    default: return hipErrorInvalidValue;
+  }
+}
