@@ -101,6 +101,9 @@ hipError_t launch_topk_rows(const void* logits, int type, int64_t ld, int n, int
                             hipStream_t st);
 
 // ---- losses of the vocabulary decoder (vocab.hip)
+// How the products dh = G W and dW = G^T h of one piece share the persistent workgroups (vocab8.hip): dh's long k is cut
+// into `splits`; a workgroup that has one dW tile less than others takes dh_more of the split tiles, the others dh_less
+struct VocabSchedule { int32_t splits, dh_less, dh_more, unused; };
 struct VocabRows {          // rows, targets and results of one call; what is null is not asked for
   int32_t n, hidden, k;     // k: targets per row (1 for labels)
   int64_t vocab;
@@ -119,11 +122,16 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   float* dbias;
   // workspace (VocabPlan)
   int32_t *count, *row_map, *state;
-  int32_t* splits;          // V_DH's splits: of every piece but the last, and of the last
-  int32_t split_tiles_n, split_pairs[2], split_cap, split_wgs;   // what they are chosen from (split_wgs 0: split_cap itself)
+  int32_t* block_base;      // live rows before every 16th row (calls of many rows), and
+  float* grad_max;          // the largest finite |gradient| of a live row
+  VocabSchedule* schedule;  // of every piece but the last, and of the last
+  int32_t tiles_h, piece_tiles[2], max_splits, wgs;   // what they are chosen from (wgs 0: max_splits itself)
+  int64_t dh_room;
+  bool with_dw;
   float *t_p, *t_logp, *out_scale;
   bf16_t* x;
-  float4* row_coef;
+  float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
+  float2* row_lc;           // distillation: (lse log2(e), c)
   int64_t* fix;
 };
 struct VocabGemm {          // arguments of vocab_gemm_kernel
@@ -135,17 +143,17 @@ struct VocabGemm {          // arguments of vocab_gemm_kernel
   float scale2;             // log2(e) / T
   float2* part; int32_t n_part;
   bf16_t* g;
-  const float4* row_coef;   // per live row (x, y, lse log2(e), c): G = y exp2(z log2(e) / T - x)
+  const float4* row_info;
   float* colsum; int64_t ld_colsum;
   float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: a slot is the live rows, padded, x hidden)
-  const int32_t* splits;
+  const VocabSchedule* schedule; bool accumulate, with_dw, with_dh;
   bf16_t* out16; int64_t ldo;
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
-  size_t count, out_scale, row_map, state, t_p, t_logp, x, part, row_coef, fix, g, colsum, dh_part, bytes;
-  int64_t piece, pieces, ld_colsum, dh_slot, dh_piece;   // dh_piece: floats of one piece's partials
-  int32_t splits;
+  size_t head, row_map, block_base, state, t_p, t_logp, x, part, row_info, row_lc, fix, g, colsum, dh_part, bytes;
+  int64_t piece, pieces, ld_colsum, dh_slot, dh_room;   // floats of one split's partials, and of all
+  int32_t splits;         // at most
   bool large;             // 256 x 256 tiles (vocab8.hip)
 };
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad);

@@ -55,11 +55,20 @@ __device__ __forceinline__ int tr_swz(int k) {
   return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) : (((k >> 1) & 1) | ((k >> 3) & 1) << 1);
 }
 
-// What the product kernels compute; A [M, K] and B [N, K] with "R-major" = stored [K, R]
+// What the product kernels compute; A [M, K] and B [N, K], "R-major" = stored [K, R]
 //   V_STATS  rows x vocabulary: every row's (max, sum of exp2) over 64 columns at a time       A = live rows, B = W
 //   V_GRAD   the same product once more -> G and the column sums of G before rounding
 //   V_DH     rows x hidden over a range of the vocabulary piece -> fp32 partial                A = G, B = W (R-major)
 //   V_DW     vocabulary x hidden over the rows -> 16-bit dW                                    A = G, B = live rows (both R-major)
-enum { V_STATS = 0, V_GRAD = 1, V_DH = 2, V_DW = 3 };
+//   V_PROD   both, sharing one launch (vocab8.hip)
+enum { V_STATS = 0, V_GRAD = 1, V_DH = 2, V_DW = 3, V_PROD = 4 };
+
+// the words at the head of the workspace
+struct VocabHead {
+  int32_t count;            // live rows
+  float grad_max;
+  float out_scale[2];       // what a sum over G, and over c, is multiplied by
+  VocabSchedule schedule[2];
+};
 
 }  // namespace

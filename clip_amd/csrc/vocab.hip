@@ -14,6 +14,12 @@
 // their products cost nothing and whatever a dropped row holds (NaN included) reaches no gradient.
 #include "vocab.h"
 
+#define TRY(expr)                          \
+  do {                                     \
+    hipError_t _e = (expr);                \
+    if (_e != hipSuccess) return _e;       \
+  } while (0)
+
 namespace {
 
 // ---- LDS image of a K tile of one operand, R rows (of the output's M or N) by 64 k:
@@ -168,13 +174,14 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
       const int r = row0 + m * 16;
-      const float4 rc = a.row_coef[r];
+      const float4 ri = a.row_info[r];
+      const int at = __float_as_int(ri.z) - (int)a.v0 - col0;   // the label, counted from this lane's first column
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float g[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          g[e] = __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -rc.x)) * rc.y;
+          g[e] = at == n * 16 + e ? ri.w : __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -ri.x)) * ri.y;
           cs[n][e] += g[e];
         }
         *reinterpret_cast<uint2*>(a.g + (int64_t)r * a.ldg + col0 + n * 16) = make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3]));
@@ -196,8 +203,10 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int n = 0; n < NB; ++n)
-        if (col0 + n * 16 < a.hidden)
-          *reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + m * 16) * a.hidden + col0 + n * 16) = acc[m][n];
+        if (col0 + n * 16 < a.hidden) {
+          f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + m * 16) * a.hidden + col0 + n * 16);
+          *o = a.accumulate ? *o + acc[m][n] : acc[m][n];
+        }
   } else {
     const float s = a.out_scale[0];
 #pragma unroll
@@ -265,123 +274,222 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
 }
 
-// dh = G W over one piece has (rows / 256)(hidden / 256) tiles and a long k of `pairs` x 128: it is cut into the number of
-// splits that fills the persistent workgroups best, a round of them costing its k plus about 8 pairs' time for the fp32
-// partials (256 KiB a tile, written here and read by the last kernel).
-__device__ int choose_splits(const VocabRows& a, int total, int pairs) {
-  const int rows = (total + 255) & ~255, tiles = (rows >> 8) * a.split_tiles_n;
-  if (tiles == 0) return 1;
-  int64_t most = (int64_t)a.split_cap * 65536 / ((int64_t)rows * a.hidden);   // split_cap: 65536 floats of room each
-  if (most > 64) most = 64;
-  if (most > pairs) most = pairs;
-  int best = 1, best_cost = 0x7fffffff;
-  for (int s = 1; s <= (int)most; ++s) {
-    const int cost = ((tiles * s + a.split_wgs - 1) / a.split_wgs) * ((pairs + s - 1) / s + 8);
-    if (cost < best_cost) { best_cost = cost; best = s; }
+// ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
+// tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
+// leave the CU; dh: 256 KB of fp32 partials leave it and are read again by the last kernel).  Lane s tries s + 1 splits, and for
+// each a few shares of the workgroups that are behind by one dW tile.
+__device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
+  const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
+  if (tiles > 0) {   // partials that there is room for
+    const int64_t room = a.dh_room / ((int64_t)rows_t * 256 * a.hidden);
+    if (room < max_splits) max_splits = (int)room;
   }
-  return best;
+  const int n_dw = a.with_dw ? vocab_tiles * a.tiles_h : 0, full = n_dw / wgs, rest = n_dw - full * wgs;
+  const int len_dw = (total + 127) / 128 + 2, splits = lane + 1;
+  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 5;
+  int best = 0x7fffffff, best_more = 0, best_less = 0;
+  if (splits <= max_splits && splits <= vocab_tiles)
+    for (int less = 0; less < 4; ++less) {   // dh tiles of a workgroup with one dW tile more
+      const int left = n_dh - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
+      const int t0 = rest ? (full + 1) * len_dw + less * len_dh : 0, t1 = full * len_dw + more * len_dh;
+      const int cost = max(t0, t1);
+      if (cost < best) { best = cost; best_less = less; best_more = more; }
+    }
+  const int low = best;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+  const int win = __ffsll(__ballot(low == best)) - 1;
+  VocabSchedule r;
+  r.splits = win + 1;
+  r.dh_less = __shfl(best_less, win, 64);
+  r.dh_more = __shfl(best_more, win, 64);
+  r.unused = 0;
+  return r;
 }
 
-// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the next multiple of 256, count = how many.  One
-// workgroup per 64 rows; each counts all rows' states itself (8 bytes a row from L2), so there is no scan kernel.
-// Backward: also every live row's (lse, c), the common factor, zeroed gradients of the dropped rows and a zeroed table.
+// 0 takes no part, 1 live, 2 live with a target outside the vocabulary
+__device__ __forceinline__ int row_state(const VocabRows& a, int r) {
+  if (a.state) return a.state[r];
+  const int64_t y = a.labels[r];
+  return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
+}
+__device__ __forceinline__ float finite_abs(float g) {
+  g = fabsf(g);
+  return g < INFINITY ? g : 0.f;
+}
+
+// what the whole call needs to know: by one wave, once
+template <bool GRAD>
+__device__ void write_head(const VocabRows& a, int total, float grad_max, int lane) {
+  // (every piece sums into the first's partials: the last must not have more of them)
+  VocabSchedule s0 = {a.max_splits, 0, 0, 0}, s1 = s0;
+  if (GRAD && a.wgs) {
+    s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
+    s1 = choose_schedule(a, total, a.piece_tiles[1], s0.splits, lane);
+  }
+  if (lane != 0) return;
+  *a.count = total;
+  if (GRAD) {
+    // the factor common to all rows; what is left of a row's gradient is c, |c| <= 1.  No live row: zeros, not 0 / 0
+    const float f = (a.grad_rows ? grad_max : a.grad[0]) * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);
+    *a.grad_max = grad_max;
+    a.out_scale[0] = f / G_SCALE;
+    a.out_scale[1] = f;
+    a.schedule[0] = s0;
+    a.schedule[1] = s1;
+  }
+}
+
+// Calls of many rows: the live rows before every 16th row, by one workgroup (a thread reads 16 rows' states at a time)
+template <bool GRAD>
+__global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
+  __shared__ int sums[16];
+  __shared__ float maxs[16];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  int before = 0;
+  float gm = 0.f;
+  for (int r0 = 0; r0 < a.n; r0 += 16384) {
+    const int r = r0 + tid * 16;
+    int live = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (r + i < a.n) {
+        const int s = row_state(a, r + i) != 0;
+        live += s;
+        if (GRAD && a.grad_rows && s) gm = fmaxf(gm, finite_abs(a.grad[r + i]));
+      }
+    int up = live;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int t = __shfl_up(up, o, 64);
+      if (lane >= o) up += t;
+    }
+    __syncthreads();
+    if (lane == 63) sums[w] = up;
+    __syncthreads();
+    int base = before, all = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < w) base += sums[i];
+      all += sums[i];
+    }
+    if (r < a.n) a.block_base[r >> 4] = base + up - live;
+    before += all;
+  }
+  if (GRAD) {
+    gm = wave_max(gm);
+    if (lane == 0) maxs[w] = gm;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; ++i) gm = fmaxf(gm, maxs[i]);
+  }
+  if (w == 0) write_head<GRAD>(a, before, gm, lane);
+}
+
+// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the next multiple of 256.  One workgroup per 16 rows;
+// without a scan before it (few rows) each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
+// zero gradients of the dropped rows, and a zeroed table of target sums.
 template <bool GRAD>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
+  __shared__ int before_s[4], total_s[4];
   __shared__ float red[4];
-  __shared__ int rows[64], n_rows, before_s[4], total_s[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * 64;
-  auto state_of = [&](int r) -> int {
-    if (a.state) return a.state[r];
-    const int64_t y = a.labels[r];
-    return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
-  };
-  int before = 0, total = 0;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * 16;
+  int before, total;
   float gm = 0.f;
-  for (int r = tid; r < a.n; r += 256) {
-    const int live = state_of(r) != 0;
-    total += live;
-    before += live && r < r0;
-    if (GRAD && a.grad_rows && live) {
-      const float g = fabsf(a.grad[r]);
-      if (g < INFINITY) gm = fmaxf(gm, g);
+  if (a.block_base) {
+    before = a.block_base[blockIdx.x];
+    total = *a.count;
+    if (GRAD) gm = *a.grad_max;
+  } else {
+    before = total = 0;
+    for (int r = tid; r < a.n; r += 256) {
+      const int live = row_state(a, r) != 0;
+      total += live;
+      before += live && r < r0;
+      if (GRAD && a.grad_rows && live) gm = fmaxf(gm, finite_abs(a.grad[r]));
     }
-  }
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    before += __shfl_xor(before, o, 64);
-    total += __shfl_xor(total, o, 64);
-  }
-  if (lane == 0) { before_s[w] = before; total_s[w] = total; }
-  if (GRAD && a.grad_rows) gm = block_max(gm, red);
-  __syncthreads();
-  before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
-  total = total_s[0] + total_s[1] + total_s[2] + total_s[3];
-  // the factor common to all rows; c = what is left of a row's gradient, |c| <= 1
-  float common = 1.f;
-  if (GRAD) {
-    if (a.grad_rows) {
-      common = gm;
-    } else {
-      common = a.grad[0];
+    for (int o = 32; o > 0; o >>= 1) {
+      before += __shfl_xor(before, o, 64);
+      total += __shfl_xor(total, o, 64);
     }
+    if (lane == 0) { before_s[w] = before; total_s[w] = total; }
+    if (GRAD) gm = block_max(gm, red);
+    __syncthreads();
+    before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
+    total = total_s[0] + total_s[1] + total_s[2] + total_s[3];
+    if (blockIdx.x == 0 && w == 0) write_head<GRAD>(a, total, gm, lane);
   }
-  if (blockIdx.x == 0 && tid == 0) {
-    *a.count = total;
-    if (GRAD) {
-      const float f = common * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);   // no live row: zeros, not 0 / 0
-      a.out_scale[0] = f / G_SCALE;
-      a.out_scale[1] = f;
-      for (int i = 0; i < 2; ++i) a.splits[i] = a.split_wgs ? choose_splits(a, total, a.split_pairs[i]) : a.split_cap;
+  // every wave ranks the 16 rows, wave 0 notes them down, wave w copies rows 4 w .. 4 w + 3
+  const int r = r0 + lane, st = lane < 16 && r < a.n ? row_state(a, r) : 0;
+  const unsigned live = (unsigned)__ballot(st != 0);
+  const int H = a.hidden;
+  {
+    const int64_t first = before + __popc(live & ((1u << (w * 4)) - 1));
+    const bf16_t* src[4];
+    bf16_t* dst[4];
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int q = w * 4 + i;
+      src[i] = a.h + (int64_t)(r0 + q) * a.ldh;
+      dst[i] = (live >> q & 1) ? a.x + (first + n++) * H : nullptr;
     }
+    if (a.h_aligned)
+      for (int c = lane * 8; c < H; c += 512) {   // four rows' loads in flight
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (dst[i]) v[i] = *reinterpret_cast<const uint4*>(src[i] + c);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + c) = v[i];
+      }
+    else
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (dst[i])
+          for (int c = lane; c < H; c += 64) dst[i][c] = src[i][c];
+    if (GRAD && a.dh)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (!dst[i] && r0 + w * 4 + i < a.n)
+          for (int c = lane; c < H; c += 64) a.dh[(int64_t)(r0 + w * 4 + i) * a.ld_dh + c] = 0;
   }
-  if (w == 0) {
-    const int r = r0 + lane;
-    const int st = r < a.n ? state_of(r) : 0;
-    const unsigned long long m = __ballot(st != 0);
-    const int local = __popcll(m & ((1ull << lane) - 1)), rank = before + local;
+  if (w == 0 && lane < 16 && r < a.n) {
     if (st != 0) {
-      rows[local] = r;
+      const int rank = before + __popc(live & ((1u << lane) - 1));
       a.row_map[rank] = st == 2 ? ~r : r;    // a row whose target is outside the vocabulary: NaN loss and gradients
       if (GRAD) {
         float c = 1.f;
         if (a.grad_rows) {
           const float g = a.grad[r];
-          c = fabsf(g) < INFINITY ? (common > 0.f ? g / common : 0.f) : g;
+          c = fabsf(g) < INFINITY ? (gm > 0.f ? g / gm : 0.f) : g;
         }
         if (st == 2) c = __builtin_nanf("");
         const float l2 = a.lse[r] * LOG2E;
-        // G = y exp2(z log2(e) / T - x): x takes |c| (and G's scale), y its sign
-        a.row_coef[rank] = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, l2, c);
+        // x takes |c| and G's scale, y its sign
+        float4 info = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, __int_as_float(-1), 0.f);
+        if (a.state) {
+          a.row_lc[rank] = make_float2(l2, c);
+        } else if (st == 1) {
+          info.z = __int_as_float((int)a.labels[r]);
+          info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -l2)) - 1.f) * G_SCALE;
+        }
+        a.row_info[rank] = info;
       }
-    } else if (r < a.n && !GRAD) {
+    } else if (!GRAD) {
       a.row_loss[r] = 0.f;
       a.lse_out[r] = 0.f;
     }
-    if (lane == 0) n_rows = __popcll(m);
-  }
-  __syncthreads();
-  const int H = a.hidden;
-  for (int i = w; i < n_rows; i += 4) {
-    const bf16_t* src = a.h + (int64_t)rows[i] * a.ldh;
-    bf16_t* dst = a.x + (int64_t)(before + i) * H;
-    if (a.h_aligned)
-      for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
-    else
-      for (int c = lane; c < H; c += 64) dst[c] = src[c];
   }
   const int pad = (total + 255) & ~255;
-  for (int r = total + blockIdx.x * 4 + w; r < pad; r += gridDim.x * 4) {
-    for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)r * H + c) = make_uint4(0, 0, 0, 0);
-    if (GRAD && lane == 0) a.row_coef[r] = make_float4(INFINITY, 1.f, 0.f, 0.f);   // G = 0
+  for (int q = total + blockIdx.x * 4 + w; q < pad; q += gridDim.x * 4) {
+    for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)q * H + c) = make_uint4(0, 0, 0, 0);
+    if (GRAD && lane == 0) a.row_info[q] = make_float4(INFINITY, 1.f, __int_as_float(-1), 0.f);   // G = 0
   }
-  if (GRAD) {
-    if (a.dh)
-      for (int i = w; i < 64 && r0 + i < a.n; i += 4)
-        if (state_of(r0 + i) == 0)
-          for (int c = lane; c < H; c += 64) a.dh[(int64_t)(r0 + i) * a.ld_dh + c] = 0;
-    if (a.fix)
-      for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
-  }
+  if (GRAD && a.fix)
+    for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
 }
 
 // score (times 1/T) of one vocabulary entry for the hidden row x: a wave's dot product, fp32
@@ -420,7 +528,7 @@ __global__ __launch_bounds__(256) void vocab_loss_kernel(VocabRows a, const floa
     for (int j = w; j < a.k; j += 4) {
       const int64_t v = a.t_index[(int64_t)row * a.ld_ti + j];
       float z = 0.f;
-      if (v >= 0) {
+      if (v >= 0 && v < a.vocab) {
         z = (wave_score(x, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
         const float pj = a.t_p[(int64_t)row * a.k + j];
         if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - z + lse);
@@ -445,42 +553,48 @@ __global__ __launch_bounds__(256) void vocab_loss_kernel(VocabRows a, const floa
 
 // loss[0] = sum of the rows' losses, over the live rows' count for the mean (0 / 0 = NaN as torch's mean over none);
 // one workgroup, fixed order
-__global__ __launch_bounds__(256) void vocab_reduce_kernel(VocabRows a) {
-  __shared__ float red[4];
-  float s = 0.f;
-  for (int i = threadIdx.x; i < a.n; i += 256) s += a.row_loss[i];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) a.loss[0] = a.mean ? s / (float)*a.count : s;
+__global__ __launch_bounds__(1024) void vocab_reduce_kernel(VocabRows a) {
+  __shared__ float red[16];
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int i = threadIdx.x; i < a.n; i += 4096)
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u * 1024 < a.n) s[u] += a.row_loss[i + u * 1024];
+  const float t = wave_sum((s[0] + s[1]) + (s[2] + s[3]));
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    float sum = 0.f;
+    for (int i = 0; i < 16; ++i) sum += red[i];
+    a.loss[0] = a.mean ? sum / (float)*a.count : sum;
+  }
 }
 
-// The targets' part of G, one wave per live row: G[r, v] = c (q_v - sum of p over the entries that name v), from the
-// forward's fp32 score of v (a difference of the rounded q would lose what is left where q is near p).  The sums of the
-// targets per vocabulary entry, which db needs, go to a table of 64-bit fixed point: integer adds commute, so their
-// order does not show (2^-38 a unit; p <= 1, n <= 2^24 rows).
-__global__ __launch_bounds__(256) void vocab_targets_kernel(VocabRows a, bf16_t* __restrict__ g, int64_t ldg, int64_t v0, int64_t v1,
-                                                            int table) {
+// The teacher's part of G, one wave per live row: G[r, v] = c (q_v - sum of p over the entries that name v), from the
+// forward's fp32 score of v (a difference of the rounded q would lose what is left where q is near p).  (A label's part is
+// set by V_GRAD itself.)  The sums of c p per vocabulary entry, which db needs, go to a table of 64-bit fixed point: integer
+// adds commute, so their order does not show (2^-38 a unit; |c| p <= 1, n <= 2^24 rows).
+__global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf16_t* __restrict__ g, int64_t ldg, int64_t v0, int64_t v1,
+                                                                 int table) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= *a.count) return;
   const int row = a.row_map[r];
   if (row < 0) return;
-  const float4 rc = a.row_coef[r];
+  const float2 lc = a.row_lc[r];
+  const int64_t* index = a.t_index + (int64_t)row * a.ld_ti;
+  const float* tp = a.t_p + (int64_t)row * a.k;
   for (int j = lane; j < a.k; j += 64) {
-    const int64_t v = a.state ? a.t_index[(int64_t)row * a.ld_ti + j] : a.labels[row];
-    if (v < 0) continue;
-    float p = 1.f;
-    if (a.state) {
-      const float own = a.t_p[(int64_t)row * a.k + j];
-      p = 0.f;
-      for (int i = 0; i < a.k; ++i)
-        if (a.t_index[(int64_t)row * a.ld_ti + i] == v) p += a.t_p[(int64_t)row * a.k + i];
-      if (table && fabsf(rc.w * own) <= 1.f)
-        atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(rc.w * own) * FIX));
-    } else if (table && fabsf(rc.w) <= 1.f) {
-      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)rc.w * FIX));
-    }
+    const int64_t v = index[j];
+    const float own = tp[j];
+    if (v < 0 || v >= a.vocab) continue;   // (not listed; beyond the vocabulary only where the value is -inf)
+    float p = 0.f;
+    for (int i = 0; i < a.k; ++i)
+      if (index[i] == v) p += tp[i];
+    if (table && fabsf(lc.y * own) <= 1.f)
+      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
     if (v < v0 || v >= v1) continue;
-    const float q = __builtin_amdgcn_exp2f(a.target_in[(int64_t)row * a.k + j] * LOG2E - rc.z);
-    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(rc.w * (q - p) * G_SCALE);
+    const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
+    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(lc.y * (q - p) * G_SCALE);
   }
 }
 
@@ -491,15 +605,21 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
   if ((int)blockIdx.x < row_blocks) {
     const int64_t total = (int64_t)count * (a.hidden / 4);
     const int64_t slot = p.large ? (int64_t)((count + 255) & ~255) * a.hidden : p.dh_slot;
+    const int n = a.schedule[0].splits;
     const float s = a.out_scale[0];
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
       const int r = (int)(i / (a.hidden / 4)), c = (int)(i % (a.hidden / 4)) * 4;
+      const float* q = part + (int64_t)r * a.hidden + c;
       f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-      for (int64_t piece = 0; piece < p.pieces; ++piece) {
-        const int n = a.splits[piece == p.pieces - 1];
-        const float* q = part + piece * p.dh_piece + (int64_t)r * a.hidden + c;
-        for (int k = 0; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
+      int k = 0;
+      for (; k + 4 <= n; k += 4) {   // four slots' loads in flight, added in order
+        f32x4_t t[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const f32x4_t*>(q + (k + u) * slot);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) v += t[u];
       }
+      for (; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
       const int m = a.row_map[r];
       bf16_t* o = a.dh + (int64_t)(m < 0 ? ~m : m) * a.ld_dh + c;
 #pragma unroll
@@ -512,7 +632,7 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
     float s = 0.f;
     for (int k = 0; k < n_sums; ++k) s += colsum[(int64_t)k * p.ld_colsum + v];
     // (s is in units of G, the table in units of c)
-    a.dbias[v] = (float)((double)s / G_SCALE - (double)a.fix[v] / FIX) * a.out_scale[1];
+    a.dbias[v] = a.fix ? (float)((double)s / G_SCALE - (double)a.fix[v] / FIX) * a.out_scale[1] : s * a.out_scale[0];
   }
 }
 
@@ -528,8 +648,7 @@ hipError_t launch_tiles(const VocabGemm& g, int tiles_m, int splits, hipStream_t
 
 #if !CLIP_OPERAND_F16
 // G of one piece of the vocabulary may take this much: the pieces are as few as that allows
-constexpr int64_t G_BYTES = 512ll << 20;
-
+constexpr int64_t G_BYTES = 1ll << 30;
 // From here on the 256 x 256 tiles
 constexpr int LARGE_ROWS = 256;
 
@@ -543,9 +662,9 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   };
   p.large = n > LARGE_ROWS && hidden % 128 == 0;
   const int64_t rows = ((int64_t)n + 255) / 256 * 256, vp = (vocab + 255) / 256 * 256;
-  p.count = take(4);
-  p.out_scale = take(16);   // and V_DH's splits
+  p.head = take(sizeof(VocabHead));
   p.row_map = take(rows * 4);
+  p.block_base = take(rows / 16 * 4);
   if (distill) {
     p.state = take(rows * 4);
     p.t_p = take((size_t)n * k * 4);
@@ -555,8 +674,11 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   if (!grad) {
     p.part = take(rows * (vp / 64) * 8);
   } else {
-    p.row_coef = take(rows * 16);
-    p.fix = take(vocab * 8);
+    p.row_info = take(rows * 16);
+    if (distill) {
+      p.row_lc = take(rows * 8);
+      p.fix = take(vocab * 8);
+    }
     // a piece: whole 256-column tiles, G within its bound, 32-bit byte offsets into the piece of W
     int64_t piece = rows > 0 ? G_BYTES / (rows * 2) : vp;
     if (piece > (1ll << 30) / ldw) piece = (1ll << 30) / ldw;
@@ -569,49 +691,69 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     p.g = take(rows * p.piece * 2);
     p.ld_colsum = vp;
     p.colsum = take((rows / 64) * vp * 4);
-    // dh = G W has few tiles and a long k: the vocabulary is split until every CU has two workgroups
+    // dh = G W has few tiles and a long k, which is split: until every CU has two workgroups, or (large) as the schedule on
+    // the device finds best, within this many fp32 partials of the rows
     const int64_t tiles = (rows / 128) * ((hidden + 127) / 128);
     int64_t s = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
     if (s > p.piece / 256) s = p.piece / 256;
     p.splits = (int32_t)(s < 1 ? 1 : s);
     p.dh_slot = rows * hidden;
-    p.dh_piece = p.splits * p.dh_slot;
-    if (p.large) {   // room for the splits that few live rows call for
+    int64_t room = p.splits * p.dh_slot;
+    if (p.large) {
       const int64_t tiles8 = (rows / 256) * ((hidden + 255) / 256);
-      p.dh_piece = (tiles8 > 256 ? 2 * tiles8 : 512) * 65536;
-      if (p.dh_piece < p.dh_slot) p.dh_piece = p.dh_slot;
+      room = (tiles8 > 256 ? 2 * tiles8 : 512) * 65536;
+      if (room < 2 * p.dh_slot) room = 2 * p.dh_slot;
     }
-    p.dh_part = take((size_t)p.pieces * p.dh_piece * 4);
+    p.dh_part = take((size_t)room * 4);
+    p.dh_room = room;
   }
   p.bytes = at;
   return p;
 }
 #endif
 
-#define TRY(expr)                          \
-  do {                                     \
-    hipError_t _e = (expr);                \
-    if (_e != hipSuccess) return _e;       \
-  } while (0)
+namespace {
 
-hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, void* work, hipStream_t st) {
-  VocabRows a = rows;
-  char* base = static_cast<char*>(work);
-  a.count = reinterpret_cast<int32_t*>(base + p.count);
+hipError_t device_cus(int* out) {
+  static DeviceOnce once;
+  return once.get([](int dev, int* val) { return hipDeviceGetAttribute(val, hipDeviceAttributeMultiprocessorCount, dev); }, out);
+}
+
+// what the forward and the backward begin with: the teacher's lists, and the live rows side by side
+template <bool GRAD>
+hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, hipStream_t st) {
+  VocabHead* head = reinterpret_cast<VocabHead*>(base + p.head);
+  a.count = &head->count;
+  a.grad_max = &head->grad_max;
+  a.out_scale = head->out_scale;
+  a.schedule = head->schedule;
   a.row_map = reinterpret_cast<int32_t*>(base + p.row_map);
   a.x = reinterpret_cast<bf16_t*>(base + p.x);
-  float2* part = reinterpret_cast<float2*>(base + p.part);
   if (a.t_index) {
     a.state = reinterpret_cast<int32_t*>(base + p.state);
     a.t_p = reinterpret_cast<float*>(base + p.t_p);
-    a.t_logp = reinterpret_cast<float*>(base + p.t_logp);
+    a.t_logp = GRAD ? nullptr : reinterpret_cast<float*>(base + p.t_logp);
     if (a.n > 0) {
       hipLaunchKernelGGL(vocab_teacher_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
       TRY(hipGetLastError());
     }
   }
-  hipLaunchKernelGGL(vocab_pack_kernel<false>, dim3(a.n > 0 ? (a.n + 63) / 64 : 1), dim3(256), 0, st, a);
-  TRY(hipGetLastError());
+  if (a.n > 1024) {   // more rows than a workgroup of the next kernel should count for itself
+    a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
+    hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
+    TRY(hipGetLastError());
+  }
+  hipLaunchKernelGGL(vocab_pack_kernel<GRAD>, dim3(a.n > 0 ? (a.n + 15) / 16 : 1), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, void* work, hipStream_t st) {
+  VocabRows a = rows;
+  char* base = static_cast<char*>(work);
+  float2* part = reinterpret_cast<float2*>(base + p.part);
+  TRY(gather_rows<false>(a, p, base, st));
   if (a.n > 0) {
     VocabGemm g = {};
     g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
@@ -629,7 +771,7 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
     TRY(hipGetLastError());
   }
   if (a.loss) {
-    hipLaunchKernelGGL(vocab_reduce_kernel, dim3(1), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(vocab_reduce_kernel, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -638,68 +780,63 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
 hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf16_t* dw, int64_t ld_dw, void* work, hipStream_t st) {
   VocabRows a = rows;
   char* base = static_cast<char*>(work);
-  a.count = reinterpret_cast<int32_t*>(base + p.count);
-  a.out_scale = reinterpret_cast<float*>(base + p.out_scale);
-  a.row_map = reinterpret_cast<int32_t*>(base + p.row_map);
-  a.row_coef = reinterpret_cast<float4*>(base + p.row_coef);
-  a.x = reinterpret_cast<bf16_t*>(base + p.x);
-  a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
+  a.row_info = reinterpret_cast<float4*>(base + p.row_info);
   if (a.t_index) {
-    a.state = reinterpret_cast<int32_t*>(base + p.state);
-    a.t_p = reinterpret_cast<float*>(base + p.t_p);
-    if (a.n > 0) {
-      hipLaunchKernelGGL(vocab_teacher_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
-      TRY(hipGetLastError());
-    }
+    a.row_lc = reinterpret_cast<float2*>(base + p.row_lc);
+    a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
   }
-  a.splits = reinterpret_cast<int32_t*>(base + p.out_scale + 8);
-  a.split_cap = p.splits;
+  a.with_dw = dw != nullptr;
+  a.max_splits = p.splits;
+  a.tiles_h = (int)((a.hidden + (p.large ? 255 : T_BN - 1)) / (p.large ? 256 : T_BN));
   if (p.large) {
-    static DeviceOnce once;
-    TRY(once.get([](int dev, int* val) { return hipDeviceGetAttribute(val, hipDeviceAttributeMultiprocessorCount, dev); }, &a.split_wgs));
-    a.split_wgs &= ~7;
-    a.split_tiles_n = (a.hidden + 255) / 256;
-    a.split_cap = (int32_t)(p.dh_piece / 65536);
-    a.split_pairs[0] = (int32_t)(p.piece / 128);
-    a.split_pairs[1] = (int32_t)((a.vocab - (p.pieces - 1) * p.piece + 255) / 256 * 2);
+    TRY(device_cus(&a.wgs));
+    a.wgs &= ~7;
+    a.dh_room = p.dh_room;
+    a.piece_tiles[0] = (int32_t)(p.piece / 256);
+    a.piece_tiles[1] = (int32_t)((a.vocab - (p.pieces - 1) * p.piece + 255) / 256);
   }
-  hipLaunchKernelGGL(vocab_pack_kernel<true>, dim3(a.n > 0 ? (a.n + 63) / 64 : 1), dim3(256), 0, st, a);
-  TRY(hipGetLastError());
+  TRY(gather_rows<true>(a, p, base, st));
   VocabGemm g = {};
   g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
   g.scale2 = LOG2E * a.inv_t;
   g.g = reinterpret_cast<bf16_t*>(base + p.g);
-  g.row_coef = a.row_coef;
+  g.row_info = a.row_info;
   g.colsum = a.dbias ? reinterpret_cast<float*>(base + p.colsum) : nullptr;
   g.ld_colsum = p.ld_colsum;
-  float* dh_part = reinterpret_cast<float*>(base + p.dh_part);
+  g.out32 = reinterpret_cast<float*>(base + p.dh_part);
   g.slot_stride = p.dh_slot;
   g.out16 = dw; g.ldo = ld_dw;
   g.out_scale = a.out_scale;
-  const int tiles_r = (a.n + T_BM - 1) / T_BM, tiles_h = (int)((a.hidden + (p.large ? 255 : T_BN - 1)) / (p.large ? 256 : T_BN));
+  g.with_dw = dw != nullptr;
+  g.with_dh = a.dh && a.n > 0;
+  const int tiles_r = (a.n + T_BM - 1) / T_BM;
   for (int64_t v0 = 0, piece = 0; v0 < a.vocab; v0 += p.piece, ++piece) {
     const int64_t v1 = v0 + p.piece < a.vocab ? v0 + p.piece : a.vocab;
     g.v0 = v0;
     g.ldg = (int)((v1 - v0 + 255) / 256 * 256);
+    g.schedule = a.schedule + (piece == p.pieces - 1 && piece > 0);
+    g.accumulate = piece > 0;
     if (a.n > 0) {
       g.tiles_n = g.ldg / (p.large ? 256 : T_BN);
       TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_tiles<V_GRAD>(g, tiles_r, 1, st));
-      hipLaunchKernelGGL(vocab_targets_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
-                         (a.fix && piece == 0) ? 1 : 0);
-      TRY(hipGetLastError());
+      if (a.t_index) {
+        hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
+                           (a.fix && piece == 0) ? 1 : 0);
+        TRY(hipGetLastError());
+      }
     }
-    g.tiles_n = tiles_h;
-    if (a.dh && a.n > 0) {
-      g.out32 = dh_part + piece * p.dh_piece;
-      g.splits = a.splits + (piece == p.pieces - 1);
-      TRY(p.large ? launch_vocab8(V_DH, g, st) : launch_tiles<V_DH>(g, tiles_r, p.splits, st));
+    g.tiles_n = a.tiles_h;
+    if (p.large) {
+      TRY(launch_vocab8(V_PROD, g, st));
+    } else {
+      if (g.with_dh) TRY(launch_tiles<V_DH>(g, tiles_r, p.splits, st));
+      if (g.with_dw) TRY(launch_tiles<V_DW>(g, (g.ldg + T_BM - 1) / T_BM, 1, st));
     }
-    if (dw) TRY(p.large ? launch_vocab8(V_DW, g, st) : launch_tiles<V_DW>(g, (g.ldg + T_BM - 1) / T_BM, 1, st));
   }
-  const int row_blocks = a.dh && a.n > 0 ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
+  const int row_blocks = g.with_dh ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
   const int b_blocks = a.dbias ? (int)((a.vocab + 255) / 256) : 0;
   if (row_blocks + b_blocks > 0) {
-    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks), dim3(256), 0, st, a, p, dh_part, g.colsum, row_blocks);
+    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks), dim3(256), 0, st, a, p, g.out32, g.colsum, row_blocks);
     TRY(hipGetLastError());
   }
   return hipSuccess;

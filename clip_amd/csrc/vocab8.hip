@@ -6,16 +6,27 @@
 //  * loads go through a buffer descriptor, so the vocabulary may end anywhere (rows past the end read as zero);
 //  * the number of live rows is read on the device: tiles past it are never visited;
 //  * epilogues: (max, sum of exp2) per row and 64 columns; the 16-bit score gradients with their column sums; fp32 partials;
-//    16-bit weight gradients.
+//    16-bit weight gradients;
+//  * dW tiles and dh tiles share one launch: either alone leaves a last round of workgroups mostly idle.
 #include "vocab.h"
 
 namespace {
+
+#ifndef V8_NT
+#define V8_NT 1
+#endif
+template <typename V>
+__device__ __forceinline__ void G_STORE(V v, V* p) {
+  if (V8_NT) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
 
 constexpr int BM = 256, BN = 256;
 constexpr int HT = 16384;              // half-tile
 constexpr int RING = 8 * HT;           // 2 K tiles
 constexpr int SCR = 2048;              // epilogue scratch per wave
-constexpr int LDS8 = RING + 8 * SCR + 2 * 1024;   // + bias[2][256]
+constexpr int SIDE = 1024 + 4096;      // of the next tile, by LDS-DMA: bias[256], row_info[256]
+constexpr int LDS8 = RING + 8 * SCR + 2 * SIDE;
 
 __device__ __forceinline__ float xor16_sum(float v) {
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -60,136 +71,164 @@ struct Cursor {
 template <int EPI>
 __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr bool A_TR = EPI == V_DW, B_TR = EPI == V_DH || EPI == V_DW, ROWS = EPI == V_STATS || EPI == V_GRAD;
+  constexpr bool ROWS = EPI == V_STATS || EPI == V_GRAD;   // else V_PROD: dW tiles, then dh tiles
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = w >> 2, wc = w & 3;   // wr: barrier group AND 64-row block inside each A half
   char* scr = smem + RING + w * SCR;
-  const float* bias_lds = reinterpret_cast<const float*>(smem + RING + 8 * SCR);
+  char* side = smem + RING + 8 * SCR;
+  // What the K loop does not need is computed again, from the arguments in memory, where it is needed (at a change of tile
+  // and in the epilogue): kept in registers it would be spilled, and the reloads wait for every staged half-tile
+  typedef const __attribute__((address_space(4))) VocabGemm* Args;
+  auto args = [&]() -> Args {
+    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();   // = &a: the only argument
+    asm volatile("" : "+s"(p));
+    return p;
+  };
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  const int rows_pad = (count + 255) & ~255;
-
-  // ---- items: (row or vocabulary panel tm, column tile tn, K tiles kt0 .. kt0 + nt)
-  const int G = gridDim.x, per_x = G >> 3;
+  int splits = 1, dh_less = 0, dh_more = 0;
+  if (!ROWS) {
+    splits = __builtin_amdgcn_readfirstlane(a.schedule->splits);
+    dh_less = __builtin_amdgcn_readfirstlane(a.schedule->dh_less);
+    dh_more = __builtin_amdgcn_readfirstlane(a.schedule->dh_more);
+  }
+  const int G = gridDim.x;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
-  const int tiles_m = EPI == V_DW ? a.ldg / BM : rows_pad / BM, tiles_n = a.tiles_n;
-  const int splits = EPI == V_DH ? __builtin_amdgcn_readfirstlane(*a.splits) : 1;
-  // the 8 XCDs take contiguous runs of the longer side: the vocabulary's tiles (each XCD its own part of W)
-  const int run_all = ROWS ? tiles_n : tiles_m, run = (run_all >> 3) + (xcd < (run_all & 7) ? 1 : 0);
-  const int run0 = xcd * (run_all >> 3) + min(xcd, run_all & 7);
-  int tm, tn, kt0, nt;
-  auto item = [&](int i, int& tm_o, int& tn_o, int& kt0_o, int& nt_o) -> bool {
+  const int lin = xcd * (G >> 3) + slot;   // neighbours share an XCD
+  const uint32_t ld_x = (uint32_t)a.hidden * 2, ld_g = (uint32_t)a.ldg * 2, ld_w = (uint32_t)a.ldw * 2;
+
+  // ---- items of this workgroup: a dW or dh tile or one of scores (panel tm, column tile tn), K tiles kt0 .. kt0 + nt
+  struct Item { bool dh; int tm, tn, kt0, nt, split; };
+  auto item = [&](int i, Item& o) -> bool {
+    const auto& a = *args();
+    const int tiles_r = (count + 255) >> 8, tiles_n = a.tiles_n;
+    o.kt0 = o.split = 0;
+    o.dh = false;
     if (ROWS) {
-      // column groups of 4 tiles (their slice of W stays in this XCD's L2), all row panels of one before the next
-      const int q = slot + per_x * i;
-      if (q >= run * tiles_m) return false;
-      const int per_group = 4 * tiles_m, g = q / per_group, r = q - g * per_group;
+      // the 8 XCDs take contiguous runs of the vocabulary's tiles, each its own part of W; within it column groups of 4 tiles
+      // (their slice of W stays in this XCD's L2), all row panels of one before the next
+      const int run = (tiles_n >> 3) + (xcd < (tiles_n & 7) ? 1 : 0), run0 = xcd * (tiles_n >> 3) + min(xcd, tiles_n & 7);
+      const int q = slot + (G >> 3) * i;
+      if (q >= run * tiles_r) return false;
+      const int per_group = 4 * tiles_r, g = q / per_group, r = q - g * per_group;
       const int wide = min(4, run - g * 4), m = r / wide;
-      tm_o = m;
-      tn_o = run0 + g * 4 + (r - m * wide);
-      kt0_o = 0;
-      nt_o = a.hidden / BK;
+      o.tm = m;
+      o.tn = run0 + g * 4 + (r - m * wide);
+      o.nt = a.hidden / BK;
       return true;
     }
-    if (EPI == V_DW) {
-      const int q = slot + per_x * i;
-      if (q >= run * tiles_n) return false;
-      tm_o = run0 + q / tiles_n;
-      tn_o = q % tiles_n;
-      kt0_o = 0;
-      nt_o = (count + 127) / 128 * 2;
+    // dW tiles dealt round-robin, then dh tiles as the schedule says
+    const int n_dw = a.with_dw ? (a.ldg >> 8) * tiles_n : 0, dw_full = n_dw / G, dw_rest = n_dw - dw_full * G;
+    const bool more_dw = lin < dw_rest;
+    const int my_dw = dw_full + (more_dw ? 1 : 0);
+    if (i < my_dw) {
+      const int q = i * G + lin;
+      o.tm = q / tiles_n;
+      o.tn = q - o.tm * tiles_n;
+      o.nt = (count + 127) / 128 * 2;
       return true;
     }
-    const int q = xcd * per_x + slot + G * i, tiles = tiles_m * tiles_n;
+    const int t = i - my_dw, tiles = tiles_r * tiles_n;
+    if (t >= (more_dw ? dh_less : dh_more) || !a.with_dh) return false;
+    const int q = more_dw ? (G - dw_rest) * dh_more + lin + dw_rest * t : (lin - dw_rest) + (G - dw_rest) * t;
     if (q >= tiles * splits) return false;
-    const int s = q / tiles, t = q - s * tiles, all = a.ldg / 128;
-    tm_o = t / tiles_n;
-    tn_o = t - tm_o * tiles_n;
-    kt0_o = all * s / splits * 2;
-    nt_o = all * (s + 1) / splits * 2 - kt0_o;
+    const int s = q / tiles, u = q - s * tiles, all = a.ldg >> 7;
+    o.dh = true;
+    o.split = s;
+    o.tm = u / tiles_n;
+    o.tn = u - o.tm * tiles_n;
+    o.kt0 = all * s / splits * 2;
+    o.nt = all * (s + 1) / splits * 2 - o.kt0;
     return true;
   };
-  if (!item(0, tm, tn, kt0, nt)) return;   // workgroup-uniform
+  Item cur;
+  if (!item(0, cur)) return;   // workgroup-uniform
 
   // ---- LDS-DMA: this wave's two 1-KiB pieces of a half-tile.  K-major image [128 rows][128 B]: rows 8 w .. and 64 + 8 w ..;
   // R-major image [64 k][256 B]: k 4 w .. and 32 + 4 w ..; the source chunk carries the swizzle
-  const uint32_t ld_a = (uint32_t)(ROWS ? a.hidden : a.ldg) * 2, ld_b = (uint32_t)((ROWS || EPI == V_DH) ? a.ldw : a.hidden) * 2;
-  auto lane_off = [&](bool tr, uint32_t ld) -> uint32_t {
-    if (!tr) {
-      const int r = w * 8 + (lane >> 3);
-      return r * ld + swz128(r, lane & 7) * 16;
-    }
-    const int k = w * 4 + (lane >> 4), c = lane & 15;
-    return k * ld + (((((c >> 1) ^ tr_swz<128>(k)) << 1) | (c & 1)) << 4);
-  };
-  const uint32_t a_off = lane_off(A_TR, ld_a), b_off = lane_off(B_TR, ld_b);
-  const uint32_t a_off2 = a_off + (A_TR ? 32 : 64) * ld_a, b_off2 = b_off + (B_TR ? 32 : 64) * ld_b;   // (same swizzle)
-  const uint32_t a_half = A_TR ? 256 : 128 * ld_a, b_half = B_TR ? 256 : 128 * ld_b;
-  const uint32_t a_step = A_TR ? BK * ld_a : BK * 2, b_step = B_TR ? BK * ld_b : BK * 2;
+  const int rk = w * 8 + (lane >> 3), rr = w * 4 + (lane >> 4), cc = lane & 15;
+  const uint32_t chunk_k = swz128(rk, lane & 7) * 16, chunk_r = ((((cc >> 1) ^ tr_swz<128>(rr)) << 1) | (cc & 1)) << 4;
+  // A: x K-major (ROWS), G R-major (dW), G K-major (dh);  B: W K-major, x R-major, W R-major
+  const uint32_t a_off0 = ROWS ? rk * ld_x + chunk_k : rr * ld_g + chunk_r, a_off1 = rk * ld_g + chunk_k;
+  const uint32_t b_off0 = ROWS ? rk * ld_w + chunk_k : rr * ld_x + chunk_r, b_off1 = rr * ld_w + chunk_r;
   const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(smem);
-  auto stage_a = [&](const Cursor& c, int half, int slot_idx) {
+  auto stage_a = [&](const Cursor& c, bool is_dh, int half, int slot_idx) {
     const uint32_t dst = lds0 + slot_idx * HT + w * 1024;
-    const u32x4_t r = c.rsrc(half ? a_half : 0);
-    dma16(r, a_off, dst);
-    dma16(r, a_off2, dst + 8192);
+    const uint32_t ld = ROWS ? ld_x : ld_g;
+    const bool tr = !ROWS && !is_dh;
+    const uint32_t off = ROWS || !is_dh ? a_off0 : a_off1;
+    const u32x4_t r = c.rsrc(half ? (tr ? 256 : 128 * ld) : 0);
+    dma16(r, off, dst);
+    dma16(r, off + (tr ? 32 : 64) * ld, dst + 8192);
   };
-  auto stage_b = [&](const Cursor& c, int half, int slot_idx) {
+  auto stage_b = [&](const Cursor& c, bool is_dh, int half, int slot_idx) {
     const uint32_t dst = lds0 + slot_idx * HT + w * 1024;
-    const u32x4_t r = c.rsrc(half ? b_half : 0);
-    dma16(r, b_off, dst);
-    dma16(r, b_off2, dst + 8192);
+    const uint32_t ld = ROWS || is_dh ? ld_w : ld_x;
+    const uint32_t off = ROWS || !is_dh ? b_off0 : b_off1;
+    const u32x4_t r = c.rsrc(half ? (ROWS ? 128 * ld : 256) : 0);
+    dma16(r, off, dst);
+    dma16(r, off + (ROWS ? 64 : 32) * ld, dst + 8192);
   };
-  auto stage_bias = [&](int tn_x, int buf) {   // every wave fetches the whole 1 KiB: uniform counts
+  // every wave fetches the bias slice and a quarter of the rows' info (waves 4..7 the same quarters): uniform counts
+  auto stage_side = [&](int tm_x, int tn_x, int buf) {
+    const auto& a = *args();
+    const uint32_t dst = lds0 + RING + 8 * SCR + buf * SIDE;
     const int64_t v0 = a.v0 + (int64_t)tn_x * BN;
-    dma16(make_rsrc(a.bias ? a.bias + v0 : nullptr, a.bias ? (a.vocab - v0) * 4 : 0), lane * 16, lds0 + RING + 8 * SCR + buf * 1024);
+    dma16(make_rsrc(a.bias ? a.bias + v0 : nullptr, a.bias ? (a.vocab - v0) * 4 : 0), lane * 16, dst);
+    if (EPI == V_GRAD) dma16(make_rsrc(a.row_info + tm_x * BM, BM * 16), (w & 3) * 1024 + lane * 16, dst + 1024 + (w & 3) * 1024);
   };
-  auto start_of = [&](int tm_x, int tn_x, int kt, Cursor& ca, Cursor& cb) {
+  auto start_of = [&](const Item& o, Cursor& ca, Cursor& cb) {
+    const auto& a = *args();
+    const int rows_pad = (count + 255) & ~255;
     if (ROWS) {
-      ca.set(a.x + (int64_t)tm_x * BM * a.hidden, (int64_t)BM * a.hidden * 2);
-      const int64_t v0 = a.v0 + (int64_t)tn_x * BN;
+      ca.set(a.x + (int64_t)o.tm * BM * a.hidden, (int64_t)BM * a.hidden * 2);
+      const int64_t v0 = a.v0 + (int64_t)o.tn * BN;
       cb.set(a.w + v0 * a.ldw, ((a.vocab - 1 - v0) * a.ldw + a.hidden) * 2);
-    } else if (EPI == V_DH) {
-      ca.set(a.g + (int64_t)tm_x * BM * a.ldg + (int64_t)kt * BK, ((int64_t)BM * a.ldg - (int64_t)kt * BK) * 2);
-      const int64_t v0 = a.v0 + (int64_t)kt * BK;
-      cb.set(a.w + v0 * a.ldw + tn_x * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - tn_x * BN) * 2);
+    } else if (o.dh) {
+      ca.set(a.g + (int64_t)o.tm * BM * a.ldg + (int64_t)o.kt0 * BK, ((int64_t)BM * a.ldg - (int64_t)o.kt0 * BK) * 2);
+      const int64_t v0 = a.v0 + (int64_t)o.kt0 * BK;
+      cb.set(a.w + v0 * a.ldw + o.tn * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - o.tn * BN) * 2);
     } else {
-      ca.set(a.g + (int64_t)tm_x * BM, ((int64_t)rows_pad * a.ldg - (int64_t)tm_x * BM) * 2);
-      cb.set(a.x + tn_x * BN, ((int64_t)rows_pad * a.hidden - tn_x * BN) * 2);
+      ca.set(a.g + (int64_t)o.tm * BM, ((int64_t)rows_pad * a.ldg - (int64_t)o.tm * BM) * 2);
+      cb.set(a.x + o.tn * BN, ((int64_t)rows_pad * a.hidden - o.tn * BN) * 2);
     }
   };
 
   // staging cursors: K tile t + 1 (c1) and t + 2 (c2) of the flattened (item, k) stream
   Cursor a1, b1, a2, b2;
-  bool v1, v2;
-  int s_it = 0, s_kt = 0, s_tm = tm, s_tn = tn, s_k0 = kt0, s_nt = nt;   // position of c2
+  bool v1, v2, d1, d2;
+  int s_it = 0, s_left = cur.nt;   // c2's item, and its K tiles from c2 on
   auto advance = [&]() {
-    a1 = a2; b1 = b2; v1 = v2;
+    a1 = a2; b1 = b2; v1 = v2; d1 = d2;
     if (!v2) return;
-    if (++s_kt == s_nt) {
-      s_kt = 0;
-      ++s_it;
-      v2 = item(s_it, s_tm, s_tn, s_k0, s_nt);
+    if (--s_left == 0) {
+      Item o;
+      v2 = item(++s_it, o);
       if (!v2) return;
-      start_of(s_tm, s_tn, s_k0, a2, b2);
+      s_left = o.nt;
+      d2 = o.dh;
+      start_of(o, a2, b2);
     } else {
-      a2.step(a_step);
-      b2.step(b_step);
+      // a K tile on: 128 bytes along a K-major row, 64 rows of an R-major operand
+      a2.step(ROWS || d2 ? BK * 2 : BK * ld_g);
+      b2.step(ROWS ? BK * 2 : BK * (d2 ? ld_w : ld_x));
     }
   };
   f32x4_t acc[2][2][4][2];
-  if (nt > 0) {   // (V_DW without a live row has no K tile; then no item has one)
-    start_of(tm, tn, kt0, a2, b2);
+  if (cur.nt > 0) {   // (a dW tile without live rows has no K tile; then no item has one)
+    start_of(cur, a2, b2);
     v2 = true;
-    stage_a(a2, 0, 0);
-    stage_b(b2, 0, 1);
-    stage_b(b2, 1, 2);
-    stage_a(a2, 1, 3);
-    if (ROWS) stage_bias(tn, 0);
+    d2 = cur.dh;
+    stage_a(a2, d2, 0, 0);
+    stage_b(b2, d2, 0, 1);
+    stage_b(b2, d2, 1, 2);
+    stage_a(a2, d2, 1, 3);
+    if (ROWS) stage_side(cur.tm, cur.tn, 0);
     advance();   // c2 = K tile 1
     advance();   // c1 = K tile 1, c2 = K tile 2 (or the next item's first)
-    stage_a(a1, 0, 4);
-    stage_b(b1, 0, 5);
+    stage_a(a1, d1, 0, 4);
+    stage_b(b1, d1, 0, 5);
     asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
     __builtin_amdgcn_s_barrier();
   }
@@ -212,118 +251,20 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
     const s16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return *reinterpret_cast<const opx8_t*>(&v);
   };
-  auto a_frag = [&](const char* half, int m, int ks) -> opx8_t {
-    if (A_TR) return tr_frag(half + a_tr[m] + ks * 8192);
+  auto a_frag = [&]<bool TR>(const char* half, int m, int ks) -> opx8_t {
+    if (TR) return tr_frag(half + a_tr[m] + ks * 8192);
     return *reinterpret_cast<const opx8_t*>(half + a_rd + m * 2048 + (ks ? c1 : c0));
   };
   auto b_frag = [&](const char* buf, int nh, int i, int ks) -> opx8_t {
-    if (B_TR) return tr_frag(buf + b_tr[nh * 2 + i] + ks * 8192);
+    if (!ROWS) return tr_frag(buf + b_tr[nh * 2 + i] + ks * 8192);
     return *reinterpret_cast<const opx8_t*>(buf + b_rd + nh * 4096 + i * 2048 + (ks ? c1 : c0));
   };
 
   int it = 0;
-  while (true) {
-    int ntm = 0, ntn = 0, nkt0 = 0, nnt = 0;
-    const bool has_next = item(it + 1, ntm, ntn, nkt0, nnt);
-    // acc[mh][nh][m][i]: lane holds n = 4 fq .. +3 of 16-column block (nh, i), row fr of 16-row block (mh, m)
-#pragma unroll
-    for (int nh = 0; nh < 2; ++nh)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f32x4_t start = {0.f, 0.f, 0.f, 0.f};
-        if (ROWS) start = *reinterpret_cast<const f32x4_t*>(bias_lds + (it & 1) * 256 + wc * 64 + fq * 4 + nh * 32 + i * 16);
-#pragma unroll
-        for (int mh = 0; mh < 2; ++mh)
-#pragma unroll
-          for (int m = 0; m < 4; ++m) acc[mh][nh][m][i] = start;
-      }
-    if (wr == 1) __builtin_amdgcn_s_barrier();   // waves 4..7 run one barrier behind
-
-    opx8_t af[4][2], bf0[2][2], bf1[2][2];
-    for (int kk = 0; kk < nt; kk += 2) {
-      auto ktile = [&]<int B>() {
-        const char* buf = smem + B * 4 * HT;
-        // ---------------- phase A: A0, both B halves -> acc[0][*]; stage (t+1).B1, (t+1).A1
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          bf0[i][0] = b_frag(buf, 0, i, 0);
-          bf0[i][1] = b_frag(buf, 0, i, 1);
-        }
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          af[m][0] = a_frag(buf, m, 0);
-          af[m][1] = a_frag(buf, m, 1);
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          bf1[i][0] = b_frag(buf, 1, i, 0);
-          bf1[i][1] = b_frag(buf, 1, i, 1);
-        }
-        if (v1) {
-          stage_b(b1, 1, (B ^ 1) * 4 + 2);
-          stage_a(a1, 1, (B ^ 1) * 4 + 3);
-          // in flight behind this wait: (t+1).A0/B0 from the previous phase and the four just issued
-          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        if (ROWS && B == 1 && kk == 0 && has_next) stage_bias(ntn, (it + 1) & 1);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              acc[0][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[0][0][m][i]);
-              acc[0][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[0][1][m][i]);
-            }
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-        // ---------------- phase B: A1 -> acc[1][*]; stage (t+2).A0, (t+2).B0; K tile t+1 retired
-#pragma unroll
-        for (int m = 0; m < 4; ++m) {
-          af[m][0] = a_frag(buf + 3 * HT, m, 0);
-          af[m][1] = a_frag(buf + 3 * HT, m, 1);
-        }
-        const bool staged2 = v2;
-        if (v2) {
-          stage_a(a2, 0, B * 4 + 0);
-          stage_b(b2, 0, B * 4 + 1);
-        }
-        advance();
-        if (staged2) {
-          asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-        } else {
-          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-        for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-          for (int m = 0; m < 4; ++m)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              acc[1][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[1][1][m][i]);
-              acc[1][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[1][0][m][i]);
-            }
-        __builtin_amdgcn_s_setprio(0);
-        __builtin_amdgcn_sched_barrier(0);
-        __builtin_amdgcn_s_barrier();
-      };
-      ktile.template operator()<0>();
-      ktile.template operator()<1>();
-    }
-    if (wr == 0) __builtin_amdgcn_s_barrier();   // balances the extra barrier of waves 4..7
-
-    // ---- epilogue.  Lane's rows: mh * 128 + wr * 64 + m * 16 + fr; its columns: wc * 64 + nh * 32 + i * 16 + 4 fq + e
+  // acc[mh][nh][m][i]: lane holds n = 4 fq .. +3 of 16-column block (nh, i), row fr of 16-row block (mh, m)
+  auto epilogue = [&](int le) {
+    const auto& a = *args();
+    const int fr = le & 15, fq = le >> 4, tm = cur.tm, tn = cur.tn;
     const int row0 = tm * BM + wr * 64 + fr, col0 = tn * BN + wc * 64 + fq * 4;
     if (ROWS && a.v0 + (int64_t)(tn + 1) * BN > a.vocab) {   // the last tile: nothing past the vocabulary
 #pragma unroll
@@ -374,28 +315,43 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
       for (int mh = 0; mh < 2; ++mh)
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-          const int r = row0 + mh * 128 + m * 16;
-          const float4 rc = a.row_coef[r];
+          const float4 ri = *reinterpret_cast<const float4*>(side + (it & 1) * SIDE + 1024 + (mh * 128 + wr * 64 + m * 16 + fr) * 16);
           // image [16 rows][128 B] in this wave's scratch, whole 128-byte row segments out
+          float g[2][2][4];
+#pragma unroll
+          for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                g[nh][i][e] = __builtin_amdgcn_exp2f(fmaf(acc[mh][nh][m][i][e], a.scale2, -ri.x)) * ri.y;
+          // a label among these 64 columns: seldom
+          const int at = __float_as_int(ri.z) - (int)a.v0 - tn * BN - wc * 64;
+          if (__any((unsigned)at < 64u)) {
+#pragma unroll
+            for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (at == nh * 32 + i * 16 + fq * 4 + e) g[nh][i][e] = ri.w;
+          }
 #pragma unroll
           for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              float g[4];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                g[e] = __builtin_amdgcn_exp2f(fmaf(acc[mh][nh][m][i][e], a.scale2, -rc.x)) * rc.y;
-                cs[nh][i][e] += g[e];
-              }
+              for (int e = 0; e < 4; ++e) cs[nh][i][e] += g[nh][i][e];
               const int sl = ((nh * 2 + i) * 4 + fq) ^ ((fr & 7) << 1);
-              *reinterpret_cast<uint2*>(scr + fr * 128 + sl * 8) = make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3]));
+              *reinterpret_cast<uint2*>(scr + fr * 128 + sl * 8) =
+                  make_uint2(pack_op2(g[nh][i][0], g[nh][i][1]), pack_op2(g[nh][i][2], g[nh][i][3]));
             }
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const int row = p * 8 + (lane >> 3), c16 = lane & 7;
+            const int row = p * 8 + (le >> 3), c16 = le & 7;
             const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
-            *reinterpret_cast<u32x4_t*>(a.g + (int64_t)(tm * BM + mh * 128 + wr * 64 + m * 16 + row) * a.ldg + tn * BN + wc * 64 +
-                                        c16 * 8) = v;
+            G_STORE(v, reinterpret_cast<u32x4_t*>(a.g + (int64_t)(tm * BM + mh * 128 + wr * 64 + m * 16 + row) * a.ldg + tn * BN +
+                                                  wc * 64 + c16 * 8));
           }
         }
       if (a.colsum) {
@@ -410,9 +366,9 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
               *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + a.v0 + col0 + nh * 32 + i * 16) = t;
           }
       }
-    } else if (EPI == V_DH) {
-      const int split = (it * G + xcd * per_x + slot) / (tiles_m * tiles_n);
-      float* out = a.out32 + (int64_t)split * rows_pad * a.hidden;
+    } else if (cur.dh) {
+      const int rows_pad = (count + 255) & ~255;
+      float* out = a.out32 + (int64_t)cur.split * rows_pad * a.hidden;
 #pragma unroll
       for (int mh = 0; mh < 2; ++mh)
 #pragma unroll
@@ -421,8 +377,10 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
           for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-              if (col0 + nh * 32 + i * 16 < a.hidden)
-                *reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + mh * 128 + m * 16) * a.hidden + col0 + nh * 32 + i * 16) = acc[mh][nh][m][i];
+              if (col0 + nh * 32 + i * 16 < a.hidden) {
+                f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + mh * 128 + m * 16) * a.hidden + col0 + nh * 32 + i * 16);
+                *o = a.accumulate ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
+              }
     } else {
       const float s = a.out_scale[0];
 #pragma unroll
@@ -439,7 +397,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
             }
 #pragma unroll
           for (int p = 0; p < 2; ++p) {
-            const int row = p * 8 + (lane >> 3), c16 = lane & 7;
+            const int row = p * 8 + (le >> 3), c16 = le & 7;
             const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
             const int64_t vocab_row = a.v0 + tm * BM + mh * 128 + wr * 64 + m * 16 + row;
             const int c = tn * BN + wc * 64 + c16 * 8;
@@ -451,9 +409,124 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
           }
         }
     }
-    if (!has_next) break;
-    tm = ntm; tn = ntn; kt0 = nkt0; nt = nnt;
+  };
+
+  while (true) {
+#pragma unroll
+    for (int nh = 0; nh < 2; ++nh)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x4_t start = {0.f, 0.f, 0.f, 0.f};
+        if (ROWS) start = *reinterpret_cast<const f32x4_t*>(side + (it & 1) * SIDE + (wc * 64 + fq * 4 + nh * 32 + i * 16) * 4);
+#pragma unroll
+        for (int mh = 0; mh < 2; ++mh)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) acc[mh][nh][m][i] = start;
+      }
+    if (wr == 1) __builtin_amdgcn_s_barrier();   // waves 4..7 run one barrier behind
+
+    opx8_t af[4][2], bf0[2][2], bf1[2][2];
+    auto ktile = [&]<bool A_TR, int B>(int kk) {
+        const char* buf = smem + B * 4 * HT;
+        // ---------------- phase A: A0, both B halves -> acc[0][*]; stage (t+1).B1, (t+1).A1
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          bf0[i][0] = b_frag(buf, 0, i, 0);
+          bf0[i][1] = b_frag(buf, 0, i, 1);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          af[m][0] = a_frag.template operator()<A_TR>(buf, m, 0);
+          af[m][1] = a_frag.template operator()<A_TR>(buf, m, 1);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          bf1[i][0] = b_frag(buf, 1, i, 0);
+          bf1[i][1] = b_frag(buf, 1, i, 1);
+        }
+        if (v1) {
+          stage_b(b1, d1, 1, (B ^ 1) * 4 + 2);
+          stage_a(a1, d1, 1, (B ^ 1) * 4 + 3);
+          // in flight behind this wait: (t+1).A0/B0 from the previous phase and the four just issued
+          asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        if (ROWS && B == 1 && kk == 0) {
+          Item o;
+          if (item(it + 1, o)) stage_side(o.tm, o.tn, (it + 1) & 1);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              acc[0][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[0][0][m][i]);
+              acc[0][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[0][1][m][i]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+        // ---------------- phase B: A1 -> acc[1][*]; stage (t+2).A0, (t+2).B0; K tile t+1 retired
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          af[m][0] = a_frag.template operator()<A_TR>(buf + 3 * HT, m, 0);
+          af[m][1] = a_frag.template operator()<A_TR>(buf + 3 * HT, m, 1);
+        }
+        const bool staged2 = v2;
+        if (v2) {
+          stage_a(a2, d2, 0, B * 4 + 0);
+          stage_b(b2, d2, 0, B * 4 + 1);
+        }
+        advance();
+        if (staged2) {
+          asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+        } else {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              acc[1][1][m][i] = MFMA_16x16x32(bf1[i][ks], af[m][ks], acc[1][1][m][i]);
+              acc[1][0][m][i] = MFMA_16x16x32(bf0[i][ks], af[m][ks], acc[1][0][m][i]);
+            }
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_barrier();
+    };
+    const int nt = cur.nt;
+    if (ROWS || cur.dh) {
+      for (int kk = 0; kk < nt; kk += 2) {
+        ktile.template operator()<false, 0>(kk);
+        ktile.template operator()<false, 1>(kk);
+      }
+    } else {
+      for (int kk = 0; kk < nt; kk += 2) {
+        ktile.template operator()<true, 0>(kk);
+        ktile.template operator()<true, 1>(kk);
+      }
+    }
+    if (wr == 0) __builtin_amdgcn_s_barrier();   // balances the extra barrier of waves 4..7
+
+    // ---- epilogue.  Lane's rows: mh * 128 + wr * 64 + m * 16 + fr; its columns: wc * 64 + nh * 32 + i * 16 + 4 fq + e.
+    // (lane id formed anew, too: see args())
+    int le;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(le));
+    epilogue(le);
     ++it;
+    if (!item(it, cur)) break;
   }
 }
 
@@ -482,8 +555,7 @@ hipError_t KSET::launch_vocab8(int what, const VocabGemm& g, hipStream_t st) {
   switch (what) {
     case V_STATS: return launch_8<V_STATS>(g, st);
     case V_GRAD: return launch_8<V_GRAD>(g, st);
-    case V_DH: return launch_8<V_DH>(g, st);
-    case V_DW: return launch_8<V_DW>(g, st);
+    case V_PROD: return launch_8<V_PROD>(g, st);
     default: return hipErrorInvalidValue;
   }
 }
