@@ -678,7 +678,7 @@ int linear_args(const char* who, const clip_linear* d, int32_t k, const int64_t*
   if (((uintptr_t)d->dev_weight & 15) || ((uintptr_t)work & 15))
     return fail(CLIP_ERR_ARG, "%s: weight and workspace must be 16-byte aligned", who);
   if (k < 0 || k > 1024) return fail(CLIP_ERR_ARG, "%s: k = %d (1 .. 1024)", who, k);
-  if (!(temperature > 0.f) || !std::isfinite(temperature)) return fail(CLIP_ERR_ARG, "%s: temperature must be positive", who);
+  if (!(temperature >= 1e-6f && temperature <= 1e6f)) return fail(CLIP_ERR_ARG, "%s: temperature must be between 1e-6 and 1e6", who);
   *p = vocab_plan(d->n, d->vocab, d->hidden_size, d->ld_weight, k ? k : 1, k != 0, grad);
   if (work_bytes < (int64_t)p->bytes)
     return fail(CLIP_ERR_CAPACITY, "%s: workspace of %lld bytes, %lld needed (clip_linear_loss_workspace)", who,

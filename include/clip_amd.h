@@ -211,7 +211,7 @@ int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t
                         const float* dev_lse, const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden,
                         int64_t ld_dhidden, uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,
                         int64_t work_bytes, void* stream);
-/* Distillation from a teacher's top scores at `temperature` T > 0: row i lists k scores teacher_values[i, :] with their
+/* Distillation from a teacher's top scores at `temperature` T (1e-6 <= T <= 1e6): row i lists k scores teacher_values[i, :] with their
  * vocabulary ids teacher_index[i, :]; p_i = softmax of the listed values / T, q_i = softmax(z_i / T) over the vocabulary,
  *   row_loss[i] = T^2 sum_j p_ij (log p_ij - log q_i[index_ij]).
  * An entry with a negative id or the value -inf is left out; a row with none left contributes nothing (loss 0, no gradient,

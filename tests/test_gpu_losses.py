@@ -9,7 +9,7 @@ import torch
 pytestmark = pytest.mark.gpu
 sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "helpers"))
 import loss_case as R  # noqa: E402
-from clip_amd import _lib, losses  # noqa: E402
+from clip_amd import losses  # noqa: E402
 
 BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 INF, NAN = float("inf"), float("nan")
@@ -455,7 +455,7 @@ def test_refusals():
             (ValueError, lambda: ce(h[:, :32], w, b, y)), (ValueError, lambda: ce(h, w, b, y[:3])),
             (ValueError, lambda: ce(h, w, b, y.float())), (ValueError, lambda: ce(h, w, b, y, reduction="batchmean")),
             (RuntimeError, lambda: ce(h, w, b, y.cpu())), (RuntimeError, lambda: ce(h, w.cpu(), b, y)),
-            (_lib.ClipError, lambda: ce(h[:, :32].contiguous(), w[:, :32].contiguous(), b, y)),
+            (ValueError, lambda: ce(h[:, :32].contiguous(), w[:, :32].contiguous(), b, y)),
             (ValueError, lambda: kd(h, w, b, v, i, temperature=0.0)), (ValueError, lambda: kd(h, w, b, v, i, temperature=float("nan"))),
             (ValueError, lambda: kd(h, w, b, v, i.int())), (ValueError, lambda: kd(h, w, b, v[:, :2], i)),
             (ValueError, lambda: kd(h, w, b, v[:, :0], i[:, :0])), (ValueError, lambda: kd(h, w, b, v[:3], i[:3])),

@@ -93,3 +93,10 @@ def test_python_refuses_cpu_tensors():
         losses.linear_cross_entropy([1.0], w, None, y)
     with pytest.raises(ValueError, match="reduction"):
         losses.linear_cross_entropy(h, w, None, y, reduction="max")
+
+
+def test_missing_binding_raises(monkeypatch):
+    monkeypatch.setattr(losses, "_ext", None)
+    monkeypatch.setattr(losses, "EXT_PATH", losses.EXT_PATH + ".missing")
+    with pytest.raises(ImportError, match="build"):
+        losses.topk_logits(torch.zeros(2, 5), 1)
