@@ -1,9 +1,11 @@
 // A row's k largest scores with their ids, ties to the lowest id: what a teacher hands to the distillation loss
 // (clip_linear_distill).  Scores are ordered as torch orders them: NaN above everything, -0 equal to +0.
-// One workgroup streams a row once.  What reaches the running threshold goes, as a 64-bit key (order-preserving bits of
-// the score above the inverted id: all keys differ, a larger key comes first), to a candidate list in LDS; the list is cut
-// back to its k largest by counting, for every candidate, how many are larger.  The first threshold is the k-th largest of
-// the 256 threads' maxima over the first chunk, at most the true one, so that few candidates are ever written.
+// One workgroup per row; a chunk of up to 32 768 scores (a whole row of BERT's vocabulary) is read at once into registers,
+// 128 per thread.  The k-th largest of the threads' maxima (found to 16 bits by bisection on ballots) is a threshold that the
+// k largest all reach and few others do; each wave notes what reaches it, one comparison per score, in its own part of LDS
+// as 64-bit keys (order-preserving bits of the score above the inverted id: all keys differ, a larger key comes first), and
+// the few keys noted are sorted by counting, for each, how many are larger.  Where too many reach the threshold (equal
+// scores) the chunk is gone through again, a list being cut back to its k largest whenever it is full.
 #include "common.h"
 #include "kernels.h"
 
@@ -26,6 +28,7 @@ struct F32 {
   typedef float elem;
   static __device__ __forceinline__ float get(const uint4& v, int i) { return __uint_as_float(reinterpret_cast<const uint32_t*>(&v)[i]); }
   static __device__ __forceinline__ float one(const elem* p) { return *p; }
+  static constexpr uint32_t one_inf_bits = 0;
 };
 struct Bf16 {
   static constexpr int VEC = 8;
@@ -36,6 +39,7 @@ struct Bf16 {
     return i & 1 ? __uint_as_float(d & 0xffff0000u) : __uint_as_float(d << 16);
   }
   static __device__ __forceinline__ float one(const elem* p) { return bits(*p); }
+  static constexpr uint32_t one_inf_bits = 0xff80;
 };
 struct F16 {
   static constexpr int VEC = 8;
@@ -46,153 +50,190 @@ struct F16 {
     return half_bits((uint16_t)(i & 1 ? d >> 16 : d));
   }
   static __device__ __forceinline__ float one(const elem* p) { return half_bits(*p); }
+  static constexpr uint32_t one_inf_bits = 0xfc00;
 };
 
-constexpr int NT = 256, PER = 16;   // threads; scores per thread and chunk
+constexpr int NT = 256, PER = 128;   // threads; scores per thread and chunk
+constexpr uint32_t KEY_LOWEST = 0x007fffffu;   // order_key(-inf)
 
-// CAP: room for candidates, at least k + 256
-template <class T, int CAP>
+// KMAX: the largest k; GROUPS: maxima per thread that the threshold is taken from (k <= 256 GROUPS); WCAP: keys a wave may note
+template <class T, int KMAX, int GROUPS, int WCAP>
 __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* __restrict__ logits, int64_t ld, int vocab, int k,
                                                        typename T::elem* __restrict__ values, int64_t* __restrict__ index) {
-  constexpr int NV = PER / T::VEC;   // 16-byte loads per thread and chunk
+  constexpr int NV = PER / T::VEC;               // 16-byte loads per thread and chunk
+  constexpr int CAP = KMAX + 4 * WCAP;           // cand[0 .. KMAX): kept so far; then the waves' notes
   __shared__ u64 cand[CAP];
-  __shared__ u64 kth_s;
-  __shared__ float max_s[NT];
+  __shared__ uint32_t max_s[NT * GROUPS];
+  __shared__ uint32_t threshold_s;
   __shared__ int wave_s[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const typename T::elem* row = logits + (int64_t)blockIdx.x * ld;
 
-  int have = 0, turn = 0;            // uniform: candidates in the list
-  u64 kth = 0;                       // uniform: a key below the threshold does not count
+  int have = 0, turn = 0;            // uniform: keys kept
+  u64 kth = 0;                       // uniform: a smaller key is not among the k largest
   float kth_f = -INFINITY;           // its score; !(x < kth_f) is the cheap test (NaN passes)
   auto key64 = [](float x, int id) { return ((u64)order_key(x) << 32) | (uint32_t)~id; };
+  auto score_of = [](uint32_t key) { return key <= KEY_LOWEST ? -INFINITY : key_score(key); };
 
-  // the list's k largest, sorted, to its front
-  auto cut = [&]() {
-    __syncthreads();
-    // (the list is rarely longer than one or two scores per thread: those keep their scores in registers)
-    u64 mine[CAP / NT];
-    int rank[CAP / NT];
+  // the k largest of the kept keys and n[w] notes of each wave, sorted, become the kept ones
+  auto cut = [&](const int (&n)[4]) {
+    constexpr int MINE = (CAP + NT - 1) / NT;
+    const int total = have + n[0] + n[1] + n[2] + n[3];
+    u64 mine[MINE];
+    int rank[MINE];
 #pragma unroll
-    for (int i = 0; i < CAP / NT; ++i) {
-      mine[i] = tid + i * NT < have ? cand[tid + i * NT] : 0;
+    for (int i = 0; i < MINE; ++i) {
+      int at = tid + i * NT;
+      if (at >= have) {
+        at -= have;
+        int seg = 0;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+          if (seg == q && at >= n[q]) { at -= n[q]; seg = q + 1; }
+        at += KMAX + seg * WCAP;
+      }
+      mine[i] = tid + i * NT < total ? cand[at] : 0;
       rank[i] = 0;
     }
 #pragma unroll
-    for (int i = 0; i < CAP / NT; ++i)
-      if (i * NT < have)
+    for (int i = 0; i < MINE; ++i)
+      if (i * NT + w * 64 < total) {   // (wave-uniform)
         for (int j = 0; j < have; ++j) rank[i] += cand[j] > mine[i];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          for (int j = 0; j < n[q]; ++j) rank[i] += cand[KMAX + q * WCAP + j] > mine[i];
+      }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < CAP / NT; ++i)
-      if (tid + i * NT < have && rank[i] < k) cand[rank[i]] = mine[i];
-    if (have > k) have = k;
+    for (int i = 0; i < MINE; ++i)
+      if (tid + i * NT < total && rank[i] < k) cand[rank[i]] = mine[i];
+    have = min(total, k);
     __syncthreads();
     if (have == k) {
       kth = cand[k - 1];
-      kth_f = key_score((uint32_t)(kth >> 32));
+      kth_f = score_of((uint32_t)(kth >> 32));
     }
   };
-  // `n` of this thread's scores pass: where its first one goes; false = no room, nothing reserved
-  auto reserve = [&](int n, int& at) -> bool {
-    int before = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int up = __shfl_up(before, o, 64);
-      if (lane >= o) before += up;
-    }
+  // where this thread's key goes if `p`; false = no room (the list, taken as one behind the kept keys, is full)
+  int noted = 0;
+  auto reserve = [&](bool p, int& at) -> bool {
+    const unsigned long long m = __ballot(p);
     turn ^= 1;
-    if (lane == 63) wave_s[turn][w] = before;
+    if (lane == 0) wave_s[turn][w] = __popcll(m);
     __syncthreads();
     const int t0 = wave_s[turn][0], t1 = wave_s[turn][1], t2 = wave_s[turn][2], t3 = wave_s[turn][3];
-    at = have + before - n + (w > 0 ? t0 : 0) + (w > 1 ? t1 : 0) + (w > 2 ? t2 : 0);
+    at = KMAX + noted + __popcll(m & ((1ull << lane) - 1)) + (w > 0 ? t0 : 0) + (w > 1 ? t1 : 0) + (w > 2 ? t2 : 0);
     const int sum = t0 + t1 + t2 + t3;
-    if (have + sum > CAP) return false;
-    have += sum;
+    if (noted + sum > 4 * WCAP) return false;
+    noted += sum;
     return true;
   };
-  auto passes = [&](float x, int id) { return !(x < kth_f) && key64(x, id) >= kth; };
+  // the list as one segment: split over the waves' parts for cut()
+  auto cut_list = [&]() {
+    __syncthreads();
+    int n[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) n[q] = min(max(noted - q * WCAP, 0), WCAP);
+    cut(n);
+    noted = 0;
+  };
 
-  // ---- the scores before the first and after the last whole 16 bytes
+  // ---- the scores before the first and after the last whole 16 bytes are kept to begin with (at most 14)
   const int head = min((int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(typename T::elem)), vocab);
   const int body = (vocab - head) / T::VEC;   // whole vectors
   {
     const int rest = vocab - head - body * T::VEC;
     const int id = tid < head ? tid : head + body * T::VEC + (tid - head);
-    const bool in = tid < head + rest;
-    int at;
-    reserve(in ? 1 : 0, at);
-    if (in) cand[at] = key64(T::one(row + id), id);
+    if (tid < head + rest) cand[tid] = key64(T::one(row + id), id);
+    have = head + rest;
   }
   const uint4* vec = reinterpret_cast<const uint4*>(row + head);
-  uint4 cur[NV], nxt[NV];
-  auto fetch = [&](int c, uint4 (&to)[NV]) {
+  for (int c0 = 0; c0 < body; c0 += NV * NT) {
+    uint4 v[NV];
+    const uint32_t neg = sizeof(typename T::elem) == 4 ? 0xff800000u : (T::one_inf_bits * 0x10001u);   // -inf
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = (c * NV + i) * NT + tid;
-      if (at < body) to[i] = vec[at];
+      const int at = c0 + i * NT + tid;
+      v[i] = make_uint4(neg, neg, neg, neg);
+      if (at < body) v[i] = vec[at];
     }
-  };
-  const int chunks = (body + NV * NT - 1) / (NV * NT);
-  fetch(0, cur);
-  for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) fetch(c + 1, nxt);
-    if (c == 0 && k <= NT) {
-      float mx = -INFINITY;
+    if (kth == 0) {   // no threshold yet
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (i * NT + tid < body)
+      for (int g = 0; g < GROUPS; ++g) {
+        float mx = -INFINITY;
 #pragma unroll
-          for (int e = 0; e < T::VEC; ++e) mx = fmaxf(mx, T::get(cur[i], e));
-      max_s[tid] = mx;
-      __syncthreads();
-      int rank = 0;   // ties by thread: ranks are 0 .. 255
-      for (int j = 0; j < NT; ++j) rank += max_s[j] > mx || (max_s[j] == mx && j < tid);
-      if (rank == k - 1) kth_s = (u64)order_key(mx) << 32;
-      __syncthreads();
-      kth = kth_s;
-      kth_f = key_score((uint32_t)(kth >> 32));
-    }
-    uint32_t mask = 0;
+        for (int i = g * NV / GROUPS; i < (g + 1) * NV / GROUPS; ++i)
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = (c * NV + i) * NT + tid;
-      if (at < body)
-#pragma unroll
-        for (int e = 0; e < T::VEC; ++e) {
-          const float x = T::get(cur[i], e);
-          if (passes(x, head + at * T::VEC + e)) mask |= 1u << (i * T::VEC + e);
-        }
-    }
-    int at;
-    if (reserve(__popc(mask), at)) {
-#pragma unroll
-      for (int s = 0; s < PER; ++s)
-        if (mask & (1u << s))
-          cand[at++] = key64(T::get(cur[s / T::VEC], s % T::VEC), head + ((c * NV + s / T::VEC) * NT + tid) * T::VEC + s % T::VEC);
-      if (have > CAP / 2) cut();
-    } else {
-      // a crowded chunk: one score per thread at a time, the list cut back whenever it is full
-#pragma unroll 1
-      for (int s = 0; s < PER; ++s) {
-        float x = 0.f;
-#pragma unroll
-        for (int q = 0; q < PER; ++q)
-          if (q == s) x = T::get(cur[q / T::VEC], q % T::VEC);
-        const int id = head + ((c * NV + s / T::VEC) * NT + tid) * T::VEC + s % T::VEC;
-        bool p = (mask >> s & 1) && passes(x, id);
-        if (!reserve(p, at)) {
-          cut();
-          p = p && passes(x, id);
-          reserve(p, at);        // k + 256 fit
-        }
-        if (p) cand[at] = key64(x, id);
+          for (int e = 0; e < T::VEC; ++e) mx = fmaxf(mx, T::get(v[i], e));
+        max_s[g * NT + tid] = order_key(mx);
       }
-    }
+      __syncthreads();
+      if (w == 0) {
+        uint32_t m[NT * GROUPS / 64], t = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) cur[i] = nxt[i];
+        for (int i = 0; i < NT * GROUPS / 64; ++i) m[i] = max_s[i * 64 + lane];
+        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+          int n = 0;
+#pragma unroll
+          for (int i = 0; i < NT * GROUPS / 64; ++i) n += __popcll(__ballot(m[i] >= (t | bit)));
+          if (n >= k) t |= bit;
+        }
+        if (lane == 0) threshold_s = t;
+      }
+      __syncthreads();
+      const uint32_t t = threshold_s;
+      kth = (u64)t << 32;
+      kth_f = score_of(t);
+    }
+    // every wave notes what reaches the threshold
+    int cnt = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < T::VEC; ++e) {
+        const float x = T::get(v[i], e);
+        if (__any(!(x < kth_f)) && cnt <= WCAP) {
+          const int at = c0 + i * NT + tid, id = head + at * T::VEC + e;
+          const u64 key = key64(x, id);
+          const bool p = at < body && !(x < kth_f) && key >= kth;
+          const unsigned long long m = __ballot(p);
+          const int to = cnt + __popcll(m & ((1ull << lane) - 1));
+          if (p && to < WCAP) cand[KMAX + w * WCAP + to] = key;
+          cnt += __popcll(m);
+        }
+      }
+    turn ^= 1;
+    if (lane == 0) wave_s[turn][w] = cnt;
+    __syncthreads();
+    int n[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) n[q] = __builtin_amdgcn_readfirstlane(wave_s[turn][q]);
+    if (n[0] <= WCAP && n[1] <= WCAP && n[2] <= WCAP && n[3] <= WCAP) {
+      cut(n);
+    } else {
+      // crowded: read again, one score per thread at a time
+      noted = 0;
+#pragma unroll 1
+      for (int q = 0; q < PER && c0 + q / T::VEC * NT < body; ++q) {
+        const int at = c0 + q / T::VEC * NT + tid, id = head + at * T::VEC + q % T::VEC;
+        const u64 key = at < body ? key64(T::one(row + id), id) : 0;
+        bool p = at < body && key >= kth;
+        int to;
+        if (!reserve(p, to)) {
+          cut_list();
+          p = p && key >= kth;
+          reserve(p, to);        // 256 always fit an empty list
+        }
+        if (p) cand[to] = key;
+      }
+      cut_list();
+    }
   }
-  cut();
+  if (body == 0) {
+    __syncthreads();
+    const int none[4] = {0, 0, 0, 0};
+    cut(none);
+  }
   for (int j = tid; j < k; j += NT) {
     const int id = (int)~(uint32_t)cand[j];
     values[(int64_t)blockIdx.x * k + j] = row[id];
@@ -205,9 +246,9 @@ hipError_t launch_t(const void* logits, int64_t ld, int n, int vocab, int k, voi
   const auto* in = static_cast<const typename T::elem*>(logits);
   auto* out = static_cast<typename T::elem*>(values);
   if (k <= 256)
-    hipLaunchKernelGGL((topk_rows_kernel<T, 1024>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
+    hipLaunchKernelGGL((topk_rows_kernel<T, 256, 1, 256>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
   else
-    hipLaunchKernelGGL((topk_rows_kernel<T, 4096>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
+    hipLaunchKernelGGL((topk_rows_kernel<T, 1024, 4, 512>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
   return hipGetLastError();
 }
 
