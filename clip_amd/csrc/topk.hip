@@ -1,11 +1,13 @@
 // A row's k largest scores with their ids, ties to the lowest id: what a teacher hands to the distillation loss
 // (clip_linear_distill).  Scores are ordered as torch orders them: NaN above everything, -0 equal to +0.
-// One workgroup per row; a chunk of up to 32 768 scores (a whole row of BERT's vocabulary) is read at once into registers,
-// 128 per thread.  The k-th largest of the threads' maxima (found to 16 bits by bisection on ballots) is a threshold that the
-// k largest all reach and few others do; each wave notes what reaches it, one comparison per score, in its own part of LDS
+// One workgroup per row; a chunk of 64 KB (16 384 fp32 scores or 32 768 of 16 bits) is read at once into registers, 64 per
+// thread.  A threshold that the k largest all reach and few others do is found to 16 bits by bisection on ballots:
+// for k <= 128 the k-th largest of the 256 threads' maxima (177 random scores reach it at k = 128, 74 at k = 64), beyond that
+// the k-th largest score itself.  Each wave notes what reaches it, one comparison per 16 bytes read, in its own part of LDS
 // as 64-bit keys (order-preserving bits of the score above the inverted id: all keys differ, a larger key comes first), and
 // the few keys noted are sorted by counting, for each, how many are larger.  Where too many reach the threshold (equal
 // scores) the chunk is gone through again, a list being cut back to its k largest whenever it is full.
+// Bound: reading the scores; 8192 x 30 522 with k 64: fp32 200 us (5.0 TB/s), bf16 138 us, fp16 119 us (4.2 TB/s); five rows 8.4 us.
 #include "common.h"
 #include "kernels.h"
 
@@ -23,9 +25,15 @@ __device__ __forceinline__ float key_score(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);   // 0xffffffff: a NaN
 }
 
+// (maximum: NaN if either is)
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 struct F32 {
   static constexpr int VEC = 4;
   typedef float elem;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    return max_nan(max_nan(get(v, 0), get(v, 1)), max_nan(get(v, 2), get(v, 3)));
+  }
   static __device__ __forceinline__ float get(const uint4& v, int i) { return __uint_as_float(reinterpret_cast<const uint32_t*>(&v)[i]); }
   static __device__ __forceinline__ float one(const elem* p) { return *p; }
   static constexpr uint32_t one_inf_bits = 0;
@@ -33,6 +41,12 @@ struct F32 {
 struct Bf16 {
   static constexpr int VEC = 8;
   typedef uint16_t elem;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    float m = max_nan(get(v, 0), get(v, 1));
+#pragma unroll
+    for (int i = 2; i < 8; i += 2) m = max_nan(max_nan(m, get(v, i)), get(v, i + 1));
+    return m;
+  }
   static __device__ __forceinline__ float bits(uint32_t h) { return __uint_as_float(h << 16); }
   static __device__ __forceinline__ float get(const uint4& v, int i) {
     const uint32_t d = reinterpret_cast<const uint32_t*>(&v)[i >> 1];
@@ -44,6 +58,13 @@ struct Bf16 {
 struct F16 {
   static constexpr int VEC = 8;
   typedef uint16_t elem;
+  static __device__ __forceinline__ float top(const uint4& v) {
+    typedef __attribute__((ext_vector_type(2))) _Float16 h2;
+    h2 h[4];
+    __builtin_memcpy(h, &v, 16);
+    const h2 m = __builtin_elementwise_maximum(__builtin_elementwise_maximum(h[0], h[1]), __builtin_elementwise_maximum(h[2], h[3]));
+    return max_nan((float)m[0], (float)m[1]);
+  }
   static __device__ __forceinline__ float half_bits(uint16_t h) { _Float16 f; __builtin_memcpy(&f, &h, 2); return (float)f; }
   static __device__ __forceinline__ float get(const uint4& v, int i) {
     const uint32_t d = reinterpret_cast<const uint32_t*>(&v)[i >> 1];
@@ -53,17 +74,20 @@ struct F16 {
   static constexpr uint32_t one_inf_bits = 0xfc00;
 };
 
-constexpr int NT = 256, PER = 128;   // threads; scores per thread and chunk
+constexpr int NT = 256;   // threads
+// 16-byte loads per thread and chunk.  8192 rows of 30 522, k 64, in us (fp32 / bf16 / fp16): 8: 234 / 137 / 118, 12: 229 / 162 /
+// 136, 16: 200 / 138 / 119, 24: 282 / 175 / 158, 32 (a whole fp32 row): 295.  16 leave room for four workgroups per CU: their
+// loads and their searches overlap
+constexpr int NV = 16;
 constexpr uint32_t KEY_LOWEST = 0x007fffffu;   // order_key(-inf)
 
-// KMAX: the largest k; GROUPS: maxima per thread that the threshold is taken from (k <= 256 GROUPS); WCAP: keys a wave may note
-template <class T, int KMAX, int GROUPS, int WCAP>
+// KMAX: the largest k; MAXIMA: the threshold from the threads' maxima (k <= 128), else from all scores; WCAP: keys a wave may note
+template <class T, int KMAX, bool MAXIMA, int WCAP>
 __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* __restrict__ logits, int64_t ld, int vocab, int k,
                                                        typename T::elem* __restrict__ values, int64_t* __restrict__ index) {
-  constexpr int NV = PER / T::VEC;               // 16-byte loads per thread and chunk
   constexpr int CAP = KMAX + 4 * WCAP;           // cand[0 .. KMAX): kept so far; then the waves' notes
   __shared__ u64 cand[CAP];
-  __shared__ uint32_t max_s[NT * GROUPS];
+  __shared__ uint32_t max_s[MAXIMA ? NT : 1];
   __shared__ uint32_t threshold_s;
   __shared__ int wave_s[2][4];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -152,56 +176,72 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
     uint4 v[NV];
     const uint32_t neg = sizeof(typename T::elem) == 4 ? 0xff800000u : (T::one_inf_bits * 0x10001u);   // -inf
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int at = c0 + i * NT + tid;
-      v[i] = make_uint4(neg, neg, neg, neg);
-      if (at < body) v[i] = vec[at];
-    }
+    for (int i = 0; i < NV; ++i) v[i] = vec[min(c0 + i * NT + tid, body - 1)];   // (no branches: all loads in flight)
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (c0 + (i + 1) * NT > body && c0 + i * NT + tid >= body) v[i] = make_uint4(neg, neg, neg, neg);
     if (kth == 0) {   // no threshold yet
+      uint32_t t = 0;
+      if (MAXIMA) {
+        float mx = T::top(v[0]);
 #pragma unroll
-      for (int g = 0; g < GROUPS; ++g) {
-        float mx = -INFINITY;
+        for (int i = 1; i < NV; ++i) mx = max_nan(mx, T::top(v[i]));
+        max_s[tid] = order_key(mx);
+        __syncthreads();
+        if (w == 0) {
+          uint32_t m[NT / 64];
 #pragma unroll
-        for (int i = g * NV / GROUPS; i < (g + 1) * NV / GROUPS; ++i)
+          for (int i = 0; i < NT / 64; ++i) m[i] = max_s[i * 64 + lane];
+          for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+            int n = 0;
 #pragma unroll
-          for (int e = 0; e < T::VEC; ++e) mx = fmaxf(mx, T::get(v[i], e));
-        max_s[g * NT + tid] = order_key(mx);
-      }
-      __syncthreads();
-      if (w == 0) {
-        uint32_t m[NT * GROUPS / 64], t = 0;
-#pragma unroll
-        for (int i = 0; i < NT * GROUPS / 64; ++i) m[i] = max_s[i * 64 + lane];
+            for (int i = 0; i < NT / 64; ++i) n += __popcll(__ballot(m[i] >= (t | bit)));
+            if (n >= k) t |= bit;
+          }
+          if (lane == 0) threshold_s = t;
+        }
+        __syncthreads();
+        t = threshold_s;
+      } else {
         for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+          const float f = score_of(t | bit);   // (a NaN: only NaN reach it)
           int n = 0;
 #pragma unroll
-          for (int i = 0; i < NT * GROUPS / 64; ++i) n += __popcll(__ballot(m[i] >= (t | bit)));
-          if (n >= k) t |= bit;
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < T::VEC; ++e) n += __popcll(__ballot(!(T::get(v[i], e) < f) && ((t | bit) <= 0xff800000u || T::get(v[i], e) != T::get(v[i], e))));
+          turn ^= 1;
+          if (lane == 0) wave_s[turn][w] = n;
+          __syncthreads();
+          if (wave_s[turn][0] + wave_s[turn][1] + wave_s[turn][2] + wave_s[turn][3] >= k) t |= bit;
         }
-        if (lane == 0) threshold_s = t;
       }
-      __syncthreads();
-      const uint32_t t = threshold_s;
       kth = (u64)t << 32;
       kth_f = score_of(t);
     }
     // every wave notes what reaches the threshold
     int cnt = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) {
+      // (what the threshold's pass formed of v is formed again: kept, it would take the registers of another workgroup)
+      asm volatile("" : "+v"(v[i].x), "+v"(v[i].y), "+v"(v[i].z), "+v"(v[i].w));
+      if (__any(!(T::top(v[i]) < kth_f)) && cnt <= WCAP) {
+        const int at = c0 + i * NT + tid;
 #pragma unroll
-      for (int e = 0; e < T::VEC; ++e) {
-        const float x = T::get(v[i], e);
-        if (__any(!(x < kth_f)) && cnt <= WCAP) {
-          const int at = c0 + i * NT + tid, id = head + at * T::VEC + e;
-          const u64 key = key64(x, id);
-          const bool p = at < body && !(x < kth_f) && key >= kth;
-          const unsigned long long m = __ballot(p);
-          const int to = cnt + __popcll(m & ((1ull << lane) - 1));
-          if (p && to < WCAP) cand[KMAX + w * WCAP + to] = key;
-          cnt += __popcll(m);
+        for (int e = 0; e < T::VEC; ++e) {
+          const float x = T::get(v[i], e);
+          if (__any(!(x < kth_f))) {
+            const int id = head + at * T::VEC + e;
+            const u64 key = key64(x, id);
+            const bool p = at < body && key >= kth;
+            const unsigned long long m = __ballot(p);
+            const int to = cnt + __popcll(m & ((1ull << lane) - 1));
+            if (p && to < WCAP) cand[KMAX + w * WCAP + to] = key;
+            cnt += __popcll(m);
+          }
         }
       }
+    }
     turn ^= 1;
     if (lane == 0) wave_s[turn][w] = cnt;
     __syncthreads();
@@ -214,7 +254,7 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
       // crowded: read again, one score per thread at a time
       noted = 0;
 #pragma unroll 1
-      for (int q = 0; q < PER && c0 + q / T::VEC * NT < body; ++q) {
+      for (int q = 0; q < NV * T::VEC && c0 + q / T::VEC * NT < body; ++q) {
         const int at = c0 + q / T::VEC * NT + tid, id = head + at * T::VEC + q % T::VEC;
         const u64 key = at < body ? key64(T::one(row + id), id) : 0;
         bool p = at < body && key >= kth;
@@ -245,10 +285,10 @@ template <class T>
 hipError_t launch_t(const void* logits, int64_t ld, int n, int vocab, int k, void* values, int64_t* index, hipStream_t st) {
   const auto* in = static_cast<const typename T::elem*>(logits);
   auto* out = static_cast<typename T::elem*>(values);
-  if (k <= 256)
-    hipLaunchKernelGGL((topk_rows_kernel<T, 256, 1, 256>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
+  if (k <= 128)
+    hipLaunchKernelGGL((topk_rows_kernel<T, 128, true, 256>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
   else
-    hipLaunchKernelGGL((topk_rows_kernel<T, 1024, 4, 512>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
+    hipLaunchKernelGGL((topk_rows_kernel<T, 1024, false, 512>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
   return hipGetLastError();
 }
 
