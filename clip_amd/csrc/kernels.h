@@ -104,6 +104,12 @@ hipError_t launch_topk_rows(const void* logits, int type, int64_t ld, int n, int
 // How the products dh = G W and dW = G^T h of one piece share the persistent workgroups (vocab8.hip): dh's long k is cut
 // into `splits`; a workgroup that has one dW tile less than others takes dh_more of the split tiles, the others dh_less
 struct VocabSchedule { int32_t splits, dh_less, dh_more, unused; };
+struct VocabHead {          // the words at the head of the workspace
+  int32_t count, done;      // live rows; workgroups of the forward's last kernel that have finished
+  float grad_max;
+  float out_scale[2];       // what a sum over G, and over c, is multiplied by
+  VocabSchedule schedule[2];
+};
 struct VocabRows {          // rows, targets and results of one call; what is null is not asked for
   int32_t n, hidden, k;     // k: targets per row (1 for labels)
   int64_t vocab;
@@ -121,7 +127,9 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   bf16_t* dh; int64_t ld_dh;
   float* dbias;
   // workspace (VocabPlan)
-  int32_t *count, *row_map, *state;
+  VocabHead* head;
+  int32_t *count, *row_map, *state, *done;   // done: workgroups that have finished (null: not counted)
+  int32_t tile_rows;
   int32_t* block_base;      // live rows before every 16th row (calls of many rows), and
   float* grad_max;          // the largest finite |gradient| of a live row
   VocabSchedule* schedule;  // of every piece but the last, and of the last
@@ -155,6 +163,7 @@ struct VocabPlan {          // workspace of one call: byte offsets, and how the 
   int64_t piece, pieces, ld_colsum, dh_slot, dh_room;   // floats of one split's partials, and of all
   int32_t splits;         // at most
   bool large;             // 256 x 256 tiles (vocab8.hip)
+  int32_t tile_rows;      // rows of a tile of scores
 };
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad);
 

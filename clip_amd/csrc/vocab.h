@@ -14,6 +14,7 @@ constexpr float G_SCALE = 1.f;       // bf16 has fp32's range
 #endif
 constexpr double FIX = 274877906944.0;   // 2^38: fixed-point unit of the target sums, |sum| <= 2^24 rows
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
 
 // ---- buffer descriptor of [p, p + bytes): loads past the end return zero, which is how ragged vocabulary tails are read
 __device__ __forceinline__ u32x4_t make_rsrc(const void* p, int64_t bytes) {
@@ -62,13 +63,5 @@ __device__ __forceinline__ int tr_swz(int k) {
 //   V_DW     vocabulary x hidden over the rows -> 16-bit dW                                    A = G, B = live rows (both R-major)
 //   V_PROD   both, sharing one launch (vocab8.hip)
 enum { V_STATS = 0, V_GRAD = 1, V_DH = 2, V_DW = 3, V_PROD = 4 };
-
-// the words at the head of the workspace
-struct VocabHead {
-  int32_t count;            // live rows
-  float grad_max;
-  float out_scale[2];       // what a sum over G, and over c, is multiplied by
-  VocabSchedule schedule[2];
-};
 
 }  // namespace

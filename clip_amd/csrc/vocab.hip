@@ -68,15 +68,28 @@ struct Operand {
   }
 };
 
-// One output tile of BM x BN per workgroup of WM x WN waves (few rows: many small tiles; vocab8.hip takes the large calls).
-template <int EPI, int BM, int BN, int WM, int WN>
+// waits until at most `n` of this wave's loads are in flight
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N <= 24, "counted");
+  if (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+  else if (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else if (N == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// One output tile of BM x BN per workgroup of WM x WN waves, 64 columns per wave, through a ring of NST K tiles (few rows: many
+// small tiles and a deep ring, the weight's bytes are the bound; vocab8.hip takes the large calls).
+template <int EPI, int BM, int BN, int WM, int WN, int NST>
 __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
   constexpr int NW = WM * WN, MB = BM / WM / 16, NB = BN / WN / 16;
+  static_assert(NB == 4, "64 columns per wave");
   constexpr bool A_TR = EPI == V_DW, B_TR = EPI == V_DH || EPI == V_DW;
   typedef Operand<BM, A_TR, NW> OA;
   typedef Operand<BN, B_TR, NW> OB;
   constexpr int STAGE = OA::BYTES + OB::BYTES;
-  __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
+  extern __shared__ __attribute__((aligned(16))) char smem[];   // NST * STAGE
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
@@ -121,19 +134,25 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
   }
 
   const uint32_t lds0 = (uint32_t)(uintptr_t)LDS_PTR(smem);
-  if (nt > 0) {
-    oa.stage(0, lds0, w);
-    ob.stage(0, lds0 + OA::BYTES, w);
-  }
-  for (int kt = 0; kt < nt; ++kt) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();   // the tile is in LDS; every wave has read the buffer that is filled next
-    const char* buf = smem + (kt & 1) * STAGE;
-    if (kt + 1 < nt) {
-      const uint32_t nxt = lds0 + ((kt + 1) & 1) * STAGE;
-      oa.stage(kt + 1, nxt, w);
-      ob.stage(kt + 1, nxt + OA::BYTES, w);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (i < nt) {
+      oa.stage(i, lds0 + i * STAGE, w);
+      ob.stage(i, lds0 + i * STAGE + OA::BYTES, w);
     }
+  int slot = 0;
+  for (int kt = 0; kt < nt; ++kt) {
+    // K tile kt has landed; behind it NST - 2 tiles are in flight, until the last ones
+    if (kt + NST - 1 <= nt) wait_loads<(NST - 2) * (OA::PIECES + OB::PIECES)>();
+    else wait_loads<0>();
+    __syncthreads();   // ... for every wave; and every wave has read the buffer that is filled next
+    const char* buf = smem + slot * STAGE;
+    if (kt + NST - 1 < nt) {
+      const uint32_t nxt = lds0 + (slot == 0 ? NST - 1 : slot - 1) * STAGE;
+      oa.stage(kt + NST - 1, nxt, w);
+      ob.stage(kt + NST - 1, nxt + OA::BYTES, w);
+    }
+    slot = slot + 1 == NST ? 0 : slot + 1;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       opx8_t af[MB], bf[NB];
@@ -148,6 +167,17 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
     }
   }
 
+  // 16-bit results leave as whole 128-byte row segments, by way of this wave's [16 rows][128 B] in the ring's LDS
+  if (EPI == V_GRAD || EPI == V_DW) __syncthreads();
+  char* scr = smem + w * 2048;
+  auto put = [&](int n, uint2 v) { *reinterpret_cast<uint2*>(scr + fr * 128 + ((n * 4 + fq) ^ ((fr & 7) << 1)) * 8) = v; };
+  auto flush = [&](auto&& store) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int row = p * 8 + (lane >> 3), c16 = lane & 7;
+      store(row, c16 * 8, *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16)));
+    }
+  };
   if (EPI == V_STATS) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
@@ -184,8 +214,11 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
           g[e] = at == n * 16 + e ? ri.w : __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -ri.x)) * ri.y;
           cs[n][e] += g[e];
         }
-        *reinterpret_cast<uint2*>(a.g + (int64_t)r * a.ldg + col0 + n * 16) = make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3]));
+        put(n, make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3])));
       }
+      flush([&](int row, int c, const u32x4_t& v) {
+        *reinterpret_cast<u32x4_t*>(a.g + (int64_t)(row0 - fr + m * 16 + row) * a.ldg + tn * BN + wn * 64 + c) = v;
+      });
     }
     if (a.colsum) {   // fp32 column sums of what was rounded above: db is not made of rounded values
 #pragma unroll
@@ -211,14 +244,17 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
     const float s = a.out_scale[0];
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-      const int64_t v = a.v0 + row0 + m * 16;
-      if (v < a.vocab && row0 + m * 16 < a.ldg) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          if (col0 + n * 16 < a.hidden)
-            *reinterpret_cast<uint2*>(a.out16 + v * a.ldo + col0 + n * 16) =
-                make_uint2(pack_op2(acc[m][n][0] * s, acc[m][n][1] * s), pack_op2(acc[m][n][2] * s, acc[m][n][3] * s));
-      }
+      for (int n = 0; n < NB; ++n)
+        put(n, make_uint2(pack_op2(acc[m][n][0] * s, acc[m][n][1] * s), pack_op2(acc[m][n][2] * s, acc[m][n][3] * s)));
+      flush([&](int row, int c, const u32x4_t& v) {
+        const int at = row0 - fr + m * 16 + row, h = tn * BN + wn * 64 + c;
+        if (at < a.ldg && a.v0 + at < a.vocab && h < a.hidden) {   // (8-byte stores: the row stride is a multiple of 4)
+          u32x2_t* o = reinterpret_cast<u32x2_t*>(a.out16 + (a.v0 + at) * a.ldo + h);
+          __builtin_nontemporal_store((u32x2_t){v[0], v[1]}, o);
+          __builtin_nontemporal_store((u32x2_t){v[2], v[3]}, o + 1);
+        }
+      });
     }
   }
 }
@@ -329,6 +365,7 @@ __device__ void write_head(const VocabRows& a, int total, float grad_max, int la
   }
   if (lane != 0) return;
   *a.count = total;
+  if (!GRAD) a.head->done = 0;
   if (GRAD) {
     // the factor common to all rows; what is left of a row's gradient is c, |c| <= 1.  No live row: zeros, not 0 / 0
     const float f = (a.grad_rows ? grad_max : a.grad[0]) * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);
@@ -386,14 +423,23 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   if (w == 0) write_head<GRAD>(a, before, gm, lane);
 }
 
-// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the next multiple of 256.  One workgroup per 16 rows;
+// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the end of their last tile.  One workgroup per 16 rows;
 // without a scan before it (few rows) each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
 // zero gradients of the dropped rows, and a zeroed table of target sums.
 template <bool GRAD>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
   __shared__ int before_s[4], total_s[4];
   __shared__ float red[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * 16;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * 16, r = r0 + lane;
+  const int H = a.hidden;
+  // this wave's four rows are on their way before it is known which of them are live
+  uint4 held[4][2];
+  if (a.h_aligned && a.n > 0)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+        held[i][c] = *reinterpret_cast<const uint4*>(a.h + (int64_t)min(r0 + w * 4 + i, a.n - 1) * a.ldh + min(lane * 8 + c * 512, H - 8));
   int before, total;
   float gm = 0.f;
   if (a.block_base) {
@@ -421,40 +467,28 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     if (blockIdx.x == 0 && w == 0) write_head<GRAD>(a, total, gm, lane);
   }
   // every wave ranks the 16 rows, wave 0 notes them down, wave w copies rows 4 w .. 4 w + 3
-  const int r = r0 + lane, st = lane < 16 && r < a.n ? row_state(a, r) : 0;
+  const int st = lane < 16 && r < a.n ? row_state(a, r) : 0;
   const unsigned live = (unsigned)__ballot(st != 0);
-  const int H = a.hidden;
   {
-    const int64_t first = before + __popc(live & ((1u << (w * 4)) - 1));
-    const bf16_t* src[4];
-    bf16_t* dst[4];
-    int n = 0;
+    int64_t rank = before + __popc(live & ((1u << (w * 4)) - 1));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int q = w * 4 + i;
-      src[i] = a.h + (int64_t)(r0 + q) * a.ldh;
-      dst[i] = (live >> q & 1) ? a.x + (first + n++) * H : nullptr;
-    }
-    if (a.h_aligned)
-      for (int c = lane * 8; c < H; c += 512) {   // four rows' loads in flight
-        uint4 v[4];
+      if (live >> q & 1) {
+        bf16_t* dst = a.x + rank++ * H;
+        const bf16_t* src = a.h + (int64_t)(r0 + q) * a.ldh;
+        if (a.h_aligned) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (dst[i]) v[i] = *reinterpret_cast<const uint4*>(src[i] + c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (dst[i]) *reinterpret_cast<uint4*>(dst[i] + c) = v[i];
+          for (int c = 0; c < 2; ++c)
+            if (lane * 8 + c * 512 < H) *reinterpret_cast<uint4*>(dst + lane * 8 + c * 512) = held[i][c];
+          for (int c = lane * 8 + 1024; c < H; c += 512) *reinterpret_cast<uint4*>(dst + c) = *reinterpret_cast<const uint4*>(src + c);
+        } else {
+          for (int c = lane; c < H; c += 64) dst[c] = src[c];
+        }
+      } else if (GRAD && a.dh && r0 + q < a.n) {
+        for (int c = lane; c < H; c += 64) a.dh[(int64_t)(r0 + q) * a.ld_dh + c] = 0;
       }
-    else
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (dst[i])
-          for (int c = lane; c < H; c += 64) dst[i][c] = src[i][c];
-    if (GRAD && a.dh)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (!dst[i] && r0 + w * 4 + i < a.n)
-          for (int c = lane; c < H; c += 64) a.dh[(int64_t)(r0 + w * 4 + i) * a.ld_dh + c] = 0;
+    }
   }
   if (w == 0 && lane < 16 && r < a.n) {
     if (st != 0) {
@@ -483,7 +517,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       a.lse_out[r] = 0.f;
     }
   }
-  const int pad = (total + 255) & ~255;
+  const int pad = (total + a.tile_rows - 1) / a.tile_rows * a.tile_rows;
   for (int q = total + blockIdx.x * 4 + w; q < pad; q += gridDim.x * 4) {
     for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)q * H + c) = make_uint4(0, 0, 0, 0);
     if (GRAD && lane == 0) a.row_info[q] = make_float4(INFINITY, 1.f, __int_as_float(-1), 0.f);   // G = 0
@@ -505,50 +539,104 @@ __device__ __forceinline__ float wave_score(const bf16_t* x, const bf16_t* wrow,
   return wave_sum(s);
 }
 
-// One workgroup per live row: lse from the tiles' (max, sum) pairs, the targets' scores, the row's loss.
-__global__ __launch_bounds__(256) void vocab_loss_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
-  __shared__ float red[4];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (r >= *a.count) return;
-  const int mapped = a.row_map[r], row = mapped < 0 ? ~mapped : mapped;
-  const float2* p = part + (int64_t)r * n_part;
-  float mx = -INFINITY;
-  for (int i = tid; i < n_part; i += 256) mx = fmaxf(mx, p[i].x);
-  mx = block_max(mx, red);
-  const float ref = mx == -INFINITY ? 0.f : mx;
+// what a row's exponentials over 64 columns at a time come to: (largest score, sum) of a wave's share of the pairs
+__device__ __forceinline__ float2 wave_pairs(const float2* p, int n_part, int lane, int step) {
+  float2 v[8];
+  float mx = -INFINITY, s = 0.f;
+  for (int i0 = lane; i0 < n_part; i0 += 8 * step) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = i0 + u * step < n_part ? p[i0 + u * step] : make_float2(-INFINITY, 0.f);
+    float m = mx;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) m = fmaxf(m, v[u].x);
+    const float ref = m == -INFINITY ? 0.f : m;
+    s *= __builtin_amdgcn_exp2f(mx - ref);
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s += v[u].y * __builtin_amdgcn_exp2f(v[u].x - ref);
+    mx = m;
+  }
+  const float m = wave_max(mx), ref = m == -INFINITY ? 0.f : m;
+  return make_float2(m, wave_sum(s * __builtin_amdgcn_exp2f(mx - ref)));
+}
+__device__ __forceinline__ float lse_of(float2 p) { return LN2 * ((p.x == -INFINITY ? 0.f : p.x) + log2f(p.y)); }
+
+// The rows' losses are summed by the last of few workgroups to finish (the others' results are stored to where every XCD
+// reads, and acknowledged, before they count themselves), or by a kernel of its own where there are many.
+__device__ __forceinline__ void finish_rows(const VocabRows& a, int groups, float* red) {
+  __shared__ int last_s;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0)
+    last_s = __hip_atomic_fetch_add(a.done, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == groups - 1;
+  __syncthreads();
+  if (!last_s) return;
   float s = 0.f;
-  for (int i = tid; i < n_part; i += 256) s += p[i].y * __builtin_amdgcn_exp2f(p[i].x - ref);
+  for (int i = threadIdx.x; i < a.n; i += 256) s += __hip_atomic_load(a.row_loss + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   s = block_sum(s, red);
-  const float lse = LN2 * (ref + log2f(s));
-  const bf16_t* x = a.x + (int64_t)r * a.hidden;
-  float loss = 0.f;
-  if (mapped < 0) {
-    loss = __builtin_nanf("");
-  } else if (a.state) {
-    for (int j = w; j < a.k; j += 4) {
-      const int64_t v = a.t_index[(int64_t)row * a.ld_ti + j];
-      float z = 0.f;
-      if (v >= 0 && v < a.vocab) {
-        z = (wave_score(x, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
-        const float pj = a.t_p[(int64_t)row * a.k + j];
-        if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - z + lse);
-      }
-      if (lane == 0) a.target[(int64_t)row * a.k + j] = z;
+  if (threadIdx.x == 0) a.loss[0] = a.mean ? s / (float)*a.count : s;
+}
+
+// Cross entropy, one wave per live row: lse from the tiles' (max, sum) pairs, the label's score, the row's loss
+__global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
+  __shared__ float red[4];
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r < *a.count) {
+    const int mapped = a.row_map[r], row = mapped < 0 ? ~mapped : mapped;
+    float loss = __builtin_nanf(""), z = 0.f;
+    if (mapped >= 0) {
+      const int64_t v = a.labels[row];
+      z = wave_score(a.x + (int64_t)r * a.hidden, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
     }
+    const float lse = lse_of(wave_pairs(part + (int64_t)r * n_part, n_part, lane, 64));
+    if (mapped >= 0) loss = lse - z;
+    if (lane == 0) {
+      a.target[row] = z;
+      a.lse_out[row] = lse;
+      __hip_atomic_store(a.row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (a.done) finish_rows(a, gridDim.x, red);
+}
+
+// Distillation, one workgroup per live row, its waves sharing the teacher's entries
+__global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
+  __shared__ float red[4];
+  __shared__ float2 pair[4];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (r < *a.count) {
+    const int mapped = a.row_map[r], row = mapped < 0 ? ~mapped : mapped;
+    const float2 mine = wave_pairs(part + (int64_t)r * n_part, n_part, tid, 256);
+    if (lane == 0) pair[w] = mine;
     __syncthreads();
+    float2 all = pair[0];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float m = fmaxf(all.x, pair[i].x), ref = m == -INFINITY ? 0.f : m;
+      all = make_float2(m, all.y * __builtin_amdgcn_exp2f(all.x - ref) + pair[i].y * __builtin_amdgcn_exp2f(pair[i].x - ref));
+    }
+    const float lse = lse_of(all);
+    const bf16_t* x = a.x + (int64_t)r * a.hidden;
+    float loss = 0.f;
+    if (mapped >= 0)
+      for (int j = w; j < a.k; j += 4) {
+        const int64_t v = a.t_index[(int64_t)row * a.ld_ti + j];
+        float z = 0.f;
+        if (v >= 0 && v < a.vocab) {   // (beyond the vocabulary only where the value is -inf)
+          z = (wave_score(x, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
+          const float pj = a.t_p[(int64_t)row * a.k + j];
+          if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - z + lse);
+        }
+        if (lane == 0) a.target[(int64_t)row * a.k + j] = z;
+      }
     if (lane == 0) red[w] = loss;
     __syncthreads();
-    loss = ((red[0] + red[1]) + (red[2] + red[3])) * a.loss_factor;
-  } else if (w == 0) {
-    const int64_t v = a.labels[row];
-    const float z = wave_score(x, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
-    if (lane == 0) a.target[row] = z;
-    loss = lse - z;
+    if (tid == 0) {
+      loss = mapped < 0 ? __builtin_nanf("") : ((red[0] + red[1]) + (red[2] + red[3])) * a.loss_factor;
+      a.lse_out[row] = lse;
+      __hip_atomic_store(a.row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
   }
-  if (tid == 0) {
-    a.row_loss[row] = loss;
-    a.lse_out[row] = lse;
-  }
+  if (a.done) finish_rows(a, gridDim.x, red);
 }
 
 // loss[0] = sum of the rows' losses, over the live rows' count for the mean (0 / 0 = NaN as torch's mean over none);
@@ -602,12 +690,13 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPlan p, const float* __restrict__ part,
                                                            const float* __restrict__ colsum, int row_blocks) {
   const int count = *a.count;
-  if ((int)blockIdx.x < row_blocks) {
+  const int b_blocks = gridDim.x - row_blocks;
+  if ((int)blockIdx.x >= b_blocks) {
     const int64_t total = (int64_t)count * (a.hidden / 4);
     const int64_t slot = p.large ? (int64_t)((count + 255) & ~255) * a.hidden : p.dh_slot;
     const int n = a.schedule[0].splits;
     const float s = a.out_scale[0];
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
+    for (int64_t i = (int64_t)(blockIdx.x - b_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
       const int r = (int)(i / (a.hidden / 4)), c = (int)(i % (a.hidden / 4)) * 4;
       const float* q = part + (int64_t)r * a.hidden + c;
       f32x4_t v = {0.f, 0.f, 0.f, 0.f};
@@ -626,22 +715,42 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
       for (int e = 0; e < 4; ++e) o[e] = f32_to_op(v[e] * s);
     }
   } else {
-    const int64_t v = (int64_t)(blockIdx.x - row_blocks) * 256 + threadIdx.x;
+    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (v >= a.vocab) return;
-    const int n_sums = p.large ? (count + 255) / 256 * 2 : (count + 127) / 128 * 2;
+    const int n_sums = (count + p.tile_rows - 1) / p.tile_rows * 2;   // one per half tile of rows
     float s = 0.f;
-    for (int k = 0; k < n_sums; ++k) s += colsum[(int64_t)k * p.ld_colsum + v];
+    int k = 0;
+    for (; k + 8 <= n_sums; k += 8) {
+      float t[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) t[u] = colsum[(int64_t)(k + u) * p.ld_colsum + v];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) s += t[u];
+    }
+    for (; k < n_sums; ++k) s += colsum[(int64_t)k * p.ld_colsum + v];
     // (s is in units of G, the table in units of c)
     a.dbias[v] = a.fix ? (float)((double)s / G_SCALE - (double)a.fix[v] / FIX) * a.out_scale[1] : s * a.out_scale[0];
   }
 }
 
-constexpr int T_BM = 128, T_BN = 128;
-
-template <int EPI>
-hipError_t launch_tiles(const VocabGemm& g, int tiles_m, int splits, hipStream_t st) {
-  hipLaunchKernelGGL((vocab_gemm_kernel<EPI, T_BM, T_BN, 2, 2>), dim3(tiles_m * g.tiles_n, splits), dim3(256), 0, st, g);
+// up to 64 rows: 64-row tiles of scores, of dh and (its k) of dW, rings 3 K tiles ahead; up to LARGE_ROWS: 128-row tiles
+template <int EPI, int BM, int NST>
+hipError_t launch_tile(const VocabGemm& g, int tiles_m, int splits, hipStream_t st) {
+  constexpr int BN = 128, lds = NST * (BM + BN) * BK * 2;
+  auto kfn = vocab_gemm_kernel<EPI, BM, BN, 2, 2, NST>;
+  static DeviceOnce once;
+  int unused;
+  TRY(once.get([&](int, int*) {
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(kfn), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  }, &unused));
+  hipLaunchKernelGGL(kfn, dim3(tiles_m * g.tiles_n, splits), dim3(256), lds, st, g);
   return hipGetLastError();
+}
+template <int EPI>
+hipError_t launch_tiles(const VocabGemm& g, const VocabPlan& p, int64_t m, int splits, hipStream_t st) {
+  if (EPI == V_DW) return launch_tile<V_DW, 128, 2>(g, (int)((m + 127) / 128), splits, st);
+  return p.tile_rows == 64 ? launch_tile<EPI, 64, 4>(g, (int)((m + 63) / 64), splits, st)
+                           : launch_tile<EPI, 128, 3>(g, (int)((m + 127) / 128), splits, st);
 }
 
 }  // namespace
@@ -661,6 +770,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     return o;
   };
   p.large = n > LARGE_ROWS && hidden % 128 == 0;
+  p.tile_rows = p.large ? 256 : (n <= 64 ? 64 : 128);
   const int64_t rows = ((int64_t)n + 255) / 256 * 256, vp = (vocab + 255) / 256 * 256;
   p.head = take(sizeof(VocabHead));
   p.row_map = take(rows * 4);
@@ -691,10 +801,10 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     p.g = take(rows * p.piece * 2);
     p.ld_colsum = vp;
     p.colsum = take((rows / 64) * vp * 4);
-    // dh = G W has few tiles and a long k, which is split: until every CU has two workgroups, or (large) as the schedule on
-    // the device finds best, within this many fp32 partials of the rows
-    const int64_t tiles = (rows / 128) * ((hidden + 127) / 128);
-    int64_t s = tiles > 0 ? (512 + tiles - 1) / tiles : 1;
+    // dh = G W has few tiles and a long k, which is split: until every CU has a workgroup (whose ring takes most of its LDS), or
+    // (large) as the schedule on the device finds best, within this many fp32 partials of the rows
+    const int64_t tiles = ((int64_t)n + p.tile_rows - 1) / p.tile_rows * ((hidden + 127) / 128);
+    int64_t s = tiles > 0 ? 256 / tiles : 1;
     if (s > p.piece / 256) s = p.piece / 256;
     p.splits = (int32_t)(s < 1 ? 1 : s);
     p.dh_slot = rows * hidden;
@@ -723,6 +833,8 @@ hipError_t device_cus(int* out) {
 template <bool GRAD>
 hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, hipStream_t st) {
   VocabHead* head = reinterpret_cast<VocabHead*>(base + p.head);
+  a.head = head;
+  a.tile_rows = p.tile_rows;
   a.count = &head->count;
   a.grad_max = &head->grad_max;
   a.out_scale = head->out_scale;
@@ -765,12 +877,14 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
       TRY(launch_vocab8(V_STATS, g, st));
     } else {
       g.tiles_n = g.n_part / 2;
-      TRY(launch_tiles<V_STATS>(g, (a.n + T_BM - 1) / T_BM, 1, st));
+      TRY(launch_tiles<V_STATS>(g, p, a.n, 1, st));
     }
-    hipLaunchKernelGGL(vocab_loss_kernel, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
+    if (a.loss && a.n <= 1024) a.done = &reinterpret_cast<VocabHead*>(base + p.head)->done;
+    if (a.t_index) hipLaunchKernelGGL(vocab_distill_kernel, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
+    else hipLaunchKernelGGL(vocab_ce_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, part, g.n_part);
     TRY(hipGetLastError());
   }
-  if (a.loss) {
+  if (a.loss && !a.done) {
     hipLaunchKernelGGL(vocab_reduce_kernel, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());
   }
@@ -787,7 +901,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   }
   a.with_dw = dw != nullptr;
   a.max_splits = p.splits;
-  a.tiles_h = (int)((a.hidden + (p.large ? 255 : T_BN - 1)) / (p.large ? 256 : T_BN));
+  a.tiles_h = p.large ? (a.hidden + 255) / 256 : (a.hidden + 127) / 128;
   if (p.large) {
     TRY(device_cus(&a.wgs));
     a.wgs &= ~7;
@@ -809,7 +923,6 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.out_scale = a.out_scale;
   g.with_dw = dw != nullptr;
   g.with_dh = a.dh && a.n > 0;
-  const int tiles_r = (a.n + T_BM - 1) / T_BM;
   for (int64_t v0 = 0, piece = 0; v0 < a.vocab; v0 += p.piece, ++piece) {
     const int64_t v1 = v0 + p.piece < a.vocab ? v0 + p.piece : a.vocab;
     g.v0 = v0;
@@ -817,8 +930,8 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     g.schedule = a.schedule + (piece == p.pieces - 1 && piece > 0);
     g.accumulate = piece > 0;
     if (a.n > 0) {
-      g.tiles_n = g.ldg / (p.large ? 256 : T_BN);
-      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_tiles<V_GRAD>(g, tiles_r, 1, st));
+      g.tiles_n = g.ldg / (p.large ? 256 : 128);
+      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_tiles<V_GRAD>(g, p, a.n, 1, st));
       if (a.t_index) {
         hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
                            (a.fix && piece == 0) ? 1 : 0);
@@ -829,8 +942,8 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     if (p.large) {
       TRY(launch_vocab8(V_PROD, g, st));
     } else {
-      if (g.with_dh) TRY(launch_tiles<V_DH>(g, tiles_r, p.splits, st));
-      if (g.with_dw) TRY(launch_tiles<V_DW>(g, (g.ldg + T_BM - 1) / T_BM, 1, st));
+      if (g.with_dh) TRY(launch_tiles<V_DH>(g, p, a.n, p.splits, st));
+      if (g.with_dw) TRY(launch_tiles<V_DW>(g, p, g.ldg, 1, st));
     }
   }
   const int row_blocks = g.with_dh ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
