@@ -135,7 +135,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   VocabSchedule* schedule;  // of every piece but the last, and of the last
   int32_t tiles_h, piece_tiles[2], max_splits, wgs;   // what they are chosen from (wgs 0: max_splits itself)
   int64_t dh_room;
-  bool with_dw;
+  bool with_dw, dh_aligned;
   float *t_p, *t_logp, *out_scale;
   bf16_t* x;
   float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
@@ -153,9 +153,9 @@ struct VocabGemm {          // arguments of vocab_gemm_kernel
   bf16_t* g;
   const float4* row_info;
   float* colsum; int64_t ld_colsum;
-  float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: a slot is the live rows, padded, x hidden)
+  float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: whole tiles, dh_partial_at)
   const VocabSchedule* schedule; bool accumulate, with_dw, with_dh;
-  bf16_t* out16; int64_t ldo;
+  bf16_t* out16; int64_t ldo; bool wide;   // wide: rows start on 16 bytes
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary

@@ -56,6 +56,23 @@ __device__ __forceinline__ int tr_swz(int k) {
   return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) : (((k >> 1) & 1) | ((k >> 3) & 1) << 1);
 }
 
+// 16 bytes of dW, written once and not read again here; rows of a caller's own stride may start on 8 bytes only
+__device__ __forceinline__ void store_dw(bf16_t* o, const u32x4_t& v, bool wide) {
+  if (wide) {
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(o));
+  } else {
+    __builtin_nontemporal_store((u32x2_t){v[0], v[1]}, reinterpret_cast<u32x2_t*>(o));
+    __builtin_nontemporal_store((u32x2_t){v[2], v[3]}, reinterpret_cast<u32x2_t*>(o) + 1);
+  }
+}
+
+// Row and column within its 256 x 256 tile of the q-th group of 4 partials that vocab8_kernel stores of a dh tile
+__device__ __forceinline__ void dh_partial_at(int q, int& row, int& col) {
+  const int lane = q & 63, i = q >> 6 & 1, nh = q >> 7 & 1, m = q >> 8 & 3, mh = q >> 10 & 1, w = q >> 11;
+  row = mh * 128 + (w >> 2) * 64 + m * 16 + (lane & 15);
+  col = (w & 3) * 64 + nh * 32 + i * 16 + (lane >> 4) * 4;
+}
+
 // What the product kernels compute; A [M, K] and B [N, K], "R-major" = stored [K, R]
 //   V_STATS  rows x vocabulary: every row's (max, sum of exp2) over 64 columns at a time       A = live rows, B = W
 //   V_GRAD   the same product once more -> G and the column sums of G before rounding

@@ -249,11 +249,7 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
         put(n, make_uint2(pack_op2(acc[m][n][0] * s, acc[m][n][1] * s), pack_op2(acc[m][n][2] * s, acc[m][n][3] * s)));
       flush([&](int row, int c, const u32x4_t& v) {
         const int at = row0 - fr + m * 16 + row, h = tn * BN + wn * 64 + c;
-        if (at < a.ldg && a.v0 + at < a.vocab && h < a.hidden) {   // (8-byte stores: the row stride is a multiple of 4)
-          u32x2_t* o = reinterpret_cast<u32x2_t*>(a.out16 + (a.v0 + at) * a.ldo + h);
-          __builtin_nontemporal_store((u32x2_t){v[0], v[1]}, o);
-          __builtin_nontemporal_store((u32x2_t){v[2], v[3]}, o + 1);
-        }
+        if (at < a.ldg && a.v0 + at < a.vocab && h < a.hidden) store_dw(a.out16 + (a.v0 + at) * a.ldo + h, v, a.wide);
       });
     }
   }
@@ -317,12 +313,12 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
 __device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
   const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
   if (tiles > 0) {   // partials that there is room for
-    const int64_t room = a.dh_room / ((int64_t)rows_t * 256 * a.hidden);
+    const int64_t room = a.dh_room / ((int64_t)tiles * 65536);
     if (room < max_splits) max_splits = (int)room;
   }
   const int n_dw = a.with_dw ? vocab_tiles * a.tiles_h : 0, full = n_dw / wgs, rest = n_dw - full * wgs;
   const int len_dw = (total + 127) / 128 + 2, splits = lane + 1;
-  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 5;
+  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 4;
   int best = 0x7fffffff, best_more = 0, best_less = 0;
   if (splits <= max_splits && splits <= vocab_tiles)
     for (int less = 0; less < 4; ++less) {   // dh tiles of a workgroup with one dW tile more
@@ -361,7 +357,7 @@ __device__ void write_head(const VocabRows& a, int total, float grad_max, int la
   VocabSchedule s0 = {a.max_splits, 0, 0, 0}, s1 = s0;
   if (GRAD && a.wgs) {
     s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
-    s1 = choose_schedule(a, total, a.piece_tiles[1], s0.splits, lane);
+    s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.splits, lane);
   }
   if (lane != 0) return;
   *a.count = total;
@@ -388,12 +384,19 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   for (int r0 = 0; r0 < a.n; r0 += 16384) {
     const int r = r0 + tid * 16;
     int live = 0;
+    int s[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if (r + i < a.n) {
-        const int s = row_state(a, r + i) != 0;
-        live += s;
-        if (GRAD && a.grad_rows && s) gm = fmaxf(gm, finite_abs(a.grad[r + i]));
+    for (int i = 0; i < 16; ++i) {   // (no branches: all loads in flight)
+      const int q = min(r + i, a.n - 1);
+      s[i] = a.state ? a.state[q] != 0 : a.labels[q] != a.ignore;
+    }
+#pragma unroll
+    for (int i = 0; i < 16; ++i) live += r + i < a.n ? s[i] : 0;
+    if (GRAD && a.grad_rows)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float g = finite_abs(a.grad[min(r + i, a.n - 1)]);
+        if (s[i]) gm = fmaxf(gm, g);
       }
     int up = live;
 #pragma unroll
@@ -526,16 +529,18 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
 }
 
-// score (times 1/T) of one vocabulary entry for the hidden row x: a wave's dot product, fp32
+// eight products of 16-bit operands in fp32, added to s
+__device__ __forceinline__ float dot8(const uint4& x, const uint4& w, float s) {
+  const uint32_t* xp = reinterpret_cast<const uint32_t*>(&x);
+  const uint32_t* wp = reinterpret_cast<const uint32_t*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s = fmaf(op2_lo(xp[i]), op2_lo(wp[i]), fmaf(op2_hi(xp[i]), op2_hi(wp[i]), s));
+  return s;
+}
+// score of one vocabulary entry for the hidden row x: a wave's dot product, fp32
 __device__ __forceinline__ float wave_score(const bf16_t* x, const bf16_t* wrow, int H, int lane) {
   float s = 0.f;
-  for (int c = lane * 8; c < H; c += 512) {
-    const uint4 xv = *reinterpret_cast<const uint4*>(x + c), wv = *reinterpret_cast<const uint4*>(wrow + c);
-    const uint32_t* xp = reinterpret_cast<const uint32_t*>(&xv);
-    const uint32_t* wp = reinterpret_cast<const uint32_t*>(&wv);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s = fmaf(op2_lo(xp[i]), op2_lo(wp[i]), fmaf(op2_hi(xp[i]), op2_hi(wp[i]), s));
-  }
+  for (int c = lane * 8; c < H; c += 512) s = dot8(*reinterpret_cast<const uint4*>(x + c), *reinterpret_cast<const uint4*>(wrow + c), s);
   return wave_sum(s);
 }
 
@@ -618,16 +623,50 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
     const bf16_t* x = a.x + (int64_t)r * a.hidden;
     float loss = 0.f;
     if (mapped >= 0)
-      for (int j = w; j < a.k; j += 4) {
-        const int64_t v = a.t_index[(int64_t)row * a.ld_ti + j];
-        float z = 0.f;
-        if (v >= 0 && v < a.vocab) {   // (beyond the vocabulary only where the value is -inf)
-          z = (wave_score(x, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
-          const float pj = a.t_p[(int64_t)row * a.k + j];
-          if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - z + lse);
+      for (int j0 = w * 8; j0 < a.k; j0 += 32) {   // eight entries' rows of W in flight
+        const bf16_t* wr[8];
+        float z[8];
+        const int64_t mine_v = lane < 8 && j0 + lane < a.k ? a.t_index[(int64_t)row * a.ld_ti + j0 + lane] : -1;
+        const int mine_at = mine_v >= 0 && mine_v < a.vocab ? (int)mine_v : -1;   // (beyond only where the value is -inf)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int v = __builtin_amdgcn_readlane(mine_at, u);
+          wr[u] = a.w + (int64_t)max(v, 0) * a.ldw;
+          z[u] = 0.f;
         }
-        if (lane == 0) a.target[(int64_t)row * a.k + j] = z;
+        for (int c = lane * 8; c < a.hidden; c += 512) {
+          uint4 wv[8];
+          const uint4 xv = *reinterpret_cast<const uint4*>(x + c);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) wv[u] = *reinterpret_cast<const uint4*>(wr[u] + c);
+#pragma unroll
+          for (int u = 0; u < 8; ++u) z[u] = dot8(xv, wv[u], z[u]);
+        }
+        // eight sums over 64 lanes: halve the values with the lanes, then lane l holds that of entry (l >> 3)
+#pragma unroll
+        for (int h = 4; h > 0; h >>= 1) {
+          const bool up = lane & (h * 8);
+#pragma unroll
+          for (int u = 0; u < h; ++u) {
+            const float send = up ? z[u] : z[u + h], keep = up ? z[u + h] : z[u];
+            z[u] = keep + __shfl_xor(send, h * 8, 64);
+          }
+        }
+        float sum = z[0];
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+        const int u = lane >> 3, j = j0 + u, v = __shfl(mine_at, u, 64);
+        if ((lane & 7) == 0 && j < a.k) {
+          float zj = 0.f;
+          if (v >= 0) {
+            zj = (sum + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
+            const float pj = a.t_p[(int64_t)row * a.k + j];
+            if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - zj + lse);
+          }
+          a.target[(int64_t)row * a.k + j] = zj;
+        }
       }
+    loss = wave_sum(loss);
     if (lane == 0) red[w] = loss;
     __syncthreads();
     if (tid == 0) {
@@ -671,13 +710,29 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
   const float2 lc = a.row_lc[r];
   const int64_t* index = a.t_index + (int64_t)row * a.ld_ti;
   const float* tp = a.t_p + (int64_t)row * a.k;
-  for (int j = lane; j < a.k; j += 64) {
-    const int64_t v = index[j];
-    const float own = tp[j];
-    if (v < 0 || v >= a.vocab) continue;   // (not listed; beyond the vocabulary only where the value is -inf)
-    float p = 0.f;
-    for (int i = 0; i < a.k; ++i)
-      if (index[i] == v) p += tp[i];
+  // (not listed, or beyond the vocabulary, which only an entry of value -inf may be: -1)
+  auto entry = [&](int j, int& v, float& p) {
+    const int64_t t = j < a.k ? index[j] : -1;
+    v = t >= 0 && t < a.vocab ? (int)t : -1;
+    p = j < a.k ? tp[j] : 0.f;
+  };
+  for (int j0 = 0; j0 < a.k; j0 += 64) {
+    const int j = j0 + lane;
+    int v;
+    float own, p = 0.f;
+    entry(j, v, own);
+    for (int i0 = 0; i0 < a.k; i0 += 64) {   // every entry that names v
+      int u = v;
+      float q = own;
+      if (i0 != j0) entry(i0 + lane, u, q);
+      const int n = min(64, a.k - i0);
+      for (int i = 0; i < n; ++i) {
+        const int ui = __builtin_amdgcn_readlane(u, i);
+        const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
+        p += ui == v ? qi : 0.f;
+      }
+    }
+    if (v < 0) continue;
     if (table && fabsf(lc.y * own) <= 1.f)
       atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
     if (v < v0 || v >= v1) continue;
@@ -692,13 +747,24 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
   const int count = *a.count;
   const int b_blocks = gridDim.x - row_blocks;
   if ((int)blockIdx.x >= b_blocks) {
-    const int64_t total = (int64_t)count * (a.hidden / 4);
-    const int64_t slot = p.large ? (int64_t)((count + 255) & ~255) * a.hidden : p.dh_slot;
     const int n = a.schedule[0].splits;
     const float s = a.out_scale[0];
+    const int tiles_r = (count + 255) >> 8, h4 = a.hidden / 4;
+    const int64_t total = p.large ? (int64_t)tiles_r * a.tiles_h * 16384 : (int64_t)count * h4;
+    const int64_t slot = p.large ? total * 4 : p.dh_slot;
     for (int64_t i = (int64_t)(blockIdx.x - b_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
-      const int r = (int)(i / (a.hidden / 4)), c = (int)(i % (a.hidden / 4)) * 4;
-      const float* q = part + (int64_t)r * a.hidden + c;
+      int r, c;
+      if (p.large) {
+        const int tile = (int)(i >> 14);
+        dh_partial_at((int)(i & 16383), r, c);
+        r += tile / a.tiles_h * 256;
+        c += tile % a.tiles_h * 256;
+        if (r >= count || c >= a.hidden) continue;
+      } else {
+        r = (int)(i / h4);
+        c = (int)(i - (int64_t)r * h4) * 4;
+      }
+      const float* q = part + i * 4;
       f32x4_t v = {0.f, 0.f, 0.f, 0.f};
       int k = 0;
       for (; k + 4 <= n; k += 4) {   // four slots' loads in flight, added in order
@@ -711,8 +777,13 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
       for (; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
       const int m = a.row_map[r];
       bf16_t* o = a.dh + (int64_t)(m < 0 ? ~m : m) * a.ld_dh + c;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = f32_to_op(v[e] * s);
+      const uint2 packed = make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
+      if (a.dh_aligned) {
+        *reinterpret_cast<uint2*>(o) = packed;
+      } else {
+        o[0] = (bf16_t)packed.x; o[1] = (bf16_t)(packed.x >> 16);
+        o[2] = (bf16_t)packed.y; o[3] = (bf16_t)(packed.y >> 16);
+      }
     }
   } else {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -812,7 +883,6 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     if (p.large) {
       const int64_t tiles8 = (rows / 256) * ((hidden + 255) / 256);
       room = (tiles8 > 256 ? 2 * tiles8 : 512) * 65536;
-      if (room < 2 * p.dh_slot) room = 2 * p.dh_slot;
     }
     p.dh_part = take((size_t)room * 4);
     p.dh_room = room;
@@ -900,6 +970,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
   }
   a.with_dw = dw != nullptr;
+  a.dh_aligned = ((uintptr_t)a.dh & 7) == 0 && a.ld_dh % 4 == 0;
   a.max_splits = p.splits;
   a.tiles_h = p.large ? (a.hidden + 255) / 256 : (a.hidden + 127) / 128;
   if (p.large) {
@@ -920,6 +991,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.out32 = reinterpret_cast<float*>(base + p.dh_part);
   g.slot_stride = p.dh_slot;
   g.out16 = dw; g.ldo = ld_dw;
+  g.wide = ((uintptr_t)dw & 15) == 0 && ld_dw % 8 == 0;
   g.out_scale = a.out_scale;
   g.with_dw = dw != nullptr;
   g.with_dh = a.dh && a.n > 0;

@@ -12,15 +12,6 @@
 
 namespace {
 
-#ifndef V8_NT
-#define V8_NT 1
-#endif
-template <typename V>
-__device__ __forceinline__ void G_STORE(V v, V* p) {
-  if (V8_NT) __builtin_nontemporal_store(v, p);
-  else *p = v;
-}
-
 constexpr int BM = 256, BN = 256;
 constexpr int HT = 16384;              // half-tile
 constexpr int RING = 8 * HT;           // 2 K tiles
@@ -350,7 +341,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
           for (int p = 0; p < 2; ++p) {
             const int row = p * 8 + (le >> 3), c16 = le & 7;
             const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
-            G_STORE(v, reinterpret_cast<u32x4_t*>(a.g + (int64_t)(tm * BM + mh * 128 + wr * 64 + m * 16 + row) * a.ldg + tn * BN +
+            __builtin_nontemporal_store(v, reinterpret_cast<u32x4_t*>(a.g + (int64_t)(tm * BM + mh * 128 + wr * 64 + m * 16 + row) * a.ldg + tn * BN +
                                                   wc * 64 + c16 * 8));
           }
         }
@@ -367,8 +358,9 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
           }
       }
     } else if (cur.dh) {
-      const int rows_pad = (count + 255) & ~255;
-      float* out = a.out32 + (int64_t)cur.split * rows_pad * a.hidden;
+      // fp32 partials in the accumulators' order (dh_partial_at): every store of a wave is 1 KiB contiguous
+      const int tiles_r = (count + 255) >> 8;
+      float* out = a.out32 + ((int64_t)(cur.split * tiles_r + tm) * a.tiles_n + tn) * 65536 + w * 8192 + le * 4;
 #pragma unroll
       for (int mh = 0; mh < 2; ++mh)
 #pragma unroll
@@ -376,11 +368,10 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
 #pragma unroll
           for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              if (col0 + nh * 32 + i * 16 < a.hidden) {
-                f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (int64_t)(row0 + mh * 128 + m * 16) * a.hidden + col0 + nh * 32 + i * 16);
-                *o = a.accumulate ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
-              }
+            for (int i = 0; i < 2; ++i) {
+              f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (((mh * 4 + m) * 2 + nh) * 2 + i) * 256);
+              *o = a.accumulate ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
+            }
     } else {
       const float s = a.out_scale[0];
 #pragma unroll
@@ -401,11 +392,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
             const u32x4_t v = *reinterpret_cast<const u32x4_t*>(scr + row * 128 + ((c16 ^ (row & 7)) * 16));
             const int64_t vocab_row = a.v0 + tm * BM + mh * 128 + wr * 64 + m * 16 + row;
             const int c = tn * BN + wc * 64 + c16 * 8;
-            if (vocab_row < a.vocab && c < a.hidden) {   // (8-byte stores: the row stride is a multiple of 4)
-              uint2* o = reinterpret_cast<uint2*>(a.out16 + vocab_row * a.ldo + c);
-              o[0] = make_uint2(v[0], v[1]);
-              o[1] = make_uint2(v[2], v[3]);
-            }
+            if (vocab_row < a.vocab && c < a.hidden) store_dw(a.out16 + vocab_row * a.ldo + c, v, a.wide);
           }
         }
     }
