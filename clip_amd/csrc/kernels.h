@@ -101,9 +101,10 @@ hipError_t launch_topk_rows(const void* logits, int type, int64_t ld, int n, int
                             hipStream_t st);
 
 // ---- losses of the vocabulary decoder (vocab.hip)
-// How the products dh = G W and dW = G^T h of one piece share the persistent workgroups (vocab8.hip): dh's long k is cut
-// into `splits`; a workgroup that has one dW tile less than others takes dh_more of the split tiles, the others dh_less
-struct VocabSchedule { int32_t splits, dh_less, dh_more, unused; };
+// How the products dh = G W and dW = G^T h of one piece share the persistent workgroups (vocab8.hip): the k of dh's tiles
+// (the vocabulary) is cut into `splits`, that of dW's (the rows) into dw_splits; a workgroup that has one dW tile less than
+// others takes dh_more of dh's split tiles, the others dh_less
+struct VocabSchedule { int32_t splits, dh_less, dh_more, dw_splits; };
 struct VocabHead {          // the words at the head of the workspace
   int32_t count, done;      // live rows; workgroups of the forward's last kernel that have finished
   float grad_max;
@@ -134,7 +135,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   float* grad_max;          // the largest finite |gradient| of a live row
   VocabSchedule* schedule;  // of every piece but the last, and of the last
   int32_t tiles_h, piece_tiles[2], max_splits, wgs;   // what they are chosen from (wgs 0: max_splits itself)
-  int64_t dh_room;
+  int64_t dh_room, dw_room;   // floats of partials
   bool with_dw, dh_aligned;
   float *t_p, *t_logp, *out_scale;
   bf16_t* x;
@@ -154,13 +155,14 @@ struct VocabGemm {          // arguments of vocab_gemm_kernel
   const float4* row_info;
   float* colsum; int64_t ld_colsum;
   float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: whole tiles, dh_partial_at)
+  float* dw32;              // dW's partials where its k is split
   const VocabSchedule* schedule; bool accumulate, with_dw, with_dh;
   bf16_t* out16; int64_t ldo; bool wide;   // wide: rows start on 16 bytes
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
-  size_t head, row_map, block_base, state, t_p, t_logp, x, part, row_info, row_lc, fix, g, colsum, dh_part, bytes;
-  int64_t piece, pieces, ld_colsum, dh_slot, dh_room;   // floats of one split's partials, and of all
+  size_t head, row_map, block_base, state, t_p, t_logp, x, part, row_info, row_lc, fix, g, colsum, dh_part, dw_part, bytes;
+  int64_t piece, pieces, ld_colsum, dh_slot, dh_room, dw_room;   // floats of one split's partials of dh, of all, and of dW's
   int32_t splits;         // at most
   bool large;             // 256 x 256 tiles (vocab8.hip)
   int32_t tile_rows;      // rows of a tile of scores

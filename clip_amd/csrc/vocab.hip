@@ -308,24 +308,28 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
 
 // ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
 // tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
-// leave the CU; dh: 256 KB of fp32 partials leave it and are read again by the last kernel).  Lane s tries s + 1 splits, and for
-// each a few shares of the workgroups that are behind by one dW tile.
+// leave the CU; partials: 256 KB leave it and are read again by the last kernel).  Lane s tries s + 1 splits of dh's tiles, and
+// for each some of dW's (where the vocabulary is so short that its tiles do not fill the workgroups: dw_room) and a few shares
+// of the workgroups that are behind by one dW tile.
 __device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
   const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
   if (tiles > 0) {   // partials that there is room for
     const int64_t room = a.dh_room / ((int64_t)tiles * 65536);
     if (room < max_splits) max_splits = (int)room;
   }
-  const int n_dw = a.with_dw ? vocab_tiles * a.tiles_h : 0, full = n_dw / wgs, rest = n_dw - full * wgs;
-  const int len_dw = (total + 127) / 128 + 2, splits = lane + 1;
+  const int dw_tiles = a.with_dw ? vocab_tiles * a.tiles_h : 0, pairs = (total + 127) / 128, splits = lane + 1;
   const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 4;
-  int best = 0x7fffffff, best_more = 0, best_less = 0;
+  int best = 0x7fffffff, best_more = 0, best_less = 0, best_dw = 1;
   if (splits <= max_splits && splits <= vocab_tiles)
-    for (int less = 0; less < 4; ++less) {   // dh tiles of a workgroup with one dW tile more
-      const int left = n_dh - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
-      const int t0 = rest ? (full + 1) * len_dw + less * len_dh : 0, t1 = full * len_dw + more * len_dh;
-      const int cost = max(t0, t1);
-      if (cost < best) { best = cost; best_less = less; best_more = more; }
+    for (int d = 1; d <= 16; d += d < 4 ? 1 : d / 2) {   // 1 2 3 4 6 9 13
+      if (d > 1 && (d > pairs || (int64_t)dw_tiles * d * 65536 > a.dw_room)) break;
+      const int n_dw = dw_tiles * d, full = n_dw / wgs, rest = n_dw - full * wgs, len_dw = (pairs + d - 1) / d + (d > 1 ? 5 : 2);
+      for (int less = 0; less < 4; ++less) {   // dh tiles of a workgroup with one dW tile more
+        const int left = n_dh - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
+        const int t0 = rest ? (full + 1) * len_dw + less * len_dh : 0, t1 = full * len_dw + more * len_dh;
+        const int cost = max(t0, t1);
+        if (cost < best) { best = cost; best_less = less; best_more = more; best_dw = d; }
+      }
     }
   const int low = best;
 #pragma unroll
@@ -335,7 +339,7 @@ __device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int voca
   r.splits = win + 1;
   r.dh_less = __shfl(best_less, win, 64);
   r.dh_more = __shfl(best_more, win, 64);
-  r.unused = 0;
+  r.dw_splits = __shfl(best_dw, win, 64);
   return r;
 }
 
@@ -354,7 +358,7 @@ __device__ __forceinline__ float finite_abs(float g) {
 template <bool GRAD>
 __device__ void write_head(const VocabRows& a, int total, float grad_max, int lane) {
   // (every piece sums into the first's partials: the last must not have more of them)
-  VocabSchedule s0 = {a.max_splits, 0, 0, 0}, s1 = s0;
+  VocabSchedule s0 = {a.max_splits, 0, 0, 1}, s1 = s0;
   if (GRAD && a.wgs) {
     s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
     s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.splits, lane);
@@ -526,7 +530,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     if (GRAD && lane == 0) a.row_info[q] = make_float4(INFINITY, 1.f, __int_as_float(-1), 0.f);   // G = 0
   }
   if (GRAD && a.fix)
-    for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
+    for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab * FIX_COPIES; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
 }
 
 // eight products of 16-bit operands in fp32, added to s
@@ -603,27 +607,31 @@ __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2
   if (a.done) finish_rows(a, gridDim.x, red);
 }
 
-// Distillation, one workgroup per live row, its waves sharing the teacher's entries
+// Distillation, WPR waves per live row sharing the teacher's entries: one for short lists, four for long ones
+template <int WPR>
 __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
   __shared__ float red[4];
   __shared__ float2 pair[4];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  if (r < *a.count) {
+  const int tid = threadIdx.x, lane = tid & 63, w = WPR == 4 ? tid >> 6 : 0;
+  const int r = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + (tid >> 6);
+  if (r < *a.count) {   // (WPR 4: the same for the whole workgroup)
     const int mapped = a.row_map[r], row = mapped < 0 ? ~mapped : mapped;
-    const float2 mine = wave_pairs(part + (int64_t)r * n_part, n_part, tid, 256);
-    if (lane == 0) pair[w] = mine;
-    __syncthreads();
-    float2 all = pair[0];
+    float2 all = wave_pairs(part + (int64_t)r * n_part, n_part, WPR == 4 ? tid : lane, 64 * WPR);
+    if (WPR == 4) {
+      if (lane == 0) pair[w] = all;
+      __syncthreads();
+      all = pair[0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      const float m = fmaxf(all.x, pair[i].x), ref = m == -INFINITY ? 0.f : m;
-      all = make_float2(m, all.y * __builtin_amdgcn_exp2f(all.x - ref) + pair[i].y * __builtin_amdgcn_exp2f(pair[i].x - ref));
+      for (int i = 1; i < 4; ++i) {
+        const float m = fmaxf(all.x, pair[i].x), ref = m == -INFINITY ? 0.f : m;
+        all = make_float2(m, all.y * __builtin_amdgcn_exp2f(all.x - ref) + pair[i].y * __builtin_amdgcn_exp2f(pair[i].x - ref));
+      }
     }
     const float lse = lse_of(all);
     const bf16_t* x = a.x + (int64_t)r * a.hidden;
     float loss = 0.f;
     if (mapped >= 0)
-      for (int j0 = w * 8; j0 < a.k; j0 += 32) {   // eight entries' rows of W in flight
+      for (int j0 = w * 8; j0 < a.k; j0 += 8 * WPR) {   // eight entries' rows of W in flight
         const bf16_t* wr[8];
         float z[8];
         const int64_t mine_v = lane < 8 && j0 + lane < a.k ? a.t_index[(int64_t)row * a.ld_ti + j0 + lane] : -1;
@@ -667,10 +675,13 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
         }
       }
     loss = wave_sum(loss);
-    if (lane == 0) red[w] = loss;
-    __syncthreads();
-    if (tid == 0) {
-      loss = mapped < 0 ? __builtin_nanf("") : ((red[0] + red[1]) + (red[2] + red[3])) * a.loss_factor;
+    if (WPR == 4) {
+      if (lane == 0) red[w] = loss;
+      __syncthreads();
+      loss = (red[0] + red[1]) + (red[2] + red[3]);
+    }
+    if (w == 0 && lane == 0) {
+      loss = mapped < 0 ? __builtin_nanf("") : loss * a.loss_factor;
       a.lse_out[row] = lse;
       __hip_atomic_store(a.row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
@@ -700,7 +711,8 @@ __global__ __launch_bounds__(1024) void vocab_reduce_kernel(VocabRows a) {
 // The teacher's part of G, one wave per live row: G[r, v] = c (q_v - sum of p over the entries that name v), from the
 // forward's fp32 score of v (a difference of the rounded q would lose what is left where q is near p).  (A label's part is
 // set by V_GRAD itself.)  The sums of c p per vocabulary entry, which db needs, go to a table of 64-bit fixed point: integer
-// adds commute, so their order does not show (2^-38 a unit; |c| p <= 1, n <= 2^24 rows).
+// adds commute, so their order does not show (2^-38 a unit; |c| p <= 1, n <= 2^24 rows); in FIX_COPIES copies by row, since a
+// teacher's frequent entries are the same in most rows.
 __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf16_t* __restrict__ g, int64_t ldg, int64_t v0, int64_t v1,
                                                                  int table) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
@@ -734,7 +746,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
     }
     if (v < 0) continue;
     if (table && fabsf(lc.y * own) <= 1.f)
-      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
+      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
     if (v < v0 || v >= v1) continue;
     const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
     g[(int64_t)r * ldg + (v - v0)] = f32_to_op(lc.y * (q - p) * G_SCALE);
@@ -743,16 +755,31 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
 
 // dh of the live rows from the fp32 partials (fixed order), and db from the column sums and the targets' table
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPlan p, const float* __restrict__ part,
-                                                           const float* __restrict__ colsum, int row_blocks) {
+                                                           const float* __restrict__ colsum, const float* __restrict__ dw_part,
+                                                           bf16_t* __restrict__ dw, int64_t ld_dw, int row_blocks, int dw_blocks) {
   const int count = *a.count;
-  const int b_blocks = gridDim.x - row_blocks;
-  if ((int)blockIdx.x >= b_blocks) {
+  const int b_blocks = gridDim.x - row_blocks - dw_blocks;
+  // the sum of n slots' partials, four of them in flight, in order; times the common factor, rounded
+  const float s = a.out_scale[0];
+  auto sum_slots = [&](const float* q, int n, int64_t slot) -> uint2 {
+    f32x4_t v = {0.f, 0.f, 0.f, 0.f};
+    int k = 0;
+    for (; k + 4 <= n; k += 4) {
+      f32x4_t t[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const f32x4_t*>(q + (k + u) * slot);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v += t[u];
+    }
+    for (; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
+    return make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
+  };
+  if ((int)blockIdx.x >= b_blocks + dw_blocks) {
     const int n = a.schedule[0].splits;
-    const float s = a.out_scale[0];
     const int tiles_r = (count + 255) >> 8, h4 = a.hidden / 4;
     const int64_t total = p.large ? (int64_t)tiles_r * a.tiles_h * 16384 : (int64_t)count * h4;
     const int64_t slot = p.large ? total * 4 : p.dh_slot;
-    for (int64_t i = (int64_t)(blockIdx.x - b_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
+    for (int64_t i = (int64_t)(blockIdx.x - b_blocks - dw_blocks) * 256 + threadIdx.x; i < total; i += (int64_t)row_blocks * 256) {
       int r, c;
       if (p.large) {
         const int tile = (int)(i >> 14);
@@ -764,20 +791,9 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
         r = (int)(i / h4);
         c = (int)(i - (int64_t)r * h4) * 4;
       }
-      const float* q = part + i * 4;
-      f32x4_t v = {0.f, 0.f, 0.f, 0.f};
-      int k = 0;
-      for (; k + 4 <= n; k += 4) {   // four slots' loads in flight, added in order
-        f32x4_t t[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) t[u] = *reinterpret_cast<const f32x4_t*>(q + (k + u) * slot);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) v += t[u];
-      }
-      for (; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
+      const uint2 packed = sum_slots(part + i * 4, n, slot);
       const int m = a.row_map[r];
       bf16_t* o = a.dh + (int64_t)(m < 0 ? ~m : m) * a.ld_dh + c;
-      const uint2 packed = make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
       if (a.dh_aligned) {
         *reinterpret_cast<uint2*>(o) = packed;
       } else {
@@ -785,26 +801,43 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
         o[2] = (bf16_t)packed.y; o[3] = (bf16_t)(packed.y >> 16);
       }
     }
+  } else if ((int)blockIdx.x >= b_blocks) {
+    const int n = a.schedule[0].dw_splits, tiles = a.piece_tiles[0] * a.tiles_h;
+    if (n == 1) return;   // written whole
+    for (int64_t i = (int64_t)(blockIdx.x - b_blocks) * 256 + threadIdx.x; i < (int64_t)tiles * 16384; i += (int64_t)dw_blocks * 256) {
+      const int tile = (int)(i >> 14);
+      int r, c;
+      dh_partial_at((int)(i & 16383), r, c);
+      const int64_t v = (int64_t)(tile / a.tiles_h) * 256 + r;
+      c += tile % a.tiles_h * 256;
+      if (v < a.vocab && c < a.hidden) *reinterpret_cast<uint2*>(dw + v * ld_dw + c) = sum_slots(dw_part + i * 4, n, (int64_t)tiles * 65536);
+    }
   } else {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (v >= a.vocab) return;
     const int n_sums = (count + p.tile_rows - 1) / p.tile_rows * 2;   // one per half tile of rows
-    float s = 0.f;
+    float sum = 0.f;
     int k = 0;
     for (; k + 8 <= n_sums; k += 8) {
       float t[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) t[u] = colsum[(int64_t)(k + u) * p.ld_colsum + v];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) s += t[u];
+      for (int u = 0; u < 8; ++u) sum += t[u];
     }
-    for (; k < n_sums; ++k) s += colsum[(int64_t)k * p.ld_colsum + v];
-    // (s is in units of G, the table in units of c)
-    a.dbias[v] = a.fix ? (float)((double)s / G_SCALE - (double)a.fix[v] / FIX) * a.out_scale[1] : s * a.out_scale[0];
+    for (; k < n_sums; ++k) sum += colsum[(int64_t)k * p.ld_colsum + v];
+    if (a.fix) {   // (the sum is in units of G, the table in units of c)
+      int64_t t = 0;
+#pragma unroll
+      for (int u = 0; u < FIX_COPIES; ++u) t += a.fix[u * a.vocab + v];
+      a.dbias[v] = (float)((double)sum / G_SCALE - (double)t / FIX) * a.out_scale[1];
+    } else {
+      a.dbias[v] = sum * s;
+    }
   }
 }
 
-// up to 64 rows: 64-row tiles of scores, of dh and (its k) of dW, rings 3 K tiles ahead; up to LARGE_ROWS: 128-row tiles
+// up to 64 rows: 64-row tiles of scores, of dh and (its k) of dW, rings 3 K tiles ahead; more: 128-row tiles
 template <int EPI, int BM, int NST>
 hipError_t launch_tile(const VocabGemm& g, int tiles_m, int splits, hipStream_t st) {
   constexpr int BN = 128, lds = NST * (BM + BN) * BK * 2;
@@ -829,8 +862,14 @@ hipError_t launch_tiles(const VocabGemm& g, const VocabPlan& p, int64_t m, int s
 #if !CLIP_OPERAND_F16
 // G of one piece of the vocabulary may take this much: the pieces are as few as that allows
 constexpr int64_t G_BYTES = 1ll << 30;
-// From here on the 256 x 256 tiles
-constexpr int LARGE_ROWS = 256;
+// Which calls run on the 256 x 256 tiles of vocab8.hip.  Loss and gradients in us, these tiles against the small ones:
+//   V 30 522, H 768: n 65 120 / 94, 128 114 / 94, 160 118 / 133, 256 114 / 135;   V 8 000, H 256: n 160 71 / 55, 256 68 / 58
+// so up to 128 rows never, up to 256 where the weight has the tiles to fill most CUs, beyond that always (the small tiles read
+// W once per 128 rows)
+bool large_tiles(int32_t n, int64_t vocab, int32_t hidden) {
+  if (hidden % 128 || n <= 128) return false;
+  return n > 256 || (vocab + 255) / 256 * ((hidden + 255) / 256) >= 192;
+}
 
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {
   VocabPlan p = {};
@@ -840,7 +879,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     at += (bytes + 255) & ~(size_t)255;
     return o;
   };
-  p.large = n > LARGE_ROWS && hidden % 128 == 0;
+  p.large = large_tiles(n, vocab, hidden);
   p.tile_rows = p.large ? 256 : (n <= 64 ? 64 : 128);
   const int64_t rows = ((int64_t)n + 255) / 256 * 256, vp = (vocab + 255) / 256 * 256;
   p.head = take(sizeof(VocabHead));
@@ -858,7 +897,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     p.row_info = take(rows * 16);
     if (distill) {
       p.row_lc = take(rows * 8);
-      p.fix = take(vocab * 8);
+      p.fix = take(vocab * 8 * FIX_COPIES);
     }
     // a piece: whole 256-column tiles, G within its bound, 32-bit byte offsets into the piece of W
     int64_t piece = rows > 0 ? G_BYTES / (rows * 2) : vp;
@@ -886,6 +925,10 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     }
     p.dh_part = take((size_t)room * 4);
     p.dh_room = room;
+    if (p.large && n >= 1024 && p.pieces == 1 && vp / 256 * ((hidden + 255) / 256) <= 256) {
+      p.dw_room = 512 * 65536;
+      p.dw_part = take((size_t)p.dw_room * 4);
+    }
   }
   p.bytes = at;
   return p;
@@ -950,7 +993,8 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
       TRY(launch_tiles<V_STATS>(g, p, a.n, 1, st));
     }
     if (a.loss && a.n <= 1024) a.done = &reinterpret_cast<VocabHead*>(base + p.head)->done;
-    if (a.t_index) hipLaunchKernelGGL(vocab_distill_kernel, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
+    if (a.t_index && a.k > 16) hipLaunchKernelGGL(vocab_distill_kernel<4>, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
+    else if (a.t_index) hipLaunchKernelGGL(vocab_distill_kernel<1>, dim3((a.n + 3) / 4), dim3(256), 0, st, a, part, g.n_part);
     else hipLaunchKernelGGL(vocab_ce_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, part, g.n_part);
     TRY(hipGetLastError());
   }
@@ -977,6 +1021,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     TRY(device_cus(&a.wgs));
     a.wgs &= ~7;
     a.dh_room = p.dh_room;
+    a.dw_room = p.dw_room;
     a.piece_tiles[0] = (int32_t)(p.piece / 256);
     a.piece_tiles[1] = (int32_t)((a.vocab - (p.pieces - 1) * p.piece + 255) / 256);
   }
@@ -989,6 +1034,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.colsum = a.dbias ? reinterpret_cast<float*>(base + p.colsum) : nullptr;
   g.ld_colsum = p.ld_colsum;
   g.out32 = reinterpret_cast<float*>(base + p.dh_part);
+  g.dw32 = reinterpret_cast<float*>(base + p.dw_part);
   g.slot_stride = p.dh_slot;
   g.out16 = dw; g.ldo = ld_dw;
   g.wide = ((uintptr_t)dw & 15) == 0 && ld_dw % 8 == 0;
@@ -1020,8 +1066,10 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   }
   const int row_blocks = g.with_dh ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
   const int b_blocks = a.dbias ? (int)((a.vocab + 255) / 256) : 0;
-  if (row_blocks + b_blocks > 0) {
-    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks), dim3(256), 0, st, a, p, g.out32, g.colsum, row_blocks);
+  const int dw_blocks = dw && p.dw_room > 0 ? 1024 : 0;
+  if (row_blocks + b_blocks + dw_blocks > 0) {
+    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks + dw_blocks), dim3(256), 0, st, a, p, g.out32, g.colsum, g.dw32, dw,
+                       ld_dw, row_blocks, dw_blocks);
     TRY(hipGetLastError());
   }
   return hipSuccess;

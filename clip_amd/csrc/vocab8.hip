@@ -78,11 +78,12 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
     return p;
   };
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  int splits = 1, dh_less = 0, dh_more = 0;
+  int splits = 1, dh_less = 0, dh_more = 0, dw_splits = 1;
   if (!ROWS) {
     splits = __builtin_amdgcn_readfirstlane(a.schedule->splits);
     dh_less = __builtin_amdgcn_readfirstlane(a.schedule->dh_less);
     dh_more = __builtin_amdgcn_readfirstlane(a.schedule->dh_more);
+    dw_splits = __builtin_amdgcn_readfirstlane(a.schedule->dw_splits);
   }
   const int G = gridDim.x;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
@@ -110,14 +111,16 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
       return true;
     }
     // dW tiles dealt round-robin, then dh tiles as the schedule says
-    const int n_dw = a.with_dw ? (a.ldg >> 8) * tiles_n : 0, dw_full = n_dw / G, dw_rest = n_dw - dw_full * G;
+    const int dw_tiles = a.with_dw ? (a.ldg >> 8) * tiles_n : 0, n_dw = dw_tiles * dw_splits, dw_full = n_dw / G, dw_rest = n_dw - dw_full * G;
     const bool more_dw = lin < dw_rest;
     const int my_dw = dw_full + (more_dw ? 1 : 0);
     if (i < my_dw) {
-      const int q = i * G + lin;
-      o.tm = q / tiles_n;
-      o.tn = q - o.tm * tiles_n;
-      o.nt = (count + 127) / 128 * 2;
+      const int q = i * G + lin, s = q / dw_tiles, u = q - s * dw_tiles, all = (count + 127) >> 7;
+      o.split = s;
+      o.tm = u / tiles_n;
+      o.tn = u - o.tm * tiles_n;
+      o.kt0 = all * s / dw_splits * 2;
+      o.nt = all * (s + 1) / dw_splits * 2 - o.kt0;
       return true;
     }
     const int t = i - my_dw, tiles = tiles_r * tiles_n;
@@ -181,8 +184,9 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
       const int64_t v0 = a.v0 + (int64_t)o.kt0 * BK;
       cb.set(a.w + v0 * a.ldw + o.tn * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - o.tn * BN) * 2);
     } else {
-      ca.set(a.g + (int64_t)o.tm * BM, ((int64_t)rows_pad * a.ldg - (int64_t)o.tm * BM) * 2);
-      cb.set(a.x + o.tn * BN, ((int64_t)rows_pad * a.hidden - o.tn * BN) * 2);
+      const int64_t k0 = (int64_t)o.kt0 * BK;
+      ca.set(a.g + k0 * a.ldg + (int64_t)o.tm * BM, ((rows_pad - k0) * a.ldg - (int64_t)o.tm * BM) * 2);
+      cb.set(a.x + k0 * a.hidden + o.tn * BN, ((rows_pad - k0) * a.hidden - o.tn * BN) * 2);
     }
   };
 
@@ -357,10 +361,11 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
               *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + a.v0 + col0 + nh * 32 + i * 16) = t;
           }
       }
-    } else if (cur.dh) {
+    } else if (cur.dh || dw_splits > 1) {
       // fp32 partials in the accumulators' order (dh_partial_at): every store of a wave is 1 KiB contiguous
-      const int tiles_r = (count + 255) >> 8;
-      float* out = a.out32 + ((int64_t)(cur.split * tiles_r + tm) * a.tiles_n + tn) * 65536 + w * 8192 + le * 4;
+      const int panels = cur.dh ? (count + 255) >> 8 : a.ldg >> 8;
+      float* out = (cur.dh ? a.out32 : a.dw32) + ((int64_t)(cur.split * panels + tm) * a.tiles_n + tn) * 65536 + w * 8192 + le * 4;
+      const bool add = cur.dh && a.accumulate;
 #pragma unroll
       for (int mh = 0; mh < 2; ++mh)
 #pragma unroll
@@ -370,7 +375,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (((mh * 4 + m) * 2 + nh) * 2 + i) * 256);
-              *o = a.accumulate ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
+              *o = add ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
             }
     } else {
       const float s = a.out_scale[0];

@@ -61,7 +61,8 @@ def _check(h, w, b, run, p, live, temperature, reduction, seed, entropy=None):
 
 
 SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64, 128, 64), (65, 129, 192), (130, 777, 320),
-         (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768)]
+         (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768), (2600, 1300, 128), (1500, 2500, 384),
+         (1030, 5, 1024)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
