@@ -102,9 +102,9 @@ hipError_t launch_topk_rows(const void* logits, int type, int64_t ld, int n, int
 
 // ---- losses of the vocabulary decoder (vocab.hip)
 // How the products dh = G W and dW = G^T h of one piece share the persistent workgroups (vocab8.hip): the k of dh's tiles
-// (the vocabulary) is cut into `splits`, that of dW's (the rows) into dw_splits; a workgroup that has one dW tile less than
-// others takes dh_more of dh's split tiles, the others dh_less
-struct VocabSchedule { int32_t splits, dh_less, dh_more, dw_splits; };
+// (the vocabulary) is cut into dh_splits, that of dW's (the rows) into dw_splits; the first `first` workgroups take dw[0] of
+// dW's tiles and dh[0] of dh's, the others dw[1] and dh[1] (as long as there are any left)
+struct VocabSchedule { int32_t dh_splits, dw_splits, first, dw[2], dh[2], unused; };
 struct VocabHead {          // the words at the head of the workspace
   int32_t count, done;      // live rows; workgroups of the forward's last kernel that have finished
   float grad_max;
@@ -156,8 +156,10 @@ struct VocabGemm {          // arguments of vocab_gemm_kernel
   float* colsum; int64_t ld_colsum;
   float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: whole tiles, dh_partial_at)
   float* dw32;              // dW's partials where its k is split
-  const VocabSchedule* schedule; bool accumulate, with_dw, with_dh;
-  bf16_t* out16; int64_t ldo; bool wide;   // wide: rows start on 16 bytes
+  const VocabSchedule* schedule;
+  int32_t accumulate, with_dw, with_dh;   // (words: a byte among the arguments is no scalar load)
+  bf16_t* out16; int64_t ldo;
+  int32_t wide;             // out16's rows start on 16 bytes
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary

@@ -309,8 +309,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
 // ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
 // tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
 // leave the CU; partials: 256 KB leave it and are read again by the last kernel).  Lane s tries s + 1 splits of dh's tiles, and
-// for each some of dW's (where the vocabulary is so short that its tiles do not fill the workgroups: dw_room) and a few shares
-// of the workgroups that are behind by one dW tile.
+// for each some of dW's (where the vocabulary is so short that its tiles do not fill the workgroups: dw_room).
 __device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
   const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
   if (tiles > 0) {   // partials that there is room for
@@ -318,28 +317,45 @@ __device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int voca
     if (room < max_splits) max_splits = (int)room;
   }
   const int dw_tiles = a.with_dw ? vocab_tiles * a.tiles_h : 0, pairs = (total + 127) / 128, splits = lane + 1;
-  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 4;
-  int best = 0x7fffffff, best_more = 0, best_less = 0, best_dw = 1;
+  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 6;
+  VocabSchedule r = {splits, 1, 0, {0, 0}, {0, 0}, 0};
+  int best = 0x7fffffff;
   if (splits <= max_splits && splits <= vocab_tiles)
-    for (int d = 1; d <= 16; d += d < 4 ? 1 : d / 2) {   // 1 2 3 4 6 9 13
+    for (int d = 1; d <= 16; d += d < 4 ? 1 : d) {   // 1 2 3 4 8 16
       if (d > 1 && (d > pairs || (int64_t)dw_tiles * d * 65536 > a.dw_room)) break;
-      const int n_dw = dw_tiles * d, full = n_dw / wgs, rest = n_dw - full * wgs, len_dw = (pairs + d - 1) / d + (d > 1 ? 5 : 2);
-      for (int less = 0; less < 4; ++less) {   // dh tiles of a workgroup with one dW tile more
-        const int left = n_dh - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
-        const int t0 = rest ? (full + 1) * len_dw + less * len_dh : 0, t1 = full * len_dw + more * len_dh;
-        const int cost = max(t0, t1);
-        if (cost < best) { best = cost; best_less = less; best_more = more; best_dw = d; }
+      const int n_dw = dw_tiles * d, len_dw = (pairs + d - 1) / d + (d > 1 ? 6 : 3);
+      // one product dealt evenly, so that some workgroups are behind by one tile; those take more of the other's
+#pragma unroll
+      for (int even_dh = 0; even_dh < 2; ++even_dh) {
+        const int n0 = even_dh ? n_dh : n_dw, l0 = even_dh ? len_dh : len_dw, n1 = even_dh ? n_dw : n_dh, l1 = even_dh ? len_dw : len_dh;
+        const int full = n0 / wgs, rest = n0 - full * wgs;
+        for (int less = 0; less < 3; ++less) {
+          const int left = n1 - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
+          const int cost = max(rest ? (full + 1) * l0 + less * l1 : 0, full * l0 + more * l1);
+          if (cost < best) {
+            best = cost;
+            r.dw_splits = d;
+            r.first = rest;
+            r.dw[0] = even_dh ? less : full + 1;
+            r.dw[1] = even_dh ? more : full;
+            r.dh[0] = even_dh ? full + 1 : less;
+            r.dh[1] = even_dh ? full : more;
+          }
+        }
       }
     }
   const int low = best;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
   const int win = __ffsll(__ballot(low == best)) - 1;
-  VocabSchedule r;
-  r.splits = win + 1;
-  r.dh_less = __shfl(best_less, win, 64);
-  r.dh_more = __shfl(best_more, win, 64);
-  r.dw_splits = __shfl(best_dw, win, 64);
+  r.dh_splits = win + 1;
+  r.dw_splits = __shfl(r.dw_splits, win, 64);
+  r.first = __shfl(r.first, win, 64);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    r.dw[i] = __shfl(r.dw[i], win, 64);
+    r.dh[i] = __shfl(r.dh[i], win, 64);
+  }
   return r;
 }
 
@@ -358,10 +374,10 @@ __device__ __forceinline__ float finite_abs(float g) {
 template <bool GRAD>
 __device__ void write_head(const VocabRows& a, int total, float grad_max, int lane) {
   // (every piece sums into the first's partials: the last must not have more of them)
-  VocabSchedule s0 = {a.max_splits, 0, 0, 1}, s1 = s0;
+  VocabSchedule s0 = {a.max_splits, 1, 0, {0, 0}, {0, 0}, 0}, s1 = s0;
   if (GRAD && a.wgs) {
     s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
-    s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.splits, lane);
+    s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.dh_splits, lane);
   }
   if (lane != 0) return;
   *a.count = total;
@@ -775,7 +791,7 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
     return make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
   };
   if ((int)blockIdx.x >= b_blocks + dw_blocks) {
-    const int n = a.schedule[0].splits;
+    const int n = a.schedule[0].dh_splits;
     const int tiles_r = (count + 255) >> 8, h4 = a.hidden / 4;
     const int64_t total = p.large ? (int64_t)tiles_r * a.tiles_h * 16384 : (int64_t)count * h4;
     const int64_t slot = p.large ? total * 4 : p.dh_slot;

@@ -78,25 +78,19 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
     return p;
   };
   const int count = __builtin_amdgcn_readfirstlane(*a.count);
-  int splits = 1, dh_less = 0, dh_more = 0, dw_splits = 1;
-  if (!ROWS) {
-    splits = __builtin_amdgcn_readfirstlane(a.schedule->splits);
-    dh_less = __builtin_amdgcn_readfirstlane(a.schedule->dh_less);
-    dh_more = __builtin_amdgcn_readfirstlane(a.schedule->dh_more);
-    dw_splits = __builtin_amdgcn_readfirstlane(a.schedule->dw_splits);
-  }
+  typedef const __attribute__((address_space(4))) VocabSchedule* Schedule;   // (scalar loads, where it is needed)
   const int G = gridDim.x;
   const int xcd = blockIdx.x & 7, slot = blockIdx.x >> 3;
   const int lin = xcd * (G >> 3) + slot;   // neighbours share an XCD
   const uint32_t ld_x = (uint32_t)a.hidden * 2, ld_g = (uint32_t)a.ldg * 2, ld_w = (uint32_t)a.ldw * 2;
 
   // ---- items of this workgroup: a dW or dh tile or one of scores (panel tm, column tile tn), K tiles kt0 .. kt0 + nt
-  struct Item { bool dh; int tm, tn, kt0, nt, split; };
+  struct Item { bool dh, whole; int tm, tn, kt0, nt, split; };   // whole: a dW tile of all rows
   auto item = [&](int i, Item& o) -> bool {
     const auto& a = *args();
     const int tiles_r = (count + 255) >> 8, tiles_n = a.tiles_n;
     o.kt0 = o.split = 0;
-    o.dh = false;
+    o.dh = o.whole = false;
     if (ROWS) {
       // the 8 XCDs take contiguous runs of the vocabulary's tiles, each its own part of W; within it column groups of 4 tiles
       // (their slice of W stays in this XCD's L2), all row panels of one before the next
@@ -110,12 +104,17 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
       o.nt = a.hidden / BK;
       return true;
     }
-    // dW tiles dealt round-robin, then dh tiles as the schedule says
-    const int dw_tiles = a.with_dw ? (a.ldg >> 8) * tiles_n : 0, n_dw = dw_tiles * dw_splits, dw_full = n_dw / G, dw_rest = n_dw - dw_full * G;
-    const bool more_dw = lin < dw_rest;
-    const int my_dw = dw_full + (more_dw ? 1 : 0);
+    // dW tiles, then dh tiles, dealt as the schedule says: workgroups < first, then the others
+    const Schedule sc = (Schedule)a.schedule;
+    const int dw_splits = sc->dw_splits, dh_splits = sc->dh_splits, first = sc->first;
+    const int dw_tiles = a.with_dw ? (a.ldg >> 8) * tiles_n : 0, dh_tiles = a.with_dh ? tiles_r * tiles_n : 0;
+    const bool front = lin < first;
+    const int step = front ? first : G - first;
+    const int dw_at = front ? lin : first * sc->dw[0] + lin - first, dw_left = dw_tiles * dw_splits - dw_at;
+    const int my_dw = dw_left <= 0 ? 0 : min((dw_left + step - 1) / step, front ? sc->dw[0] : sc->dw[1]);
     if (i < my_dw) {
-      const int q = i * G + lin, s = q / dw_tiles, u = q - s * dw_tiles, all = (count + 127) >> 7;
+      o.whole = dw_splits == 1;
+      const int q = dw_at + i * step, s = q / dw_tiles, u = q - s * dw_tiles, all = (count + 127) >> 7;
       o.split = s;
       o.tm = u / tiles_n;
       o.tn = u - o.tm * tiles_n;
@@ -123,17 +122,15 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
       o.nt = all * (s + 1) / dw_splits * 2 - o.kt0;
       return true;
     }
-    const int t = i - my_dw, tiles = tiles_r * tiles_n;
-    if (t >= (more_dw ? dh_less : dh_more) || !a.with_dh) return false;
-    const int q = more_dw ? (G - dw_rest) * dh_more + lin + dw_rest * t : (lin - dw_rest) + (G - dw_rest) * t;
-    if (q >= tiles * splits) return false;
-    const int s = q / tiles, u = q - s * tiles, all = a.ldg >> 7;
+    const int t = i - my_dw, q = (front ? lin : first * sc->dh[0] + lin - first) + t * step;
+    if (t >= (front ? sc->dh[0] : sc->dh[1]) || q >= dh_tiles * dh_splits) return false;
+    const int s = q / dh_tiles, u = q - s * dh_tiles, all = a.ldg >> 7;
     o.dh = true;
     o.split = s;
     o.tm = u / tiles_n;
     o.tn = u - o.tm * tiles_n;
-    o.kt0 = all * s / splits * 2;
-    o.nt = all * (s + 1) / splits * 2 - o.kt0;
+    o.kt0 = all * s / dh_splits * 2;
+    o.nt = all * (s + 1) / dh_splits * 2 - o.kt0;
     return true;
   };
   Item cur;
@@ -361,22 +358,22 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
               *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + a.v0 + col0 + nh * 32 + i * 16) = t;
           }
       }
-    } else if (cur.dh || dw_splits > 1) {
+    } else if (!cur.whole) {
       // fp32 partials in the accumulators' order (dh_partial_at): every store of a wave is 1 KiB contiguous
       const int panels = cur.dh ? (count + 255) >> 8 : a.ldg >> 8;
       float* out = (cur.dh ? a.out32 : a.dw32) + ((int64_t)(cur.split * panels + tm) * a.tiles_n + tn) * 65536 + w * 8192 + le * 4;
-      const bool add = cur.dh && a.accumulate;
+      auto each = [&](auto&& f) {
 #pragma unroll
-      for (int mh = 0; mh < 2; ++mh)
+        for (int mh = 0; mh < 2; ++mh)
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+          for (int m = 0; m < 4; ++m)
 #pragma unroll
-          for (int nh = 0; nh < 2; ++nh)
+            for (int nh = 0; nh < 2; ++nh)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              f32x4_t* o = reinterpret_cast<f32x4_t*>(out + (((mh * 4 + m) * 2 + nh) * 2 + i) * 256);
-              *o = add ? *o + acc[mh][nh][m][i] : acc[mh][nh][m][i];
-            }
+              for (int i = 0; i < 2; ++i) f(reinterpret_cast<f32x4_t*>(out + (((mh * 4 + m) * 2 + nh) * 2 + i) * 256), acc[mh][nh][m][i]);
+      };
+      if (cur.dh && a.accumulate) each([](f32x4_t* o, const f32x4_t& v) { *o += v; });
+      else each([](f32x4_t* o, const f32x4_t& v) { *o = v; });
     } else {
       const float s = a.out_scale[0];
 #pragma unroll
