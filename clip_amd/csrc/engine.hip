@@ -656,9 +656,11 @@ int check_linear(const char* who, const clip_linear* d) {
   if (!d) return fail(CLIP_ERR_ARG, "%s: null argument", who);
   if (d->operand != CLIP_PRECISION_BF16 && d->operand != CLIP_PRECISION_F16)
     return fail(CLIP_ERR_ARG, "%s: operand type %d (CLIP_PRECISION_BF16 or CLIP_PRECISION_F16)", who, d->operand);
-  if (d->n < 0 || d->n >= (1 << 24) || d->hidden_size < 64 || d->hidden_size > 8192 || d->hidden_size % 64 || d->vocab < 1 ||
-      d->vocab > (1ll << 30))
-    return fail(CLIP_ERR_ARG, "%s: unsupported sizes n %d, hidden %d, vocab %lld (n < 2^24; hidden a multiple of 64, <= 8192; vocab <= 2^30)",
+  // (the kernels walk the rows with 32-bit byte offsets, and 256 columns of their score gradients within the piece's bound)
+  if (d->n < 0 || d->n >= (1 << 21) || d->hidden_size < 64 || d->hidden_size > 8192 || d->hidden_size % 64 ||
+      ((int64_t)d->n + 256) * d->hidden_size >= (1ll << 31) || d->vocab < 1 || d->vocab > (1ll << 30) ||
+      ((int64_t)d->n / 128 + 1) * (d->vocab / 128 + 1) >= (1ll << 31))
+    return fail(CLIP_ERR_ARG, "%s: unsupported sizes n %d, hidden %d, vocab %lld (n < 2^21, n hidden < 2^31; hidden a multiple of 64, <= 8192)",
                 who, d->n, d->hidden_size, (long long)d->vocab);
   if (d->ld_weight < d->hidden_size || d->ld_weight % 8 || d->ld_weight > (1 << 22) || (d->n > 1 && d->ld_hidden < d->hidden_size))
     return fail(CLIP_ERR_ARG, "%s: row strides %lld / %lld (weight: a multiple of 8, <= 2^22)", who, (long long)d->ld_hidden,

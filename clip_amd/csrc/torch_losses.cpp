@@ -5,6 +5,8 @@
 // Nothing is computed here, and there is no fallback: every call goes to libclip_amd.so, whose entry points the Python host
 // hands over (so that CLIP_AMD_LIB holds for both).
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -172,7 +174,9 @@ void check_linear(const Tensor& hidden, const Tensor& weight, const MaybeTensor&
                     " does not fit a [vocab, hidden] weight of ", shape_of(weight.sizes()));
   TORCH_CHECK_VALUE(weight.size(0) >= 1 && weight.size(1) >= 64 && weight.size(1) <= 8192 && weight.size(1) % 64 == 0,
                     "hidden size ", weight.size(1), " (a multiple of 64 up to 8192)");
-  TORCH_CHECK_VALUE(hidden.numel() / weight.size(1) < (1 << 24), "more than 2^24 - 1 rows");
+  const int64_t n = hidden.numel() / weight.size(1);
+  TORCH_CHECK_VALUE(n < (1 << 21) && (n + 256) * weight.size(1) < (1ll << 31), n, " rows of ", weight.size(1),
+                    " (fewer than 2^21, and 2^31 elements)");
   TORCH_CHECK(weight.device() == hidden.device(), "tensors on ", hidden.device(), " and ", weight.device());
   if (bias) {
     TORCH_CHECK_TYPE(bias->scalar_type() == at::kFloat && bias->dim() == 1 && bias->size(0) == weight.size(0), "bias must be float32 [",
@@ -181,11 +185,25 @@ void check_linear(const Tensor& hidden, const Tensor& weight, const MaybeTensor&
   }
 }
 
+// While a stream is being captured, a leaf whose gradient accumulation node still belongs to a graph of another stream would
+// make the backward pass record a wait across streams into the capture, and end the process: refused here, with the reason.
+void check_capture(const Tensor& t) {
+  if (!t.defined() || !t.requires_grad() || !t.is_leaf()) return;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!node) return;
+  const auto stream = node->stream();
+  TORCH_CHECK(!stream || *stream == c10::impl::VirtualGuardImpl(t.device().type()).getStream(t.device()),
+              "clip_amd.losses: a HIP graph is being captured while an earlier loss of the same leaf is still alive (its gradient belongs "
+              "to another stream): let go of eager losses before the capture");
+}
+
 Tensor apply(const Tensor& hidden, const Tensor& weight, const MaybeTensor& bias, const MaybeTensor& labels, const MaybeTensor& values,
              const MaybeTensor& index, int64_t ignore_index, double temperature, int64_t reduction) {
   const Tensor b = bias ? *bias : Tensor();
   Tensor loss;
   if (at::GradMode::is_enabled() && (hidden.requires_grad() || weight.requires_grad() || (b.defined() && b.requires_grad()))) {
+    if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None)
+      for (const Tensor* t : {&hidden, &weight, &b}) check_capture(*t);
     loss = LinearLoss::apply(hidden, weight, bias, labels, values, index, ignore_index, temperature, reduction);
   } else {
     const auto given = [](const MaybeTensor& t) { return t ? *t : Tensor(); };

@@ -180,13 +180,13 @@ int clip_ce_loss(const float* dev_logits, const int32_t* dev_labels, int32_t n, 
  * of their own. */
 typedef struct clip_linear {
   int32_t operand;               /* CLIP_PRECISION_BF16 or CLIP_PRECISION_F16: type of hidden, weight and their gradients */
-  int32_t n;                     /* hidden rows, 0 <= n < 2^24 */
+  int32_t n;                     /* hidden rows, 0 <= n < 2^21, (n + 256) hidden_size < 2^31 */
   int32_t hidden_size;           /* a multiple of 64, <= 8192 */
-  int64_t vocab;                 /* decoder rows, 1 .. 2^30 */
+  int64_t vocab;                 /* decoder rows, 1 .. 2^30; n x vocab < 2^45 */
   const uint16_t* dev_hidden;    /* [n, hidden_size], row stride ld_hidden (elements, >= hidden_size) */
   int64_t ld_hidden;
   const uint16_t* dev_weight;    /* [vocab, hidden_size], row stride ld_weight (a multiple of 8), 16-byte aligned */
-  int64_t ld_weight;
+  int64_t ld_weight;             /* <= 2^22 */
   const float* dev_bias;         /* [vocab] fp32, or NULL; -inf leaves an entry out of the softmax */
 } clip_linear;
 
@@ -206,7 +206,7 @@ int clip_linear_ce(const clip_linear* d, const int64_t* dev_labels, int64_t igno
  * dbias = column sums of dz; g_i = dev_grad[i] for reduction 0, dev_grad[0] / count for 1, dev_grad[0] for 2 (fp32).  Ignored
  * rows get zero dhidden rows and reach nothing else, whatever they hold.  Any of the three outputs may be NULL.  dz is rounded
  * once to the operand type for the two products (relative, 2^-9 or 2^-12); dbias is summed from unrounded values.  dweight
- * must be 8-byte aligned with a row stride that is a multiple of 4.  Same bits on every call. */
+ * must be 8-byte aligned with a row stride that is a multiple of 4.  Every call that asks for the same outputs gives the same bits. */
 int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t ignore_index, int32_t reduction,
                         const float* dev_lse, const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden,
                         int64_t ld_dhidden, uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,

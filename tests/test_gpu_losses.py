@@ -62,7 +62,7 @@ def _check(h, w, b, run, p, live, temperature, reduction, seed, entropy=None):
 
 SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64, 128, 64), (65, 129, 192), (130, 777, 320),
          (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768), (2600, 1300, 128), (1500, 2500, 384),
-         (1030, 5, 1024)]
+         (1030, 5, 1024), (70, 500, 2048), (300, 600, 1152), (130, 300, 8192)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -442,6 +442,150 @@ def test_captured_step_replays():
         kept = [t.clone() for t in out]
         for got, want in zip(kept, step()):
             assert torch.equal(got, want) or (got.isnan().all() and want.isnan().all())
+
+
+def test_capture_beside_a_living_eager_loss_is_refused():
+    h, w, b = R.make(40, 300, 64, BF16, 70)
+    y = _labels(40, 300, 71)
+    h.requires_grad_()
+    alive = losses.linear_cross_entropy(h, w, b, y)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="let go of eager losses"):
+        with torch.cuda.graph(graph, stream=side):
+            losses.linear_cross_entropy(h, w, b, y)
+    want, = torch.autograd.grad(alive, h)
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got, = torch.autograd.grad(losses.linear_cross_entropy(h, w, b, y), h)
+    for _ in range(3):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_backward_accumulates_and_repeats():
+    """.backward() into .grad, twice over one graph, and a weight shared by two losses"""
+    h, w, b = R.make(60, 500, 128, BF16, 90)
+    y = _labels(60, 500, 91, 0.2)
+    h, w, b = (t.requires_grad_() for t in (h, w, b))
+    loss = losses.linear_cross_entropy(h, w, b, y)
+    loss.backward(retain_graph=True)
+    first = [t.grad.clone() for t in (h, w, b)]
+    loss.backward()
+    assert all(torch.equal(t.grad, 2 * g) for t, g in zip((h, w, b), first))
+    two = losses.linear_cross_entropy(h, w, b, y) + losses.linear_cross_entropy(h[:30], w, b, y[:30], reduction="sum")
+    sep = torch.autograd.grad(losses.linear_cross_entropy(h[:30], w, b, y[:30], reduction="sum"), w)[0]
+    assert torch.equal(torch.autograd.grad(two, w)[0], (first[1] + sep))
+
+
+@pytest.mark.parametrize("up", [0.0, -2.0, 65536.0, 1e-30])
+def test_upstream_gradients(up):
+    n, vocab = 90, 700
+    h, w, b = R.make(n, vocab, 128, BF16, 40)
+    y = _labels(n, vocab, 41)
+    p, live = R.targets_ce(y, vocab, -100)
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    for red in ("sum", "none"):
+        loss = losses.linear_cross_entropy(*leaves, y, reduction=red)
+        g = torch.full_like(loss, up)
+        if red == "none":
+            g[::3] *= -1
+            g[7] = 0
+        rows = g if red == "none" else g.expand(n)
+        want, err = R.reference(h, w, b, p, live, 1.0, rows)
+        for name, got, a, e in zip(("dh", "dw", "db"), torch.autograd.grad(loss, leaves, g), want[1:], err[1:]):
+            R.assert_within(name, got, a, e)
+    # an infinite or NaN gradient shows
+    for bad in (INF, NAN):
+        loss = losses.linear_cross_entropy(*leaves, y)
+        assert not any(t.isfinite().all() for t in torch.autograd.grad(loss, leaves, torch.tensor(bad).cuda()))
+
+
+def test_ignore_index_inside_the_vocabulary():
+    n, vocab = 300, 260
+    h, w, b = R.make(n, vocab, 128, BF16, 44)
+    y = _labels(n, vocab, 45)
+    y[::3] = 5
+    p, live = R.targets_ce(y, vocab, 5)
+    assert not live.all()
+    _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y, ignore_index=5), p, live, 1.0, "mean", 5)
+
+
+# ---------------------------------------------------------------- the C ABI itself
+@pytest.mark.parametrize("n,vocab,hidden,ld_dh,ld_dw,k", [(50, 300, 64, 71, 68, 0), (100, 1000, 128, 128, 132, 5), (300, 1111, 128, 129, 136, 0),
+                                                          (700, 4000, 384, 384, 388, 70), (1500, 257, 128, 128, 128, 0)])
+def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
+    """Row strides of the outputs, a workspace of exactly the size asked for and full of NaN, and untouched bytes around
+    every output and behind the workspace; the same bits as the Python call."""
+    import ctypes as C
+    from clip_amd import _lib
+    lib = _lib.load()
+    h, w, b = R.make(n, vocab, hidden, BF16, 17)
+    y = _labels(n, vocab, 18, 0.1)
+    values, index = _teacher(n, vocab, max(k, 1), 19, 0.2)
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_distillation(*leaves, values, index, temperature=2.0) if k else losses.linear_cross_entropy(*leaves, y)
+    want = torch.autograd.grad(loss, leaves)
+    d = _lib.ClipLinear(_lib.PRECISION_BF16, n, hidden, vocab, h.data_ptr(), hidden, w.data_ptr(), hidden, b.data_ptr())
+    GUARD = 4096
+
+    def guarded(nbytes):
+        t = torch.full((nbytes + 2 * GUARD,), 0xA5, dtype=torch.uint8, device="cuda")
+        return t, t.data_ptr() + GUARD
+
+    def intact(t, nbytes):
+        return bool((t[:GUARD] == 0xA5).all()) and bool((t[GUARD + nbytes:] == 0xA5).all())
+    st = torch.cuda.current_stream().cuda_stream
+    need = C.c_int64()
+    bufs = {}
+    for name, size in (("row", 4 * n), ("lse", 4 * n), ("target", 4 * n * max(k, 1)), ("loss", 4), ("dh", 2 * n * ld_dh), ("dw", 2 * vocab * ld_dw),
+                       ("db", 4 * vocab)):
+        bufs[name] = (*guarded(size), size)
+    at = {name: v[1] for name, v in bufs.items()}
+    one = torch.ones((), device="cuda")
+    for grad in (0, 1):
+        _lib.check(lib.clip_linear_loss_workspace(C.byref(d), k, grad, C.byref(need)))
+        work, base = guarded(need.value)
+        work[GUARD:GUARD + need.value] = 0xFF          # NaN in every type
+        if not grad:
+            tail = (1, at["row"], at["lse"], at["target"], at["loss"], base, need.value, st)
+            rc = lib.clip_linear_distill(C.byref(d), values.data_ptr(), index.data_ptr(), k, 2.0, *tail) if k else \
+                lib.clip_linear_ce(C.byref(d), y.data_ptr(), -100, *tail)
+        else:
+            tail = (1, at["lse"], at["target"], one.data_ptr(), at["dh"], ld_dh, at["dw"], ld_dw, at["db"], base, need.value, st)
+            rc = lib.clip_linear_distill_grad(C.byref(d), values.data_ptr(), index.data_ptr(), k, 2.0, *tail) if k else \
+                lib.clip_linear_ce_grad(C.byref(d), y.data_ptr(), -100, *tail)
+        _lib.check(rc)
+        torch.cuda.synchronize()
+        assert intact(work, need.value)
+    assert all(intact(t, size) for t, _, size in bufs.values())
+
+    def rows(name, dtype, ld, cols):
+        t, _, size = bufs[name]
+        m = t[GUARD:GUARD + size].view(torch.int16).view(-1, ld)
+        assert (m[:, cols:] == torch.tensor(0xA5A5 - 0x10000, dtype=torch.int16)).all(), name
+        return m[:, :cols].contiguous().view(dtype)
+    assert torch.equal(rows("dh", BF16, ld_dh, hidden), want[0]) and torch.equal(rows("dw", BF16, ld_dw, hidden), want[1])
+    assert torch.equal(bufs["db"][0][GUARD:GUARD + 4 * vocab].view(F32), want[2])
+    assert torch.equal(bufs["loss"][0][GUARD:GUARD + 4].view(F32)[0], loss.detach())
+    # one output at a time
+    for name in ("dh", "dw", "db"):
+        bufs[name][0][GUARD:GUARD + bufs[name][2]] = 0xA5
+        a = {x: (at[x] if x == name else None) for x in ("dh", "dw", "db")}
+        tail = (1, at["lse"], at["target"], one.data_ptr(), a["dh"], ld_dh, a["dw"], ld_dw, a["db"], base, need.value, st)
+        rc = lib.clip_linear_distill_grad(C.byref(d), values.data_ptr(), index.data_ptr(), k, 2.0, *tail) if k else \
+            lib.clip_linear_ce_grad(C.byref(d), y.data_ptr(), -100, *tail)
+        _lib.check(rc)
+    torch.cuda.synchronize()
+    # dh and dW: the split of their long sums depends on what shares the workgroups, so a value may round to its neighbour
+    for name, ld, ref in (("dh", ld_dh, want[0]), ("dw", ld_dw, want[1])):
+        off = (rows(name, BF16, ld, hidden).float() - ref.float()).abs()
+        assert (off <= 2 * R.half_step(BF16) * ref.float().abs() + 1e-6).all()
+    assert torch.equal(bufs["db"][0][GUARD:GUARD + 4 * vocab].view(F32), want[2])
 
 
 # ---------------------------------------------------------------- refusals

@@ -20,7 +20,7 @@ def _need(k=0, grad=0, **kw):
     return rc, out.value
 
 
-@pytest.mark.parametrize("kw", [dict(operand=_lib.PRECISION_FP32), dict(operand=7), dict(n=-1), dict(n=1 << 24), dict(hidden_size=0),
+@pytest.mark.parametrize("kw", [dict(operand=_lib.PRECISION_FP32), dict(operand=7), dict(n=-1), dict(n=1 << 21), dict(n=1 << 18, hidden_size=8192, ld_hidden=8192, ld_weight=8192), dict(n=1 << 20, vocab=1 << 30), dict(hidden_size=0),
                                 dict(hidden_size=96), dict(hidden_size=8256, ld_weight=8256, ld_hidden=8256), dict(vocab=0),
                                 dict(vocab=(1 << 30) + 1), dict(ld_weight=120), dict(ld_weight=132), dict(ld_weight=(1 << 22) + 8),
                                 dict(ld_hidden=64)])
