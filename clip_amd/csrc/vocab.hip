@@ -12,11 +12,13 @@
 // the products are stored.
 // Rows that take no part (ignored label, empty teacher list) are dropped first: the live rows are copied side by side, so
 // their products cost nothing and whatever a dropped row holds (NaN included) reaches no gradient.
+#include <type_traits>
+
 #include "vocab.h"
 
-#define TRY(expr)                          \
+#define TRY(...)                           \
   do {                                     \
-    hipError_t _e = (expr);                \
+    hipError_t _e = (__VA_ARGS__);         \
     if (_e != hipSuccess) return _e;       \
   } while (0)
 
@@ -48,6 +50,16 @@ struct Operand {
       }
     }
   }
+  // rows base[map[r]] (K-major); a row that is not there (-1) lies past the end: zeros.  bytes < 2^31
+  __device__ __forceinline__ void init_rows(const bf16_t* base, int64_t bytes, int64_t ld, const int* map, int w, int lane) {
+    rsrc = make_rsrc(base, bytes);
+    step = BK * 2;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int at = (w * PIECES + p) * 1024 + lane * 16, r = at >> 7, from = map[r];
+      off[p] = from < 0 ? 0x80000000u : (uint32_t)(from * ld * 2) + swz128(r, (at >> 4) & 7) * 16;
+    }
+  }
   __device__ __forceinline__ void stage(uint32_t kt, uint32_t lds, int w) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) dma16(rsrc, off[p] + kt * step, lds + (w * PIECES + p) * 1024);
@@ -68,6 +80,175 @@ struct Operand {
   }
 };
 
+// ---- block-wide sums (256 threads) through LDS, every thread gets the result; fixed order
+__device__ __forceinline__ float block_sum(float v, float* red) {
+  v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (red[0] + red[1]) + (red[2] + red[3]);
+}
+__device__ __forceinline__ float block_max(float v, float* red) {
+  v = wave_max(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
+// tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
+// leave the CU; partials: 256 KB leave it and are read again by the last kernel).  Lane s tries s + 1 splits of dh's tiles, and
+// for each some of dW's (where the vocabulary is so short that its tiles do not fill the workgroups: dw_room).
+__device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
+  const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
+  if (tiles > 0) {   // partials that there is room for
+    const int64_t room = a.dh_room / ((int64_t)tiles * 65536);
+    if (room < max_splits) max_splits = (int)room;
+  }
+  const int dw_tiles = a.with_dw ? vocab_tiles * a.tiles_h : 0, pairs = (total + 127) / 128, splits = lane + 1;
+  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 6;
+  VocabSchedule r = {splits, 1, 0, {0, 0}, {0, 0}, 0};
+  int best = 0x7fffffff;
+  if (splits <= max_splits && splits <= vocab_tiles)
+    for (int d = 1; d <= 16; d += d < 4 ? 1 : d) {   // 1 2 3 4 8 16
+      if (d > 1 && (d > pairs || (int64_t)dw_tiles * d * 65536 > a.dw_room)) break;
+      const int n_dw = dw_tiles * d, len_dw = (pairs + d - 1) / d + (d > 1 ? 6 : 3);
+      // one product dealt evenly, so that some workgroups are behind by one tile; those take more of the other's
+#pragma unroll
+      for (int even_dh = 0; even_dh < 2; ++even_dh) {
+        const int n0 = even_dh ? n_dh : n_dw, l0 = even_dh ? len_dh : len_dw, n1 = even_dh ? n_dw : n_dh, l1 = even_dh ? len_dw : len_dh;
+        const int full = n0 / wgs, rest = n0 - full * wgs;
+        for (int less = 0; less < 3; ++less) {
+          const int left = n1 - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
+          const int cost = max(rest ? (full + 1) * l0 + less * l1 : 0, full * l0 + more * l1);
+          if (cost < best) {
+            best = cost;
+            r.dw_splits = d;
+            r.first = rest;
+            r.dw[0] = even_dh ? less : full + 1;
+            r.dw[1] = even_dh ? more : full;
+            r.dh[0] = even_dh ? full + 1 : less;
+            r.dh[1] = even_dh ? full : more;
+          }
+        }
+      }
+    }
+  const int low = best;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
+  const int win = __ffsll(__ballot(low == best)) - 1;
+  r.dh_splits = win + 1;
+  r.dw_splits = __shfl(r.dw_splits, win, 64);
+  r.first = __shfl(r.first, win, 64);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    r.dw[i] = __shfl(r.dw[i], win, 64);
+    r.dh[i] = __shfl(r.dh[i], win, 64);
+  }
+  return r;
+}
+
+// 0 takes no part, 1 live, 2 live with a target outside the vocabulary
+__device__ __forceinline__ int row_state(const VocabRows& a, int r) {
+  if (a.state) return a.state[r];
+  const int64_t y = a.labels[r];
+  return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
+}
+__device__ __forceinline__ float finite_abs(float g) {
+  g = fabsf(g);
+  return g < INFINITY ? g : 0.f;
+}
+
+// what the whole call needs to know: by one wave, once
+template <bool GRAD>
+__device__ void write_head(const VocabRows& a, int total, float grad_max, int lane) {
+  // (every piece sums into the first's partials: the last must not have more of them)
+  VocabSchedule s0 = {a.max_splits, 1, 0, {0, 0}, {0, 0}, 0}, s1 = s0;
+  if (GRAD && a.wgs) {
+    s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
+    s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.dh_splits, lane);
+  }
+  if (lane != 0) return;
+  *a.count = total;
+  if (!GRAD) a.head->done = 0;
+  if (GRAD) {
+    // the factor common to all rows; what is left of a row's gradient is c, |c| <= 1.  No live row: zeros, not 0 / 0
+    const float f = (a.grad_rows ? grad_max : a.grad[0]) * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);
+    *a.grad_max = grad_max;
+    a.out_scale[0] = f / G_SCALE;
+    a.out_scale[1] = f;
+    a.schedule[0] = s0;
+    a.schedule[1] = s1;
+  }
+}
+
+// what V_GRAD needs of a live row: (x, y, label, t), G = y exp2(z log2(e) / T - x) but t at the label; lc: (lse log2(e), c)
+__device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st, float grad_max, float2& lc) {
+  float c = 1.f;
+  if (a.grad_rows) {
+    const float g = a.grad[r];
+    c = fabsf(g) < INFINITY ? (grad_max > 0.f ? g / grad_max : 0.f) : g;
+  }
+  if (st == 2) c = __builtin_nanf("");   // the target is outside the vocabulary
+  const float l2 = a.lse[r] * LOG2E;
+  lc = make_float2(l2, c);
+  // x takes |c| and G's scale, y its sign
+  float4 info = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, __int_as_float(-1), 0.f);
+  if (!a.state && st == 1) {
+    info.z = __int_as_float((int)a.labels[r]);
+    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -l2)) - 1.f) * G_SCALE;
+  }
+  return info;
+}
+__device__ __forceinline__ float4 no_row() { return make_float4(INFINITY, 1.f, __int_as_float(-1), 0.f); }   // G = 0
+
+// Calls of at most 64 rows: what vocab_pack_kernel does otherwise, by the product kernel itself.  Every workgroup finds the
+// live rows for itself (map, in LDS; and info); workgroup 0 notes them down for the kernels that follow, and all of them share
+// the copies.  Returns the number of live rows.
+template <bool GRAD>
+__device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, int* map, float4* info) {
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, groups = gridDim.x;
+  const int st = lane < a.n ? row_state(a, lane) : 0;
+  const unsigned long long live = __ballot(st != 0);
+  const int count = __popcll(live), rank = __popcll(live & ((1ull << lane) - 1));
+  const float gm = GRAD && a.grad_rows ? wave_max(st != 0 ? finite_abs(a.grad[lane]) : 0.f) : 0.f;
+  if (w == 0) {
+    if (GRAD && lane >= count) info[lane] = no_row();
+    if (lane >= count) map[lane] = -1;
+    if (st != 0) {
+      map[rank] = lane;
+      float2 lc;
+      if (GRAD) info[rank] = row_info_of(a, lane, st, gm, lc);
+      if (blockIdx.x == 0) {
+        a.row_map[rank] = st == 2 ? ~lane : lane;
+        if (GRAD && a.state) a.row_lc[rank] = lc;
+      }
+    } else if (!GRAD && blockIdx.x == 0 && lane < a.n) {
+      a.row_loss[lane] = 0.f;
+      a.lse_out[lane] = 0.f;
+    }
+    if (blockIdx.x == 0) write_head<GRAD>(a, count, gm, lane);
+  }
+  __syncthreads();
+  if (GRAD) {
+    // dW reads the rows k by k: side by side, and zeros up to 64
+    for (int q = blockIdx.x * 4 + w; q < 64; q += groups * 4) {
+      const int r = map[q];
+      for (int c = lane * 8; c < a.hidden; c += 512)
+        *reinterpret_cast<uint4*>(a.x + (int64_t)q * a.hidden + c) =
+            r < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(a.h + (int64_t)r * a.ldh + c);
+      if (a.dh && q < a.n && !(live >> q & 1))
+        for (int c = lane; c < a.hidden; c += 64) a.dh[(int64_t)q * a.ld_dh + c] = 0;
+    }
+    if (a.fix && first_piece)
+      for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab * FIX_COPIES; v += (int64_t)groups * 256) a.fix[v] = 0;
+  }
+  return count;
+}
+
+struct NoRows {};
+
 // waits until at most `n` of this wave's loads are in flight
 template <int N>
 __device__ __forceinline__ void wait_loads() {
@@ -81,8 +262,9 @@ __device__ __forceinline__ void wait_loads() {
 
 // One output tile of BM x BN per workgroup of WM x WN waves, 64 columns per wave, through a ring of NST K tiles (few rows: many
 // small tiles and a deep ring, the weight's bytes are the bound; vocab8.hip takes the large calls).
-template <int EPI, int BM, int BN, int WM, int WN, int NST>
-__global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
+// FEW: calls of at most 64 rows, whose live rows this kernel finds and reads in place (gather_few).
+template <int EPI, int BM, int BN, int WM, int WN, int NST, bool FEW>
+__global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, std::conditional_t<FEW, VocabRows, NoRows> rows) {
   constexpr int NW = WM * WN, MB = BM / WM / 16, NB = BN / WN / 16;
   static_assert(NB == 4, "64 columns per wave");
   constexpr bool A_TR = EPI == V_DW, B_TR = EPI == V_DH || EPI == V_DW;
@@ -93,7 +275,11 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
-  const int count = *a.count;                       // live rows
+  __shared__ int map_s[FEW ? 64 : 1];
+  __shared__ float4 info_s[FEW ? 64 : 1];
+  int count;                                        // live rows
+  if constexpr (FEW) count = gather_few<EPI == V_GRAD>(rows, a.v0 == 0, map_s, info_s);
+  else count = *a.count;
   const int tn = blockIdx.x % a.tiles_n, tm = blockIdx.x / a.tiles_n, split = blockIdx.y;
   if (EPI != V_DW && tm * BM >= count) return;      // workgroup-uniform
 
@@ -102,7 +288,8 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
   OB ob;
   if (EPI == V_STATS || EPI == V_GRAD) {
     nt = a.hidden / BK;
-    oa.init(a.x + (int64_t)tm * BM * a.hidden, (int64_t)BM * a.hidden * 2, a.hidden, w, lane);
+    if constexpr (FEW) oa.init_rows(rows.h, ((int64_t)(rows.n - 1) * rows.ldh + a.hidden) * 2, rows.ldh, map_s, w, lane);
+    else oa.init(a.x + (int64_t)tm * BM * a.hidden, (int64_t)BM * a.hidden * 2, a.hidden, w, lane);
     const int64_t v0 = a.v0 + (int64_t)tn * BN;
     ob.init(a.w + v0 * a.ldw, ((a.vocab - 1 - v0) * a.ldw + a.hidden) * 2, a.ldw, w, lane);
   } else if (EPI == V_DH) {
@@ -204,7 +391,7 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
       const int r = row0 + m * 16;
-      const float4 ri = a.row_info[r];
+      const float4 ri = FEW ? info_s[r & 63] : a.row_info[r];
       const int at = __float_as_int(ri.z) - (int)a.v0 - col0;   // the label, counted from this lane's first column
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -255,22 +442,6 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a) {
   }
 }
 
-// ---- block-wide sums (256 threads) through LDS, every thread gets the result; fixed order
-__device__ __forceinline__ float block_sum(float v, float* red) {
-  v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
-}
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-
 // Teacher lists of a distillation: p = softmax(values / T) over a row's entries with index >= 0 and a value above -inf
 // (0 elsewhere), log_p beside it, state[row] = 0 no entry, 1 live, 2 an index beyond the vocabulary or a value that is
 // NaN or +inf.  One wave per row.
@@ -304,93 +475,6 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
   }
   const bool any_in = __any(n_in), any_bad = __any(bad);
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
-}
-
-// ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
-// tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
-// leave the CU; partials: 256 KB leave it and are read again by the last kernel).  Lane s tries s + 1 splits of dh's tiles, and
-// for each some of dW's (where the vocabulary is so short that its tiles do not fill the workgroups: dw_room).
-__device__ VocabSchedule choose_schedule(const VocabRows& a, int total, int vocab_tiles, int max_splits, int lane) {
-  const int rows_t = (total + 255) >> 8, tiles = a.dh ? rows_t * a.tiles_h : 0, wgs = a.wgs;
-  if (tiles > 0) {   // partials that there is room for
-    const int64_t room = a.dh_room / ((int64_t)tiles * 65536);
-    if (room < max_splits) max_splits = (int)room;
-  }
-  const int dw_tiles = a.with_dw ? vocab_tiles * a.tiles_h : 0, pairs = (total + 127) / 128, splits = lane + 1;
-  const int n_dh = tiles * splits, len_dh = (vocab_tiles * 2 + splits - 1) / splits + 6;
-  VocabSchedule r = {splits, 1, 0, {0, 0}, {0, 0}, 0};
-  int best = 0x7fffffff;
-  if (splits <= max_splits && splits <= vocab_tiles)
-    for (int d = 1; d <= 16; d += d < 4 ? 1 : d) {   // 1 2 3 4 8 16
-      if (d > 1 && (d > pairs || (int64_t)dw_tiles * d * 65536 > a.dw_room)) break;
-      const int n_dw = dw_tiles * d, len_dw = (pairs + d - 1) / d + (d > 1 ? 6 : 3);
-      // one product dealt evenly, so that some workgroups are behind by one tile; those take more of the other's
-#pragma unroll
-      for (int even_dh = 0; even_dh < 2; ++even_dh) {
-        const int n0 = even_dh ? n_dh : n_dw, l0 = even_dh ? len_dh : len_dw, n1 = even_dh ? n_dw : n_dh, l1 = even_dh ? len_dw : len_dh;
-        const int full = n0 / wgs, rest = n0 - full * wgs;
-        for (int less = 0; less < 3; ++less) {
-          const int left = n1 - less * rest, more = left > 0 ? (left + wgs - rest - 1) / (wgs - rest) : 0;
-          const int cost = max(rest ? (full + 1) * l0 + less * l1 : 0, full * l0 + more * l1);
-          if (cost < best) {
-            best = cost;
-            r.dw_splits = d;
-            r.first = rest;
-            r.dw[0] = even_dh ? less : full + 1;
-            r.dw[1] = even_dh ? more : full;
-            r.dh[0] = even_dh ? full + 1 : less;
-            r.dh[1] = even_dh ? full : more;
-          }
-        }
-      }
-    }
-  const int low = best;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) best = min(best, __shfl_xor(best, o, 64));
-  const int win = __ffsll(__ballot(low == best)) - 1;
-  r.dh_splits = win + 1;
-  r.dw_splits = __shfl(r.dw_splits, win, 64);
-  r.first = __shfl(r.first, win, 64);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    r.dw[i] = __shfl(r.dw[i], win, 64);
-    r.dh[i] = __shfl(r.dh[i], win, 64);
-  }
-  return r;
-}
-
-// 0 takes no part, 1 live, 2 live with a target outside the vocabulary
-__device__ __forceinline__ int row_state(const VocabRows& a, int r) {
-  if (a.state) return a.state[r];
-  const int64_t y = a.labels[r];
-  return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
-}
-__device__ __forceinline__ float finite_abs(float g) {
-  g = fabsf(g);
-  return g < INFINITY ? g : 0.f;
-}
-
-// what the whole call needs to know: by one wave, once
-template <bool GRAD>
-__device__ void write_head(const VocabRows& a, int total, float grad_max, int lane) {
-  // (every piece sums into the first's partials: the last must not have more of them)
-  VocabSchedule s0 = {a.max_splits, 1, 0, {0, 0}, {0, 0}, 0}, s1 = s0;
-  if (GRAD && a.wgs) {
-    s0 = choose_schedule(a, total, a.piece_tiles[0], 64, lane);
-    s1 = a.piece_tiles[1] == a.piece_tiles[0] ? s0 : choose_schedule(a, total, a.piece_tiles[1], s0.dh_splits, lane);
-  }
-  if (lane != 0) return;
-  *a.count = total;
-  if (!GRAD) a.head->done = 0;
-  if (GRAD) {
-    // the factor common to all rows; what is left of a row's gradient is c, |c| <= 1.  No live row: zeros, not 0 / 0
-    const float f = (a.grad_rows ? grad_max : a.grad[0]) * a.grad_factor / (a.mean ? (float)max(total, 1) : 1.f);
-    *a.grad_max = grad_max;
-    a.out_scale[0] = f / G_SCALE;
-    a.out_scale[1] = f;
-    a.schedule[0] = s0;
-    a.schedule[1] = s1;
-  }
 }
 
 // Calls of many rows: the live rows before every 16th row, by one workgroup (a thread reads 16 rows' states at a time)
@@ -518,22 +602,9 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       const int rank = before + __popc(live & ((1u << lane) - 1));
       a.row_map[rank] = st == 2 ? ~r : r;    // a row whose target is outside the vocabulary: NaN loss and gradients
       if (GRAD) {
-        float c = 1.f;
-        if (a.grad_rows) {
-          const float g = a.grad[r];
-          c = fabsf(g) < INFINITY ? (gm > 0.f ? g / gm : 0.f) : g;
-        }
-        if (st == 2) c = __builtin_nanf("");
-        const float l2 = a.lse[r] * LOG2E;
-        // x takes |c| and G's scale, y its sign
-        float4 info = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, __int_as_float(-1), 0.f);
-        if (a.state) {
-          a.row_lc[rank] = make_float2(l2, c);
-        } else if (st == 1) {
-          info.z = __int_as_float((int)a.labels[r]);
-          info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -l2)) - 1.f) * G_SCALE;
-        }
-        a.row_info[rank] = info;
+        float2 lc;
+        a.row_info[rank] = row_info_of(a, r, st, gm, lc);
+        if (a.state) a.row_lc[rank] = lc;
       }
     } else if (!GRAD) {
       a.row_loss[r] = 0.f;
@@ -543,7 +614,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
   const int pad = (total + a.tile_rows - 1) / a.tile_rows * a.tile_rows;
   for (int q = total + blockIdx.x * 4 + w; q < pad; q += gridDim.x * 4) {
     for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)q * H + c) = make_uint4(0, 0, 0, 0);
-    if (GRAD && lane == 0) a.row_info[q] = make_float4(INFINITY, 1.f, __int_as_float(-1), 0.f);   // G = 0
+    if (GRAD && lane == 0) a.row_info[q] = no_row();
   }
   if (GRAD && a.fix)
     for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab * FIX_COPIES; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
@@ -610,7 +681,7 @@ __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2
     float loss = __builtin_nanf(""), z = 0.f;
     if (mapped >= 0) {
       const int64_t v = a.labels[row];
-      z = wave_score(a.x + (int64_t)r * a.hidden, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
+      z = wave_score(a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
     }
     const float lse = lse_of(wave_pairs(part + (int64_t)r * n_part, n_part, lane, 64));
     if (mapped >= 0) loss = lse - z;
@@ -644,7 +715,7 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
       }
     }
     const float lse = lse_of(all);
-    const bf16_t* x = a.x + (int64_t)r * a.hidden;
+    const bf16_t* x = a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh;
     float loss = 0.f;
     if (mapped >= 0)
       for (int j0 = w * 8; j0 < a.k; j0 += 8 * WPR) {   // eight entries' rows of W in flight
@@ -854,16 +925,16 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
 }
 
 // up to 64 rows: 64-row tiles of scores, of dh and (its k) of dW, rings 3 K tiles ahead; more: 128-row tiles
-template <int EPI, int BM, int NST>
-hipError_t launch_tile(const VocabGemm& g, int tiles_m, int splits, hipStream_t st) {
+template <int EPI, int BM, int NST, bool FEW = false>
+hipError_t launch_tile(const VocabGemm& g, int tiles_m, int splits, hipStream_t st, const std::conditional_t<FEW, VocabRows, NoRows>& rows = {}) {
   constexpr int BN = 128, lds = NST * (BM + BN) * BK * 2;
-  auto kfn = vocab_gemm_kernel<EPI, BM, BN, 2, 2, NST>;
+  auto kfn = vocab_gemm_kernel<EPI, BM, BN, 2, 2, NST, FEW>;
   static DeviceOnce once;
   int unused;
   TRY(once.get([&](int, int*) {
     return hipFuncSetAttribute(reinterpret_cast<const void*>(kfn), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   }, &unused));
-  hipLaunchKernelGGL(kfn, dim3(tiles_m * g.tiles_n, splits), dim3(256), lds, st, g);
+  hipLaunchKernelGGL(kfn, dim3(tiles_m * g.tiles_n, splits), dim3(256), lds, st, g, rows);
   return hipGetLastError();
 }
 template <int EPI>
@@ -960,7 +1031,7 @@ hipError_t device_cus(int* out) {
 
 // what the forward and the backward begin with: the teacher's lists, and the live rows side by side
 template <bool GRAD>
-hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, hipStream_t st) {
+hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, hipStream_t st) {
   VocabHead* head = reinterpret_cast<VocabHead*>(base + p.head);
   a.head = head;
   a.tile_rows = p.tile_rows;
@@ -979,12 +1050,17 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, hipStream_t
       TRY(hipGetLastError());
     }
   }
+  // few rows, read in place by the product kernel (16-byte loads, 31-bit offsets): no kernel of their own
+  few = p.tile_rows == 64 && a.n > 0 && a.h_aligned && ((int64_t)(a.n - 1) * a.ldh + a.hidden) * 2 < (1ll << 31);
+  if (few) return hipSuccess;
   if (a.n > 1024) {   // more rows than a workgroup of the next kernel should count for itself
     a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
     hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());
   }
-  hipLaunchKernelGGL(vocab_pack_kernel<GRAD>, dim3(a.n > 0 ? (a.n + 15) / 16 : 1), dim3(256), 0, st, a);
+  int groups = a.n > 0 ? (a.n + 15) / 16 : 1;
+  if (GRAD && a.fix && groups < 64) groups = 64;   // (they clear its table, too)
+  hipLaunchKernelGGL(vocab_pack_kernel<GRAD>, dim3(groups), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -994,7 +1070,8 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
   VocabRows a = rows;
   char* base = static_cast<char*>(work);
   float2* part = reinterpret_cast<float2*>(base + p.part);
-  TRY(gather_rows<false>(a, p, base, st));
+  bool few;
+  TRY(gather_rows<false>(a, p, base, few, st));
   if (a.n > 0) {
     VocabGemm g = {};
     g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
@@ -1006,8 +1083,9 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
       TRY(launch_vocab8(V_STATS, g, st));
     } else {
       g.tiles_n = g.n_part / 2;
-      TRY(launch_tiles<V_STATS>(g, p, a.n, 1, st));
+      TRY(few ? launch_tile<V_STATS, 64, 4, true>(g, 1, 1, st, a) : launch_tiles<V_STATS>(g, p, a.n, 1, st));
     }
+    if (few) a.x = nullptr;   // rows stay where they are
     if (a.loss && a.n <= 1024) a.done = &reinterpret_cast<VocabHead*>(base + p.head)->done;
     if (a.t_index && a.k > 16) hipLaunchKernelGGL(vocab_distill_kernel<4>, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
     else if (a.t_index) hipLaunchKernelGGL(vocab_distill_kernel<1>, dim3((a.n + 3) / 4), dim3(256), 0, st, a, part, g.n_part);
@@ -1041,7 +1119,8 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     a.piece_tiles[0] = (int32_t)(p.piece / 256);
     a.piece_tiles[1] = (int32_t)((a.vocab - (p.pieces - 1) * p.piece + 255) / 256);
   }
-  TRY(gather_rows<true>(a, p, base, st));
+  bool few;
+  TRY(gather_rows<true>(a, p, base, few, st));
   VocabGemm g = {};
   g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
   g.scale2 = LOG2E * a.inv_t;
@@ -1065,7 +1144,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     g.accumulate = piece > 0;
     if (a.n > 0) {
       g.tiles_n = g.ldg / (p.large ? 256 : 128);
-      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_tiles<V_GRAD>(g, p, a.n, 1, st));
+      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : few ? launch_tile<V_GRAD, 64, 4, true>(g, 1, 1, st, a) : launch_tiles<V_GRAD>(g, p, a.n, 1, st));
       if (a.t_index) {
         hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
                            (a.fix && piece == 0) ? 1 : 0);

@@ -192,6 +192,27 @@ def test_strides_and_shapes(dtype):
     assert one.shape == () and torch.equal(one, row3.view(-1)[live][0])
 
 
+@pytest.mark.parametrize("n", [1, 30, 64, 100, 300])
+def test_row_strides_by_size(n):
+    """rows read in place (few), copied by aligned and by unaligned loads: the same bits from every layout"""
+    vocab, hidden = 500, 128
+    big = torch.randn(n, 3 * hidden, generator=torch.Generator().manual_seed(n)).to(BF16).cuda()
+    _, w, b = R.make(1, vocab, hidden, BF16, 2)
+    y = _labels(n, vocab, 3, 0.3)
+    values, index = _teacher(n, vocab, 5, 4, 0.2)
+    y[0] = 7
+    seen = []
+    for at in (0, 8, 3, 2 * hidden):
+        big2 = torch.zeros_like(big)
+        big2[:, at:at + hidden] = big[:, :hidden]
+        for h in (big2[:, at:at + hidden], big2[:, at:at + hidden].contiguous()):
+            leaves = [t.detach().requires_grad_() for t in (h, w, b)]
+            for loss in (losses.linear_cross_entropy(*leaves, y), losses.linear_distillation(*leaves, values, index)):
+                seen.append((loss.detach(), *torch.autograd.grad(loss, leaves)))
+    for i, got in enumerate(seen):
+        assert all(torch.equal(a, b) for a, b in zip(got, seen[i % 2])), i
+
+
 def test_gradients_of_some_inputs_only():
     h, w, b = R.make(70, 200, 64, BF16, 4)
     y = _labels(70, 200, 4)
