@@ -141,6 +141,8 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   bf16_t* x;
   float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
   float2* row_lc;           // distillation: (lse log2(e), c)
+  float2* row_fix;          // distillation: up to ROW_FIX (vocabulary id, what G's rounding left of its entry) per live row
+  bool low;                 // G's rows 64 .. 127 hold what the rounding of its rows 0 .. 63 left (few rows)
   int64_t* fix;
 };
 struct VocabGemm {          // arguments of vocab_gemm_kernel
@@ -157,13 +159,13 @@ struct VocabGemm {          // arguments of vocab_gemm_kernel
   float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: whole tiles, dh_partial_at)
   float* dw32;              // dW's partials where its k is split
   const VocabSchedule* schedule;
-  int32_t accumulate, with_dw, with_dh;   // (words: a byte among the arguments is no scalar load)
+  int32_t accumulate, with_dw, with_dh, low;   // (words: a byte among the arguments is no scalar load)
   bf16_t* out16; int64_t ldo;
   int32_t wide;             // out16's rows start on 16 bytes
   const float* out_scale;
 };
 struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
-  size_t head, row_map, block_base, state, t_p, t_logp, x, part, row_info, row_lc, fix, g, colsum, dh_part, dw_part, bytes;
+  size_t head, row_map, block_base, state, t_p, t_logp, x, part, row_info, row_lc, row_fix, fix, g, colsum, dh_part, dw_part, bytes;
   int64_t piece, pieces, ld_colsum, dh_slot, dh_room, dw_room;   // floats of one split's partials of dh, of all, and of dW's
   int32_t splits;         // at most
   bool large;             // 256 x 256 tiles (vocab8.hip)

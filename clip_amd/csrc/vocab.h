@@ -14,6 +14,7 @@ constexpr float G_SCALE = 1.f;       // bf16 has fp32's range
 #endif
 constexpr double FIX = 274877906944.0;   // 2^38: fixed-point unit of the target sums, |sum| <= 2^24 rows
 constexpr int FIX_COPIES = 8;            // copies of their table
+constexpr int ROW_FIX = 8;               // large entries of a row of G that dh is corrected for
 typedef __attribute__((ext_vector_type(4))) unsigned int u32x4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned int u32x2_t;
 

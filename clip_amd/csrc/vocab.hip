@@ -10,6 +10,10 @@
 // G = c (softmax - targets) of two products, dh += G W and dW = G^T h.  G holds c = g_i / max|g|, |c| <= 1, so that fp16's
 // range holds it (times 2^15 there: softmax values down to 2e-9 stay normal numbers); the factor is put back in fp32 when
 // the products are stored.
+// What G's rounding costs: most of a row's gradient sits in few entries (its targets), whose rounding errors do not average
+// out.  dh gets them back in fp32: the residuals of a row's largest entries times their rows of W, added where the partials are
+// joined.  dW of few rows (at most 64) is a product of G's high AND low parts, k twice as long under an output that is the
+// bound; with more rows its errors average out like those of the operands.
 // Rows that take no part (ignored label, empty teacher list) are dropped first: the live rows are copied side by side, so
 // their products cost nothing and whatever a dropped row holds (NaN included) reaches no gradient.
 #include <type_traits>
@@ -222,6 +226,7 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
       if (GRAD) info[rank] = row_info_of(a, lane, st, gm, lc);
       if (blockIdx.x == 0) {
         a.row_map[rank] = st == 2 ? ~lane : lane;
+        if (GRAD) a.row_info[rank] = info[rank];
         if (GRAD && a.state) a.row_lc[rank] = lc;
       }
     } else if (!GRAD && blockIdx.x == 0 && lane < a.n) {
@@ -235,9 +240,11 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
     // dW reads the rows k by k: side by side, and zeros up to 64
     for (int q = blockIdx.x * 4 + w; q < 64; q += groups * 4) {
       const int r = map[q];
-      for (int c = lane * 8; c < a.hidden; c += 512)
-        *reinterpret_cast<uint4*>(a.x + (int64_t)q * a.hidden + c) =
-            r < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(a.h + (int64_t)r * a.ldh + c);
+      for (int c = lane * 8; c < a.hidden; c += 512) {   // twice: beside G's high and its low part
+        const uint4 v = r < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(a.h + (int64_t)r * a.ldh + c);
+        *reinterpret_cast<uint4*>(a.x + (int64_t)q * a.hidden + c) = v;
+        *reinterpret_cast<uint4*>(a.x + (int64_t)(q + 64) * a.hidden + c) = v;
+      }
       if (a.dh && q < a.n && !(live >> q & 1))
         for (int c = lane; c < a.hidden; c += 64) a.dh[(int64_t)q * a.ld_dh + c] = 0;
     }
@@ -248,6 +255,12 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
 }
 
 struct NoRows {};
+
+// what rounding to the operand type leaves of x (0 of what is not finite)
+__device__ __forceinline__ float residual(float x) {
+  const float r = x - op_to_f32(f32_to_op(x));
+  return fabsf(r) < INFINITY ? r : 0.f;
+}
 
 // waits until at most `n` of this wave's loads are in flight
 template <int N>
@@ -300,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
     const int64_t v0 = a.v0 + (int64_t)kt0 * BK;
     ob.init(a.w + v0 * a.ldw + tn * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - tn * BN) * 2, a.ldw, w, lane);
   } else {
-    nt = (count + BK - 1) / BK;
+    nt = (count + BK - 1) / BK * (a.low ? 2 : 1);
     oa.init(a.g + (int64_t)tm * BM, ((int64_t)nt * BK * a.ldg - (int64_t)tm * BM) * 2, a.ldg, w, lane);
     ob.init(a.x + tn * BN, ((int64_t)nt * BK * a.hidden - tn * BN) * 2, a.hidden, w, lane);
   }
@@ -393,6 +406,7 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
       const int r = row0 + m * 16;
       const float4 ri = FEW ? info_s[r & 63] : a.row_info[r];
       const int at = __float_as_int(ri.z) - (int)a.v0 - col0;   // the label, counted from this lane's first column
+      float low[NB][4];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float g[4];
@@ -402,10 +416,20 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
           cs[n][e] += g[e];
         }
         put(n, make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3])));
+        if (FEW) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) low[n][e] = residual(g[e]);
+        }
       }
-      flush([&](int row, int c, const u32x4_t& v) {
+      auto store = [&](int row, int c, const u32x4_t& v) {
         *reinterpret_cast<u32x4_t*>(a.g + (int64_t)(row0 - fr + m * 16 + row) * a.ldg + tn * BN + wn * 64 + c) = v;
-      });
+      };
+      flush(store);
+      if (FEW) {   // G's rows 64 .. 127
+#pragma unroll
+        for (int n = 0; n < NB; ++n) put(n, make_uint2(pack_op2(low[n][0], low[n][1]), pack_op2(low[n][2], low[n][3])));
+        flush([&](int row, int c, const u32x4_t& v) { store(row + 64, c, v); });
+      }
     }
     if (a.colsum) {   // fp32 column sums of what was rounded above: db is not made of rounded values
 #pragma unroll
@@ -620,6 +644,11 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab * FIX_COPIES; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
 }
 
+// few rows that 16-byte loads with 31-bit offsets cannot read where they are, a row a workgroup
+__global__ __launch_bounds__(256) void vocab_copy_kernel(const bf16_t* __restrict__ from, int64_t ld, bf16_t* __restrict__ to, int hidden) {
+  for (int c = threadIdx.x; c < hidden; c += 256) to[(int64_t)blockIdx.x * hidden + c] = from[blockIdx.x * ld + c];
+}
+
 // eight products of 16-bit operands in fp32, added to s
 __device__ __forceinline__ float dot8(const uint4& x, const uint4& w, float s) {
   const uint32_t* xp = reinterpret_cast<const uint32_t*>(&x);
@@ -805,7 +834,10 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= *a.count) return;
   const int row = a.row_map[r];
-  if (row < 0) return;
+  if (row < 0) {   // (a row of NaN: nothing to correct)
+    if (table && lane < ROW_FIX) a.row_fix[(int64_t)r * ROW_FIX + lane] = make_float2(__int_as_float(-1), 0.f);
+    return;
+  }
   const float2 lc = a.row_lc[r];
   const int64_t* index = a.t_index + (int64_t)row * a.ld_ti;
   const float* tp = a.t_p + (int64_t)row * a.k;
@@ -815,9 +847,10 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
     v = t >= 0 && t < a.vocab ? (int)t : -1;
     p = j < a.k ? tp[j] : 0.f;
   };
+  int fixed = 0;   // entries noted for dh
   for (int j0 = 0; j0 < a.k; j0 += 64) {
     const int j = j0 + lane;
-    int v;
+    int v, earlier = 0;
     float own, p = 0.f;
     entry(j, v, own);
     for (int i0 = 0; i0 < a.k; i0 += 64) {   // every entry that names v
@@ -829,15 +862,25 @@ __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf
         const int ui = __builtin_amdgcn_readlane(u, i);
         const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
         p += ui == v ? qi : 0.f;
+        earlier += ui == v && i0 + i < j;
       }
     }
-    if (v < 0) continue;
-    if (table && fabsf(lc.y * own) <= 1.f)
+    if (a.fix && table && v >= 0 && fabsf(lc.y * own) <= 1.f)
       atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
-    if (v < v0 || v >= v1) continue;
-    const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
-    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(lc.y * (q - p) * G_SCALE);
+    const float q = v < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
+    const float e = lc.y * (q - p) * G_SCALE;
+    if (v >= v0 && v < v1) {
+      g[(int64_t)r * ldg + (v - v0)] = f32_to_op(e);
+      if (a.low) g[(int64_t)(r + 64) * ldg + (v - v0)] = f32_to_op(residual(e));
+    }
+    if (table && a.dh) {   // the first ROW_FIX entries of a sixteenth or more of the row (of an id named twice: the first)
+      const unsigned long long big = __ballot(v >= 0 && earlier == 0 && fabsf(q - p) >= 0.0625f);
+      const int at = fixed + __popcll(big & ((1ull << lane) - 1));
+      if ((big >> lane & 1) && at < ROW_FIX) a.row_fix[(int64_t)r * ROW_FIX + at] = make_float2(__int_as_float(v), residual(e));
+      fixed += __popcll(big);
+    }
   }
+  if (table && a.dh && lane < ROW_FIX && lane >= fixed) a.row_fix[(int64_t)r * ROW_FIX + lane] = make_float2(__int_as_float(-1), 0.f);
 }
 
 // dh of the live rows from the fp32 partials (fixed order), and db from the column sums and the targets' table
@@ -846,9 +889,9 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
                                                            bf16_t* __restrict__ dw, int64_t ld_dw, int row_blocks, int dw_blocks) {
   const int count = *a.count;
   const int b_blocks = gridDim.x - row_blocks - dw_blocks;
-  // the sum of n slots' partials, four of them in flight, in order; times the common factor, rounded
+  // the sum of n slots' partials, four of them in flight, in order; rounded: times the common factor
   const float s = a.out_scale[0];
-  auto sum_slots = [&](const float* q, int n, int64_t slot) -> uint2 {
+  auto sum_slots = [&](const float* q, int n, int64_t slot) -> f32x4_t {
     f32x4_t v = {0.f, 0.f, 0.f, 0.f};
     int k = 0;
     for (; k + 4 <= n; k += 4) {
@@ -859,8 +902,9 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
       for (int u = 0; u < 4; ++u) v += t[u];
     }
     for (; k < n; ++k) v += *reinterpret_cast<const f32x4_t*>(q + k * slot);
-    return make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s));
+    return v;
   };
+  auto rounded = [&](const f32x4_t& v) { return make_uint2(pack_op2(v[0] * s, v[1] * s), pack_op2(v[2] * s, v[3] * s)); };
   if ((int)blockIdx.x >= b_blocks + dw_blocks) {
     const int n = a.schedule[0].dh_splits;
     const int tiles_r = (count + 255) >> 8, h4 = a.hidden / 4;
@@ -878,7 +922,24 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
         r = (int)(i / h4);
         c = (int)(i - (int64_t)r * h4) * 4;
       }
-      const uint2 packed = sum_slots(part + i * 4, n, slot);
+      f32x4_t v = sum_slots(part + i * 4, n, slot);
+      // what G's rounding left of the row's largest entries
+      auto correct = [&](int id, float rest) {
+        const uint2 wv = *reinterpret_cast<const uint2*>(a.w + (int64_t)id * a.ldw + c);
+        v[0] = fmaf(rest, op2_lo(wv.x), v[0]); v[1] = fmaf(rest, op2_hi(wv.x), v[1]);
+        v[2] = fmaf(rest, op2_lo(wv.y), v[2]); v[3] = fmaf(rest, op2_hi(wv.y), v[3]);
+      };
+      if (a.row_fix) {
+        for (int k = 0; k < ROW_FIX; ++k) {
+          const float2 f = a.row_fix[(int64_t)r * ROW_FIX + k];
+          if (__float_as_int(f.x) < 0) break;
+          correct(__float_as_int(f.x), f.y);
+        }
+      } else {
+        const float4 ri = a.row_info[r];
+        if (__float_as_int(ri.z) >= 0) correct(__float_as_int(ri.z), residual(ri.w));
+      }
+      const uint2 packed = rounded(v);
       const int m = a.row_map[r];
       bf16_t* o = a.dh + (int64_t)(m < 0 ? ~m : m) * a.ld_dh + c;
       if (a.dh_aligned) {
@@ -897,7 +958,7 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
       dh_partial_at((int)(i & 16383), r, c);
       const int64_t v = (int64_t)(tile / a.tiles_h) * 256 + r;
       c += tile % a.tiles_h * 256;
-      if (v < a.vocab && c < a.hidden) *reinterpret_cast<uint2*>(dw + v * ld_dw + c) = sum_slots(dw_part + i * 4, n, (int64_t)tiles * 65536);
+      if (v < a.vocab && c < a.hidden) *reinterpret_cast<uint2*>(dw + v * ld_dw + c) = rounded(sum_slots(dw_part + i * 4, n, (int64_t)tiles * 65536));
     }
   } else {
     const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -984,6 +1045,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     p.row_info = take(rows * 16);
     if (distill) {
       p.row_lc = take(rows * 8);
+      p.row_fix = take(rows * 8 * ROW_FIX);
       p.fix = take(vocab * 8 * FIX_COPIES);
     }
     // a piece: whole 256-column tiles, G within its bound, 32-bit byte offsets into the piece of W
@@ -1051,8 +1113,17 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
     }
   }
   // few rows, read in place by the product kernel (16-byte loads, 31-bit offsets): no kernel of their own
-  few = p.tile_rows == 64 && a.n > 0 && a.h_aligned && ((int64_t)(a.n - 1) * a.ldh + a.hidden) * 2 < (1ll << 31);
-  if (few) return hipSuccess;
+  few = p.tile_rows == 64 && a.n > 0;
+  if (few) {
+    if (!a.h_aligned || ((int64_t)(a.n - 1) * a.ldh + a.hidden) * 2 >= (1ll << 31)) {   // ... but these, copied to where they can be
+      bf16_t* to = a.x + (int64_t)128 * a.hidden;   // (x has room for 256 rows, of which the products of few rows use 128)
+      hipLaunchKernelGGL(vocab_copy_kernel, dim3(a.n), dim3(256), 0, st, a.h, a.ldh, to, a.hidden);
+      TRY(hipGetLastError());
+      a.h = to;
+      a.ldh = a.hidden;
+    }
+    return hipSuccess;
+  }
   if (a.n > 1024) {   // more rows than a workgroup of the next kernel should count for itself
     a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
     hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
@@ -1105,6 +1176,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   a.row_info = reinterpret_cast<float4*>(base + p.row_info);
   if (a.t_index) {
     a.row_lc = reinterpret_cast<float2*>(base + p.row_lc);
+    a.row_fix = reinterpret_cast<float2*>(base + p.row_fix);
     a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
   }
   a.with_dw = dw != nullptr;
@@ -1121,6 +1193,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   }
   bool few;
   TRY(gather_rows<true>(a, p, base, few, st));
+  a.low = few;
   VocabGemm g = {};
   g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
   g.scale2 = LOG2E * a.inv_t;
@@ -1135,6 +1208,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.wide = ((uintptr_t)dw & 15) == 0 && ld_dw % 8 == 0;
   g.out_scale = a.out_scale;
   g.with_dw = dw != nullptr;
+  g.low = few;
   g.with_dh = a.dh && a.n > 0;
   for (int64_t v0 = 0, piece = 0; v0 < a.vocab; v0 += p.piece, ++piece) {
     const int64_t v1 = v0 + p.piece < a.vocab ? v0 + p.piece : a.vocab;
@@ -1147,7 +1221,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
       TRY(p.large ? launch_vocab8(V_GRAD, g, st) : few ? launch_tile<V_GRAD, 64, 4, true>(g, 1, 1, st, a) : launch_tiles<V_GRAD>(g, p, a.n, 1, st));
       if (a.t_index) {
         hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
-                           (a.fix && piece == 0) ? 1 : 0);
+                           piece == 0 ? 1 : 0);
         TRY(hipGetLastError());
       }
     }

@@ -205,8 +205,10 @@ int clip_linear_ce(const clip_linear* d, const int64_t* dev_labels, int64_t igno
 /* Gradients of the same loss: dz_i = g_i (softmax(z_i) - onehot(labels[i])), dhidden = dz weight, dweight = dz^T hidden,
  * dbias = column sums of dz; g_i = dev_grad[i] for reduction 0, dev_grad[0] / count for 1, dev_grad[0] for 2 (fp32).  Ignored
  * rows get zero dhidden rows and reach nothing else, whatever they hold.  Any of the three outputs may be NULL.  dz is rounded
- * once to the operand type for the two products (relative, 2^-9 or 2^-12); dbias is summed from unrounded values.  dweight
- * must be 8-byte aligned with a row stride that is a multiple of 4.  Every call that asks for the same outputs gives the same bits. */
+ * once to the operand type for the two products (relative, 2^-8 or 2^-11), but the label's entry reaches dhidden with the
+ * rounding's residual added back, calls of at most 64 rows form dweight from two such parts of dz, and dbias is summed from
+ * unrounded values.  dweight must be 8-byte aligned with a row stride that is a multiple of 4.  Every call that asks for the
+ * same outputs gives the same bits. */
 int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t ignore_index, int32_t reduction,
                         const float* dev_lse, const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden,
                         int64_t ld_dhidden, uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,
@@ -220,7 +222,7 @@ int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t
 int clip_linear_distill(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index, int32_t k,
                         float temperature, int32_t reduction, float* dev_row_loss, float* dev_lse, float* dev_target,
                         float* dev_loss, void* dev_work, int64_t work_bytes, void* stream);
-/* Its gradients, dz_i = g_i T (q_i - p_i), as clip_linear_ce_grad. */
+/* Its gradients, dz_i = g_i T (q_i - p_i), as clip_linear_ce_grad (residuals for the teacher's ids with |q - p| >= 1/16). */
 int clip_linear_distill_grad(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index,
                              int32_t k, float temperature, int32_t reduction, const float* dev_lse,
                              const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden, int64_t ld_dhidden,

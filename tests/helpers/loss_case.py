@@ -37,9 +37,10 @@ def targets_distill(values, index, vocab, temperature):
     return p, live, entropy
 
 
-def reference(h, w, b, p, live, temperature, row_grad, entropy=None):
+def reference(h, w, b, p, live, temperature, row_grad, entropy=None, rounded_h=1.0, rounded_w=1.0):
     """Row losses, (dh, dw, db) for upstream row gradients, and bounds on the kernels' errors: every rounding counted
-    once at its half step, fp32 sums of m terms at m half steps of the sum of magnitudes."""
+    once at its half step, fp32 sums of m terms at m half steps of the sum of magnitudes.  rounded_h, rounded_w: how many half
+    steps the score gradients lose on their way into dh and into dw (each a number or [n, vocab])."""
     hd, wd = h.double(), w.double()
     hd = torch.where(live[:, None], hd, 0.0)
     zero = torch.zeros(w.shape[0], dtype=torch.float64, device=w.device)
@@ -62,10 +63,10 @@ def reference(h, w, b, p, live, temperature, row_grad, entropy=None):
     # q's relative error: its exponent's, exp2 (2 half steps), the sum of a row's exponentials (vocab terms, tree of 64s)
     rel = 2 * z_err + (16 + vocab / 64) * F32
     size = g.abs() * (q + p)
-    dz_err = u * dz.abs() + rel[:, None] * size + 2.0 ** -39 * g.abs().max().clamp(min=1e-300) * (q > 0)
+    dz_err = rel[:, None] * size + 2.0 ** -39 * g.abs().max().clamp(min=1e-300) * (q > 0)
     dh, dw, db = dz @ wd, dz.t() @ hd, dz.sum(0)
-    dh_err = dz_err @ wd.abs() + vocab * F32 * (size @ wd.abs()) + u * dh.abs() * 1.01 + TINY[h.dtype]
-    dw_err = dz_err.t() @ hd.abs() + n * F32 * (size.t() @ hd.abs()) + u * dw.abs() * 1.01 + TINY[h.dtype]
+    dh_err = (dz_err + u * rounded_h * dz.abs()) @ wd.abs() + vocab * F32 * (size @ wd.abs()) + u * dh.abs() * 1.01 + TINY[h.dtype]
+    dw_err = (dz_err + u * rounded_w * dz.abs()).t() @ hd.abs() + n * F32 * (size.t() @ hd.abs()) + u * dw.abs() * 1.01 + TINY[h.dtype]
     db_err = (rel[:, None] * size).sum(0) + (n + 4) * F32 * size.sum(0) + n * 2.0 ** -38 * g.abs().max()
     return (loss, dh, dw, db), (loss_err, dh_err, dw_err, db_err)
 

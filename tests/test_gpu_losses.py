@@ -213,6 +213,37 @@ def test_row_strides_by_size(n):
         assert all(torch.equal(a, b) for a, b in zip(got, seen[i % 2])), i
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("distill", [False, True])
+@pytest.mark.parametrize("n", [1, 40, 64, 100, 700])
+def test_what_the_rounded_score_gradients_leave_is_put_back(n, distill, dtype):
+    """The large entries of a row reach dhidden unrounded; dweight of at most 64 rows is made of high and low parts, whose
+    product is off by the square of a half step."""
+    vocab, hidden = 600, 128
+    h, w, b = R.make(n, vocab, hidden, dtype, n)
+    w[2:] = 0                                     # the targets, each in columns of its own
+    w[0, 64:] = 0
+    w[1, :64] = 0
+    up = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
+    if distill:
+        values, index = torch.tensor([[1.0, 0.5]]).cuda().expand(n, 2), torch.tensor([[0, 1]]).cuda().expand(n, 2)
+        p, live, entropy = R.targets_distill(values, index, vocab, 1.0)
+    else:
+        y = torch.arange(n).cuda() % 2
+        (p, live), entropy = R.targets_ce(y, vocab, -100), None
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = (losses.linear_distillation(*leaves, values, index, reduction="none") if distill else
+            losses.linear_cross_entropy(*leaves, y, reduction="none"))
+    dh, dw, _ = torch.autograd.grad(loss, leaves, up)
+    q = torch.softmax(h.double() @ w.double().t() + b.double(), 1)
+    large = (q - p).abs() >= 0.07 if distill else p > 0          # (a sixteenth, and away from it)
+    u = R.half_step(dtype)
+    (_, want_h, want_w, _), (_, e_h, e_w, _) = R.reference(h, w, b, p, live, 1.0, up, entropy, rounded_h=~large * 1.0,
+                                                          rounded_w=u if n <= 64 else 1.0)
+    R.assert_within("dh", dh, want_h, e_h)
+    R.assert_within("dw", dw, want_w, e_w)
+
+
 def test_gradients_of_some_inputs_only():
     h, w, b = R.make(70, 200, 64, BF16, 4)
     y = _labels(70, 200, 4)
