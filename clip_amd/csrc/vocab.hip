@@ -159,6 +159,7 @@ __device__ __forceinline__ int row_state(const VocabRows& a, int r) {
   const int64_t y = a.labels[r];
   return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
 }
+__device__ __forceinline__ bool taking_part(const VocabRows& a, int r) { return a.state ? a.state[r] != 0 : a.labels[r] != a.ignore; }
 __device__ __forceinline__ float finite_abs(float g) {
   g = fabsf(g);
   return g < INFINITY ? g : 0.f;
@@ -277,14 +278,14 @@ __device__ __forceinline__ void wait_loads() {
 // small tiles and a deep ring, the weight's bytes are the bound; vocab8.hip takes the large calls).
 // FEW: calls of at most 64 rows, whose live rows this kernel finds and reads in place (gather_few).
 template <int EPI, int BM, int BN, int WM, int WN, int NST, bool FEW>
-__global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, std::conditional_t<FEW, VocabRows, NoRows> rows) {
+__device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::conditional_t<FEW, VocabRows, NoRows>& rows, char* smem, int tn,
+                                           int tm, int split, int splits) {
   constexpr int NW = WM * WN, MB = BM / WM / 16, NB = BN / WN / 16;
   static_assert(NB == 4, "64 columns per wave");
   constexpr bool A_TR = EPI == V_DW, B_TR = EPI == V_DH || EPI == V_DW;
   typedef Operand<BM, A_TR, NW> OA;
   typedef Operand<BN, B_TR, NW> OB;
-  constexpr int STAGE = OA::BYTES + OB::BYTES;
-  extern __shared__ __attribute__((aligned(16))) char smem[];   // NST * STAGE
+  constexpr int STAGE = OA::BYTES + OB::BYTES;   // of NST in smem
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WN, wn = w % WN, fr = lane & 15, fq = lane >> 4;
@@ -293,7 +294,6 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
   int count;                                        // live rows
   if constexpr (FEW) count = gather_few<EPI == V_GRAD>(rows, a.v0 == 0, map_s, info_s);
   else count = *a.count;
-  const int tn = blockIdx.x % a.tiles_n, tm = blockIdx.x / a.tiles_n, split = blockIdx.y;
   if (EPI != V_DW && tm * BM >= count) return;      // workgroup-uniform
 
   int nt, kt0 = 0;
@@ -307,8 +307,8 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
     ob.init(a.w + v0 * a.ldw, ((a.vocab - 1 - v0) * a.ldw + a.hidden) * 2, a.ldw, w, lane);
   } else if (EPI == V_DH) {
     const int all = a.ldg / BK;
-    kt0 = (int)((int64_t)all * split / gridDim.y);
-    nt = (int)((int64_t)all * (split + 1) / gridDim.y) - kt0;
+    kt0 = (int)((int64_t)all * split / splits);
+    nt = (int)((int64_t)all * (split + 1) / splits) - kt0;
     oa.init(a.g + (int64_t)tm * BM * a.ldg + (int64_t)kt0 * BK, (int64_t)BM * a.ldg * 2, a.ldg, w, lane);
     const int64_t v0 = a.v0 + (int64_t)kt0 * BK;
     ob.init(a.w + v0 * a.ldw + tn * BN, ((a.vocab - 1 - v0) * a.ldw + a.hidden - tn * BN) * 2, a.ldw, w, lane);
@@ -466,6 +466,26 @@ __global__ __launch_bounds__(64 * WM * WN) void vocab_gemm_kernel(VocabGemm a, s
   }
 }
 
+// scores (V_STATS, V_GRAD): a tile per workgroup
+template <int EPI, int BM, int NST, bool FEW>
+__global__ __launch_bounds__(256) void vocab_scores_kernel(VocabGemm a, std::conditional_t<FEW, VocabRows, NoRows> rows) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  vocab_tile<EPI, BM, 128, 2, 2, NST, FEW>(a, rows, smem, blockIdx.x % a.tiles_n, blockIdx.x / a.tiles_n, 0, 1);
+}
+// Both products with G in one launch, which need nothing of each other: dh's tiles of BM rows first (few, with a long k in
+// `splits` parts), then dW's of 128 vocabulary entries.  Rings short enough that a CU holds a workgroup of each.
+template <int BM, int NST>
+__global__ __launch_bounds__(256) void vocab_products_kernel(VocabGemm a, int tiles_m, int splits) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int id = blockIdx.x, tiles = tiles_m * a.tiles_n, n_dh = tiles * splits;
+  if (id < n_dh) {
+    const int split = id / tiles, t = id - split * tiles;
+    vocab_tile<V_DH, BM, 128, 2, 2, NST, false>(a, {}, smem, t % a.tiles_n, t / a.tiles_n, split, splits);
+  } else {
+    vocab_tile<V_DW, 128, 128, 2, 2, 2, false>(a, {}, smem, (id - n_dh) % a.tiles_n, (id - n_dh) / a.tiles_n, 0, 1);
+  }
+}
+
 // Teacher lists of a distillation: p = softmax(values / T) over a row's entries with index >= 0 and a value above -inf
 // (0 elsewhere), log_p beside it, state[row] = 0 no entry, 1 live, 2 an index beyond the vocabulary or a value that is
 // NaN or +inf.  One wave per row.
@@ -516,7 +536,7 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {   // (no branches: all loads in flight)
       const int q = min(r + i, a.n - 1);
-      s[i] = a.state ? a.state[q] != 0 : a.labels[q] != a.ignore;
+      s[i] = taking_part(a, q);
     }
 #pragma unroll
     for (int i = 0; i < 16; ++i) live += r + i < a.n ? s[i] : 0;
@@ -579,11 +599,24 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     if (GRAD) gm = *a.grad_max;
   } else {
     before = total = 0;
-    for (int r = tid; r < a.n; r += 256) {
-      const int live = row_state(a, r) != 0;
-      total += live;
-      before += live && r < r0;
-      if (GRAD && a.grad_rows && live) gm = fmaxf(gm, finite_abs(a.grad[r]));
+    for (int q0 = 0; q0 < a.n; q0 += 256 * 8) {   // eight loads in flight
+      int s[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int q = q0 + i * 256 + tid;
+        s[i] = q0 + i * 256 < a.n ? (q < a.n) & (int)taking_part(a, min(q, a.n - 1)) : 0;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        total += s[i];
+        before += q0 + i * 256 + tid < r0 ? s[i] : 0;
+      }
+      if (GRAD && a.grad_rows)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float g = finite_abs(a.grad[min(q0 + i * 256 + tid, a.n - 1)]);
+          if (s[i]) gm = fmaxf(gm, g);
+        }
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
@@ -985,24 +1018,29 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
   }
 }
 
-// up to 64 rows: 64-row tiles of scores, of dh and (its k) of dW, rings 3 K tiles ahead; more: 128-row tiles
-template <int EPI, int BM, int NST, bool FEW = false>
-hipError_t launch_tile(const VocabGemm& g, int tiles_m, int splits, hipStream_t st, const std::conditional_t<FEW, VocabRows, NoRows>& rows = {}) {
-  constexpr int BN = 128, lds = NST * (BM + BN) * BK * 2;
-  auto kfn = vocab_gemm_kernel<EPI, BM, BN, 2, 2, NST, FEW>;
+template <auto KERNEL, typename... Args>
+hipError_t launch_tiles(int lds, int64_t groups, hipStream_t st, const Args&... args) {
   static DeviceOnce once;
   int unused;
   TRY(once.get([&](int, int*) {
-    return hipFuncSetAttribute(reinterpret_cast<const void*>(kfn), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    return hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   }, &unused));
-  hipLaunchKernelGGL(kfn, dim3(tiles_m * g.tiles_n, splits), dim3(256), lds, st, g, rows);
+  hipLaunchKernelGGL(KERNEL, dim3((uint32_t)groups), dim3(256), lds, st, args...);
   return hipGetLastError();
 }
+// up to 64 rows: 64-row tiles of scores and dh, (its k) of dW; more: 128-row tiles
+constexpr int ring_bytes(int rows, int stages) { return stages * (rows + 128) * BK * 2; }
 template <int EPI>
-hipError_t launch_tiles(const VocabGemm& g, const VocabPlan& p, int64_t m, int splits, hipStream_t st) {
-  if (EPI == V_DW) return launch_tile<V_DW, 128, 2>(g, (int)((m + 127) / 128), splits, st);
-  return p.tile_rows == 64 ? launch_tile<EPI, 64, 4>(g, (int)((m + 63) / 64), splits, st)
-                           : launch_tile<EPI, 128, 3>(g, (int)((m + 127) / 128), splits, st);
+hipError_t launch_scores(const VocabGemm& g, const VocabRows& a, bool few, hipStream_t st) {
+  if (few) return launch_tiles<vocab_scores_kernel<EPI, 64, 4, true>>(ring_bytes(64, 4), g.tiles_n, st, g, a);
+  return launch_tiles<vocab_scores_kernel<EPI, 128, 3, false>>(ring_bytes(128, 3), (a.n + 127) / 128 * (int64_t)g.tiles_n, st, g, NoRows());
+}
+hipError_t launch_products(const VocabGemm& g, const VocabPlan& p, int n, hipStream_t st) {
+  const int tiles_m = g.with_dh ? (n + p.tile_rows - 1) / p.tile_rows : 0;
+  const int64_t groups = (int64_t)g.tiles_n * (tiles_m * p.splits + (g.with_dw ? g.ldg / 128 : 0));
+  if (groups == 0) return hipSuccess;
+  return p.tile_rows == 64 ? launch_tiles<vocab_products_kernel<64, 3>>(ring_bytes(64, 3), groups, st, g, tiles_m, (int)p.splits)
+                           : launch_tiles<vocab_products_kernel<128, 2>>(ring_bytes(128, 2), groups, st, g, tiles_m, (int)p.splits);
 }
 
 }  // namespace
@@ -1010,13 +1048,16 @@ hipError_t launch_tiles(const VocabGemm& g, const VocabPlan& p, int64_t m, int s
 #if !CLIP_OPERAND_F16
 // G of one piece of the vocabulary may take this much: the pieces are as few as that allows
 constexpr int64_t G_BYTES = 1ll << 30;
-// Which calls run on the 256 x 256 tiles of vocab8.hip.  Loss and gradients in us, these tiles against the small ones:
-//   V 30 522, H 768: n 65 120 / 94, 128 114 / 94, 160 118 / 133, 256 114 / 135;   V 8 000, H 256: n 160 71 / 55, 256 68 / 58
-// so up to 128 rows never, up to 256 where the weight has the tiles to fill most CUs, beyond that always (the small tiles read
-// W once per 128 rows)
+// Which calls run on the 256 x 256 tiles of vocab8.hip.  Loss and gradients in us, these tiles / the small ones, and how many
+// 256^3 blocks the call has (rows x vocabulary x hidden):
+//   H 768, V 30 522: n 128 110 / 88, 160 (360) 117 / 125, 257 (720) 130 / 168, 2048 386 / 630
+//   H 768, V 8 000: n 512 (192) 96 / 84, 768 (288) 104 / 114, 2048 151 / 196;   V 2 000: n 2048 (192) 112 / 89
+//   H 256, V 8 000: n 512 (64) 75 / 58, 1024 (128) 88 / 81, 2048 (256) 100 / 120;   V 2 000: n 2048 (64) 83 / 74
+//   H 128, V 30 522: n 257 (240) 91 / 82, 400 (240) 86 / 92, 512 (240) 86 / 93, 1024 116 / 146
+// so up to 128 rows never (the small tiles read W once per 128 rows), then from about as many blocks as there are CUs
 bool large_tiles(int32_t n, int64_t vocab, int32_t hidden) {
   if (hidden % 128 || n <= 128) return false;
-  return n > 256 || (vocab + 255) / 256 * ((hidden + 255) / 256) >= 192;
+  return ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
 }
 
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {
@@ -1124,7 +1165,9 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
     }
     return hipSuccess;
   }
-  if (a.n > 1024) {   // more rows than a workgroup of the next kernel should count for itself
+  // more rows than a workgroup of the next kernel should count for itself (a forward of 15 % live rows, us, counting here / there:
+  // n 1100 22.8 / 19.9, 2048 23.3 / 20.5, 4096 24.6 / 22.4, 8192 28.0 / 27.4, 16384 36.6 / 44.9)
+  if (a.n > 4096) {
     a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
     hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());
@@ -1154,9 +1197,11 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
       TRY(launch_vocab8(V_STATS, g, st));
     } else {
       g.tiles_n = g.n_part / 2;
-      TRY(few ? launch_tile<V_STATS, 64, 4, true>(g, 1, 1, st, a) : launch_tiles<V_STATS>(g, p, a.n, 1, st));
+      TRY(launch_scores<V_STATS>(g, a, few, st));
     }
     if (few) a.x = nullptr;   // rows stay where they are
+    // (a loss of 15 % live rows, us, summed by the last workgroup / by a kernel more: n 1100 23.8 / 24.8, 1500 24.9 / 24.9,
+    // 2048 27.0 / 25.4: every workgroup's count is an atomic on one word)
     if (a.loss && a.n <= 1024) a.done = &reinterpret_cast<VocabHead*>(base + p.head)->done;
     if (a.t_index && a.k > 16) hipLaunchKernelGGL(vocab_distill_kernel<4>, dim3(a.n), dim3(256), 0, st, a, part, g.n_part);
     else if (a.t_index) hipLaunchKernelGGL(vocab_distill_kernel<1>, dim3((a.n + 3) / 4), dim3(256), 0, st, a, part, g.n_part);
@@ -1218,7 +1263,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     g.accumulate = piece > 0;
     if (a.n > 0) {
       g.tiles_n = g.ldg / (p.large ? 256 : 128);
-      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : few ? launch_tile<V_GRAD, 64, 4, true>(g, 1, 1, st, a) : launch_tiles<V_GRAD>(g, p, a.n, 1, st));
+      TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_scores<V_GRAD>(g, a, few, st));
       if (a.t_index) {
         hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
                            piece == 0 ? 1 : 0);
@@ -1226,12 +1271,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
       }
     }
     g.tiles_n = a.tiles_h;
-    if (p.large) {
-      TRY(launch_vocab8(V_PROD, g, st));
-    } else {
-      if (g.with_dh) TRY(launch_tiles<V_DH>(g, p, a.n, p.splits, st));
-      if (g.with_dw) TRY(launch_tiles<V_DW>(g, p, g.ldg, 1, st));
-    }
+    TRY(p.large ? launch_vocab8(V_PROD, g, st) : launch_products(g, p, a.n, st));
   }
   const int row_blocks = g.with_dh ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
   const int b_blocks = a.dbias ? (int)((a.vocab + 255) / 256) : 0;

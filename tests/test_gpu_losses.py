@@ -62,7 +62,9 @@ def _check(h, w, b, run, p, live, temperature, reduction, seed, entropy=None):
 
 SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64, 128, 64), (65, 129, 192), (130, 777, 320),
          (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768), (2600, 1300, 128), (1500, 2500, 384),
-         (1030, 5, 1024), (70, 500, 2048), (300, 600, 1152), (130, 300, 8192)]
+         (1030, 5, 1024), (70, 500, 2048), (300, 600, 1152), (130, 300, 8192),
+         # large tiles: 240 blocks of 256^3
+         (257, 30700, 128), (129, 10300, 1408), (300, 9001, 1152), (1030, 4099, 1024), (2600, 8003, 128), (1500, 10001, 384), (20500, 700, 256)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -77,8 +79,9 @@ def test_cross_entropy_sizes(n, vocab, hidden, dtype):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("ignored", [0.0, 0.6, 0.97, 1.1])
-def test_cross_entropy_reductions_and_ignored_rows(dtype, reduction, ignored):
-    n, vocab, hidden = 401, 523, 128
+@pytest.mark.parametrize("vocab", [523, 30523])
+def test_cross_entropy_reductions_and_ignored_rows(vocab, dtype, reduction, ignored):
+    n, hidden = 401, 128
     h, w, b = R.make(n, vocab, hidden, dtype, 3)
     y = _labels(n, vocab, 4, ignored, ignore=-7)
     p, live = R.targets_ce(y, vocab, -7)
@@ -136,15 +139,15 @@ def test_without_bias_and_with_entries_left_out(dtype):
     assert losses.linear_cross_entropy(h, w, torch.full_like(b, -INF), y, reduction="none").isnan().all()
 
 
-def test_non_finite_rows_stay_in_their_rows():
-    n, vocab, hidden = 140, 300, 64
+@pytest.mark.parametrize("n,vocab,hidden", [(140, 300, 64), (300, 30800, 128), (50, 300, 64)])
+def test_non_finite_rows_stay_in_their_rows(n, vocab, hidden):
     h, w, b = R.make(n, vocab, hidden, BF16, 12)
-    h[5], h[77, 3] = NAN, INF
+    h[5], h[37, 3] = NAN, INF
     y = _labels(n, vocab, 13)
     y[9] = vocab                      # no such entry
     y[11] = -1
     bad = torch.zeros(n, dtype=torch.bool).cuda()
-    bad[[5, 77, 9, 11]] = True
+    bad[[5, 37, 9, 11]] = True
     leaves = [t.requires_grad_() for t in (h, w, b)]
     loss = losses.linear_cross_entropy(*leaves, y, reduction="none")
     assert torch.equal(loss.isnan(), bad)
@@ -192,10 +195,10 @@ def test_strides_and_shapes(dtype):
     assert one.shape == () and torch.equal(one, row3.view(-1)[live][0])
 
 
-@pytest.mark.parametrize("n", [1, 30, 64, 100, 300])
-def test_row_strides_by_size(n):
+@pytest.mark.parametrize("n,vocab", [(1, 500), (30, 500), (64, 500), (100, 500), (300, 500), (300, 31000), (1300, 31000)])
+def test_row_strides_by_size(n, vocab):
     """rows read in place (few), copied by aligned and by unaligned loads: the same bits from every layout"""
-    vocab, hidden = 500, 128
+    hidden = 128
     big = torch.randn(n, 3 * hidden, generator=torch.Generator().manual_seed(n)).to(BF16).cuda()
     _, w, b = R.make(1, vocab, hidden, BF16, 2)
     y = _labels(n, vocab, 3, 0.3)
@@ -215,11 +218,11 @@ def test_row_strides_by_size(n):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("distill", [False, True])
-@pytest.mark.parametrize("n", [1, 40, 64, 100, 700])
-def test_what_the_rounded_score_gradients_leave_is_put_back(n, distill, dtype):
+@pytest.mark.parametrize("n,vocab", [(1, 600), (40, 600), (64, 600), (100, 600), (700, 600), (700, 21000)])
+def test_what_the_rounded_score_gradients_leave_is_put_back(n, vocab, distill, dtype):
     """The large entries of a row reach dhidden unrounded; dweight of at most 64 rows is made of high and low parts, whose
     product is off by the square of a half step."""
-    vocab, hidden = 600, 128
+    hidden = 128
     h, w, b = R.make(n, vocab, hidden, dtype, n)
     w[2:] = 0                                     # the targets, each in columns of its own
     w[0, 64:] = 0
@@ -301,9 +304,9 @@ def test_loss_differences():
     assert abs(slope - (gb.double() * db_dir).sum()) <= n * step ** 2 / 6 * 8 + e_loss.sum() / step + e_b.sum()
 
 
-def test_vocabulary_in_several_pieces():
+@pytest.mark.parametrize("n,vocab,hidden", [(4500, 65537, 64), (4500, 120001, 128)])
+def test_vocabulary_in_several_pieces(n, vocab, hidden):
     # 16-bit score gradients of 4500 x 65 536 are beyond one piece's bound: the products run piece by piece
-    n, vocab, hidden = 4500, 65537, 64
     h, w, b = R.make(n, vocab, hidden, BF16, 77)
     y = _labels(n, vocab, 78, 0.01)
     y[0], y[1] = vocab - 1, 0
@@ -315,7 +318,8 @@ def test_vocabulary_in_several_pieces():
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("n,vocab,hidden,k,temperature", [
     (1, 1, 64, 1, 1.0), (1, 30, 64, 30, 2.0), (3, 65, 128, 7, 0.5), (70, 1000, 128, 64, 2.0), (130, 777, 320, 65, 4.0),
-    (33, 2000, 64, 200, 1.0), (300, 3001, 256, 16, 1.5), (9, 1500, 64, 1024, 3.0), (19, 30522, 768, 8, 1.0)])
+    (33, 2000, 64, 200, 1.0), (300, 3001, 256, 16, 1.5), (9, 1500, 64, 1024, 3.0), (19, 30522, 768, 8, 1.0),
+    (300, 30801, 128, 16, 1.5), (1100, 12345, 256, 100, 2.0)])
 def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
     h, w, b = R.make(n, vocab, hidden, dtype, n + k)
     values, index = _teacher(n, vocab, k, n)
@@ -326,28 +330,30 @@ def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
 
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_distillation_ragged_empty_and_repeated_entries(dtype, reduction):
-    n, vocab, hidden, k = 150, 400, 128, 12
+@pytest.mark.parametrize("n,vocab", [(150, 400), (300, 30800), (60, 400)])
+def test_distillation_ragged_empty_and_repeated_entries(n, vocab, dtype, reduction):
+    hidden, k = 128, 12
     h, w, b = R.make(n, vocab, hidden, dtype, 5)
     values, index = _teacher(n, vocab, k, 6, dropped=0.4)
-    index[[0, 17, 149]] = -1              # nothing listed
+    index[[0, 17, n - 1]] = -1            # nothing listed
     index[40] = -5
     values[41] = -INF
     values[42, 3:] = -INF
     values[43] = torch.finfo(F32).min     # the lowest finite value everywhere: a uniform teacher
     index[44, :5] = index[44, 5].clamp(min=0)   # one id several times
-    index[45] = 399
+    index[45] = vocab - 1
     p, live, entropy = R.targets_distill(values, index, vocab, 2.0)
-    assert not live[[0, 17, 149, 40, 41]].any()
+    assert not live[[0, 17, n - 1, 40, 41]].any()
     h[~live] = NAN
     _, grads = _check(h, w, b, lambda h, w, b: losses.linear_distillation(h, w, b, values, index, temperature=2.0, reduction=reduction),
                       p, live, 2.0, reduction, 9, entropy)
     assert not grads[0][~live].any()
 
 
-def test_distillation_of_bad_entries_is_nan():
-    n, vocab, k = 30, 100, 4
-    h, w, b = R.make(n, vocab, 64, BF16, 5)
+@pytest.mark.parametrize("n,vocab", [(30, 100), (100, 100), (300, 30800)])
+def test_distillation_of_bad_entries_is_nan(n, vocab):
+    k = 4
+    h, w, b = R.make(n, vocab, 128, BF16, 5)
     values, index = _teacher(n, vocab, k, 6)
     index[3, 1] = vocab
     values[4, 2] = NAN
@@ -447,9 +453,10 @@ def test_teacher_to_student_step():
         R.assert_within(name, got, x + y_, e + f + (u if name != "db" else R.F32) * 1.01 * (x + y_).abs())
 
 
-def test_other_stream():
-    h, w, b = R.make(500, 3000, 128, BF16, 60)
-    y = _labels(500, 3000, 61)
+@pytest.mark.parametrize("n,vocab", [(500, 3000), (500, 31000), (50, 3000)])
+def test_other_stream(n, vocab):
+    h, w, b = R.make(n, vocab, 128, BF16, 60)
+    y = _labels(n, vocab, 61)
     leaves = [t.requires_grad_() for t in (h, w, b)]
     want = torch.autograd.grad(losses.linear_cross_entropy(*leaves, y), leaves)
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
@@ -463,8 +470,9 @@ def test_other_stream():
         assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
-def test_captured_step_replays():
-    n, vocab, hidden = 90, 1111, 128
+@pytest.mark.parametrize("n,vocab", [(90, 1111), (50, 1111), (400, 31111), (4200, 4000)])
+def test_captured_step_replays(n, vocab):
+    hidden = 128
     h, w, b = R.make(n, vocab, hidden, BF16, 70)
     y = _labels(n, vocab, 71, 0.3)
     values, index = _teacher(n, vocab, 9, 72)
@@ -535,8 +543,8 @@ def test_backward_accumulates_and_repeats():
 
 
 @pytest.mark.parametrize("up", [0.0, -2.0, 65536.0, 1e-30])
-def test_upstream_gradients(up):
-    n, vocab = 90, 700
+@pytest.mark.parametrize("n,vocab", [(90, 700), (40, 700), (300, 30800)])
+def test_upstream_gradients(n, vocab, up):
     h, w, b = R.make(n, vocab, 128, BF16, 40)
     y = _labels(n, vocab, 41)
     p, live = R.targets_ce(y, vocab, -100)
@@ -569,7 +577,8 @@ def test_ignore_index_inside_the_vocabulary():
 
 # ---------------------------------------------------------------- the C ABI itself
 @pytest.mark.parametrize("n,vocab,hidden,ld_dh,ld_dw,k", [(50, 300, 64, 71, 68, 0), (100, 1000, 128, 128, 132, 5), (300, 1111, 128, 129, 136, 0),
-                                                          (700, 4000, 384, 384, 388, 70), (1500, 257, 128, 128, 128, 0)])
+                                                          (700, 4000, 384, 384, 388, 70), (1500, 257, 128, 128, 128, 0),
+                                                          (300, 31111, 128, 129, 136, 0), (700, 24001, 128, 128, 132, 70), (5000, 3300, 128, 128, 128, 0)])
 def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     """Row strides of the outputs, a workspace of exactly the size asked for and full of NaN, and untouched bytes around
     every output and behind the workspace; the same bits as the Python call."""
