@@ -8,6 +8,12 @@
 //  * epilogues: (max, sum of exp2) per row and 64 columns; the 16-bit score gradients with their column sums; fp32 partials;
 //    16-bit weight gradients;
 //  * dW tiles and dh tiles share one launch: either alone leaves a last round of workgroups mostly idle.
+// Bound: the matrix cores at the clock that the card's power limit leaves them (1.55 - 1.7 GHz in these loops, busy 68 % of the
+// cycles); 256 x 256 tiles because each byte that a CU takes in feeds twice the MFMAs that it does in a 128 x 128 tile (of which
+// two fit: 16 384 rows 4.6 ms instead of 2.7).  bf16, V 30 522, H 768, us (2 n V H, twice that for the pair; 1.29 PF is the rate
+// of a large library product):
+//   4096 rows:   scores 164 - 181 (1.06 - 1.17 PF), G 184 - 206 (0.93 - 1.04 PF; 250 MB leave it), dW + dh 342 - 389 (0.99 - 1.12 PF)
+//   16 384 rows: scores 612 - 647 (1.19 - 1.25 PF), G 686 - 724 (1.06 - 1.12 PF; 1 GB leaves it), dW + dh 1250 - 1306 (1.18 - 1.23 PF)
 #include "vocab.h"
 
 namespace {

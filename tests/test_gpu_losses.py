@@ -314,6 +314,29 @@ def test_vocabulary_in_several_pieces(n, vocab, hidden):
     _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y), p, live, 1.0, "mean", 5)
 
 
+@pytest.mark.parametrize("distill", [False, True])
+@pytest.mark.parametrize("n", [20, 100, 300])
+def test_few_rows_in_several_pieces(n, distill):
+    # rows of the weight so far apart that 32-bit byte offsets reach 256 of them
+    vocab, hidden, ld = 600, 128, 1 << 22
+    h, w, b = R.make(n, vocab, hidden, BF16, 79)
+    far = torch.empty(vocab, ld, dtype=BF16, device="cuda")[:, :hidden]
+    far.copy_(w)
+    if distill:
+        values, index = _teacher(n, vocab, 10, 80, 0.1)
+        p, live, entropy = R.targets_distill(values, index, vocab, 1.5)
+    else:
+        y = _labels(n, vocab, 80, 0.2)
+        (p, live), entropy = R.targets_ce(y, vocab, -100), None
+    leaves = [h.clone().requires_grad_(), far.requires_grad_(), b.clone().requires_grad_()]
+    loss = (losses.linear_distillation(*leaves, values, index, temperature=1.5, reduction="none") if distill else
+            losses.linear_cross_entropy(*leaves, y, reduction="none"))
+    grads = torch.autograd.grad(loss.sum(), leaves)
+    want, err = R.reference(h, w, b, p, live, 1.5 if distill else 1.0, torch.ones(n).cuda(), entropy)
+    for name, got, a, e in zip(("loss", "dh", "dw", "db"), (loss.detach(), *grads), want, err):
+        R.assert_within(name, got, a, e)
+
+
 # ---------------------------------------------------------------- distillation
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("n,vocab,hidden,k,temperature", [
