@@ -285,10 +285,14 @@ template <class T>
 hipError_t launch_t(const void* logits, int64_t ld, int n, int vocab, int k, void* values, int64_t* index, hipStream_t st) {
   const auto* in = static_cast<const typename T::elem*>(logits);
   auto* out = static_cast<typename T::elem*>(values);
-  if (k <= 128)
-    hipLaunchKernelGGL((topk_rows_kernel<T, 128, true, 256>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
-  else
-    hipLaunchKernelGGL((topk_rows_kernel<T, 1024, false, 512>), dim3(n), dim3(NT), 0, st, in, ld, vocab, k, out, index);
+  constexpr int MOST = 1 << 22;   // (a grid may have 2^32 threads)
+  for (int r0 = 0; r0 < n; r0 += n - r0 < MOST ? n - r0 : MOST) {
+    const dim3 rows(n - r0 < MOST ? n - r0 : MOST);
+    const auto* from = in + r0 * ld;
+    auto* to = out + (int64_t)r0 * k;
+    if (k <= 128) hipLaunchKernelGGL((topk_rows_kernel<T, 128, true, 256>), rows, dim3(NT), 0, st, from, ld, vocab, k, to, index + (int64_t)r0 * k);
+    else hipLaunchKernelGGL((topk_rows_kernel<T, 1024, false, 512>), rows, dim3(NT), 0, st, from, ld, vocab, k, to, index + (int64_t)r0 * k);
+  }
   return hipGetLastError();
 }
 

@@ -1207,8 +1207,14 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
       g.tiles_n = (int)((a.vocab + 255) / 256);
       TRY(launch_vocab8(V_STATS, g, st));
     } else {
-      g.tiles_n = g.n_part / 2;
-      TRY(launch_scores<V_STATS>(g, a, few, st));
+      // (a grid may have 2^32 threads: the vocabulary in as many parts as that takes)
+      const int tiles = g.n_part / 2, most = max(1, (1 << 23) / ((a.n + 127) / 128));
+      for (int t0 = 0; t0 < tiles; t0 += most) {
+        g.v0 = (int64_t)t0 * 128;
+        g.part = part + t0 * 2;
+        g.tiles_n = min(most, tiles - t0);
+        TRY(launch_scores<V_STATS>(g, a, few, st));
+      }
     }
     if (few) a.x = nullptr;   // rows stay where they are
     // (a loss of 15 % live rows, us, summed by the last workgroup / by a kernel more: n 1100 23.8 / 24.8, 1500 24.9 / 24.9,

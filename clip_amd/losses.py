@@ -12,7 +12,7 @@ fp32.  Rows that take no part (labels equal to ignore_index, teacher rows withou
 Everything is queued on the current stream of the tensors' device; there is no host wait and no CPU execution path.
 The tensor handling is in csrc/torch_losses.cpp (lib/_clip_torch.so), over the C ABI (clip_linear_ce and its neighbours).
 
-In a HIP graph: make one eager call per device first, and let go of eager losses of the same leaves before the capture (torch
+In a HIP graph: make one eager call of the same sizes first, and let go of eager losses of the same leaves before the capture (torch
 ties a leaf's gradient accumulation to the stream of the graph that is alive)."""
 import ctypes as C
 import importlib.util

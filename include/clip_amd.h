@@ -176,7 +176,7 @@ int clip_ce_loss(const float* dev_logits, const int32_t* dev_labels, int32_t n, 
  * [n_rows, vocab] fp32 scores.  The entry points below take any hidden rows and any decoder and give the loss AND the
  * gradients with a workspace of n x hidden plus one bounded piece of 16-bit score gradients.  Stateless: no engine, all
  * memory is the caller's, all work is queued on `stream` of the current device, nothing waits on the host, and calls can be
- * captured into HIP graphs (after one eager call per device) and replayed; calls that run at the same time need workspaces
+ * captured into HIP graphs (after one eager call of the same sizes) and replayed; calls that run at the same time need workspaces
  * of their own. */
 typedef struct clip_linear {
   int32_t operand;               /* CLIP_PRECISION_BF16 or CLIP_PRECISION_F16: type of hidden, weight and their gradients */

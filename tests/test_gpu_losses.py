@@ -456,6 +456,33 @@ def test_topk_strides_and_shapes(dtype):
     assert v.shape == i.shape == (0, 4)
 
 
+def test_topk_of_more_rows_than_one_grid():
+    n = (1 << 24) + 70001
+    x = torch.randint(-3, 3, (n, 3), generator=torch.Generator().manual_seed(5), dtype=torch.int8).cuda().to(BF16)
+    values, index = losses.topk_logits(x, 1)
+    want = x.max(1).values
+    first = torch.where(x[:, 0] == want, 0, torch.where(x[:, 1] == want, 1, 2))
+    assert torch.equal(values[:, 0], want) and torch.equal(index[:, 0], first)
+
+
+def test_losses_of_more_tiles_than_one_grid():
+    # 2^20 rows of 64 columns over 2^18 + 77 entries: 2^24 tiles and more
+    n, vocab, hidden = 1 << 20, (1 << 18) + 77, 64
+    h, w, b = R.make(4096, vocab, hidden, BF16, 99)
+    y = torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(6)).cuda()
+    y[-1] = vocab - 1
+    loss = losses.linear_cross_entropy(h.repeat(n // 4096, 1), w, b, y, reduction="none")
+    for at in (slice(0, 128), slice(n - 128, n)):
+        rows = h[at.start % 4096:at.start % 4096 + 128]
+        p, live = R.targets_ce(y[at], vocab, -100)
+        (want, *_), (err, *_) = R.reference(rows, w, b, p, live, 1.0, torch.ones(128).cuda())
+        R.assert_within("loss", loss[at], want, err)
+    # equal hidden rows have equal logsumexps: loss + score is off by the score's 64 fp32 sums (|h| |w| < 16) and the loss's rounding
+    z = torch.cat([(h.double() * w.double()[y[i:i + 4096]]).sum(1) + b.double()[y[i:i + 4096]] for i in range(0, n, 4096)])
+    lse = (loss.double() + z).view(-1, 4096)
+    assert ((lse - lse[0]).abs() <= 2 * (66 * 16 + 32) * R.F32).all()
+
+
 # ---------------------------------------------------------------- used together, streams, graphs
 def test_teacher_to_student_step():
     """a teacher's scores -> its top entries -> the student's distillation and cross entropy on the same rows"""
