@@ -161,7 +161,6 @@ __device__ __forceinline__ int row_state(const VocabRows& a, int r) {
   const int64_t y = a.labels[r];
   return y == a.ignore ? 0 : (y < 0 || y >= a.vocab ? 2 : 1);
 }
-__device__ __forceinline__ bool taking_part(const VocabRows& a, int r) { return a.state ? a.state[r] != 0 : a.labels[r] != a.ignore; }
 __device__ __forceinline__ float finite_abs(float g) {
   g = fabsf(g);
   return g < INFINITY ? g : 0.f;
@@ -528,7 +527,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
 }
 
 // Calls of many rows: the live rows before every 16th row, by one workgroup (a thread reads 16 rows' states at a time); 16 384
-// labels 11 us, latency
+// labels in 11 us, latency
 template <bool GRAD>
 __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   __shared__ int sums[16];
@@ -539,20 +538,27 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   for (int r0 = 0; r0 < a.n; r0 += 16384) {
     const int r = r0 + tid * 16;
     int live = 0;
-    int s[16];
+    int s[16];   // (clamped, not skipped: all loads in flight)
+    if (a.state) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {   // (no branches: all loads in flight)
-      const int q = min(r + i, a.n - 1);
-      s[i] = taking_part(a, q);
+      for (int i = 0; i < 16; ++i) s[i] = a.state[min(r + i, a.n - 1)];
+    } else {
+      int64_t y[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) y[i] = a.labels[min(r + i, a.n - 1)];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = y[i] != a.ignore;
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) live += r + i < a.n ? s[i] : 0;
+    float g[16];
     if (GRAD && a.grad_rows)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float g = finite_abs(a.grad[min(r + i, a.n - 1)]);
-        if (s[i]) gm = fmaxf(gm, g);
-      }
+      for (int i = 0; i < 16; ++i) g[i] = a.grad[min(r + i, a.n - 1)];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const bool takes_part = r + i < a.n && s[i] != 0;
+      live += takes_part;
+      if (GRAD && a.grad_rows && takes_part) gm = fmaxf(gm, finite_abs(g[i]));
+    }
     int up = live;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -583,8 +589,8 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
 
 // Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the end of their last tile.  One workgroup per 16 rows;
 // without a scan before it (few rows) each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
-// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 20 us (50 MB), 4096 rows 18 us (12.6 MB:
-// latency of count, then states, then rows).
+// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 30 us (50 MB and every workgroup's count),
+// 4096 rows 14 us (12.6 MB).
 template <bool GRAD>
 __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
   __shared__ int before_s[4], total_s[4];
@@ -599,6 +605,7 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         held[i][c] = *reinterpret_cast<const uint4*>(a.h + (int64_t)min(r0 + w * 4 + i, a.n - 1) * a.ldh + min(lane * 8 + c * 512, H - 8));
+  const int st = lane < 16 && r < a.n ? row_state(a, r) : 0;
   int before, total;
   float gm = 0.f;
   if (a.block_base) {
@@ -607,25 +614,34 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     if (GRAD) gm = *a.grad_max;
   } else {
     before = total = 0;
-    for (int q0 = 0; q0 < a.n; q0 += 256 * 8) {   // eight loads in flight
-      int s[8];
+    auto count = [&]<int U>(int q0) {   // U loads in flight: clamped, not skipped
+      int s[U];
+      if (a.state) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int q = q0 + i * 256 + tid;
-        s[i] = q0 + i * 256 < a.n ? (q < a.n) & (int)taking_part(a, min(q, a.n - 1)) : 0;
-      }
+        for (int i = 0; i < U; ++i) s[i] = a.state[min(q0 + i * 256 + tid, a.n - 1)];
+      } else {
+        int64_t y[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        total += s[i];
-        before += q0 + i * 256 + tid < r0 ? s[i] : 0;
+        for (int i = 0; i < U; ++i) y[i] = a.labels[min(q0 + i * 256 + tid, a.n - 1)];
+#pragma unroll
+        for (int i = 0; i < U; ++i) s[i] = y[i] != a.ignore;
       }
+      float g[U];
       if (GRAD && a.grad_rows)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float g = finite_abs(a.grad[min(q0 + i * 256 + tid, a.n - 1)]);
-          if (s[i]) gm = fmaxf(gm, g);
-        }
-    }
+        for (int i = 0; i < U; ++i) g[i] = a.grad[min(q0 + i * 256 + tid, a.n - 1)];
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int q = q0 + i * 256 + tid;
+        const bool live = q < a.n && s[i] != 0;
+        total += live;
+        before += live && q < r0;
+        if (GRAD && a.grad_rows && live) gm = fmaxf(gm, finite_abs(g[i]));
+      }
+    };
+    int q0 = 0;
+    for (; q0 + 512 < a.n; q0 += 256 * 8) count.template operator()<8>(q0);
+    for (; q0 < a.n; q0 += 256) count.template operator()<1>(q0);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       before += __shfl_xor(before, o, 64);
@@ -639,7 +655,6 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     if (blockIdx.x == 0 && w == 0) write_head<GRAD>(a, total, gm, lane);
   }
   // every wave ranks the 16 rows, wave 0 notes them down, wave w copies rows 4 w .. 4 w + 3
-  const int st = lane < 16 && r < a.n ? row_state(a, r) : 0;
   const unsigned live = (unsigned)__ballot(st != 0);
   {
     int64_t rank = before + __popc(live & ((1u << (w * 4)) - 1));
@@ -1065,10 +1080,14 @@ constexpr int64_t G_BYTES = 1ll << 30;
 //   H 768, V 8 000: n 512 (192) 96 / 84, 768 (288) 104 / 114, 2048 151 / 196;   V 2 000: n 2048 (192) 112 / 89
 //   H 256, V 8 000: n 512 (64) 75 / 58, 1024 (128) 88 / 81, 2048 (256) 100 / 120;   V 2 000: n 2048 (64) 83 / 74
 //   H 128, V 30 522: n 257 (240) 91 / 82, 400 (240) 86 / 92, 512 (240) 86 / 93, 1024 116 / 146
-// so up to 128 rows never (the small tiles read W once per 128 rows), then from about as many blocks as there are CUs
-bool large_tiles(int32_t n, int64_t vocab, int32_t hidden) {
+//   (gradients only: the small tiles do not split dW's k)  H 256, V 2 000: n 3000 (96) 89 / 95, 4096 (128) 93 / 113, 6000 102 / 148;
+//   H 128, V 500: n 4096 (32) 78 / 83, 16 384 148 / 258;   H 1024, V 1 000: n 4096 (256) 127 / 119, 6000 153 / 173
+//   (the loss alone)  H 768, V 500: n 16 384 (384) 81 / 68;   V 2 000: n 4096 (384) 40 / 43;   H 256, V 1 000: n 8192 (128) 36 / 38
+// so up to 128 rows never (the small tiles read W once per 128 rows), then from about as many blocks as there are CUs, and for
+// gradients from 4096 rows
+bool large_tiles(int32_t n, int64_t vocab, int32_t hidden, bool grad) {
   if (hidden % 128 || n <= 128) return false;
-  return ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
+  return (grad && n >= 4096) || ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
 }
 
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {
@@ -1079,7 +1098,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     at += (bytes + 255) & ~(size_t)255;
     return o;
   };
-  p.large = large_tiles(n, vocab, hidden);
+  p.large = large_tiles(n, vocab, hidden, grad);
   p.tile_rows = p.large ? 256 : (n <= 64 ? 64 : 128);
   const int64_t rows = ((int64_t)n + 255) / 256 * 256, vp = (vocab + 255) / 256 * 256;
   p.head = take(sizeof(VocabHead));
@@ -1177,8 +1196,8 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
     return hipSuccess;
   }
   // more rows than a workgroup of the next kernel should count for itself (a forward of 15 % live rows, us, counting here / there:
-  // n 1100 22.8 / 19.9, 2048 23.3 / 20.5, 4096 24.6 / 22.4, 8192 28.0 / 27.4, 16384 36.6 / 44.9)
-  if (a.n > 4096) {
+  // n 1100 18.8 / 15.5, 4096 20.9 / 17.4, 8192 28.1 / 25.0, 16 384 36.9 / 36.5)
+  if (a.n > 16384) {
     a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
     hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());

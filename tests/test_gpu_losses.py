@@ -64,7 +64,7 @@ SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64
          (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768), (2600, 1300, 128), (1500, 2500, 384),
          (1030, 5, 1024), (70, 500, 2048), (300, 600, 1152), (130, 300, 8192),
          # large tiles: 240 blocks of 256^3
-         (257, 30700, 128), (129, 10300, 1408), (300, 9001, 1152), (1030, 4099, 1024), (2600, 8003, 128), (1500, 10001, 384), (20500, 700, 256)]
+         (257, 30700, 128), (129, 10300, 1408), (300, 9001, 1152), (1030, 4099, 1024), (2600, 8003, 128), (1500, 10001, 384), (20500, 700, 256), (4100, 65, 256)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -628,7 +628,7 @@ def test_ignore_index_inside_the_vocabulary():
 # ---------------------------------------------------------------- the C ABI itself
 @pytest.mark.parametrize("n,vocab,hidden,ld_dh,ld_dw,k", [(50, 300, 64, 71, 68, 0), (100, 1000, 128, 128, 132, 5), (300, 1111, 128, 129, 136, 0),
                                                           (700, 4000, 384, 384, 388, 70), (1500, 257, 128, 128, 128, 0),
-                                                          (300, 31111, 128, 129, 136, 0), (700, 24001, 128, 128, 132, 70), (5000, 3300, 128, 128, 128, 0)])
+                                                          (300, 31111, 128, 129, 136, 0), (700, 24001, 128, 128, 132, 70), (5000, 3300, 128, 128, 128, 0), (4100, 257, 128, 128, 128, 3)])
 def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     """Row strides of the outputs, a workspace of exactly the size asked for and full of NaN, and untouched bytes around
     every output and behind the workspace; the same bits as the Python call."""
