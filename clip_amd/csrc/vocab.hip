@@ -587,15 +587,15 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   if (w == 0) write_head<GRAD>(a, before, gm, lane);
 }
 
-// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the end of their last tile.  One workgroup per 16 rows;
-// without a scan before it (few rows) each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
-// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 30 us (50 MB and every workgroup's count),
-// 4096 rows 14 us (12.6 MB).
-template <bool GRAD>
-__global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
-  __shared__ int before_s[4], total_s[4];
-  __shared__ float red[4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * 16, r = r0 + lane;
+// Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the end of their last tile.  A workgroup per NT / 16 rows,
+// four to a wave; without a scan before it each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
+// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 24 us (50 MB), 4096 rows 14 us (12.6 MB).
+template <bool GRAD, int NT>
+__global__ __launch_bounds__(NT) void vocab_pack_kernel(VocabRows a) {
+  constexpr int NW = NT / 64, ROWS = NT / 16;
+  __shared__ int before_s[NW], total_s[NW];
+  __shared__ float max_s[NW];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, r0 = blockIdx.x * ROWS, r = r0 + lane;
   const int H = a.hidden;
   // this wave's four rows are on their way before it is known which of them are live
   uint4 held[4][2];
@@ -605,11 +605,11 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
         held[i][c] = *reinterpret_cast<const uint4*>(a.h + (int64_t)min(r0 + w * 4 + i, a.n - 1) * a.ldh + min(lane * 8 + c * 512, H - 8));
-  const int st = lane < 16 && r < a.n ? row_state(a, r) : 0;
+  const int st = lane < ROWS && r < a.n ? row_state(a, r) : 0;
   int before, total;
   float gm = 0.f;
   if (a.block_base) {
-    before = a.block_base[blockIdx.x];
+    before = a.block_base[r0 >> 4];
     total = *a.count;
     if (GRAD) gm = *a.grad_max;
   } else {
@@ -618,21 +618,21 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       int s[U];
       if (a.state) {
 #pragma unroll
-        for (int i = 0; i < U; ++i) s[i] = a.state[min(q0 + i * 256 + tid, a.n - 1)];
+        for (int i = 0; i < U; ++i) s[i] = a.state[min(q0 + i * NT + tid, a.n - 1)];
       } else {
         int64_t y[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) y[i] = a.labels[min(q0 + i * 256 + tid, a.n - 1)];
+        for (int i = 0; i < U; ++i) y[i] = a.labels[min(q0 + i * NT + tid, a.n - 1)];
 #pragma unroll
         for (int i = 0; i < U; ++i) s[i] = y[i] != a.ignore;
       }
       float g[U];
       if (GRAD && a.grad_rows)
 #pragma unroll
-        for (int i = 0; i < U; ++i) g[i] = a.grad[min(q0 + i * 256 + tid, a.n - 1)];
+        for (int i = 0; i < U; ++i) g[i] = a.grad[min(q0 + i * NT + tid, a.n - 1)];
 #pragma unroll
       for (int i = 0; i < U; ++i) {
-        const int q = q0 + i * 256 + tid;
+        const int q = q0 + i * NT + tid;
         const bool live = q < a.n && s[i] != 0;
         total += live;
         before += live && q < r0;
@@ -640,24 +640,29 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       }
     };
     int q0 = 0;
-    for (; q0 + 512 < a.n; q0 += 256 * 8) count.template operator()<8>(q0);
-    for (; q0 < a.n; q0 += 256) count.template operator()<1>(q0);
+    for (; q0 + 2 * NT < a.n; q0 += NT * 8) count.template operator()<8>(q0);
+    for (; q0 < a.n; q0 += NT) count.template operator()<1>(q0);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
       before += __shfl_xor(before, o, 64);
       total += __shfl_xor(total, o, 64);
     }
-    if (lane == 0) { before_s[w] = before; total_s[w] = total; }
-    if (GRAD) gm = block_max(gm, red);
+    if (GRAD) gm = wave_max(gm);
+    if (lane == 0) { before_s[w] = before; total_s[w] = total; if (GRAD) max_s[w] = gm; }
     __syncthreads();
-    before = before_s[0] + before_s[1] + before_s[2] + before_s[3];
-    total = total_s[0] + total_s[1] + total_s[2] + total_s[3];
+    before = total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      before += before_s[i];
+      total += total_s[i];
+      if (GRAD) gm = fmaxf(gm, max_s[i]);
+    }
     if (blockIdx.x == 0 && w == 0) write_head<GRAD>(a, total, gm, lane);
   }
-  // every wave ranks the 16 rows, wave 0 notes them down, wave w copies rows 4 w .. 4 w + 3
-  const unsigned live = (unsigned)__ballot(st != 0);
+  // every wave ranks its workgroup's rows, wave 0 notes them down, wave w copies rows 4 w .. 4 w + 3
+  const unsigned long long live = __ballot(st != 0);
   {
-    int64_t rank = before + __popc(live & ((1u << (w * 4)) - 1));
+    int64_t rank = before + __popcll(live & ((1ull << (w * 4)) - 1));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int q = w * 4 + i;
@@ -677,9 +682,9 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
       }
     }
   }
-  if (w == 0 && lane < 16 && r < a.n) {
+  if (w == 0 && lane < ROWS && r < a.n) {
     if (st != 0) {
-      const int rank = before + __popc(live & ((1u << lane) - 1));
+      const int rank = before + __popcll(live & ((1ull << lane) - 1));
       a.row_map[rank] = st == 2 ? ~r : r;    // a row whose target is outside the vocabulary: NaN loss and gradients
       if (GRAD) {
         float2 lc;
@@ -692,12 +697,12 @@ __global__ __launch_bounds__(256) void vocab_pack_kernel(VocabRows a) {
     }
   }
   const int pad = (total + a.tile_rows - 1) / a.tile_rows * a.tile_rows;
-  for (int q = total + blockIdx.x * 4 + w; q < pad; q += gridDim.x * 4) {
+  for (int q = total + blockIdx.x * NW + w; q < pad; q += gridDim.x * NW) {
     for (int c = lane * 8; c < H; c += 512) *reinterpret_cast<uint4*>(a.x + (int64_t)q * H + c) = make_uint4(0, 0, 0, 0);
     if (GRAD && lane == 0) a.row_info[q] = no_row();
   }
   if (GRAD && a.fix)
-    for (int64_t v = (int64_t)blockIdx.x * 256 + tid; v < a.vocab * FIX_COPIES; v += (int64_t)gridDim.x * 256) a.fix[v] = 0;
+    for (int64_t v = (int64_t)blockIdx.x * NT + tid; v < a.vocab * FIX_COPIES; v += (int64_t)gridDim.x * NT) a.fix[v] = 0;
 }
 
 // few rows that 16-byte loads with 31-bit offsets cannot read where they are, a row a workgroup
@@ -1080,14 +1085,14 @@ constexpr int64_t G_BYTES = 1ll << 30;
 //   H 768, V 8 000: n 512 (192) 96 / 84, 768 (288) 104 / 114, 2048 151 / 196;   V 2 000: n 2048 (192) 112 / 89
 //   H 256, V 8 000: n 512 (64) 75 / 58, 1024 (128) 88 / 81, 2048 (256) 100 / 120;   V 2 000: n 2048 (64) 83 / 74
 //   H 128, V 30 522: n 257 (240) 91 / 82, 400 (240) 86 / 92, 512 (240) 86 / 93, 1024 116 / 146
-//   (gradients only: the small tiles do not split dW's k)  H 256, V 2 000: n 3000 (96) 89 / 95, 4096 (128) 93 / 113, 6000 102 / 148;
-//   H 128, V 500: n 4096 (32) 78 / 83, 16 384 148 / 258;   H 1024, V 1 000: n 4096 (256) 127 / 119, 6000 153 / 173
+//   (gradients only: the small tiles do not split dW's k)  H 256, V 2 000: n 3000 (96) 89 / 95, 4096 (128) 93 / 113 (but 75 / 56
+//   where 15 % of the rows are live), 6000 102 / 148;   H 128, V 500: n 16 384 148 / 258;   H 1024, V 1 000: n 6000 153 / 173
 //   (the loss alone)  H 768, V 500: n 16 384 (384) 81 / 68;   V 2 000: n 4096 (384) 40 / 43;   H 256, V 1 000: n 8192 (128) 36 / 38
 // so up to 128 rows never (the small tiles read W once per 128 rows), then from about as many blocks as there are CUs, and for
-// gradients from 4096 rows
+// gradients beyond 4096 rows
 bool large_tiles(int32_t n, int64_t vocab, int32_t hidden, bool grad) {
   if (hidden % 128 || n <= 128) return false;
-  return (grad && n >= 4096) || ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
+  return (grad && n > 4096) || ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
 }
 
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {
@@ -1162,6 +1167,10 @@ hipError_t device_cus(int* out) {
   return once.get([](int dev, int* val) { return hipDeviceGetAttribute(val, hipDeviceAttributeMultiprocessorCount, dev); }, out);
 }
 
+// More rows than this: copied by workgroups of 64 rows, each of which counts all rows' states, instead of 16; and more than this
+// are counted by a kernel of their own.  A forward of 15 % live rows (V 2 000, H 256), us, 16 rows / 64 rows / 64 rows and a
+// counting kernel: n 4096 17 / 21 / -, 8192 25 / 26 / -, 16 384 36 / 30 / -, 32 768 64 / 41 / 53, 65 536 172 / 85 / 96
+constexpr int PACK_WIDE = 8192, PACK_COUNTS = 65536;
 // what the forward and the backward begin with: the teacher's lists, and the live rows side by side
 template <bool GRAD>
 hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, hipStream_t st) {
@@ -1195,16 +1204,18 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
     }
     return hipSuccess;
   }
-  // more rows than a workgroup of the next kernel should count for itself (a forward of 15 % live rows, us, counting here / there:
-  // n 1100 18.8 / 15.5, 4096 20.9 / 17.4, 8192 28.1 / 25.0, 16 384 36.9 / 36.5)
-  if (a.n > 16384) {
+  if (a.n > PACK_COUNTS) {
     a.block_base = reinterpret_cast<int32_t*>(base + p.block_base);
     hipLaunchKernelGGL(vocab_scan_kernel<GRAD>, dim3(1), dim3(1024), 0, st, a);
     TRY(hipGetLastError());
   }
+  if (a.n > PACK_WIDE) {
+    hipLaunchKernelGGL((vocab_pack_kernel<GRAD, 1024>), dim3((a.n + 63) / 64), dim3(1024), 0, st, a);
+    return hipGetLastError();
+  }
   int groups = a.n > 0 ? (a.n + 15) / 16 : 1;
   if (GRAD && a.fix && groups < 64) groups = 64;   // (they clear its table, too)
-  hipLaunchKernelGGL(vocab_pack_kernel<GRAD>, dim3(groups), dim3(256), 0, st, a);
+  hipLaunchKernelGGL((vocab_pack_kernel<GRAD, 256>), dim3(groups), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -95,6 +95,25 @@ def test_cross_entropy_reductions_and_ignored_rows(vocab, dtype, reduction, igno
         assert not any(g.any() for g in grads)
 
 
+@pytest.mark.parametrize("reduction", ["none", "mean"])
+@pytest.mark.parametrize("distill", [False, True])
+@pytest.mark.parametrize("n", [1500, 4097, 9001, 70001])
+def test_ignored_rows_among_many(n, distill, reduction):
+    # live rows counted by the copying workgroups, small and large, or beforehand
+    vocab, hidden = 200, 128
+    h, w, b = R.make(n, vocab, hidden, BF16, n)
+    if distill:
+        values, index = _teacher(n, vocab, 3, n, 0.8)
+        p, live, entropy = R.targets_distill(values, index, vocab, 2.0)
+    else:
+        y = _labels(n, vocab, n, 0.6)
+        (p, live), entropy = R.targets_ce(y, vocab, -100), None
+    h[~live] = NAN
+    _, grads = _check(h, w, b, lambda h, w, b: losses.linear_distillation(h, w, b, values, index, temperature=2.0, reduction=reduction) if distill
+                      else losses.linear_cross_entropy(h, w, b, y, reduction=reduction), p, live, 2.0 if distill else 1.0, reduction, 6, entropy)
+    assert not grads[0][~live].any()
+
+
 def test_mean_over_no_rows():
     h, w, b = R.make(5, 70, 64, BF16, 1)
     y = torch.full((5,), -100).cuda()
