@@ -12,8 +12,8 @@
 // cycles); 256 x 256 tiles because each byte that a CU takes in feeds twice the MFMAs that it does in a 128 x 128 tile (of which
 // two fit: 16 384 rows 4.6 ms instead of 2.7).  bf16, V 30 522, H 768, us (2 n V H, twice that for the pair; 1.29 PF is the rate
 // of a large library product):
-//   4096 rows:   scores 164 - 181 (1.06 - 1.17 PF), G 184 - 206 (0.93 - 1.04 PF; 250 MB leave it), dW + dh 342 - 389 (0.99 - 1.12 PF)
-//   16 384 rows: scores 612 - 647 (1.19 - 1.25 PF), G 686 - 724 (1.06 - 1.12 PF; 1 GB leaves it), dW + dh 1250 - 1306 (1.18 - 1.23 PF)
+//   4096 rows:   scores 160 - 177 (1.08 - 1.20 PF), G 180 - 198 (0.97 - 1.07 PF; 250 MB leave it), dW + dh 339 - 371 (1.03 - 1.13 PF)
+//   16 384 rows: scores 590 - 635 (1.21 - 1.30 PF), G 649 - 706 (1.09 - 1.18 PF; 1 GB leaves it), dW + dh 1220 - 1294 (1.19 - 1.26 PF)
 #include "vocab.h"
 
 namespace {
