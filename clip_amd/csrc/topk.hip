@@ -3,11 +3,12 @@
 // One workgroup per row; a chunk of 64 KB (16 384 fp32 scores or 32 768 of 16 bits) is read at once into registers, 64 per
 // thread.  A threshold that the k largest all reach and few others do is found to 16 bits by bisection on ballots:
 // for k <= 128 the k-th largest of the 256 threads' maxima (177 random scores reach it at k = 128, 74 at k = 64), beyond that
-// the k-th largest score itself.  Each wave notes what reaches it, one comparison per 16 bytes read, in its own part of LDS
+// the k-th largest of the maxima of 16 bytes, and the k-th largest score itself where a row has not twice k of these.  Each wave notes what reaches it, one comparison per 16 bytes read, in its own part of LDS
 // as 64-bit keys (order-preserving bits of the score above the inverted id: all keys differ, a larger key comes first), and
 // the few keys noted are sorted by counting, for each, how many are larger.  Where too many reach the threshold (equal
 // scores) the chunk is gone through again, a list being cut back to its k largest whenever it is full.
-// Bound: reading the scores; 8192 x 30 522 with k 64: fp32 200 us (5.0 TB/s), bf16 138 us, fp16 119 us (4.2 TB/s); five rows 8.4 us.
+// Bound: reading the scores; 8192 x 30 522 with k 64: fp32 200 us (5.0 TB/s), bf16 138 us, fp16 119 us (4.2 TB/s); five rows 8.4 us;
+// k 300 on 4096 rows: fp32 360 us, bf16 290 us (the search's 16 barriers; 540 and 940 us with every score searched).
 #include "common.h"
 #include "kernels.h"
 
@@ -162,6 +163,20 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
     noted = 0;
   };
 
+  // the largest threshold, to 16 bits, that k scores reach; count(reaches) = how many of this wave's do
+  auto search = [&](auto&& count) -> uint32_t {
+    uint32_t t = 0;
+    for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
+      const float f = score_of(t | bit);
+      const int n = (t | bit) <= 0xff800000u ? count([&](float x) { return !(x < f); }) : count([](float x) { return x != x; });
+      turn ^= 1;
+      if (lane == 0) wave_s[turn][w] = n;
+      __syncthreads();
+      if (wave_s[turn][0] + wave_s[turn][1] + wave_s[turn][2] + wave_s[turn][3] >= k) t |= bit;
+    }
+    return t;
+  };
+
   // ---- the scores before the first and after the last whole 16 bytes are kept to begin with (at most 14)
   const int head = min((int)(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(typename T::elem)), vocab);
   const int body = (vocab - head) / T::VEC;   // whole vectors
@@ -182,7 +197,8 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
       if (c0 + (i + 1) * NT > body && c0 + i * NT + tid >= body) v[i] = make_uint4(neg, neg, neg, neg);
     if (kth == 0) {   // no threshold yet
       uint32_t t = 0;
-      if (MAXIMA) {
+      const int left = min(body - c0, NV * NT);
+      if (MAXIMA && left >= min(NT, 2 * k)) {
         float mx = T::top(v[0]);
 #pragma unroll
         for (int i = 1; i < NV; ++i) mx = max_nan(mx, T::top(v[i]));
@@ -202,19 +218,27 @@ __global__ __launch_bounds__(NT) void topk_rows_kernel(const typename T::elem* _
         }
         __syncthreads();
         t = threshold_s;
-      } else {
-        for (uint32_t bit = 0x80000000u; bit >= 0x10000u; bit >>= 1) {
-          const float f = score_of(t | bit);   // (a NaN: only NaN reach it)
+      } else if (!MAXIMA && left >= 2 * k) {
+        float mx[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) mx[i] = T::top(v[i]);
+        t = search([&](auto&& reaches) {
           int n = 0;
 #pragma unroll
-          for (int i = 0; i < NV; ++i)
+          for (int i = 0; i < NV; ++i) n += __popcll(__ballot(reaches(mx[i])));
+          return n;
+        });
+      } else {
+        constexpr int FEW = MAXIMA ? 1 : 2 * KMAX / NT;   // 16-byte pieces per thread
+        t = search([&](auto&& reaches) {
+          int n = 0;
 #pragma unroll
-            for (int e = 0; e < T::VEC; ++e) n += __popcll(__ballot(!(T::get(v[i], e) < f) && ((t | bit) <= 0xff800000u || T::get(v[i], e) != T::get(v[i], e))));
-          turn ^= 1;
-          if (lane == 0) wave_s[turn][w] = n;
-          __syncthreads();
-          if (wave_s[turn][0] + wave_s[turn][1] + wave_s[turn][2] + wave_s[turn][3] >= k) t |= bit;
-        }
+          for (int i = 0; i < FEW; ++i)
+            if (i * NT < left)
+#pragma unroll
+              for (int e = 0; e < T::VEC; ++e) n += __popcll(__ballot(reaches(T::get(v[i], e))));
+          return n;
+        });
       }
       kth = (u64)t << 32;
       kth_f = score_of(t);

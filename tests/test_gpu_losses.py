@@ -442,16 +442,17 @@ def _same_topk(x, k):
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("n,vocab,k", [(1, 1, 1), (2, 3, 3), (5, 17, 5), (7, 1000, 1000), (3, 255, 256 - 1), (4, 4097, 64), (9, 30522, 10),
-                                       (2, 30522, 257), (3, 50001, 1024), (1, 200003, 128), (70, 8192, 1)])
+                                       (2, 30522, 257), (3, 50001, 1024), (1, 200003, 128), (70, 8192, 1), (5, 300, 100), (5, 301, 128),
+                                       (4, 1000, 128), (4, 1030, 64), (6, 1003, 200), (3, 2051, 256), (3, 3000, 1024), (2, 4099, 1024),
+                                       (2, 9001, 1024), (2, 16500, 1024), (2, 5000, 700), (2, 17001, 129)])
 def test_topk_sizes(n, vocab, k, dtype):
     g = torch.Generator().manual_seed(vocab)
     _same_topk((2.5 * torch.randn(n, vocab, generator=g)).to(dtype).cuda(), k)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
-@pytest.mark.parametrize("k", [1, 64, 300])
-def test_topk_orders_that_fill_the_list(dtype, k):
-    vocab = 20000
+@pytest.mark.parametrize("vocab,k", [(20000, 1), (20000, 64), (20000, 300), (20000, 1000), (600, 64), (600, 128), (600, 500), (5000, 700)])
+def test_topk_orders_that_fill_the_list(dtype, vocab, k):
     up = torch.linspace(-50, 50, vocab)
     rows = [up, up.flip(0), torch.zeros(vocab), torch.full((vocab,), -INF), torch.full((vocab,), NAN), (torch.arange(vocab) % 7).float(),
             torch.where(torch.arange(vocab) % 2 == 0, 0.0, -0.0), torch.where(torch.arange(vocab) < 100, INF, -INF),
