@@ -494,33 +494,49 @@ __global__ __launch_bounds__(256) void vocab_products_kernel(VocabGemm a, int ti
 // Teacher lists of a distillation: p = softmax(values / T) over a row's entries with index >= 0 and a value above -inf
 // (0 elsewhere), log_p beside it, state[row] = 0 no entry, 1 live, 2 an index beyond the vocabulary or a value that is
 // NaN or +inf.  One wave per row.  4096 x 64 entries: 5.5 us (3 MB read; latency).
+template <int EACH>   // entries per lane
 __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
   const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (row >= a.n) return;
-  const float* t = a.t_values + (int64_t)row * a.ld_t;
-  const int64_t* ix = a.t_index + (int64_t)row * a.ld_ti;
+  float t[EACH];
+  int64_t id[EACH];
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    t[u] = -INFINITY;
+    id[u] = -1;
+    if (u * 64 < a.k) {   // (clamped, not skipped: all loads in flight)
+      const int j = min(u * 64 + lane, a.k - 1);
+      t[u] = a.t_values[(int64_t)row * a.ld_t + j];
+      id[u] = a.t_index[(int64_t)row * a.ld_ti + j];
+    }
+  }
   float mx = -INFINITY;
   int n_in = 0, bad = 0;
-  auto in_list = [&](int j) { return ix[j] >= 0 && t[j] != -INFINITY; };
-  for (int j = lane; j < a.k; j += 64)
-    if (in_list(j)) {
-      mx = fmaxf(mx, t[j] * a.inv_t);
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    if (u * 64 + lane >= a.k || id[u] < 0) t[u] = -INFINITY;   // not in the list
+    if (t[u] != -INFINITY) {
+      mx = fmaxf(mx, t[u] * a.inv_t);
       ++n_in;
-      bad |= ix[j] >= a.vocab;
+      bad |= id[u] >= a.vocab;
     }
+  }
   mx = wave_max(mx);
   const float ref = mx == -INFINITY ? 0.f : mx;
   float s = 0.f;
-  for (int j = lane; j < a.k; j += 64)
-    if (in_list(j)) s += expf(t[j] * a.inv_t - ref);
+#pragma unroll
+  for (int u = 0; u < EACH; ++u)
+    if (u * 64 < a.k && t[u] != -INFINITY) s += expf(t[u] * a.inv_t - ref);
   s = wave_sum(s);
   bad |= !(s < INFINITY);   // a NaN or +inf among the teacher's values
   const float log_s = logf(s);
-  for (int j = lane; j < a.k; j += 64) {
-    const bool in = in_list(j);
-    const float lp = t[j] * a.inv_t - ref - log_s;
-    a.t_p[(int64_t)row * a.k + j] = in ? expf(t[j] * a.inv_t - ref) / s : 0.f;
-    if (a.t_logp) a.t_logp[(int64_t)row * a.k + j] = lp;
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    const int j = u * 64 + lane;
+    if (j >= a.k) continue;
+    const float x = t[u] * a.inv_t - ref;
+    a.t_p[(int64_t)row * a.k + j] = t[u] != -INFINITY ? expf(x) / s : 0.f;
+    if (a.t_logp) a.t_logp[(int64_t)row * a.k + j] = x - log_s;
   }
   const bool any_in = __any(n_in), any_bad = __any(bad);
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
@@ -887,63 +903,121 @@ __global__ __launch_bounds__(1024) void vocab_reduce_kernel(VocabRows a) {
   }
 }
 
-// The teacher's part of G, one wave per live row: G[r, v] = c (q_v - sum of p over the entries that name v), from the
-// forward's fp32 score of v (a difference of the rounded q would lose what is left where q is near p).  (A label's part is
-// set by V_GRAD itself.)  The sums of c p per vocabulary entry, which db needs, go to a table of 64-bit fixed point: integer
-// adds commute, so their order does not show (2^-38 a unit; |c| p <= 1, n <= 2^24 rows); in FIX_COPIES copies by row, since a
-// teacher's frequent entries are the same in most rows.  4096 x 64 entries: 23 us, mostly the adds' (262 k of them).
+// The teacher's part of G: G[r, v] = c (q_v - sum of p over the entries that name v), from the forward's fp32 score of v (a
+// difference of the rounded q would lose what is left where q is near p).  (A label's part is set by V_GRAD itself.)  The sums
+// of c p per vocabulary entry, which db needs, go to a table of 64-bit fixed point: integer adds commute, so their order does
+// not show (2^-38 a unit; |c| p <= 1, n <= 2^24 rows); in FIX_COPIES copies by row, since a teacher's frequent entries are the
+// same in most rows.
+// `first`: this entry is the first of its row to name v (0 <= v), `p` what they add up to, `own` its own part.  Returns whether
+// the entry is a sixteenth or more of the row, and what rounding leaves of it.
+__device__ __forceinline__ bool teacher_entry(const VocabRows& a, const float2& lc, int r, int row, int j, int v, float own, float p, bool first,
+                                              bf16_t* g, int64_t ldg, int64_t v0, int64_t v1, int table, float& rest) {
+  if (a.fix && table && v >= 0 && fabsf(lc.y * own) <= 1.f)
+    atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
+  if (!first) return false;
+  const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
+  const float e = lc.y * (q - p) * G_SCALE;
+  if (v >= v0 && v < v1) {
+    g[(int64_t)r * ldg + (v - v0)] = f32_to_op(e);
+    if (a.low) g[(int64_t)(r + 64) * ldg + (v - v0)] = f32_to_op(residual(e));
+  }
+  rest = residual(e);
+  return fabsf(q - p) >= 0.0625f;
+}
+__device__ __forceinline__ void teacher_list(const VocabRows& a, int row, int j, int& v, float& own) {
+  // (not listed, or beyond the vocabulary, which only an entry of value -inf may be: -1)
+  const int64_t t = j < a.k ? a.t_index[(int64_t)row * a.ld_ti + j] : -1;
+  v = t >= 0 && t < a.vocab ? (int)t : -1;
+  own = j < a.k ? a.t_p[(int64_t)row * a.k + j] : 0.f;
+}
+// up to 64 entries a row: one wave per live row, every entry against every other.  4096 x 64 entries: 23 us, mostly the table's
+// adds (262 k of them)
 __global__ __launch_bounds__(256) void vocab_teacher_grad_kernel(VocabRows a, bf16_t* __restrict__ g, int64_t ldg, int64_t v0, int64_t v1,
                                                                  int table) {
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r >= *a.count) return;
   const int row = a.row_map[r];
-  if (row < 0) {   // (a row of NaN: nothing to correct)
-    if (table && lane < ROW_FIX) a.row_fix[(int64_t)r * ROW_FIX + lane] = make_float2(__int_as_float(-1), 0.f);
+  unsigned long long big = 0;
+  float rest = 0.f;
+  int v = -1;
+  if (row >= 0) {   // (else a row of NaN: nothing to put in or to correct)
+    int earlier = 0;
+    float own, p = 0.f;
+    teacher_list(a, row, lane, v, own);
+    for (int i = 0; i < a.k; ++i) {   // every entry that names v
+      const int ui = __builtin_amdgcn_readlane(v, i);
+      const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), i));
+      p += ui == v ? qi : 0.f;
+      earlier += ui == v && i < lane;
+    }
+    big = __ballot(teacher_entry(a, a.row_lc[r], r, row, lane, v, own, p, v >= 0 && earlier == 0, g, ldg, v0, v1, table, rest));
+  }
+  if (table && a.dh) {   // the row's first ROW_FIX large entries
+    float2* fix = a.row_fix + (int64_t)r * ROW_FIX;
+    const int at = __popcll(big & ((1ull << lane) - 1));
+    if ((big >> lane & 1) && at < ROW_FIX) fix[at] = make_float2(__int_as_float(v), rest);
+    if (lane < ROW_FIX && lane >= __popcll(big)) fix[lane] = make_float2(__int_as_float(-1), 0.f);
+  }
+}
+// more entries: a workgroup per live row, the sums by way of a hash table in LDS that is at most half full (64-bit fixed point
+// again, of 2^-62 a unit).  4096 rows: 128 entries 35 us, 1024 200 us (every entry against every other: 51 us, 1530 us)
+__global__ __launch_bounds__(256) void vocab_teacher_hash_kernel(VocabRows a, bf16_t* __restrict__ g, int64_t ldg, int64_t v0, int64_t v1,
+                                                                 int table) {
+  constexpr int SIZE = 2048, EACH = 4;   // 1024 entries
+  constexpr double UNIT = 4611686018427387904.0;
+  __shared__ int id_s[SIZE], first_s[SIZE];
+  __shared__ unsigned long long sum_s[SIZE], big_s[EACH][4];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  if (r >= *a.count) return;
+  const int row = a.row_map[r];
+  float2* fix = table && a.dh ? a.row_fix + (int64_t)r * ROW_FIX : nullptr;
+  if (row < 0) {
+    if (fix && tid < ROW_FIX) fix[tid] = make_float2(__int_as_float(-1), 0.f);
     return;
   }
   const float2 lc = a.row_lc[r];
-  const int64_t* index = a.t_index + (int64_t)row * a.ld_ti;
-  const float* tp = a.t_p + (int64_t)row * a.k;
-  // (not listed, or beyond the vocabulary, which only an entry of value -inf may be: -1)
-  auto entry = [&](int j, int& v, float& p) {
-    const int64_t t = j < a.k ? index[j] : -1;
-    v = t >= 0 && t < a.vocab ? (int)t : -1;
-    p = j < a.k ? tp[j] : 0.f;
-  };
-  int fixed = 0;   // entries noted for dh
-  for (int j0 = 0; j0 < a.k; j0 += 64) {
-    const int j = j0 + lane;
-    int v, earlier = 0;
-    float own, p = 0.f;
-    entry(j, v, own);
-    for (int i0 = 0; i0 < a.k; i0 += 64) {   // every entry that names v
-      int u = v;
-      float q = own;
-      if (i0 != j0) entry(i0 + lane, u, q);
-      const int n = min(64, a.k - i0);
-      for (int i = 0; i < n; ++i) {
-        const int ui = __builtin_amdgcn_readlane(u, i);
-        const float qi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(q), i));
-        p += ui == v ? qi : 0.f;
-        earlier += ui == v && i0 + i < j;
-      }
-    }
-    if (a.fix && table && v >= 0 && fabsf(lc.y * own) <= 1.f)
-      atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
-    const float q = v < 0 ? 0.f : __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
-    const float e = lc.y * (q - p) * G_SCALE;
-    if (v >= v0 && v < v1) {
-      g[(int64_t)r * ldg + (v - v0)] = f32_to_op(e);
-      if (a.low) g[(int64_t)(r + 64) * ldg + (v - v0)] = f32_to_op(residual(e));
-    }
-    if (table && a.dh) {   // the first ROW_FIX entries of a sixteenth or more of the row (of an id named twice: the first)
-      const unsigned long long big = __ballot(v >= 0 && earlier == 0 && fabsf(q - p) >= 0.0625f);
-      const int at = fixed + __popcll(big & ((1ull << lane) - 1));
-      if ((big >> lane & 1) && at < ROW_FIX) a.row_fix[(int64_t)r * ROW_FIX + at] = make_float2(__int_as_float(v), residual(e));
-      fixed += __popcll(big);
-    }
+  int v[EACH], slot[EACH];
+  float own[EACH], rest[EACH];
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) teacher_list(a, row, u * 256 + tid, v[u], own[u]);
+  for (int i = tid; i < SIZE; i += 256) {
+    id_s[i] = -1;
+    first_s[i] = 1 << 30;
+    sum_s[i] = 0;
   }
-  if (table && a.dh && lane < ROW_FIX && lane >= fixed) a.row_fix[(int64_t)r * ROW_FIX + lane] = make_float2(__int_as_float(-1), 0.f);
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    slot[u] = 0;
+    if (v[u] < 0) continue;
+    int h = (int)((uint32_t)v[u] * 2654435761u >> 21);
+    for (int at; (at = atomicCAS(&id_s[h], -1, v[u])) != -1 && at != v[u];) h = (h + 1) & (SIZE - 1);
+    slot[u] = h;
+    atomicAdd(&sum_s[h], (unsigned long long)__double2ull_rn((double)own[u] * UNIT));
+    atomicMin(&first_s[h], u * 256 + tid);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < EACH; ++u) {
+    const int j = u * 256 + tid;
+    const bool first = v[u] >= 0 && first_s[slot[u]] == j;
+    const float p = (float)((double)sum_s[slot[u]] / UNIT);
+    const unsigned long long big = __ballot(teacher_entry(a, lc, r, row, j, v[u], own[u], p, first, g, ldg, v0, v1, table, rest[u]));
+    if (lane == 0) big_s[u][w] = big;
+  }
+  if (!fix) return;
+  __syncthreads();
+  int before = 0;   // large entries ahead, in the list's order
+#pragma unroll
+  for (int u = 0; u < EACH; ++u)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const unsigned long long big = big_s[u][q];
+      const int at = before + __popcll(big & ((1ull << lane) - 1));
+      if (q == w && (big >> lane & 1) && at < ROW_FIX) fix[at] = make_float2(__int_as_float(v[u]), rest[u]);
+      before += __popcll(big);
+    }
+  if (tid < ROW_FIX && tid >= before) fix[tid] = make_float2(__int_as_float(-1), 0.f);
 }
 
 // dh of the live rows from the fp32 partials (fixed order), and db from the column sums and the targets' table; dW from its
@@ -1188,7 +1262,8 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
     a.t_p = reinterpret_cast<float*>(base + p.t_p);
     a.t_logp = GRAD ? nullptr : reinterpret_cast<float*>(base + p.t_logp);
     if (a.n > 0) {
-      hipLaunchKernelGGL(vocab_teacher_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
+      const auto kfn = a.k > 64 ? vocab_teacher_kernel<16> : vocab_teacher_kernel<1>;
+      hipLaunchKernelGGL(kfn, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
       TRY(hipGetLastError());
     }
   }
@@ -1312,8 +1387,8 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
       g.tiles_n = g.ldg / (p.large ? 256 : 128);
       TRY(p.large ? launch_vocab8(V_GRAD, g, st) : launch_scores<V_GRAD>(g, a, few, st));
       if (a.t_index) {
-        hipLaunchKernelGGL(vocab_teacher_grad_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1,
-                           piece == 0 ? 1 : 0);
+        const auto kfn = a.k > 64 ? vocab_teacher_hash_kernel : vocab_teacher_grad_kernel;
+        hipLaunchKernelGGL(kfn, dim3(a.k > 64 ? a.n : (a.n + 3) / 4), dim3(256), 0, st, a, g.g, (int64_t)g.ldg, v0, v1, piece == 0 ? 1 : 0);
         TRY(hipGetLastError());
       }
     }

@@ -236,7 +236,7 @@ def test_row_strides_by_size(n, vocab):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("distill", [False, True])
+@pytest.mark.parametrize("distill", [0, 2, 70])
 @pytest.mark.parametrize("n,vocab", [(1, 600), (40, 600), (64, 600), (100, 600), (700, 600), (700, 21000)])
 def test_what_the_rounded_score_gradients_leave_is_put_back(n, vocab, distill, dtype):
     """The large entries of a row reach dhidden unrounded; dweight of at most 64 rows is made of high and low parts, whose
@@ -248,7 +248,8 @@ def test_what_the_rounded_score_gradients_leave_is_put_back(n, vocab, distill, d
     w[1, :64] = 0
     up = torch.randn(n, generator=torch.Generator().manual_seed(n)).cuda()
     if distill:
-        values, index = torch.tensor([[1.0, 0.5]]).cuda().expand(n, 2), torch.tensor([[0, 1]]).cuda().expand(n, 2)
+        values, index = torch.full((n, distill), -INF).cuda(), torch.full((n, distill), -1).cuda()
+        values[:, 0], values[:, -1], index[:, 0], index[:, -1] = 1.0, 0.5, 0, 1
         p, live, entropy = R.targets_distill(values, index, vocab, 1.0)
     else:
         y = torch.arange(n).cuda() % 2
@@ -372,9 +373,9 @@ def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
 
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("n,vocab", [(150, 400), (300, 30800), (60, 400)])
-def test_distillation_ragged_empty_and_repeated_entries(n, vocab, dtype, reduction):
-    hidden, k = 128, 12
+@pytest.mark.parametrize("n,vocab,k", [(150, 400, 12), (300, 30800, 12), (60, 400, 12), (150, 400, 65), (60, 400, 300), (300, 30800, 300)])
+def test_distillation_ragged_empty_and_repeated_entries(n, vocab, k, dtype, reduction):
+    hidden = 128
     h, w, b = R.make(n, vocab, hidden, dtype, 5)
     values, index = _teacher(n, vocab, k, 6, dropped=0.4)
     index[[0, 17, n - 1]] = -1            # nothing listed
@@ -383,6 +384,8 @@ def test_distillation_ragged_empty_and_repeated_entries(n, vocab, dtype, reducti
     values[42, 3:] = -INF
     values[43] = torch.finfo(F32).min     # the lowest finite value everywhere: a uniform teacher
     index[44, :5] = index[44, 5].clamp(min=0)   # one id several times
+    index[46, k // 2:] = index[46, :k - k // 2].clone()  # the list twice
+    index[47] = 7
     index[45] = vocab - 1
     p, live, entropy = R.targets_distill(values, index, vocab, 2.0)
     assert not live[[0, 17, n - 1, 40, 41]].any()
@@ -392,9 +395,8 @@ def test_distillation_ragged_empty_and_repeated_entries(n, vocab, dtype, reducti
     assert not grads[0][~live].any()
 
 
-@pytest.mark.parametrize("n,vocab", [(30, 100), (100, 100), (300, 30800)])
-def test_distillation_of_bad_entries_is_nan(n, vocab):
-    k = 4
+@pytest.mark.parametrize("n,vocab,k", [(30, 100, 4), (100, 100, 4), (300, 30800, 4), (30, 100, 90)])
+def test_distillation_of_bad_entries_is_nan(n, vocab, k):
     h, w, b = R.make(n, vocab, 128, BF16, 5)
     values, index = _teacher(n, vocab, k, 6)
     index[3, 1] = vocab
