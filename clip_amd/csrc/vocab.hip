@@ -468,9 +468,11 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::condit
   }
 }
 
-// Scores (V_STATS, V_GRAD), a tile per workgroup.  Few rows: bound by W's bytes, one row 10.9 us for 47 MB (4.3 TB/s); ring of
-// four 24-KiB K tiles, three in flight: the 239 workgroups, one a CU, must hide the memory's latency alone.  64 .. 128 rows:
-// three 32-KiB K tiles.  G with its low part (19 rows) 15 us for 47 MB read and 15.6 MB written.
+// Scores (V_STATS, V_GRAD), a tile per workgroup.  Few rows: bound by W's bytes, one row 10.9 us for 47 MB (4.3 TB/s).  Rings that
+// leave room for two workgroups on a CU, so that 257 tiles and more are not two rounds (us of a loss, one 4-deep ring a CU / two
+// 3-deep: V 30 522, H 768 18.0 / 17.8; V 33 000 25 / 20; V 40 000, H 1024 30 / 26; 128-row tiles, one 3-deep / two 2-deep: 128 rows of
+// V 30 522 27.5 / 28.6, V 50 257 38 / 32; 4096 rows, H 704 314 / 229).  G with its low part (19 rows) 15 us for 47 MB read and
+// 15.6 MB written.
 template <int EPI, int BM, int NST, bool FEW>
 __global__ __launch_bounds__(256) void vocab_scores_kernel(VocabGemm a, std::conditional_t<FEW, VocabRows, NoRows> rows) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1137,8 +1139,8 @@ hipError_t launch_tiles(int lds, int64_t groups, hipStream_t st, const Args&... 
 constexpr int ring_bytes(int rows, int stages) { return stages * (rows + 128) * BK * 2; }
 template <int EPI>
 hipError_t launch_scores(const VocabGemm& g, const VocabRows& a, bool few, hipStream_t st) {
-  if (few) return launch_tiles<vocab_scores_kernel<EPI, 64, 4, true>>(ring_bytes(64, 4), g.tiles_n, st, g, a);
-  return launch_tiles<vocab_scores_kernel<EPI, 128, 3, false>>(ring_bytes(128, 3), (a.n + 127) / 128 * (int64_t)g.tiles_n, st, g, NoRows());
+  if (few) return launch_tiles<vocab_scores_kernel<EPI, 64, 3, true>>(ring_bytes(64, 3), g.tiles_n, st, g, a);
+  return launch_tiles<vocab_scores_kernel<EPI, 128, 2, false>>(ring_bytes(128, 2), (a.n + 127) / 128 * (int64_t)g.tiles_n, st, g, NoRows());
 }
 hipError_t launch_products(const VocabGemm& g, const VocabPlan& p, int n, hipStream_t st) {
   const int tiles_m = g.with_dh ? (n + p.tile_rows - 1) / p.tile_rows : 0;
@@ -1153,20 +1155,18 @@ hipError_t launch_products(const VocabGemm& g, const VocabPlan& p, int n, hipStr
 #if !CLIP_OPERAND_F16
 // G of one piece of the vocabulary may take this much: the pieces are as few as that allows
 constexpr int64_t G_BYTES = 1ll << 30;
-// Which calls run on the 256 x 256 tiles of vocab8.hip.  Loss and gradients in us, these tiles / the small ones, and how many
-// 256^3 blocks the call has (rows x vocabulary x hidden):
-//   H 768, V 30 522: n 128 110 / 88, 160 (360) 117 / 125, 257 (720) 130 / 168, 2048 386 / 630
-//   H 768, V 8 000: n 512 (192) 96 / 84, 768 (288) 104 / 114, 2048 151 / 196;   V 2 000: n 2048 (192) 112 / 89
-//   H 256, V 8 000: n 512 (64) 75 / 58, 1024 (128) 88 / 81, 2048 (256) 100 / 120;   V 2 000: n 2048 (64) 83 / 74
-//   H 128, V 30 522: n 257 (240) 91 / 82, 400 (240) 86 / 92, 512 (240) 86 / 93, 1024 116 / 146
-//   (gradients only: the small tiles do not split dW's k)  H 256, V 2 000: n 3000 (96) 89 / 95, 4096 (128) 93 / 113 (but 75 / 56
-//   where 15 % of the rows are live), 6000 102 / 148;   H 128, V 500: n 16 384 148 / 258;   H 1024, V 1 000: n 6000 153 / 173
-//   (the loss alone)  H 768, V 500: n 16 384 (384) 81 / 68;   V 2 000: n 4096 (384) 40 / 43;   H 256, V 1 000: n 8192 (128) 36 / 38
-// so up to 128 rows never (the small tiles read W once per 128 rows), then from about as many blocks as there are CUs, and for
-// gradients beyond 4096 rows
+// Which calls run on the 256 x 256 tiles of vocab8.hip: up to 128 rows none (the small tiles read W once per 128 rows).
+// The loss alone from 192 tiles, in us, these / the small ones:  V 30 522, H 768: n 256 (120 tiles) 35 / 32, 300 (240) 38 / 42;
+//   H 128: n 257 (240) 22 / 25;   V 8 000, H 256: n 1024 (128) 26 / 24, 2048 (256) 26 / 32;   V 2 000, H 768: n 4096 (128) 42 / 40
+// Loss and gradients from 500 blocks of 256^3:  V 30 522, H 768: n 256 (360 blocks) 119 / 116, 300 (720) 136 / 155, 1024 230 / 305;
+//   H 128: n 1024 (240) 117 / 114, 2048 (480) 176 / 171, 8192 571 / 623;   V 8 000, H 768: n 1024 (384) 115 / 112, 2048 148 / 174;
+//   H 256: n 2048 (256) 101 / 99, 4096 (512) 142 / 160;   V 2 000, H 768: n 4096 (384) 132 / 126
+// and beyond 4096 rows, where the small tiles' unsplit k makes dW late:  V 2 000, H 256: n 4096 (128) 92 / 103, but 75 / 56 if 15 % of
+//   the rows are live, 6000 (192) 104 / 138
 bool large_tiles(int32_t n, int64_t vocab, int32_t hidden, bool grad) {
   if (hidden % 128 || n <= 128) return false;
-  return (grad && n > 4096) || ((int64_t)n + 255) / 256 * ((vocab + 255) / 256) * ((hidden + 255) / 256) >= 240;
+  const int64_t tiles = ((int64_t)n + 255) / 256 * ((vocab + 255) / 256);
+  return grad ? n > 4096 || tiles * hidden >= 500 * 256 : tiles >= 192;
 }
 
 VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int32_t k, bool distill, bool grad) {

@@ -63,8 +63,9 @@ def _check(h, w, b, run, p, live, temperature, reduction, seed, entropy=None):
 SIZES = [(1, 1, 64), (1, 2, 64), (2, 63, 64), (3, 65, 128), (37, 2000, 128), (64, 128, 64), (65, 129, 192), (130, 777, 320),
          (257, 1000, 768), (300, 4099, 256), (1000, 300, 512), (513, 30522, 128), (20, 30522, 768), (2600, 1300, 128), (1500, 2500, 384),
          (1030, 5, 1024), (70, 500, 2048), (300, 600, 1152), (130, 300, 8192),
-         # large tiles: 240 blocks of 256^3
-         (257, 30700, 128), (129, 10300, 1408), (300, 9001, 1152), (1030, 4099, 1024), (2600, 8003, 128), (1500, 10001, 384), (20500, 700, 256), (4100, 65, 256)]
+         # large tiles for the loss (192 of them), and below for gradients (500 blocks of 256^3)
+         (257, 30700, 128), (129, 10300, 1408), (300, 9001, 1152), (1030, 4099, 1024), (2600, 8003, 128), (1500, 10001, 384), (20500, 700, 256), (4100, 65, 256),
+         (257, 128100, 128), (129, 24001, 1408), (300, 14501, 1152), (1030, 6500, 1024), (2600, 24003, 128), (1500, 15001, 384)]
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -79,7 +80,7 @@ def test_cross_entropy_sizes(n, vocab, hidden, dtype):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("ignored", [0.0, 0.6, 0.97, 1.1])
-@pytest.mark.parametrize("vocab", [523, 30523])
+@pytest.mark.parametrize("vocab", [523, 30523, 128100])
 def test_cross_entropy_reductions_and_ignored_rows(vocab, dtype, reduction, ignored):
     n, hidden = 401, 128
     h, w, b = R.make(n, vocab, hidden, dtype, 3)
@@ -158,7 +159,7 @@ def test_without_bias_and_with_entries_left_out(dtype):
     assert losses.linear_cross_entropy(h, w, torch.full_like(b, -INF), y, reduction="none").isnan().all()
 
 
-@pytest.mark.parametrize("n,vocab,hidden", [(140, 300, 64), (300, 30800, 128), (50, 300, 64)])
+@pytest.mark.parametrize("n,vocab,hidden", [(140, 300, 64), (300, 30800, 128), (300, 128100, 128), (50, 300, 64)])
 def test_non_finite_rows_stay_in_their_rows(n, vocab, hidden):
     h, w, b = R.make(n, vocab, hidden, BF16, 12)
     h[5], h[37, 3] = NAN, INF
@@ -214,7 +215,7 @@ def test_strides_and_shapes(dtype):
     assert one.shape == () and torch.equal(one, row3.view(-1)[live][0])
 
 
-@pytest.mark.parametrize("n,vocab", [(1, 500), (30, 500), (64, 500), (100, 500), (300, 500), (300, 31000), (1300, 31000)])
+@pytest.mark.parametrize("n,vocab", [(1, 500), (30, 500), (64, 500), (100, 500), (300, 500), (300, 31000), (1300, 31000), (300, 128100), (1300, 43000)])
 def test_row_strides_by_size(n, vocab):
     """rows read in place (few), copied by aligned and by unaligned loads: the same bits from every layout"""
     hidden = 128
@@ -237,7 +238,7 @@ def test_row_strides_by_size(n, vocab):
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("distill", [0, 2, 70])
-@pytest.mark.parametrize("n,vocab", [(1, 600), (40, 600), (64, 600), (100, 600), (700, 600), (700, 21000)])
+@pytest.mark.parametrize("n,vocab", [(1, 600), (40, 600), (64, 600), (100, 600), (700, 600), (700, 21000), (700, 85500)])
 def test_what_the_rounded_score_gradients_leave_is_put_back(n, vocab, distill, dtype):
     """The large entries of a row reach dhidden unrounded; dweight of at most 64 rows is made of high and low parts, whose
     product is off by the square of a half step."""
@@ -362,7 +363,7 @@ def test_few_rows_in_several_pieces(n, distill):
 @pytest.mark.parametrize("n,vocab,hidden,k,temperature", [
     (1, 1, 64, 1, 1.0), (1, 30, 64, 30, 2.0), (3, 65, 128, 7, 0.5), (70, 1000, 128, 64, 2.0), (130, 777, 320, 65, 4.0),
     (33, 2000, 64, 200, 1.0), (300, 3001, 256, 16, 1.5), (9, 1500, 64, 1024, 3.0), (19, 30522, 768, 8, 1.0),
-    (300, 30801, 128, 16, 1.5), (1100, 12345, 256, 100, 2.0)])
+    (300, 30801, 128, 16, 1.5), (1100, 12345, 256, 100, 2.0), (300, 128100, 128, 16, 1.5), (1100, 25701, 256, 100, 2.0)])
 def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
     h, w, b = R.make(n, vocab, hidden, dtype, n + k)
     values, index = _teacher(n, vocab, k, n)
@@ -373,7 +374,8 @@ def test_distillation_sizes(n, vocab, hidden, k, temperature, dtype):
 
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("n,vocab,k", [(150, 400, 12), (300, 30800, 12), (60, 400, 12), (150, 400, 65), (60, 400, 300), (300, 30800, 300)])
+@pytest.mark.parametrize("n,vocab,k", [(150, 400, 12), (300, 30800, 12), (60, 400, 12), (150, 400, 65), (60, 400, 300), (300, 30800, 300),
+                                       (300, 128100, 12), (300, 128100, 300)])
 def test_distillation_ragged_empty_and_repeated_entries(n, vocab, k, dtype, reduction):
     hidden = 128
     h, w, b = R.make(n, vocab, hidden, dtype, 5)
@@ -395,7 +397,7 @@ def test_distillation_ragged_empty_and_repeated_entries(n, vocab, k, dtype, redu
     assert not grads[0][~live].any()
 
 
-@pytest.mark.parametrize("n,vocab,k", [(30, 100, 4), (100, 100, 4), (300, 30800, 4), (30, 100, 90)])
+@pytest.mark.parametrize("n,vocab,k", [(30, 100, 4), (100, 100, 4), (300, 30800, 4), (300, 128100, 4), (30, 100, 90)])
 def test_distillation_of_bad_entries_is_nan(n, vocab, k):
     h, w, b = R.make(n, vocab, 128, BF16, 5)
     values, index = _teacher(n, vocab, k, 6)
@@ -525,7 +527,7 @@ def test_teacher_to_student_step():
         R.assert_within(name, got, x + y_, e + f + (u if name != "db" else R.F32) * 1.01 * (x + y_).abs())
 
 
-@pytest.mark.parametrize("n,vocab", [(500, 3000), (500, 31000), (50, 3000)])
+@pytest.mark.parametrize("n,vocab", [(500, 3000), (500, 31000), (500, 128100), (50, 3000)])
 def test_other_stream(n, vocab):
     h, w, b = R.make(n, vocab, 128, BF16, 60)
     y = _labels(n, vocab, 61)
@@ -542,7 +544,7 @@ def test_other_stream(n, vocab):
         assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
-@pytest.mark.parametrize("n,vocab", [(90, 1111), (50, 1111), (400, 31111), (4200, 4000)])
+@pytest.mark.parametrize("n,vocab", [(90, 1111), (50, 1111), (400, 31111), (400, 128111), (4200, 4000)])
 def test_captured_step_replays(n, vocab):
     hidden = 128
     h, w, b = R.make(n, vocab, hidden, BF16, 70)
@@ -615,7 +617,7 @@ def test_backward_accumulates_and_repeats():
 
 
 @pytest.mark.parametrize("up", [0.0, -2.0, 65536.0, 1e-30])
-@pytest.mark.parametrize("n,vocab", [(90, 700), (40, 700), (300, 30800)])
+@pytest.mark.parametrize("n,vocab", [(90, 700), (40, 700), (300, 30800), (300, 128100)])
 def test_upstream_gradients(n, vocab, up):
     h, w, b = R.make(n, vocab, 128, BF16, 40)
     y = _labels(n, vocab, 41)
@@ -650,7 +652,8 @@ def test_ignore_index_inside_the_vocabulary():
 # ---------------------------------------------------------------- the C ABI itself
 @pytest.mark.parametrize("n,vocab,hidden,ld_dh,ld_dw,k", [(50, 300, 64, 71, 68, 0), (100, 1000, 128, 128, 132, 5), (300, 1111, 128, 129, 136, 0),
                                                           (700, 4000, 384, 384, 388, 70), (1500, 257, 128, 128, 128, 0),
-                                                          (300, 31111, 128, 129, 136, 0), (700, 24001, 128, 128, 132, 70), (5000, 3300, 128, 128, 128, 0), (4100, 257, 128, 128, 128, 3)])
+                                                          (300, 31111, 128, 129, 136, 0), (700, 24001, 128, 128, 132, 70), (5000, 3300, 128, 128, 128, 0), (4100, 257, 128, 128, 128, 3),
+                                                          (300, 128111, 128, 129, 136, 0), (700, 85501, 128, 128, 132, 70)])
 def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     """Row strides of the outputs, a workspace of exactly the size asked for and full of NaN, and untouched bytes around
     every output and behind the workspace; the same bits as the Python call."""
