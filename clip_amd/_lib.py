@@ -55,7 +55,7 @@ SIGNATURES = {
     "clip_linear_ce": [_p, _p, _i64, _i32, _p, _p, _p, _p, _p, _i64, _p],
     "clip_linear_ce_grad": [_p, _p, _i64, _i32, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p],
     "clip_linear_distill": [_p, _p, _p, _i32, _f, _i32, _p, _p, _p, _p, _p, _i64, _p],
-    "clip_linear_distill_grad": [_p, _p, _p, _i32, _f, _i32, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p],
+    "clip_linear_distill_grad": [_p, _p, _i32, _f, _i32, _p, _p, _p, _p, _i64, _p, _i64, _p, _p, _i64, _p],
     "clip_topk_scores": [_i32, _p, _i64, _i32, _i32, _i32, _p, _p, _p],
     "clip_gemm_bf16": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],
     "clip_gemm_f16": [_p, _p, _p, _p, _p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p],

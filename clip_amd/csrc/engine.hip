@@ -675,7 +675,7 @@ int linear_args(const char* who, const clip_linear* d, int32_t k, const int64_t*
   int rc = check_linear(who, d);
   if (rc) return rc;
   if (!d->dev_weight || !work || reduction < REDUCE_NONE || reduction > REDUCE_SUM ||
-      (d->n > 0 && (!d->dev_hidden || (k ? !t_values || !t_index : !labels))))
+      (d->n > 0 && (!d->dev_hidden || (k ? (!grad && !t_values) || !t_index : !labels))))
     return fail(CLIP_ERR_ARG, "%s: bad argument", who);
   if (((uintptr_t)d->dev_weight & 15) || ((uintptr_t)work & 15))
     return fail(CLIP_ERR_ARG, "%s: weight and workspace must be 16-byte aligned", who);
@@ -713,12 +713,12 @@ int linear_loss(const char* who, const clip_linear* d, int32_t k, const int64_t*
   return CLIP_OK;
 }
 
-int linear_grad(const char* who, const clip_linear* d, int32_t k, const int64_t* labels, int64_t ignore, const float* t_values,
-                const int64_t* t_index, float temperature, int32_t reduction, const float* lse, const float* target, const float* grad,
+int linear_grad(const char* who, const clip_linear* d, int32_t k, const int64_t* labels, int64_t ignore, const int64_t* t_index,
+                float temperature, int32_t reduction, const float* lse, const float* target, const float* grad,
                 uint16_t* dh, int64_t ld_dh, uint16_t* dw, int64_t ld_dw, float* dbias, void* work, int64_t work_bytes, void* stream) {
   VocabRows a;
   VocabPlan p;
-  const int rc = linear_args(who, d, k, labels, ignore, t_values, t_index, temperature, reduction, true, work, work_bytes, &a, &p);
+  const int rc = linear_args(who, d, k, labels, ignore, nullptr, t_index, temperature, reduction, true, work, work_bytes, &a, &p);
   if (rc) return rc;
   if ((d->n > 0 && (!lse || !target || !grad)) || (!grad && reduction != REDUCE_NONE)) return fail(CLIP_ERR_ARG, "%s: null argument", who);
   if (dh && d->n > 1 && ld_dh < d->hidden_size) return fail(CLIP_ERR_ARG, "%s: row stride of dhidden", who);
@@ -1033,7 +1033,7 @@ int clip_linear_ce(const clip_linear* d, const int64_t* labels, int64_t ignore_i
 int clip_linear_ce_grad(const clip_linear* d, const int64_t* labels, int64_t ignore_index, int32_t reduction, const float* lse,
                         const float* target, const float* grad, uint16_t* dhidden, int64_t ld_dhidden, uint16_t* dweight,
                         int64_t ld_dweight, float* dbias, void* work, int64_t work_bytes, void* stream) {
-  return linear_grad("clip_linear_ce_grad", d, 0, labels, ignore_index, nullptr, nullptr, 1.f, reduction, lse, target, grad, dhidden,
+  return linear_grad("clip_linear_ce_grad", d, 0, labels, ignore_index, nullptr, 1.f, reduction, lse, target, grad, dhidden,
                      ld_dhidden, dweight, ld_dweight, dbias, work, work_bytes, stream);
 }
 
@@ -1045,12 +1045,12 @@ int clip_linear_distill(const clip_linear* d, const float* teacher_values, const
                      target, loss, work, work_bytes, stream);
 }
 
-int clip_linear_distill_grad(const clip_linear* d, const float* teacher_values, const int64_t* teacher_index, int32_t k,
-                             float temperature, int32_t reduction, const float* lse, const float* target, const float* grad,
+int clip_linear_distill_grad(const clip_linear* d, const int64_t* teacher_index, int32_t k, float temperature,
+                             int32_t reduction, const float* lse, const float* target, const float* grad,
                              uint16_t* dhidden, int64_t ld_dhidden, uint16_t* dweight, int64_t ld_dweight, float* dbias, void* work,
                              int64_t work_bytes, void* stream) {
   if (k < 1) return fail(CLIP_ERR_ARG, "clip_linear_distill_grad: k = %d (1 .. 1024)", k);
-  return linear_grad("clip_linear_distill_grad", d, k, nullptr, 0, teacher_values, teacher_index, temperature, reduction, lse, target,
+  return linear_grad("clip_linear_distill_grad", d, k, nullptr, 0, teacher_index, temperature, reduction, lse, target,
                      grad, dhidden, ld_dhidden, dweight, ld_dweight, dbias, work, work_bytes, stream);
 }
 

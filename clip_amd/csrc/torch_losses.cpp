@@ -79,11 +79,11 @@ struct Call {
     check(entry.workspace(&d, k, grad, &bytes));
     return at::empty({bytes}, rows.options().dtype(at::kByte));
   }
-  // -> loss, and what the backward pass needs of it: the rows' lse and target scores
+  // -> loss, and what the backward pass needs of it: the rows' lse and dev_target
   Tensor forward(Tensor& kept) {
     const c10::DeviceGuard guard(rows.device());
     describe();
-    const int64_t n = d.n, kt = k ? k : 1;
+    const int64_t n = d.n, kt = k ? 2 * k + 1 : 1;   // floats a row of dev_target
     const auto f32 = rows.options().dtype(at::kFloat);
     // (the loss has storage of its own: a caller may change it in place before the backward pass reads what is kept)
     Tensor loss = reduction == 0 ? at::empty({n}, f32) : at::empty({}, f32);
@@ -107,7 +107,7 @@ struct Call {
     const Tensor work = workspace(1);
     const float *lse = ptr<>(kept), *target = lse + n;
     const int64_t ld = d.hidden_size;
-    check(k ? entry.distill_grad(&d, ptr<>(values), ptr<int64_t>(index), k, (float)temperature, (int32_t)reduction, lse, target, ptr<>(grad),
+    check(k ? entry.distill_grad(&d, ptr<int64_t>(index), k, (float)temperature, (int32_t)reduction, lse, target, ptr<>(grad),
                                  ptr<uint16_t>(dh), ld, ptr<uint16_t>(dw), ld, ptr<>(db), ptr<void>(work), work.numel(), stream_of(rows))
             : entry.ce_grad(&d, ptr<int64_t>(labels), ignore_index, (int32_t)reduction, lse, target, ptr<>(grad), ptr<uint16_t>(dh), ld,
                             ptr<uint16_t>(dw), ld, ptr<>(db), ptr<void>(work), work.numel(), stream_of(rows)));
@@ -121,7 +121,7 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
     Call call{hidden, weight, given(bias), given(labels), given(values), given(index), ignore_index, temperature, reduction, {}, 0};
     Tensor kept;
     Tensor loss = call.forward(kept);
-    ctx->save_for_backward({hidden, weight, given(bias), given(labels), given(values), given(index), kept});
+    ctx->save_for_backward({hidden, weight, given(bias), given(labels), given(index), kept});
     ctx->saved_data["args"] = std::vector<double>{(double)reduction, temperature};
     ctx->saved_data["ignore"] = ignore_index;
     return loss;
@@ -133,9 +133,9 @@ struct LinearLoss : torch::autograd::Function<LinearLoss> {
     variable_list out(9);
     {
       const at::AutoGradMode off(false);
-      Call call{hidden, saved[1], saved[2], saved[3], saved[4], saved[5], ctx->saved_data["ignore"].toInt(), args[1], (int64_t)args[0], {}, 0};
+      Call call{hidden, saved[1], saved[2], saved[3], Tensor(), saved[4], ctx->saved_data["ignore"].toInt(), args[1], (int64_t)args[0], {}, 0};
       Tensor dh;
-      call.backward(saved[6], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), saved[2].defined() && ctx->needs_input_grad(2),
+      call.backward(saved[5], grads[0], ctx->needs_input_grad(0), ctx->needs_input_grad(1), saved[2].defined() && ctx->needs_input_grad(2),
                     dh, out[1], out[2]);
       if (dh.defined()) out[0] = dh.view(hidden.sizes());
     }

@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
     if (j >= a.k) continue;
     const float x = t[u] * a.inv_t - ref;
     a.t_p[(int64_t)row * a.k + j] = t[u] != -INFINITY ? expf(x) / s : 0.f;
-    if (a.t_logp) a.t_logp[(int64_t)row * a.k + j] = x - log_s;
+    a.t_logp[(int64_t)row * a.k + j] = x - log_s;
   }
   const bool any_in = __any(n_in), any_bad = __any(bad);
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
@@ -1183,11 +1183,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   p.head = take(sizeof(VocabHead));
   p.row_map = take(rows * 4);
   p.block_base = take(rows / 16 * 4);
-  if (distill) {
-    p.state = take(rows * 4);
-    p.t_p = take((size_t)n * k * 4);
-    if (!grad) p.t_logp = take((size_t)n * k * 4);
-  }
+  if (distill && !grad) p.t_logp = take((size_t)n * k * 4);
   p.x = take(rows * hidden * 2);
   if (!grad) {
     p.part = take(rows * (vp / 64) * 8);
@@ -1258,10 +1254,12 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
   a.row_map = reinterpret_cast<int32_t*>(base + p.row_map);
   a.x = reinterpret_cast<bf16_t*>(base + p.x);
   if (a.t_index) {
-    a.state = reinterpret_cast<int32_t*>(base + p.state);
-    a.t_p = reinterpret_cast<float*>(base + p.t_p);
-    a.t_logp = GRAD ? nullptr : reinterpret_cast<float*>(base + p.t_logp);
-    if (a.n > 0) {
+    // kept by the forward for the backward: scores [n, k], p [n, k], states [n]
+    float* kept = GRAD ? const_cast<float*>(a.target_in) : a.target;
+    a.t_p = kept + (int64_t)a.n * a.k;
+    a.state = reinterpret_cast<int32_t*>(kept + (int64_t)a.n * a.k * 2);
+    if (!GRAD && a.n > 0) {
+      a.t_logp = reinterpret_cast<float*>(base + p.t_logp);
       const auto kfn = a.k > 64 ? vocab_teacher_kernel<16> : vocab_teacher_kernel<1>;
       hipLaunchKernelGGL(kfn, dim3((a.n + 3) / 4), dim3(256), 0, st, a);
       TRY(hipGetLastError());

@@ -218,13 +218,14 @@ int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t
  *   row_loss[i] = T^2 sum_j p_ij (log p_ij - log q_i[index_ij]).
  * An entry with a negative id or the value -inf is left out; a row with none left contributes nothing (loss 0, no gradient,
  * not counted by the mean).  Ids may repeat within a row.  An id >= vocab, a NaN or a +inf makes the row's loss NaN (and the
- * gradients).  1 <= k <= 1024.  dev_target is [n, k].  No counterpart in the reference. */
+ * gradients).  1 <= k <= 1024.  dev_target [n (2 k + 1)] is what the gradient call
+ * needs of the lists, which it does not read again.  No counterpart in the reference. */
 int clip_linear_distill(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index, int32_t k,
                         float temperature, int32_t reduction, float* dev_row_loss, float* dev_lse, float* dev_target,
                         float* dev_loss, void* dev_work, int64_t work_bytes, void* stream);
 /* Its gradients, dz_i = g_i T (q_i - p_i), as clip_linear_ce_grad (residuals for the teacher's ids with |q - p| >= 1/16). */
-int clip_linear_distill_grad(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index,
-                             int32_t k, float temperature, int32_t reduction, const float* dev_lse,
+int clip_linear_distill_grad(const clip_linear* d, const int64_t* dev_teacher_index, int32_t k, float temperature,
+                             int32_t reduction, const float* dev_lse,
                              const float* dev_target, const float* dev_grad, uint16_t* dev_dhidden, int64_t ld_dhidden,
                              uint16_t* dev_dweight, int64_t ld_dweight, float* dev_dbias, void* dev_work,
                              int64_t work_bytes, void* stream);

@@ -678,7 +678,7 @@ def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     st = torch.cuda.current_stream().cuda_stream
     need = C.c_int64()
     bufs = {}
-    for name, size in (("row", 4 * n), ("lse", 4 * n), ("target", 4 * n * max(k, 1)), ("loss", 4), ("dh", 2 * n * ld_dh), ("dw", 2 * vocab * ld_dw),
+    for name, size in (("row", 4 * n), ("lse", 4 * n), ("target", 4 * n * (2 * k + 1)), ("loss", 4), ("dh", 2 * n * ld_dh), ("dw", 2 * vocab * ld_dw),
                        ("db", 4 * vocab)):
         bufs[name] = (*guarded(size), size)
     at = {name: v[1] for name, v in bufs.items()}
@@ -693,7 +693,7 @@ def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
                 lib.clip_linear_ce(C.byref(d), y.data_ptr(), -100, *tail)
         else:
             tail = (1, at["lse"], at["target"], one.data_ptr(), at["dh"], ld_dh, at["dw"], ld_dw, at["db"], base, need.value, st)
-            rc = lib.clip_linear_distill_grad(C.byref(d), values.data_ptr(), index.data_ptr(), k, 2.0, *tail) if k else \
+            rc = lib.clip_linear_distill_grad(C.byref(d), index.data_ptr(), k, 2.0, *tail) if k else \
                 lib.clip_linear_ce_grad(C.byref(d), y.data_ptr(), -100, *tail)
         _lib.check(rc)
         torch.cuda.synchronize()
@@ -713,7 +713,7 @@ def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
         bufs[name][0][GUARD:GUARD + bufs[name][2]] = 0xA5
         a = {x: (at[x] if x == name else None) for x in ("dh", "dw", "db")}
         tail = (1, at["lse"], at["target"], one.data_ptr(), a["dh"], ld_dh, a["dw"], ld_dw, a["db"], base, need.value, st)
-        rc = lib.clip_linear_distill_grad(C.byref(d), values.data_ptr(), index.data_ptr(), k, 2.0, *tail) if k else \
+        rc = lib.clip_linear_distill_grad(C.byref(d), index.data_ptr(), k, 2.0, *tail) if k else \
             lib.clip_linear_ce_grad(C.byref(d), y.data_ptr(), -100, *tail)
         _lib.check(rc)
     torch.cuda.synchronize()

@@ -65,7 +65,7 @@ def test_calls_refused_without_a_device():
         assert lib.clip_linear_ce(C.byref(bad), *ok) == _lib.CLIP_ERR_ARG
     for k, t in ((0, 1.0), (1025, 1.0), (4, 0.0), (4, -1.0), (4, float("inf")), (4, float("nan"))):
         assert lib.clip_linear_distill(C.byref(d), p, p, k, t, 1, p, p, p, p, p, big, None) == _lib.CLIP_ERR_ARG
-        assert lib.clip_linear_distill_grad(C.byref(d), p, p, k, t, 1, p, p, p, p, 128, p, 128, p, p, big, None) == _lib.CLIP_ERR_ARG
+        assert lib.clip_linear_distill_grad(C.byref(d), p, k, t, 1, p, p, p, p, 128, p, 128, p, p, big, None) == _lib.CLIP_ERR_ARG
     grad = [p, -100, 1, p, p, p, p, 128, p, 128, p, p, big, None]
     for i, v in ((0, None), (3, None), (4, None), (5, None), (7, 64), (8, C.c_void_p(4100)), (9, 64), (9, 130), (11, None)):
         args = list(grad)
