@@ -122,7 +122,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   const int64_t* t_index; int64_t ld_ti;          // their vocabulary ids (negative: left out)
   float inv_t, loss_factor, grad_factor;          // 1 / T, T^2, T
   bool mean;                                      // the mean over live rows (else the sum, or the rows)
-  float *row_loss, *lse_out, *target, *loss;      // forward: [n], [n], [n, k] scores / T of the targets, [1]
+  float *row_loss, *lse_out, *target, *loss;      // forward: [n], [n], [n, k] scores / T of the targets (and t_p, state), [1]
   const float *lse, *target_in;                   // backward: what the forward left
   const float* grad; bool grad_rows;              // upstream gradient: [n] or [1]
   bf16_t* dh; int64_t ld_dh;
@@ -137,7 +137,8 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   int32_t tiles_h, piece_tiles[2], max_splits, wgs;   // what they are chosen from (wgs 0: max_splits itself)
   int64_t dh_room, dw_room;   // floats of partials
   bool with_dw, dh_aligned;
-  float *t_p, *t_logp, *out_scale;
+  float *t_p, *t_logp;      // distillation: the teacher's p and log p, [n, k]; state: 0 no entry, 1 live, 2 a bad entry
+  float* out_scale;
   bf16_t* x;
   float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
   float2* row_lc;           // distillation: (lse log2(e), c)
@@ -145,7 +146,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   bool low;                 // G's rows 64 .. 127 hold what the rounding of its rows 0 .. 63 left (few rows)
   int64_t* fix;
 };
-struct VocabGemm {          // arguments of vocab_gemm_kernel
+struct VocabGemm {          // arguments of the product kernels
   const bf16_t *x, *w;
   const float* bias;
   int64_t ldw, vocab, v0;   // v0: first vocabulary entry of the piece

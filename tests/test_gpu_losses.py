@@ -413,6 +413,19 @@ def test_distillation_of_bad_entries_is_nan(n, vocab, k):
     assert torch.equal(dh.isnan().any(1), bad) and dw.isnan().all() and db.isnan().all()
 
 
+@pytest.mark.parametrize("k", [1, 100])
+def test_distillation_of_no_rows(k):
+    h, w, b = (t.requires_grad_() for t in R.make(3, 200, 128, BF16, 5))
+    values, index = _teacher(3, 200, k, 6)
+    for rows in (0, 3):                       # none at all; none with an entry
+        ix = index[:rows].clone().fill_(-1)
+        for red in ("mean", "sum", "none"):
+            loss = losses.linear_distillation(h[:rows], w, b, values[:rows], ix, reduction=red)
+            assert loss.isnan() if red == "mean" else not loss.any()
+            grads = torch.autograd.grad(loss.sum(), (h, w, b))
+            assert not any(g.any() for g in grads)
+
+
 def test_distillation_of_itself_is_zero():
     # the teacher lists the whole vocabulary with the student's own scores: loss and gradient vanish up to rounding
     n, vocab, hidden = 40, 60, 64
