@@ -706,7 +706,8 @@ int linear_loss(const char* who, const clip_linear* d, int32_t k, const int64_t*
   const int rc = linear_args(who, d, k, labels, ignore, t_values, t_index, temperature, reduction, false, work, work_bytes, &a, &p);
   if (rc) return rc;
   if ((d->n > 0 && (!row_loss || !lse || !target)) || (reduction != REDUCE_NONE && !loss)) return fail(CLIP_ERR_ARG, "%s: null output", who);
-  a.row_loss = row_loss; a.lse_out = lse; a.target = target;
+  if ((uintptr_t)lse & 7) return fail(CLIP_ERR_ARG, "%s: dev_lse must be 8-byte aligned", who);
+  a.row_loss = row_loss; a.lse_out = reinterpret_cast<float2*>(lse); a.target = target;
   a.loss = reduction == REDUCE_NONE ? nullptr : loss;
   HIP_TRY(d->operand == CLIP_PRECISION_F16 ? k_f16::launch_vocab_loss(a, p, work, (hipStream_t)stream)
                                            : k_bf16::launch_vocab_loss(a, p, work, (hipStream_t)stream));
@@ -724,7 +725,8 @@ int linear_grad(const char* who, const clip_linear* d, int32_t k, const int64_t*
   if (dh && d->n > 1 && ld_dh < d->hidden_size) return fail(CLIP_ERR_ARG, "%s: row stride of dhidden", who);
   if (dw && (((uintptr_t)dw & 7) || ld_dw % 4 || ld_dw < d->hidden_size))
     return fail(CLIP_ERR_ARG, "%s: dweight must be 8-byte aligned with a row stride that is a multiple of 4", who);
-  a.lse = lse; a.target_in = target; a.grad = grad;
+  if ((uintptr_t)lse & 7) return fail(CLIP_ERR_ARG, "%s: dev_lse must be 8-byte aligned", who);
+  a.lse = reinterpret_cast<const float2*>(lse); a.target_in = target; a.grad = grad;
   a.grad_rows = reduction == REDUCE_NONE;
   a.dh = dh; a.ld_dh = ld_dh; a.dbias = dbias;
   HIP_TRY(d->operand == CLIP_PRECISION_F16 ? k_f16::launch_vocab_grad(a, p, dw, ld_dw, work, (hipStream_t)stream)

@@ -122,8 +122,9 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   const int64_t* t_index; int64_t ld_ti;          // their vocabulary ids (negative: left out)
   float inv_t, loss_factor, grad_factor;          // 1 / T, T^2, T
   bool mean;                                      // the mean over live rows (else the sum, or the rows)
-  float *row_loss, *lse_out, *target, *loss;      // forward: [n], [n], [n, k] scores / T of the targets (and t_p, state), [1]
-  const float *lse, *target_in;                   // backward: what the forward left
+  float *row_loss, *target, *loss; float2* lse_out;   // forward: [n], [n, k] scores / T of the targets (and t_p, state), [1],
+                                                  // [n] (m, s): logsumexp = ln2 m + ln s, m the largest score / T * log2(e)
+  const float2* lse; const float* target_in;      // backward: what the forward left
   const float* grad; bool grad_rows;              // upstream gradient: [n] or [1]
   bf16_t* dh; int64_t ld_dh;
   float* dbias;
@@ -141,7 +142,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   float* out_scale;
   bf16_t* x;
   float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
-  float2* row_lc;           // distillation: (lse log2(e), c)
+  float4* row_lc;           // distillation: (m, 1 / s, c)
   float2* row_fix;          // distillation: up to ROW_FIX (vocabulary id, what G's rounding left of its entry) per live row
   bool low;                 // G's rows 64 .. 127 hold what the rounding of its rows 0 .. 63 left (few rows)
   int64_t* fix;

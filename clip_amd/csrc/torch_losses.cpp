@@ -87,8 +87,8 @@ struct Call {
     const auto f32 = rows.options().dtype(at::kFloat);
     // (the loss has storage of its own: a caller may change it in place before the backward pass reads what is kept)
     Tensor loss = reduction == 0 ? at::empty({n}, f32) : at::empty({}, f32);
-    kept = at::empty({(reduction == 0 ? 1 + kt : 2 + kt) * n}, f32);
-    float *lse = ptr<>(kept), *target = lse + n, *row_loss = reduction == 0 ? ptr<>(loss) : target + kt * n;
+    kept = at::empty({(reduction == 0 ? 2 + kt : 3 + kt) * n}, f32);
+    float *lse = ptr<>(kept), *target = lse + 2 * n, *row_loss = reduction == 0 ? ptr<>(loss) : target + kt * n;
     const Tensor work = workspace(0);
     check(k ? entry.distill(&d, ptr<>(values), ptr<int64_t>(index), k, (float)temperature, (int32_t)reduction, row_loss, lse, target,
                             ptr<>(loss), ptr<void>(work), work.numel(), stream_of(rows))
@@ -105,7 +105,7 @@ struct Call {
     if (need_w) dw = at::empty(weight.sizes(), weight.options());
     if (need_b) db = at::empty({weight.size(0)}, rows.options().dtype(at::kFloat));
     const Tensor work = workspace(1);
-    const float *lse = ptr<>(kept), *target = lse + n;
+    const float *lse = ptr<>(kept), *target = lse + 2 * n;
     const int64_t ld = d.hidden_size;
     check(k ? entry.distill_grad(&d, ptr<int64_t>(index), k, (float)temperature, (int32_t)reduction, lse, target, ptr<>(grad),
                                  ptr<uint16_t>(dh), ld, ptr<uint16_t>(dw), ld, ptr<>(db), ptr<void>(work), work.numel(), stream_of(rows))

@@ -189,21 +189,22 @@ __device__ void write_head(const VocabRows& a, int total, float grad_max, int la
   }
 }
 
-// what V_GRAD needs of a live row: (x, y, label, t), G = y exp2(z log2(e) / T - x) but t at the label; lc: (lse log2(e), c)
-__device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st, float grad_max, float2& lc) {
+// what V_GRAD needs of a live row: (x, y, label, t), G = y exp2(z log2(e) / T - x) but t at the label; lc: (x, 1 / sum, c).  x is the
+// row's largest score and not its logsumexp: where q is large the exponent is small, and so is its rounding
+__device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st, float grad_max, float4& lc) {
   float c = 1.f;
   if (a.grad_rows) {
     const float g = a.grad[r];
     c = fabsf(g) < INFINITY ? (grad_max > 0.f ? g / grad_max : 0.f) : g;
   }
   if (st == 2) c = __builtin_nanf("");   // the target is outside the vocabulary
-  const float l2 = a.lse[r] * LOG2E;
-  lc = make_float2(l2, c);
-  // x takes |c| and G's scale, y its sign
-  float4 info = make_float4(l2 - log2f(fabsf(c) * G_SCALE), c < 0.f ? -1.f : 1.f, __int_as_float(-1), 0.f);
+  const float2 lse = a.lse[r];
+  const float x = lse.x == -INFINITY ? 0.f : lse.x, inv = 1.f / lse.y;
+  lc = make_float4(x, inv, c, 0.f);
+  float4 info = make_float4(x, c * G_SCALE * inv, __int_as_float(-1), 0.f);
   if (!a.state && st == 1) {
     info.z = __int_as_float((int)a.labels[r]);
-    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -l2)) - 1.f) * G_SCALE;
+    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -x)) * inv - 1.f) * G_SCALE;
   }
   return info;
 }
@@ -225,7 +226,7 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
     if (lane >= count) map[lane] = -1;
     if (st != 0) {
       map[rank] = lane;
-      float2 lc;
+      float4 lc;
       if (GRAD) info[rank] = row_info_of(a, lane, st, gm, lc);
       if (blockIdx.x == 0) {
         a.row_map[rank] = st == 2 ? ~lane : lane;
@@ -234,7 +235,7 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
       }
     } else if (!GRAD && blockIdx.x == 0 && lane < a.n) {
       a.row_loss[lane] = 0.f;
-      a.lse_out[lane] = 0.f;
+      a.lse_out[lane] = make_float2(0.f, 1.f);
     }
     if (blockIdx.x == 0) write_head<GRAD>(a, count, gm, lane);
   }
@@ -705,13 +706,13 @@ __global__ __launch_bounds__(NT) void vocab_pack_kernel(VocabRows a) {
       const int rank = before + __popcll(live & ((1ull << lane) - 1));
       a.row_map[rank] = st == 2 ? ~r : r;    // a row whose target is outside the vocabulary: NaN loss and gradients
       if (GRAD) {
-        float2 lc;
+        float4 lc;
         a.row_info[rank] = row_info_of(a, r, st, gm, lc);
         if (a.state) a.row_lc[rank] = lc;
       }
     } else if (!GRAD) {
       a.row_loss[r] = 0.f;
-      a.lse_out[r] = 0.f;
+      a.lse_out[r] = make_float2(0.f, 1.f);
     }
   }
   const int pad = (total + a.tile_rows - 1) / a.tile_rows * a.tile_rows;
@@ -792,11 +793,11 @@ __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2
       const int64_t v = a.labels[row];
       z = wave_score(a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
     }
-    const float lse = lse_of(wave_pairs(part + (int64_t)r * n_part, n_part, lane, 64));
-    if (mapped >= 0) loss = lse - z;
+    const float2 all = wave_pairs(part + (int64_t)r * n_part, n_part, lane, 64);
+    if (mapped >= 0) loss = lse_of(all) - z;
     if (lane == 0) {
       a.target[row] = z;
-      a.lse_out[row] = lse;
+      a.lse_out[row] = all;
       __hip_atomic_store(a.row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
@@ -879,7 +880,7 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
     }
     if (w == 0 && lane == 0) {
       loss = mapped < 0 ? __builtin_nanf("") : loss * a.loss_factor;
-      a.lse_out[row] = lse;
+      a.lse_out[row] = all;
       __hip_atomic_store(a.row_loss + row, loss, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
@@ -912,13 +913,13 @@ __global__ __launch_bounds__(1024) void vocab_reduce_kernel(VocabRows a) {
 // same in most rows.
 // `first`: this entry is the first of its row to name v (0 <= v), `p` what they add up to, `own` its own part.  Returns whether
 // the entry is a sixteenth or more of the row, and what rounding leaves of it.
-__device__ __forceinline__ bool teacher_entry(const VocabRows& a, const float2& lc, int r, int row, int j, int v, float own, float p, bool first,
+__device__ __forceinline__ bool teacher_entry(const VocabRows& a, const float4& lc, int r, int row, int j, int v, float own, float p, bool first,
                                               bf16_t* g, int64_t ldg, int64_t v0, int64_t v1, int table, float& rest) {
-  if (a.fix && table && v >= 0 && fabsf(lc.y * own) <= 1.f)
-    atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.y * own) * FIX));
+  if (a.fix && table && v >= 0 && fabsf(lc.z * own) <= 1.f)
+    atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.z * own) * FIX));
   if (!first) return false;
-  const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x));
-  const float e = lc.y * (q - p) * G_SCALE;
+  const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x)) * lc.y;
+  const float e = lc.z * (q - p) * G_SCALE;
   if (v >= v0 && v < v1) {
     g[(int64_t)r * ldg + (v - v0)] = f32_to_op(e);
     if (a.low) g[(int64_t)(r + 64) * ldg + (v - v0)] = f32_to_op(residual(e));
@@ -977,7 +978,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_hash_kernel(VocabRows a, bf
     if (fix && tid < ROW_FIX) fix[tid] = make_float2(__int_as_float(-1), 0.f);
     return;
   }
-  const float2 lc = a.row_lc[r];
+  const float4 lc = a.row_lc[r];
   int v[EACH], slot[EACH];
   float own[EACH], rest[EACH];
 #pragma unroll
@@ -1190,7 +1191,7 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   } else {
     p.row_info = take(rows * 16);
     if (distill) {
-      p.row_lc = take(rows * 8);
+      p.row_lc = take(rows * 16);
       p.row_fix = take(rows * 8 * ROW_FIX);
       p.fix = take(vocab * 8 * FIX_COPIES);
     }
@@ -1340,7 +1341,7 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   char* base = static_cast<char*>(work);
   a.row_info = reinterpret_cast<float4*>(base + p.row_info);
   if (a.t_index) {
-    a.row_lc = reinterpret_cast<float2*>(base + p.row_lc);
+    a.row_lc = reinterpret_cast<float4*>(base + p.row_lc);
     a.row_fix = reinterpret_cast<float2*>(base + p.row_fix);
     a.fix = a.dbias ? reinterpret_cast<int64_t*>(base + p.fix) : nullptr;
   }

@@ -691,7 +691,7 @@ def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     st = torch.cuda.current_stream().cuda_stream
     need = C.c_int64()
     bufs = {}
-    for name, size in (("row", 4 * n), ("lse", 4 * n), ("target", 4 * n * (2 * k + 1)), ("loss", 4), ("dh", 2 * n * ld_dh), ("dw", 2 * vocab * ld_dw),
+    for name, size in (("row", 4 * n), ("lse", 8 * n), ("target", 4 * n * (2 * k + 1)), ("loss", 4), ("dh", 2 * n * ld_dh), ("dw", 2 * vocab * ld_dw),
                        ("db", 4 * vocab)):
         bufs[name] = (*guarded(size), size)
     at = {name: v[1] for name, v in bufs.items()}
