@@ -94,13 +94,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   __syncthreads();
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = wave_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
 
 // ---- how the two products of a piece share the workgroups (one wave; result in lane 0).  Time is counted in pairs of K
 // tiles: a dW tile takes rows / 128 of them, a dh tile 2 x (vocabulary tiles) / splits, and an epilogue some more (dW: 128 KB
@@ -1207,10 +1200,13 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     p.g = take(rows * p.piece * 2);
     p.ld_colsum = vp;
     p.colsum = take((rows / 64) * vp * 4);
-    // dh = G W has few tiles and a long k, which is split: until every CU has a workgroup (whose ring takes most of its LDS), or
-    // (large) as the schedule on the device finds best, within this many fp32 partials of the rows
-    const int64_t tiles = ((int64_t)n + p.tile_rows - 1) / p.tile_rows * ((hidden + 127) / 128);
-    int64_t s = tiles > 0 ? 256 / tiles : 1;
+    // dh = G W has few tiles and a long k, which is split: so that half of the CUs have a workgroup (dW's take the rest of them) or,
+    // where its parts would be longer than 64 K tiles, up to all; (large) as the schedule on the device finds best, within this many
+    // fp32 partials of the rows.  A step, us, all CUs / half: 19 rows of V 30 522 68 / 65, 64 rows (V 40 000, H 1024) 102 / 97, 1000 rows
+    // (V 2 000, H 512) 68 / 64; 4000 rows (V 30 522, H 192) 421 / 473
+    const int64_t tiles = ((int64_t)n + p.tile_rows - 1) / p.tile_rows * ((hidden + 127) / 128), parts = p.piece / BK / 64;
+    int64_t s = tiles > 0 ? (p.large ? 256 : 128) / tiles : 1;
+    if (!p.large && tiles > 0 && s < parts) s = parts < 256 / tiles ? parts : 256 / tiles;
     if (s > p.piece / 256) s = p.piece / 256;
     p.splits = (int32_t)(s < 1 ? 1 : s);
     p.dh_slot = rows * hidden;
