@@ -557,6 +557,46 @@ def test_other_stream(n, vocab):
         assert all(torch.equal(a, b) for a, b in zip(g, want))
 
 
+def test_calls_from_several_threads():
+    from concurrent.futures import ThreadPoolExecutor
+    cases = []
+    for n, vocab in ((40, 3000), (300, 2000), (1, 500), (600, 31000)):
+        h, w, b = R.make(n, vocab, 128, BF16, n)
+        y, (values, index) = _labels(n, vocab, n, 0.2), _teacher(n, vocab, 9, n)
+        y[0] = 5
+        cases.append((h, w, b, y, values, index))
+
+    def step(case):
+        h, w, b, y, values, index = case
+        with torch.cuda.stream(torch.cuda.Stream()):
+            leaves = [t.detach().requires_grad_() for t in (h, w, b)]
+            ce = losses.linear_cross_entropy(*leaves, y)
+            kd = losses.linear_distillation(*leaves, values, index, reduction="sum")
+            out = (ce.detach(), kd.detach(), *torch.autograd.grad(ce, leaves), *torch.autograd.grad(kd, leaves), *losses.topk_logits(w, 5))
+            torch.cuda.current_stream().synchronize()
+        return out
+    torch.cuda.synchronize()
+    want = [step(c) for c in cases]
+    with ThreadPoolExecutor(4) as pool:
+        for _ in range(3):
+            for got, ref in zip(pool.map(step, cases), want):
+                assert all(torch.equal(x, r) for x, r in zip(got, ref))
+
+
+def test_empty_shapes_and_inference_mode():
+    h, w, b = R.make(6, 300, 128, BF16, 5)
+    y = _labels(6, 300, 6)
+    with torch.inference_mode():
+        assert torch.equal(losses.linear_cross_entropy(h, w, b, y, reduction="none"),
+                           losses.linear_cross_entropy(h.clone(), w.clone(), b.clone(), y.clone(), reduction="none"))
+    empty = h[:0].view(2, 0, 128)
+    assert losses.linear_cross_entropy(empty, w, b, y[:0].view(2, 0), reduction="none").shape == (2, 0)
+    values, index = _teacher(0, 300, 4, 1)
+    assert losses.linear_distillation(empty, w, b, values.view(2, 0, 4), index.view(2, 0, 4), reduction="none").shape == (2, 0)
+    v, i = losses.topk_logits(w.view(3, 100, 128)[:, :0], 2)
+    assert v.shape == i.shape == (3, 0, 2)
+
+
 @pytest.mark.parametrize("n,vocab", [(90, 1111), (50, 1111), (400, 31111), (400, 128111), (4200, 4000)])
 def test_captured_step_replays(n, vocab):
     hidden = 128
