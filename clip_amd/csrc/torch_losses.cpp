@@ -47,11 +47,12 @@ Tensor rows_of(const Tensor& t) {
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
   return r.stride(1) == 1 && (r.size(0) < 2 || r.stride(0) >= r.size(1)) ? r : r.contiguous();
 }
-// [V, H] as the kernels read it: 16-byte aligned rows (a parameter is; anything else is copied)
+// [V, H] as the kernels read it: 16-byte aligned rows (a parameter is; anything else is copied.  contiguous() would hand back
+// what is contiguous already, wherever it starts and whatever the stride of a single row)
 Tensor decoder_of(const Tensor& w) {
   const bool ok = w.stride(1) == 1 && w.stride(0) % 8 == 0 && w.stride(0) >= w.size(1) && w.stride(0) <= (1 << 22) &&
                   reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0;
-  return ok ? w : w.contiguous();
+  return ok ? w : at::empty(w.sizes(), w.options()).copy_(w);
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 template <typename T = float>

@@ -215,6 +215,43 @@ def test_strides_and_shapes(dtype):
     assert one.shape == () and torch.equal(one, row3.view(-1)[live][0])
 
 
+@pytest.mark.parametrize("n,vocab", [(40, 333), (130, 333), (300, 30801), (300, 128101)])
+def test_weight_anywhere_in_a_flat_buffer(n, vocab):
+    """a contiguous weight whose first row starts on 2 or 8 bytes, as a view into flat parameters may: loss and gradients"""
+    hidden = 128
+    h, w, b = R.make(n, vocab, hidden, BF16, 15)
+    y = _labels(n, vocab, 16, 0.1)
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y)
+    want = (loss.detach(), *torch.autograd.grad(loss, leaves))
+    for at in (1, 4):
+        flat = torch.full((vocab * hidden + 8,), NAN, dtype=BF16, device="cuda")
+        flat[at:at + vocab * hidden] = w.view(-1)
+        flat.requires_grad_()
+        view = flat[at:at + vocab * hidden].view(vocab, hidden)
+        assert view.is_contiguous() and view.data_ptr() % 16 != 0
+        loss = losses.linear_cross_entropy(leaves[0], view, leaves[2], y)
+        dh, dflat, db = torch.autograd.grad(loss, (leaves[0], flat, leaves[2]))
+        got = (loss.detach(), dh, dflat[at:at + vocab * hidden].view(vocab, hidden), db)
+        assert all(torch.equal(g, r) for g, r in zip(got, want))
+        assert not dflat[:at].any() and not dflat[at + vocab * hidden:].any()
+
+
+def test_one_decoder_row_of_any_stride():
+    # (torch calls a single row contiguous whatever its stride is)
+    h, _, _ = R.make(9, 1, 64, BF16, 3)
+    y = torch.zeros(9, dtype=torch.int64).cuda()
+    wide = torch.randn(2, 131, generator=torch.Generator().manual_seed(4)).to(BF16).cuda()
+    one = wide[:1, :64]
+    assert one.is_contiguous() and one.stride(0) == 131
+    leaves = [h.clone().requires_grad_(), one.detach().requires_grad_()]
+    loss = losses.linear_cross_entropy(*leaves, None, y, reduction="none")
+    p, live = R.targets_ce(y, 1, -100)
+    want, err = R.reference(h, one, None, p, live, 1.0, torch.ones(9).cuda())
+    for name, got, a, e in zip(("loss", "dh", "dw"), (loss.detach(), *torch.autograd.grad(loss.sum(), leaves)), want, err):
+        R.assert_within(name, got, a, e)
+
+
 @pytest.mark.parametrize("n,vocab", [(1, 500), (30, 500), (64, 500), (100, 500), (300, 500), (300, 31000), (1300, 31000), (300, 128100), (1300, 43000)])
 def test_row_strides_by_size(n, vocab):
     """rows read in place (few), copied by aligned and by unaligned loads: the same bits from every layout"""
