@@ -9,6 +9,7 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include "../../include/clip_amd.h"
@@ -17,6 +18,7 @@ namespace {
 
 using at::Tensor;
 using torch::autograd::AutogradContext;
+using torch::autograd::isFwGradDefined;
 using torch::autograd::variable_list;
 typedef std::optional<Tensor> MaybeTensor;
 
@@ -168,6 +170,9 @@ int64_t reduction_code(const std::string& r) {
 }
 
 void check_linear(const Tensor& hidden, const Tensor& weight, const MaybeTensor& bias) {
+  // (the kernels read values only: the tangent of a dual number would be dropped, as if it were zero)
+  TORCH_CHECK_NOT_IMPLEMENTED(!isFwGradDefined(hidden) && !isFwGradDefined(weight) && !(bias && isFwGradDefined(*bias)),
+                              "clip_amd.losses: no forward-mode derivatives");
   TORCH_CHECK(hidden.is_cuda(), "hidden must be on an MI355X (cuda); clip_amd has no CPU execution path");
   TORCH_CHECK_TYPE((hidden.scalar_type() == at::kBFloat16 || hidden.scalar_type() == at::kHalf) && weight.scalar_type() == hidden.scalar_type(),
                    "hidden and weight must both be bfloat16 or float16, not ", hidden.scalar_type(), " and ", weight.scalar_type());

@@ -100,3 +100,20 @@ def test_missing_binding_raises(monkeypatch):
     monkeypatch.setattr(losses, "EXT_PATH", losses.EXT_PATH + ".missing")
     with pytest.raises(ImportError, match="build"):
         losses.topk_logits(torch.zeros(2, 5), 1)
+
+
+def test_forward_mode_derivatives_are_refused():
+    """a dual number's tangent would be lost without a word: the kernels read values only"""
+    import torch.autograd.forward_ad as fw
+    h, w, b = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(5, 64, dtype=torch.bfloat16), torch.zeros(5)
+    y = torch.zeros(2, dtype=torch.int64)
+    with fw.dual_level():
+        for i in range(3):
+            for grad in (False, True):
+                args = [fw.make_dual(t, torch.ones_like(t)) if i == j else t.clone().requires_grad_(grad) for j, t in enumerate((h, w, b))]
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    losses.linear_cross_entropy(*args, y)
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    losses.linear_distillation(*args, torch.zeros(2, 1), y[:, None])
+        with pytest.raises(RuntimeError, match="no CPU"):       # plain tensors pass that check
+            losses.linear_cross_entropy(h, w, b, y)
