@@ -4,7 +4,9 @@
 // caches on every line (forward + backward of 37 rows: 215 us through a Python autograd.Function and ctypes).
 // Nothing is computed here, and there is no fallback: every call goes to libclip_amd.so, whose entry points the Python host
 // hands over (so that CLIP_AMD_LIB holds for both).
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
@@ -169,7 +171,15 @@ int64_t reduction_code(const std::string& r) {
   return 2;
 }
 
+// A trace (torch.jit.trace, make_fx) would hold the allocation of the outputs and none of the kernels that fill them
+void check_tracing() {
+  TORCH_CHECK_NOT_IMPLEMENTED(!at::tracer::impl::is_dispatch_enabled() &&
+                                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                              "clip_amd.losses: the calls cannot be traced (torch.compile runs them outside its graphs)");
+}
+
 void check_linear(const Tensor& hidden, const Tensor& weight, const MaybeTensor& bias) {
+  check_tracing();
   // (the kernels read values only: the tangent of a dual number would be dropped, as if it were zero)
   TORCH_CHECK_NOT_IMPLEMENTED(!isFwGradDefined(hidden) && !isFwGradDefined(weight) && !(bias && isFwGradDefined(*bias)),
                               "clip_amd.losses: no forward-mode derivatives");
@@ -251,6 +261,7 @@ Tensor linear_distillation(const Tensor& hidden, const Tensor& weight, const May
 }
 
 std::tuple<Tensor, Tensor> topk_logits(const Tensor& logits, int64_t k) {
+  check_tracing();
   TORCH_CHECK(logits.is_cuda(), "logits must be on an MI355X (cuda); clip_amd has no CPU execution path");
   const auto type = logits.scalar_type();
   TORCH_CHECK_TYPE((type == at::kFloat || type == at::kBFloat16 || type == at::kHalf) && logits.dim() >= 1,

@@ -10,6 +10,8 @@ What sentclf/bert_model.py:165,175-179 computes as decoder scores + CrossEntropy
 [n, vocab] scores, forward or backward.  hidden and weight are bf16 or fp16 (their gradients too), the bias and all losses
 fp32.  Rows that take no part (labels equal to ignore_index, teacher rows without an entry) cost nothing in the products.
 Everything is queued on the current stream of the tensors' device; there is no host wait and no CPU execution path.
+Refused: second and forward-mode derivatives, and tracing (a trace would hold the outputs' allocation and not what fills them;
+torch.compile runs these calls outside its graphs).
 The tensor handling is in csrc/torch_losses.cpp (lib/_clip_torch.so), over the C ABI (clip_linear_ce and its neighbours).
 
 In a HIP graph: make one eager call of the same sizes first, and let go of eager losses of the same leaves before the capture (torch

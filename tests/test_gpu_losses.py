@@ -691,6 +691,20 @@ def test_capture_beside_a_living_eager_loss_is_refused():
         assert torch.equal(got, want)
 
 
+def test_compiled_caller():
+    # torch.compile leaves the calls outside its graphs: the same bits
+    h, w, b = R.make(66, 333, 128, BF16, 1)
+    y = _labels(66, 333, 2)
+
+    def step(h, w, b):
+        return 3 * losses.linear_cross_entropy((2 * h).relu(), w, b, y)
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    want = step(*leaves)
+    got = torch.compile(step, backend="eager")(*leaves)
+    assert torch.equal(got, want)
+    assert all(torch.equal(x, r) for x, r in zip(torch.autograd.grad(got, leaves), torch.autograd.grad(want, leaves)))
+
+
 def test_backward_accumulates_and_repeats():
     """.backward() into .grad, twice over one graph, and a weight shared by two losses"""
     h, w, b = R.make(60, 500, 128, BF16, 90)

@@ -117,3 +117,18 @@ def test_forward_mode_derivatives_are_refused():
                     losses.linear_distillation(*args, torch.zeros(2, 1), y[:, None])
         with pytest.raises(RuntimeError, match="no CPU"):       # plain tensors pass that check
             losses.linear_cross_entropy(h, w, b, y)
+
+
+def test_tracing_is_refused():
+    """a trace would hold the outputs' allocation and nothing that fills them"""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    h, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(5, 64, dtype=torch.bfloat16)
+    y = torch.zeros(2, dtype=torch.int64)
+    for call in (lambda h: losses.linear_cross_entropy(h, w, None, y), lambda h: losses.linear_distillation(h, w, None, torch.zeros(2, 1), y[:, None]),
+                 lambda h: losses.topk_logits(h, 3)[0]):
+        with pytest.raises(NotImplementedError, match="traced"):
+            torch.jit.trace(call, (h,), check_trace=False)
+        with pytest.raises(NotImplementedError, match="traced"):
+            make_fx(call)(h)
+        with pytest.raises(RuntimeError, match="no CPU"):
+            call(h)
