@@ -166,8 +166,8 @@ struct VocabGemm {          // arguments of the product kernels
   int32_t wide;             // out16's rows start on 16 bytes
   const float* out_scale;
 };
-struct VocabPlan {          // workspace of one call: byte offsets, and how the backward cuts the vocabulary
-  size_t head, row_map, block_base, t_logp, x, part, row_info, row_lc, row_fix, fix, g, colsum, dh_part, dw_part, bytes;
+struct VocabPlan {          // workspace of one call: byte offsets, and how it cuts the vocabulary
+  size_t head, row_map, block_base, t_logp, x, part, joined, row_info, row_lc, row_fix, fix, g, colsum, dh_part, dw_part, bytes;
   int64_t piece, pieces, ld_colsum, dh_slot, dh_room, dw_room;   // floats of one split's partials of dh, of all, and of dW's
   int32_t splits;         // at most
   bool large;             // 256 x 256 tiles (vocab8.hip)

@@ -756,7 +756,23 @@ __device__ __forceinline__ float2 wave_pairs(const float2* p, int n_part, int la
   const float m = wave_max(mx), ref = m == -INFINITY ? 0.f : m;
   return make_float2(m, wave_sum(s * __builtin_amdgcn_exp2f(mx - ref)));
 }
+__device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.f : m;
+  return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
+}
 __device__ __forceinline__ float lse_of(float2 p) { return LN2 * ((p.x == -INFINITY ? 0.f : p.x) + log2f(p.y)); }
+
+// Forward over several pieces of the vocabulary: a piece's n pairs of every live row (rows n_part apart), and what the pieces before
+// it (`more`) came to, in one pair.  One wave per row; bound by the pairs' bytes.  A loss in one piece / several: 131 072 rows (H 128),
+// V 70 001 (2 pieces) 4.17 / 4.25 ms, V 262 221 (5) 13.6 / 13.8; 2^20 rows (H 64), V 262 221 (33) 129 / 138
+__global__ __launch_bounds__(256) void vocab_join_kernel(const int32_t* __restrict__ count, const float2* __restrict__ part, int n_part, int n,
+                                                         float2* __restrict__ joined, int more) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (r >= *count) return;
+  float2 all = wave_pairs(part + (int64_t)r * n_part, n, lane, 64);
+  if (more) all = join_pairs(joined[r], all);
+  if (lane == 0) joined[r] = all;
+}
 
 // The rows' losses are summed by the last of few workgroups to finish (the others' results are stored to where every XCD
 // reads, and acknowledged, before they count themselves), or by a kernel of its own where there are many.
@@ -813,10 +829,7 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
       __syncthreads();
       all = pair[0];
 #pragma unroll
-      for (int i = 1; i < 4; ++i) {
-        const float m = fmaxf(all.x, pair[i].x), ref = m == -INFINITY ? 0.f : m;
-        all = make_float2(m, all.y * __builtin_amdgcn_exp2f(all.x - ref) + pair[i].y * __builtin_amdgcn_exp2f(pair[i].x - ref));
-      }
+      for (int i = 1; i < 4; ++i) all = join_pairs(all, pair[i]);
     }
     const float lse = lse_of(all);
     const bf16_t* x = a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh;
@@ -1147,8 +1160,9 @@ hipError_t launch_products(const VocabGemm& g, const VocabPlan& p, int n, hipStr
 }  // namespace
 
 #if !CLIP_OPERAND_F16
-// G of one piece of the vocabulary may take this much: the pieces are as few as that allows
-constexpr int64_t G_BYTES = 1ll << 30;
+// G of one piece of the vocabulary may take this much in the backward pass, (max, sum) pairs in the forward: the pieces are as few
+// as that allows
+constexpr int64_t PIECE_BYTES = (int64_t)1 << 30;
 // Which calls run on the 256 x 256 tiles of vocab8.hip: up to 128 rows none (the small tiles read W once per 128 rows).
 // The loss alone from 192 tiles, in us, these / the small ones:  V 30 522, H 768: n 256 (120 tiles) 35 / 32, 300 (240) 38 / 42;
 //   H 128: n 257 (240) 22 / 25;   V 8 000, H 256: n 1024 (128) 26 / 24, 2048 (256) 26 / 32;   V 2 000, H 768: n 4096 (128) 42 / 40
@@ -1179,8 +1193,18 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
   p.block_base = take(rows / 16 * 4);
   if (distill && !grad) p.t_logp = take((size_t)n * k * 4);
   p.x = take(rows * hidden * 2);
+  // pieces of whole 256-column tiles, at most `most` columns each, of about the same size
+  auto cut = [&](int64_t most) {
+    const int64_t piece = max((int64_t)256, min(most / 256 * 256, vp));
+    p.pieces = (vp + piece - 1) / piece;
+    p.piece = ((vp / 256 + p.pieces - 1) / p.pieces) * 256;
+    p.pieces = (vp + p.piece - 1) / p.piece;
+  };
   if (!grad) {
-    p.part = take(rows * (vp / 64) * 8);
+    const int64_t pair_rows = p.tile_rows == 64 ? (n > 0 ? 64 : 0) : rows;   // 8 bytes per row and 64 columns
+    cut(pair_rows > 0 ? PIECE_BYTES / (pair_rows * 8) * 64 : vp);
+    p.part = take(pair_rows * (p.piece / 64) * 8);
+    if (p.pieces > 1) p.joined = take(pair_rows * 8);
   } else {
     p.row_info = take(rows * 16);
     if (distill) {
@@ -1188,15 +1212,8 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
       p.row_fix = take(rows * 8 * ROW_FIX);
       p.fix = take(vocab * 8 * FIX_COPIES);
     }
-    // a piece: whole 256-column tiles, G within its bound, 32-bit byte offsets into the piece of W
-    int64_t piece = rows > 0 ? G_BYTES / (rows * 2) : vp;
-    if (piece > (1ll << 30) / ldw) piece = (1ll << 30) / ldw;
-    piece = piece / 256 * 256;
-    if (piece < 256) piece = 256;
-    if (piece > vp) piece = vp;
-    p.pieces = (vp + piece - 1) / piece;
-    p.piece = ((vp / 256 + p.pieces - 1) / p.pieces) * 256;   // of about the same size
-    p.pieces = (vp + p.piece - 1) / p.piece;
+    // G within its bound, 32-bit byte offsets into the piece of W
+    cut(min(rows > 0 ? PIECE_BYTES / (rows * 2) : vp, ((int64_t)1 << 30) / ldw));
     p.g = take(rows * p.piece * 2);
     p.ld_colsum = vp;
     p.colsum = take((rows / 64) * vp * 4);
@@ -1294,7 +1311,7 @@ hipError_t gather_rows(VocabRows& a, const VocabPlan& p, char* base, bool& few, 
 hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, void* work, hipStream_t st) {
   VocabRows a = rows;
   char* base = static_cast<char*>(work);
-  float2* part = reinterpret_cast<float2*>(base + p.part);
+  float2 *part = reinterpret_cast<float2*>(base + p.part), *joined = reinterpret_cast<float2*>(base + p.joined);
   bool few;
   TRY(gather_rows<false>(a, p, base, few, st));
   if (a.n > 0) {
@@ -1302,19 +1319,20 @@ hipError_t KSET::launch_vocab_loss(const VocabRows& rows, const VocabPlan& p, vo
     g.x = a.x; g.w = a.w; g.bias = a.bias; g.ldw = a.ldw; g.vocab = a.vocab; g.hidden = a.hidden; g.count = a.count;
     g.scale2 = LOG2E * a.inv_t;
     g.part = part;
-    g.n_part = (int)((a.vocab + 255) / 256 * 4);   // 64 columns each
-    if (p.large) {
-      g.tiles_n = (int)((a.vocab + 255) / 256);
-      TRY(launch_vocab8(V_STATS, g, st));
-    } else {
-      // (a grid may have 2^32 threads: the vocabulary in as many parts as that takes)
-      const int tiles = g.n_part / 2, most = max(1, (1 << 23) / ((a.n + 127) / 128));
-      for (int t0 = 0; t0 < tiles; t0 += most) {
-        g.v0 = (int64_t)t0 * 128;
-        g.part = part + t0 * 2;
-        g.tiles_n = min(most, tiles - t0);
-        TRY(launch_scores<V_STATS>(g, a, few, st));
+    g.n_part = (int)(p.piece / 64);
+    for (int64_t v0 = 0; v0 < a.vocab; v0 += p.piece) {   // (one piece: as a rule)
+      const int cols = (int)((min(p.piece, a.vocab - v0) + 255) / 256 * 256);
+      g.v0 = v0;
+      g.tiles_n = cols / (p.large ? 256 : 128);
+      TRY(p.large ? launch_vocab8(V_STATS, g, st) : launch_scores<V_STATS>(g, a, few, st));
+      if (p.pieces > 1) {
+        hipLaunchKernelGGL(vocab_join_kernel, dim3((a.n + 3) / 4), dim3(256), 0, st, a.count, part, g.n_part, cols / 64, joined, v0 > 0 ? 1 : 0);
+        TRY(hipGetLastError());
       }
+    }
+    if (p.pieces > 1) {
+      part = joined;
+      g.n_part = 1;
     }
     if (few) a.x = nullptr;   // rows stay where they are
     // (a loss of 15 % live rows, us, summed by the last workgroup / by a kernel more: n 1100 23.8 / 24.8, 1500 24.9 / 24.9,

@@ -395,6 +395,67 @@ def test_few_rows_in_several_pieces(n, distill):
         R.assert_within(name, got, a, e)
 
 
+@pytest.mark.parametrize("distill", [0, 3, 20])
+def test_loss_of_pairs_beyond_one_piece(distill):
+    # 2^17 rows x 70 001 entries: the (max, sum) pairs of the whole vocabulary are beyond one piece's bound
+    n, vocab, hidden, step = 1 << 17, 70001, 128, 4096
+    h, w, b = R.make(n, vocab, hidden, BF16, 83)
+    if distill:
+        values, index = _teacher(step, vocab, distill, 84, 0.2)
+        values, index = values.repeat(n // step, 1), index.repeat(n // step, 1)
+        index[:, 0] = torch.arange(n).cuda() % vocab
+        index[::7] = -1
+        loss = losses.linear_distillation(h, w, b, values, index, temperature=2.0, reduction="none")
+    else:
+        y = _labels(n, vocab, 85, 0.3)
+        y[-1], y[-2] = vocab - 1, 0
+        loss = losses.linear_cross_entropy(h, w, b, y, reduction="none")
+    for i in (0, step * 13, n - step):
+        at = slice(i, i + step)
+        if distill:
+            p, live, entropy = R.targets_distill(values[at], index[at], vocab, 2.0)
+        else:
+            (p, live), entropy = R.targets_ce(y[at], vocab, -100), None
+        (want, *_), (err, *_) = R.reference(h[at], w, b, p, live, 2.0 if distill else 1.0, torch.ones(step).cuda(), entropy)
+        R.assert_within("loss", loss[at], want, err)
+        del p, want, err
+    if distill:
+        return
+    for i in range(0, n, step):      # every row, by R.reference's bound of the loss
+        hd, yi = h[i:i + step].double(), y[i:i + step]
+        z = hd @ w.double().t() + b.double()
+        lse = torch.logsumexp(z, 1)
+        mag = z.abs().amax(1) + lse.abs()
+        z_err = ((hidden + 2) * R.F32 * (hd.abs() @ w.double().abs().t() + b.abs())).amax(1) + 8 * R.F32 * mag
+        off = (loss[i:i + step] - (lse - z.gather(1, yi.clamp(min=0)[:, None])[:, 0])).abs()
+        assert (off <= 2 * z_err + (16 + vocab / 64) * R.F32 * (1 + mag))[yi >= 0].all()
+        assert not loss[i:i + step][yi < 0].any()
+
+
+def test_few_rows_of_pairs_beyond_one_piece():
+    # 2^27 entries and more: a vocabulary of which 64 rows' pairs are beyond the bound (17 GB of weight)
+    vocab, hidden, n = (1 << 27) + 77, 64, 64
+    h, w, _ = R.make(n, 1 << 20, hidden, BF16, 86)
+    w = w.repeat(129, 1)[:vocab]
+    b = (torch.arange(vocab, device="cuda") % 1009).float() / 1009
+    b[-1] = 18.0        # weighs as much as all others: it is in the second piece
+    y = torch.randint(0, vocab, (n,), generator=torch.Generator().manual_seed(87)).cuda()
+    y[0], y[1], y[2] = vocab - 1, -100, 5
+    loss = losses.linear_cross_entropy(h, w, b, y, reduction="none")
+    hd, parts = h.double(), []
+    for v in range(0, vocab, 1 << 20):
+        parts.append(torch.logsumexp(hd @ w[v:v + (1 << 20)].double().t() + b[v:v + (1 << 20)].double(), 1))
+    lse = torch.logsumexp(torch.stack(parts), 0)
+    z = (hd * w[y.clamp(min=0)].double()).sum(1) + b[y.clamp(min=0)].double()
+    assert loss[1] == 0
+    # a score: 66 fp32 steps of its magnitudes' sum; the exponentials' sum: 64 columns in a tree, then 2^21 / 64 pairs one after the
+    # other in a lane, rescaled once per eight
+    z_err = 66 * R.F32 * (hd.abs().sum(1) * w[:1 << 20].abs().amax().double() + 18)
+    err = 2 * z_err + (64 + (1 << 15) * 9 / 8) * R.F32 + 16 * R.F32 * (1 + lse.abs())
+    off = (loss.double() - (lse - z))[y >= 0].abs()
+    assert (off <= err[y >= 0]).all(), (off.max(), err.min())
+
+
 # ---------------------------------------------------------------- distillation
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("n,vocab,hidden,k,temperature", [

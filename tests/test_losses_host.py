@@ -43,6 +43,22 @@ def test_workspace_is_bounded():
     assert _need(k=64)[1] > _need()[1]
 
 
+BOUND = 1 << 30                  # bytes of a piece's score gradients, and of its (max, sum) pairs
+SHAPES = [(1, 30522, 768, 0), (64, 1 << 24, 64, 0), (64, 1 << 30, 64, 0), (300, 30522, 768, 8), (4096, 30522, 768, 1024), (16384, 30522, 768, 0), (16384, 1 << 22, 128, 3),
+          (1 << 17, 262221, 64, 0), (1 << 20, 262221, 64, 0), (1 << 20, 262221, 64, 64), ((1 << 21) - 256, 30522, 768, 0), ((1 << 21) - 257, 1 << 23, 128, 16)]
+
+
+@pytest.mark.parametrize("n,vocab,hidden,k", SHAPES)
+def test_workspace_of_a_loss(n, vocab, hidden, k):
+    """the copied rows, a list's log p, and (max, sum) pairs: of the whole vocabulary (8 bytes per row and 64 columns) or of a
+    bounded piece, with one joined pair per row"""
+    rc, need = _need(k=k, n=n, vocab=vocab, hidden_size=hidden, ld_hidden=hidden, ld_weight=hidden)
+    assert rc == 0
+    rows, pair_rows = -(-n // 256) * 256, 64 if n <= 64 else -(-n // 256) * 256
+    pairs = pair_rows * -(-vocab // 256) * 32
+    assert need <= rows * (2 * hidden + 8) + 4 * n * k + (pairs if pairs <= BOUND else BOUND + 8 * rows) + 8 * 256
+
+
 def test_calls_refused_without_a_device():
     lib, d = _lib.load(), _desc()
     p = C.c_void_p(4096)
