@@ -434,7 +434,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::condit
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = fr_sum(cs[n][e]);
         if (fr == 0)
-          *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * WM + wm) * a.ld_colsum + a.v0 + col0 + n * 16) = t;
+          *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * WM + wm) * a.ld_colsum + col0 + n * 16) = t;
       }
     }
   } else if (EPI == V_DH) {
@@ -1029,11 +1029,11 @@ __global__ __launch_bounds__(256) void vocab_teacher_hash_kernel(VocabRows a, bf
   if (tid < ROW_FIX && tid >= before) fix[tid] = make_float2(__int_as_float(-1), 0.f);
 }
 
-// dh of the live rows from the fp32 partials (fixed order), and db from the column sums and the targets' table; dW from its
-// partials where its k was split.  Bound: the partials' bytes; 16 384 rows 46 us, 4096 rows 14 us
+// dh of the live rows from the fp32 partials (fixed order), and db of the entries v0 .. v1 (a piece of the vocabulary) from its column
+// sums and the targets' table; dW from its partials where its k was split.  Bound: the partials' bytes; 16 384 rows 46 us, 4096 rows 14 us
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPlan p, const float* __restrict__ part,
                                                            const float* __restrict__ colsum, const float* __restrict__ dw_part,
-                                                           bf16_t* __restrict__ dw, int64_t ld_dw, int row_blocks, int dw_blocks) {
+                                                           bf16_t* __restrict__ dw, int64_t ld_dw, int row_blocks, int dw_blocks, int64_t v0, int64_t v1) {
   const int count = *a.count;
   const int b_blocks = gridDim.x - row_blocks - dw_blocks;
   // the sum of n slots' partials, four of them in flight, in order; rounded: times the common factor
@@ -1108,19 +1108,19 @@ __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPla
       if (v < a.vocab && c < a.hidden) *reinterpret_cast<uint2*>(dw + v * ld_dw + c) = rounded(sum_slots(dw_part + i * 4, n, (int64_t)tiles * 65536));
     }
   } else {
-    const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (v >= a.vocab) return;
+    const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x, v = v0 + at;
+    if (v >= v1) return;
     const int n_sums = (count + p.tile_rows - 1) / p.tile_rows * 2;   // one per half tile of rows
     float sum = 0.f;
     int k = 0;
     for (; k + 8 <= n_sums; k += 8) {
       float t[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) t[u] = colsum[(int64_t)(k + u) * p.ld_colsum + v];
+      for (int u = 0; u < 8; ++u) t[u] = colsum[(int64_t)(k + u) * p.ld_colsum + at];
 #pragma unroll
       for (int u = 0; u < 8; ++u) sum += t[u];
     }
-    for (; k < n_sums; ++k) sum += colsum[(int64_t)k * p.ld_colsum + v];
+    for (; k < n_sums; ++k) sum += colsum[(int64_t)k * p.ld_colsum + at];
     if (a.fix) {   // (the sum is in units of G, the table in units of c)
       int64_t t = 0;
 #pragma unroll
@@ -1215,8 +1215,8 @@ VocabPlan vocab_plan(int32_t n, int64_t vocab, int32_t hidden, int64_t ldw, int3
     // G within its bound, 32-bit byte offsets into the piece of W
     cut(min(rows > 0 ? PIECE_BYTES / (rows * 2) : vp, ((int64_t)1 << 30) / ldw));
     p.g = take(rows * p.piece * 2);
-    p.ld_colsum = vp;
-    p.colsum = take((rows / 64) * vp * 4);
+    p.ld_colsum = p.piece;
+    p.colsum = take((rows / 64) * p.piece * 4);
     // dh = G W has few tiles and a long k, which is split: so that half of the CUs have a workgroup (dW's take the rest of them) or,
     // where its parts would be longer than 64 K tiles, up to all; (large) as the schedule on the device finds best, within this many
     // fp32 partials of the rows.  A step, us, all CUs / half: 19 rows of V 30 522 68 / 65, 64 rows (V 40 000, H 1024) 102 / 97, 1000 rows
@@ -1390,7 +1390,15 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
   g.with_dw = dw != nullptr;
   g.low = few;
   g.with_dh = a.dh && a.n > 0;
-  for (int64_t v0 = 0, piece = 0; v0 < a.vocab; v0 += p.piece, ++piece) {
+  auto finish = [&](int row_blocks, int dw_blocks, int64_t v0, int64_t v1) -> hipError_t {
+    const int b_blocks = a.dbias ? (int)((v1 - v0 + 255) / 256) : 0;
+    if (row_blocks + b_blocks + dw_blocks == 0) return hipSuccess;
+    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks + dw_blocks), dim3(256), 0, st, a, p, g.out32, g.colsum, g.dw32, dw,
+                       ld_dw, row_blocks, dw_blocks, v0, v1);
+    return hipGetLastError();
+  };
+  int64_t v0 = 0;
+  for (int64_t piece = 0;; ++piece, v0 += p.piece) {
     const int64_t v1 = v0 + p.piece < a.vocab ? v0 + p.piece : a.vocab;
     g.v0 = v0;
     g.ldg = (int)((v1 - v0 + 255) / 256 * 256);
@@ -1407,14 +1415,10 @@ hipError_t KSET::launch_vocab_grad(const VocabRows& rows, const VocabPlan& p, bf
     }
     g.tiles_n = a.tiles_h;
     TRY(p.large ? launch_vocab8(V_PROD, g, st) : launch_products(g, p, a.n, st));
+    if (v1 == a.vocab) break;
+    TRY(finish(0, 0, v0, v1));   // db of this piece: the next one's column sums take the place of its own
   }
   const int row_blocks = g.with_dh ? (int)min((int64_t)2048, ((int64_t)a.n * (a.hidden / 4) + 255) / 256) : 0;
-  const int b_blocks = a.dbias ? (int)((a.vocab + 255) / 256) : 0;
-  const int dw_blocks = dw && p.dw_room > 0 ? 1024 : 0;
-  if (row_blocks + b_blocks + dw_blocks > 0) {
-    hipLaunchKernelGGL(vocab_finish_kernel, dim3(row_blocks + b_blocks + dw_blocks), dim3(256), 0, st, a, p, g.out32, g.colsum, g.dw32, dw,
-                       ld_dw, row_blocks, dw_blocks);
-    TRY(hipGetLastError());
-  }
+  TRY(finish(row_blocks, dw && p.dw_room > 0 ? 1024 : 0, v0, a.vocab));
   return hipSuccess;
 }

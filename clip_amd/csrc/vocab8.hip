@@ -361,7 +361,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) t[e] = fr_sum(cs[nh][i][e]);
             if (fr == 0)
-              *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + a.v0 + col0 + nh * 32 + i * 16) = t;
+              *reinterpret_cast<f32x4_t*>(a.colsum + (int64_t)(tm * 2 + wr) * a.ld_colsum + col0 + nh * 32 + i * 16) = t;
           }
       }
     } else if (!cur.whole) {

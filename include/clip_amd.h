@@ -174,7 +174,9 @@ int clip_ce_loss(const float* dev_logits, const int32_t* dev_labels, int32_t n, 
  * The reference trains BertContextMLMSwitch's LM head with CrossEntropyLoss over scores = decoder(hidden)
  * (bert_model.py:165,175-179; its loop is pretrain_tasks.py:333-466); clip_mlm_head evaluates that loss and keeps
  * [n_rows, vocab] fp32 scores.  The entry points below take any hidden rows and any decoder and give the loss AND the
- * gradients with a workspace of n x hidden plus one bounded piece of 16-bit score gradients.  Stateless: no engine, all
+ * gradients with a workspace that does not grow as n x vocab: of the order of n x hidden (and n x k), 64 bytes per vocabulary entry
+ * for a distillation's gradients, and one piece of the vocabulary, at most 1 GiB of 16-bit score gradients, or of (max, sum) pairs
+ * for a loss.  Stateless: no engine, all
  * memory is the caller's, all work is queued on `stream` of the current device, nothing waits on the host, and calls can be
  * captured into HIP graphs (after one eager call of the same sizes) and replayed; calls that run at the same time need workspaces
  * of their own. */

@@ -889,6 +889,66 @@ def test_c_abi_writes_only_its_outputs(n, vocab, hidden, ld_dh, ld_dw, k):
     assert torch.equal(bufs["db"][0][GUARD:GUARD + 4 * vocab].view(F32), want[2])
 
 
+@pytest.mark.parametrize("k", [0, 5])
+def test_c_abi_workspace_of_several_pieces(k):
+    """a loss and its gradients whose pairs and score gradients are beyond one piece's bound: nothing is written behind a workspace
+    of exactly the size asked for, full of NaN before; dbias, which is summed piece by piece, against 64 bits"""
+    import ctypes as C
+    from clip_amd import _lib
+    lib = _lib.load()
+    n, vocab, hidden, T = 1 << 17, 70001, 128, 2.0 if k else 1.0
+    h, w, b = R.make(n, vocab, hidden, BF16, 93)
+    if k:
+        values, index = (t.repeat(n // 1024, 1) for t in _teacher(1024, vocab, k, 94, 0.2))
+        index[::5] = -1
+    else:
+        y = _labels(n, vocab, 95, 0.4)
+    d = _lib.ClipLinear(_lib.PRECISION_BF16, n, hidden, vocab, h.data_ptr(), hidden, w.data_ptr(), hidden, b.data_ptr())
+    new = lambda *shape, dtype=F32: torch.empty(*shape, dtype=dtype, device="cuda")  # noqa: E731
+    row, lse, target, total = new(n), new(n, 2), new(n, 2 * k + 1), new(())
+    dh, dw, db = new(n, hidden, dtype=BF16), new(vocab, hidden, dtype=BF16), new(vocab)
+    up = torch.ones((), device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    for grad in (0, 1):
+        need = C.c_int64()
+        _lib.check(lib.clip_linear_loss_workspace(C.byref(d), k, grad, C.byref(need)))
+        work = torch.full((need.value + 8192,), 0xFF, dtype=torch.uint8, device="cuda")
+        at = work.data_ptr() + 4096
+        if not grad:
+            tail = (2, row.data_ptr(), lse.data_ptr(), target.data_ptr(), total.data_ptr(), at, need.value, st)
+            _lib.check(lib.clip_linear_distill(C.byref(d), values.data_ptr(), index.data_ptr(), k, T, *tail) if k else
+                       lib.clip_linear_ce(C.byref(d), y.data_ptr(), -100, *tail))
+        else:
+            tail = (2, lse.data_ptr(), target.data_ptr(), up.data_ptr(), dh.data_ptr(), hidden, dw.data_ptr(), hidden, db.data_ptr(), at,
+                    need.value, st)
+            _lib.check(lib.clip_linear_distill_grad(C.byref(d), index.data_ptr(), k, T, *tail) if k else
+                       lib.clip_linear_ce_grad(C.byref(d), y.data_ptr(), -100, *tail))
+        torch.cuda.synchronize()
+        assert (work[:4096] == 0xFF).all() and (work[4096 + need.value:] == 0xFF).all()
+        del work
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = (losses.linear_distillation(*leaves, values, index, temperature=T, reduction="sum") if k else
+            losses.linear_cross_entropy(*leaves, y, reduction="sum"))
+    assert torch.equal(loss.detach(), total)
+    for got, want in zip((dh, dw, db), torch.autograd.grad(loss, leaves)):
+        assert torch.equal(got, want)
+    # db = T sum (q - p): bounds as R.reference makes them, its sums taken over all rows
+    want, each, size = (torch.zeros(vocab, dtype=torch.float64, device="cuda") for _ in range(3))
+    for i in range(0, n, 4096):
+        part = slice(i, i + 4096)
+        p, live = R.targets_distill(values[part], index[part], vocab, T)[:2] if k else R.targets_ce(y[part], vocab, -100)
+        z = (h[part].double() @ w.double().t() + b.double()) / T
+        lse_ = torch.logsumexp(z, 1)
+        mag = z.abs().amax(1) + lse_.abs()
+        z_err = ((hidden + 2) * R.F32 * (h[part].double().abs() @ w.double().abs().t() + b.abs()) / T).amax(1) + 8 * R.F32 * mag
+        q = (z - lse_[:, None]).exp() * live[:, None]
+        want += T * (q - p).sum(0)
+        s = T * (q + p)
+        each += ((2 * z_err + (16 + vocab / 64) * R.F32)[:, None] * s).sum(0)
+        size += s.sum(0)
+    R.assert_within("db", db, want, each + (n + 4) * R.F32 * size + n * 2.0 ** -38 * T)
+
+
 # ---------------------------------------------------------------- refusals
 def test_refusals():
     h, w, b = R.make(4, 10, 64, BF16, 1)

@@ -148,3 +148,15 @@ def test_tracing_is_refused():
             make_fx(call)(h)
         with pytest.raises(RuntimeError, match="no CPU"):
             call(h)
+
+
+@pytest.mark.parametrize("n,vocab,hidden,k", SHAPES)
+def test_workspace_of_the_gradients(n, vocab, hidden, k):
+    """rows, what is known of each, fp32 partials of their gradient, a distillation's table of target sums, and one piece of 16-bit
+    score gradients with its column sums"""
+    rc, need = _need(k=k, grad=1, n=n, vocab=vocab, hidden_size=hidden, ld_hidden=hidden, ld_weight=hidden)
+    assert rc == 0
+    rows = -(-n // 256) * 256
+    piece = min(2 * rows * (-(-vocab // 256) * 256), BOUND)
+    table = rows * (16 + 64) + 64 * vocab if k else 0
+    assert need <= rows * (2 * hidden + 24) + table + piece * 33 // 32 + max(8 * rows * (hidden + 255), 2 * 128 << 20) + 12 * 256
