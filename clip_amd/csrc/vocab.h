@@ -55,7 +55,8 @@ __device__ __forceinline__ float fq_max(float v) {
 // 32-byte slot swizzle of an R-major K tile image [64 k][2 R bytes]
 template <int R>
 __device__ __forceinline__ int tr_swz(int k) {
-  return R >= 128 ? ((k & 3) | ((k >> 3) & 1) << 2) : (((k >> 1) & 1) | ((k >> 3) & 1) << 1);
+  static_assert(R >= 128, "rows of eight slots and more");
+  return (k & 3) | ((k >> 3) & 1) << 2;
 }
 
 // 16 bytes of dW, written once and not read again here; rows of a caller's own stride may start on 8 bytes only

@@ -47,7 +47,7 @@ struct Operand {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int at = (w * PIECES + p) * 1024 + lane * 16;   // byte of the image this lane fills
-      if (TR) {
+      if constexpr (TR) {
         const int k = at / (2 * R), c = (at % (2 * R)) >> 4;
         off[p] = (uint32_t)(k * ld * 2) + ((((c >> 1) ^ tr_swz<R>(k)) << 1) | (c & 1)) * 16;
       } else {
@@ -73,16 +73,17 @@ struct Operand {
   // MFMA operand of 16 rows starting at r0 (a multiple of 16), k 32 ks + 8 (lane >> 4) .. + 7
   static __device__ __forceinline__ opx8_t frag(const char* img, int r0, int ks, int lane) {
     const int fr = lane & 15, fq = lane >> 4;
-    if (!TR) {
+    if constexpr (!TR) {
       const int r = r0 + fr;
       return *reinterpret_cast<const opx8_t*>(img + r * 128 + swz128(r, ks * 4 + fq) * 16);
+    } else {
+      const int qq = fr >> 2, pp = fr & 3, k = ks * 32 + fq * 8 + qq;   // (k + 4 has the same swizzle)
+      const char* a = img + k * (2 * R) + ((r0 >> 4) ^ tr_swz<R>(k)) * 32 + pp * 8;
+      const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(a));
+      const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(a + 4 * 2 * R));
+      const s16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+      return *reinterpret_cast<const opx8_t*>(&v);
     }
-    const int qq = fr >> 2, pp = fr & 3, k = ks * 32 + fq * 8 + qq;   // (k + 4 has the same swizzle)
-    const char* a = img + k * (2 * R) + ((r0 >> 4) ^ tr_swz<R>(k)) * 32 + pp * 8;
-    const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(a));
-    const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(a + 4 * 2 * R));
-    const s16x8_t v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    return *reinterpret_cast<const opx8_t*>(&v);
   }
 };
 
@@ -259,15 +260,11 @@ __device__ __forceinline__ float residual(float x) {
   return fabsf(r) < INFINITY ? r : 0.f;
 }
 
-// waits until at most `n` of this wave's loads are in flight
+// waits until at most N of this wave's loads are in flight
 template <int N>
 __device__ __forceinline__ void wait_loads() {
-  static_assert(N <= 24, "counted");
-  if (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else if (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
-  else if (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  else if (N == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  static_assert(N >= 0 && N <= 63, "counted");
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
 // One output tile of BM x BN per workgroup of WM x WN waves, 64 columns per wave, through a ring of NST K tiles (few rows: many
