@@ -30,15 +30,6 @@ constexpr int STAGE = PM * 128 + PN * 128;            // 8 KiB of A rows + 32 Ki
 constexpr int NSTAGE = 3;
 constexpr int LDS4 = NSTAGE * STAGE + 4 * 512 + 2 * 512;   // + row partials per wave + this tile's sums + (mean, rstd)
 
-__device__ __forceinline__ float xor16_sum4(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float xor32_sum4(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // res_mode: 0 residual = fp16 rows (row stride ldres; may be the output buffer itself: every lane reads exactly the
 //             elements it rewrites), 1 = fp16 tiled (xres_tiled_offset), 2 = fp32 tiled (xres32_tiled_offset)
 // out_mode: 0 no residual copy out (fp16 operand set: x is the copy), 1 = fp16 tiled, 2 = fp32 tiled
@@ -194,8 +185,8 @@ __global__ __launch_bounds__(512) void gemm4_lnout_kernel(
         q2 = __builtin_elementwise_fma(hi2, hi2, q2);
       }
     float sm = s2[0] + s2[1], sq = q2[0] + q2[1];
-    sm = xor16_sum4(sm); sq = xor16_sum4(sq);
-    sm = xor32_sum4(sm); sq = xor32_sum4(sq);
+    sm = xor16_sum(sm); sq = xor16_sum(sq);
+    sm = xor32_sum(sm); sq = xor32_sum(sq);
     if (fq == 0) part_own[m * 16 + fr] = make_float2(sm, sq);
   }
   __syncthreads();
@@ -460,8 +451,8 @@ __global__ __launch_bounds__(256) void gemm4n_lnout_kernel(
       q2 = __builtin_elementwise_fma(hi2, hi2, q2);
     }
   float sm = s2[0] + s2[1], sq = q2[0] + q2[1];
-  sm = xor16_sum4(sm); sq = xor16_sum4(sq);
-  sm = xor32_sum4(sm); sq = xor32_sum4(sq);
+  sm = xor16_sum(sm); sq = xor16_sum(sq);
+  sm = xor32_sum(sm); sq = xor32_sum(sq);
   // (3) published per chunk as two 8-byte words {value, epoch}: the tag travels WITH the data, so a reader needs one
   // round trip through memory (poll the words themselves) instead of three (data, then flag, then read) — on a call
   // this small the exchange sits on the critical path of every launch

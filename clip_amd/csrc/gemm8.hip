@@ -85,16 +85,6 @@ __device__ __forceinline__ void out_store(V v, V* p) {
   else *p = v;
 }
 
-// v + (v of the lane 16 / 32 away): every lane of the pair ends with the sum
-__device__ __forceinline__ float xor16_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-__device__ __forceinline__ float xor32_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // SINGLE (EPI_BIAS_LNOUT, fp16 operands only): the LayerNorm output is written ONCE, row-major, and serves as the
 // next GEMM's operand AND as the next residual (in the f16 setting the two copies of the bf16 setting hold the
 // same bits); the residual is then read from the row-major buffer this tile rewrites in place (every wave reads
