@@ -8,8 +8,9 @@
 // exp2) pair per row and 64 columns; a second kernel joins the pairs and forms the target scores as k dot products per row.
 // Backward: the scores are formed once more, piece by piece of the vocabulary, and leave as the 16-bit operand
 // G = c (softmax - targets) of two products, dh += G W and dW = G^T h.  G holds c = g_i / max|g|, |c| <= 1, so that fp16's
-// range holds it (times 2^15 there: softmax values down to 2e-9 stay normal numbers); the factor is put back in fp32 when
-// the products are stored.
+// range holds it (times 2^15 there: c q down to 2e-9 stays a normal number, and 2^-40 is its smallest half step: dh rows with c of 2^-20
+// and more are as exact as the largest one's, V 30 522; the factor is common to all rows because dW sums over them); it is put back
+// in fp32 when the products are stored.
 // What G's rounding costs: most of a row's gradient sits in few entries (its targets), whose rounding errors do not average
 // out.  dh gets them back in fp32: the residuals of a row's largest entries times their rows of W, added where the partials are
 // joined.  dW of few rows (at most 64) is a product of G's high AND low parts, k twice as long under an output that is the

@@ -48,8 +48,9 @@ def load():
 def linear_cross_entropy(hidden, weight, bias, labels, *, ignore_index=-100, reduction="mean"):
     """F.cross_entropy(hidden @ weight.T + bias, labels, ignore_index=..., reduction=...) without the scores, differentiable in
     hidden [..., H] and weight [V, H] (bf16 or fp16; H a multiple of 64, at most 8192) and in bias (fp32 [V], or None).  labels:
-    integers of hidden's leading shape.  The mean is over the rows that are not ignored (NaN if there is none, with zero
-    gradients); a label outside [0, V) that is not ignore_index makes the loss and the gradients NaN."""
+    int64 or int32 of hidden's leading shape.  The mean is over the rows that are not ignored (NaN if there is none, with zero
+    gradients); a label outside [0, V) that is not ignore_index makes the loss and the gradients NaN.  fp16 with reduction="none":
+    the score gradients are held to 2^-40 of the largest upstream gradient, so rows weighted below 2^-20 of it lose bits of theirs."""
     return (_ext or load()).linear_cross_entropy(hidden, weight, bias, labels, ignore_index, reduction)
 
 

@@ -804,6 +804,32 @@ def test_upstream_gradients(n, vocab, up):
         assert not any(t.isfinite().all() for t in torch.autograd.grad(loss, leaves, torch.tensor(bad).cuda()))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,vocab", [(40, 700), (90, 700), (300, 128100)])
+def test_rows_weighted_over_a_wide_range(n, vocab, dtype):
+    """upstream gradients from 2^14 down to 2^-16 (whose dh both types still hold as normal numbers): fp16 score gradients are no
+    finer than 2^-40 of the largest, as R.reference has it; rows of 2^-20 of it and more are as exact as the largest"""
+    h, w, b = R.make(n, vocab, 128, dtype, 47)
+    y = _labels(n, vocab, 48)
+    p, live = R.targets_ce(y, vocab, -100)
+    up = 2.0 ** (14 - torch.tensor([0, 10, 20, 24, 30]).repeat(n // 5)).cuda()
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    got = torch.autograd.grad(losses.linear_cross_entropy(*leaves, y, reduction="none"), leaves, up)
+    want, err = R.reference(h, w, b, p, live, 1.0, up)
+    for name, g, a, e in zip(("dh", "dw", "db"), got, want[1:], err[1:]):
+        if g.dtype == F16:      # 2^14 |h| of a label's row beyond 4: more than the type's 65 504 is infinite
+            a = torch.where(a.abs() < 65520, a, a.sign() * INF)
+        R.assert_within(name, g, a, e)
+    # rows 2^0, 2^-10 and 2^-20: dh's own rounding (half a step of each value), what 2^-40 an entry comes to where all of a
+    # row's entries are off by it, and the relative rounding of the entries
+    u = R.half_step(dtype)
+    wide = (torch.arange(n) % 5 < 3).cuda()
+    q = torch.softmax(h.double() @ w.double().t() + b.double(), 1)
+    dz = (up.double()[:, None] * (q - p)).abs()
+    each = (2 * u * dz) @ w.double().abs() + (2.0 ** -40 * 2.0 ** 14 if dtype == F16 else 0.0) * w.double().abs().sum(0)
+    assert ((got[0].double() - want[1]).abs() <= each + 2 * u * want[1].abs() + R.TINY[dtype])[wide].all()
+
+
 def test_ignore_index_inside_the_vocabulary():
     n, vocab = 300, 260
     h, w, b = R.make(n, vocab, 128, BF16, 44)
