@@ -189,7 +189,7 @@ typedef struct clip_linear {
   int64_t ld_hidden;
   const uint16_t* dev_weight;    /* [vocab, hidden_size], row stride ld_weight (a multiple of 8), 16-byte aligned */
   int64_t ld_weight;             /* <= 2^22 */
-  const float* dev_bias;         /* [vocab] fp32, or NULL; -inf leaves an entry out of the softmax */
+  const float* dev_bias;         /* [vocab] fp32 (4-byte aligned), or NULL; -inf leaves an entry out of the softmax */
 } clip_linear;
 
 /* Bytes of workspace (16-byte aligned) of the calls below for these sizes: k = 0 for the cross entropy, else the teacher's

@@ -830,6 +830,54 @@ def test_rows_weighted_over_a_wide_range(n, vocab, dtype):
     assert ((got[0].double() - want[1]).abs() <= each + 2 * u * want[1].abs() + R.TINY[dtype])[wide].all()
 
 
+@pytest.mark.parametrize("n,vocab,hidden", [(40, 701, 128), (130, 701, 128), (300, 30803, 128), (300, 128101, 128), (1300, 15003, 384)])
+def test_bias_on_four_bytes(n, vocab, hidden):
+    # (the 256-row tiles fetch it 16 bytes at a time)
+    h, w, b = R.make(n, vocab, hidden, BF16, 49)
+    y = _labels(n, vocab, 50, 0.1)
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y)
+    want = (loss.detach(), *torch.autograd.grad(loss, leaves))
+    for at in (1, 2, 3):
+        flat = torch.full((vocab + 8,), NAN, device="cuda")
+        flat[at:at + vocab] = b
+        bias = flat[at:at + vocab].requires_grad_()
+        assert bias.data_ptr() % 16 == 4 * at
+        loss = losses.linear_cross_entropy(leaves[0], leaves[1], bias, y)
+        got = (loss.detach(), *torch.autograd.grad(loss, (leaves[0], leaves[1], bias)))
+        assert all(torch.equal(g, r) for g, r in zip(got, want))
+
+
+@pytest.mark.parametrize("n,vocab,hidden,dtype", [(300, 2301, 8192, BF16), (600, 5003, 4096, F16), (1100, 900, 2176, BF16)])
+def test_wide_hidden_on_the_large_tiles(n, vocab, hidden, dtype):
+    h, w, b = R.make(n, vocab, hidden, dtype, 51, spread=0.02)
+    y = _labels(n, vocab, 52, 0.1)
+    p, live = R.targets_ce(y, vocab, -100)
+    _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y), p, live, 1.0, "mean", 5)
+
+
+@pytest.mark.parametrize("k", [0, 6])
+def test_large_tiles_of_rows_far_apart(k):
+    # a weight whose rows lie 90 000 elements apart (4.3 GB in all): pieces as 32-bit byte offsets allow, on the 256-row tiles
+    n, vocab, hidden, ld, T = 2600, 24001, 128, 90000, 1.5 if k else 1.0
+    h, w, b = R.make(n, vocab, hidden, BF16, 53)
+    far = torch.empty(vocab, ld, dtype=BF16, device="cuda")[:, :hidden]
+    far.copy_(w)
+    if k:
+        values, index = _teacher(n, vocab, k, 54, 0.1)
+        p, live, entropy = R.targets_distill(values, index, vocab, T)
+    else:
+        y = _labels(n, vocab, 55, 0.2)
+        (p, live), entropy = R.targets_ce(y, vocab, -100), None
+    leaves = [h.clone().requires_grad_(), far.requires_grad_(), b.clone().requires_grad_()]
+    loss = (losses.linear_distillation(*leaves, values, index, temperature=T, reduction="none") if k else
+            losses.linear_cross_entropy(*leaves, y, reduction="none"))
+    grads = torch.autograd.grad(loss.sum(), leaves)
+    want, err = R.reference(h, w, b, p, live, T, torch.ones(n).cuda(), entropy)
+    for name, got, a, e in zip(("loss", "dh", "dw", "db"), (loss.detach(), *grads), want, err):
+        R.assert_within(name, got, a, e)
+
+
 def test_ignore_index_inside_the_vocabulary():
     n, vocab = 300, 260
     h, w, b = R.make(n, vocab, 128, BF16, 44)
