@@ -141,7 +141,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   float *t_p, *t_logp;      // distillation: the teacher's p and log p, [n, k]; state: 0 no entry, 1 live, 2 a bad entry
   float* out_scale;
   bf16_t* x;
-  float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), less t at the label, which V_GRAD puts in t's place
+  float4* row_info;         // per live row (x, y, label, t): G = y exp2(z log2(e) / T - x), but t at the label
   float4* row_lc;           // distillation: (m, 1 / s, c)
   float2* row_fix;          // distillation: up to ROW_FIX (vocabulary id, what G's rounding left of its entry) per live row
   bool low;                 // G's rows 64 .. 127 hold what the rounding of its rows 0 .. 63 left (few rows)
@@ -156,7 +156,7 @@ struct VocabGemm {          // arguments of the product kernels
   float scale2;             // log2(e) / T
   float2* part; int32_t n_part;
   bf16_t* g;
-  float4* row_info;
+  const float4* row_info;
   float* colsum; int64_t ld_colsum;
   float* out32; int64_t slot_stride;   // V_DH partials of this piece (vocab8: whole tiles, dh_partial_at)
   float* dw32;              // dW's partials where its k is split

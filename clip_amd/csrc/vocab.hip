@@ -184,7 +184,7 @@ __device__ void write_head(const VocabRows& a, int total, float grad_max, int la
   }
 }
 
-// what V_GRAD needs of a live row: (x, y, label, c), G = y exp2(z log2(e) / T - x), less c at the label; lc: (x, 1 / sum, c).  x is the
+// what V_GRAD needs of a live row: (x, y, label, t), G = y exp2(z log2(e) / T - x) but t at the label; lc: (x, 1 / sum, c).  x is the
 // row's largest score and not its logsumexp: where q is large the exponent is small, and so is its rounding
 __device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st, float grad_max, float4& lc) {
   float c = 1.f;
@@ -199,7 +199,7 @@ __device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st,
   float4 info = make_float4(x, c * G_SCALE * inv, __int_as_float(-1), 0.f);
   if (!a.state && st == 1) {
     info.z = __int_as_float((int)a.labels[r]);
-    info.w = c * G_SCALE;
+    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -x)) * inv - 1.f) * G_SCALE;
   }
   return info;
 }
@@ -225,10 +225,7 @@ __device__ __forceinline__ int gather_few(const VocabRows& a, bool first_piece, 
       if (GRAD) info[rank] = row_info_of(a, lane, st, gm, lc);
       if (blockIdx.x == 0) {
         a.row_map[rank] = st == 2 ? ~lane : lane;
-        if (GRAD) {   // (without its last word, which is written where the label's entry is formed)
-          float* to = reinterpret_cast<float*>(a.row_info + rank);
-          to[0] = info[rank].x; to[1] = info[rank].y; to[2] = info[rank].z;
-        }
+        if (GRAD) a.row_info[rank] = info[rank];
         if (GRAD && a.state) a.row_lc[rank] = lc;
       }
     } else if (!GRAD && blockIdx.x == 0 && lane < a.n) {
@@ -403,15 +400,13 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::condit
       const int r = row0 + m * 16;
       const float4 ri = FEW ? info_s[r & 63] : a.row_info[r];
       const int at = __float_as_int(ri.z) - (int)a.v0 - col0;   // the label, counted from this lane's first column
-      float low[NB][4], at_label = 0.f;
+      float low[NB][4];
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         float g[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bool is = at == n * 16 + e;
-          g[e] = fmaf(__builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -ri.x)), ri.y, is ? -ri.w : 0.f);
-          at_label = is ? g[e] : at_label;
+          g[e] = at == n * 16 + e ? ri.w : __builtin_amdgcn_exp2f(fmaf(acc[m][n][e], a.scale2, -ri.x)) * ri.y;
           cs[n][e] += g[e];
         }
         put(n, make_uint2(pack_op2(g[0], g[1]), pack_op2(g[2], g[3])));
@@ -420,7 +415,6 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::condit
           for (int e = 0; e < 4; ++e) low[n][e] = residual(g[e]);
         }
       }
-      if ((unsigned)at < 64u && (at & 15) < 4) a.row_info[r].w = at_label;   // unrounded, for dh
       auto store = [&](int row, int c, const u32x4_t& v) {
         *reinterpret_cast<u32x4_t*>(a.g + (int64_t)(row0 - fr + m * 16 + row) * a.ldg + tn * BN + wn * 64 + c) = v;
       };

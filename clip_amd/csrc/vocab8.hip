@@ -315,10 +315,7 @@ __global__ __launch_bounds__(512) void vocab8_kernel(VocabGemm a) {
               for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                  if (at == nh * 32 + i * 16 + fq * 4 + e) {
-                    g[nh][i][e] -= ri.w;
-                    a.row_info[tm * BM + mh * 128 + wr * 64 + m * 16 + fr].w = g[nh][i][e];   // unrounded, for dh
-                  }
+                  if (at == nh * 32 + i * 16 + fq * 4 + e) g[nh][i][e] = ri.w;
           }
 #pragma unroll
           for (int nh = 0; nh < 2; ++nh)

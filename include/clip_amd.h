@@ -200,9 +200,8 @@ int clip_linear_loss_workspace(const clip_linear* d, int32_t k, int32_t grad, in
  * 0 where labels[i] == ignore_index; NaN (with NaN gradients) where a label is neither that nor in [0, vocab).
  *   reduction 0: rows only;  1: loss[0] = mean over the rows that are not ignored (NaN when there is none, as torch);
  *   2: loss[0] = sum.   dev_loss may be NULL for 0.
- * dev_lse [n, 2] (m, s, with logsumexp(z_i) = ln 2 m + ln s; 8-byte aligned) is what the gradient call needs of the forward;
- * dev_target [n] is z_i[labels[i]] (an argument of that call as of the distillation's; it takes a label's probability from the same
- * sums as all others'). */
+ * dev_lse [n, 2] (m, s, with logsumexp(z_i) = ln 2 m + ln s; 8-byte aligned) and dev_target [n] (z_i[labels[i]]) are what the gradient
+ * call needs of the forward. */
 int clip_linear_ce(const clip_linear* d, const int64_t* dev_labels, int64_t ignore_index, int32_t reduction,
                    float* dev_row_loss, float* dev_lse, float* dev_target, float* dev_loss, void* dev_work,
                    int64_t work_bytes, void* stream);
