@@ -122,7 +122,7 @@ struct VocabRows {          // rows, targets and results of one call; what is nu
   const int64_t* t_index; int64_t ld_ti;          // their vocabulary ids (negative: left out)
   float inv_t, loss_factor, grad_factor;          // 1 / T, T^2, T
   bool mean;                                      // the mean over live rows (else the sum, or the rows)
-  float *row_loss, *target, *loss; float2* lse_out;   // forward: [n], [n, k] scores / T of the targets (and t_p, state), [1],
+  float *row_loss, *target, *loss; float2* lse_out;   // forward: [n], [n, k] scores of the targets (and t_p, state), [1],
                                                   // [n] (m, s): logsumexp = ln2 m + ln s, m the largest score / T * log2(e)
   const float2* lse; const float* target_in;      // backward: what the forward left
   const float* grad; bool grad_rows;              // upstream gradient: [n] or [1]

@@ -199,7 +199,7 @@ __device__ __forceinline__ float4 row_info_of(const VocabRows& a, int r, int st,
   float4 info = make_float4(x, c * G_SCALE * inv, __int_as_float(-1), 0.f);
   if (!a.state && st == 1) {
     info.z = __int_as_float((int)a.labels[r]);
-    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E, -x)) * inv - 1.f) * G_SCALE;
+    info.w = c * (__builtin_amdgcn_exp2f(fmaf(a.target_in[r], LOG2E * a.inv_t, -x)) * inv - 1.f) * G_SCALE;
   }
   return info;
 }
@@ -720,19 +720,44 @@ __global__ __launch_bounds__(256) void vocab_copy_kernel(const bf16_t* __restric
   for (int c = threadIdx.x; c < hidden; c += 256) to[(int64_t)blockIdx.x * hidden + c] = from[blockIdx.x * ld + c];
 }
 
-// eight products of 16-bit operands in fp32, added to s
-__device__ __forceinline__ float dot8(const uint4& x, const uint4& w, float s) {
-  const uint32_t* xp = reinterpret_cast<const uint32_t*>(&x);
-  const uint32_t* wp = reinterpret_cast<const uint32_t*>(&w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) s = fmaf(op2_lo(xp[i]), op2_lo(wp[i]), fmaf(op2_hi(xp[i]), op2_hi(wp[i]), s));
-  return s;
+// Scores of 16 vocabulary entries for one hidden row x, acc = their bias to begin with: by the same instruction as the tiles of
+// scores, in the same order of k, so that they have the bits that the row's softmax is made of (in any other order they would be off
+// from these by fp32's rounding of a score, which a small temperature or large scores make a wrong probability).  x passes through
+// this wave's KB of LDS, every entry's row of W (lane & 15: which) comes in pieces of 64 bytes; the result is acc[e] = the score of
+// entry 4 (lane >> 4) + e.  ONE: all entries are the same, and its row passes through a second KB of LDS.  `p`: the first KB of either
+// (a lane's 16 bytes), loaded by the caller before it waits for anything else.
+struct RowPieces { uint4 x, w; };
+template <bool ONE>
+__device__ __forceinline__ RowPieces row_pieces(const bf16_t* x, const bf16_t* wrow, int c0, int H, int lane) {
+  RowPieces p = {};
+  const int at = min(c0 + lane * 8, H - 8);
+  p.x = *reinterpret_cast<const uint4*>(x + at);
+  if (ONE) p.w = *reinterpret_cast<const uint4*>(wrow + at);
+  return p;
 }
-// score of one vocabulary entry for the hidden row x: a wave's dot product, fp32
-__device__ __forceinline__ float wave_score(const bf16_t* x, const bf16_t* wrow, int H, int lane) {
-  float s = 0.f;
-  for (int c = lane * 8; c < H; c += 512) s = dot8(*reinterpret_cast<const uint4*>(x + c), *reinterpret_cast<const uint4*>(wrow + c), s);
-  return wave_sum(s);
+template <bool ONE>
+__device__ __forceinline__ f32x4_t tile_scores(RowPieces p, const bf16_t* x, const bf16_t* wrow, f32x4_t acc, int H, int lane, char* lds) {
+  const int fq = lane >> 4;
+  for (int c0 = 0; c0 < H; c0 += 512) {
+    const int steps = min(H - c0, 512) / 32;
+    *reinterpret_cast<uint4*>(lds + lane * 16) = p.x;
+    if (ONE) *reinterpret_cast<uint4*>(lds + 1024 + lane * 16) = p.w;
+    if (c0 + 512 < H) p = row_pieces<ONE>(x, wrow, c0 + 512, H, lane);
+    for (int s0 = 0; s0 < steps; s0 += 8) {   // eight pieces of every row in flight
+      uint4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int s = min(s0 + u, steps - 1);
+        v[u] = ONE ? *reinterpret_cast<const uint4*>(lds + 1024 + s * 64 + fq * 16)
+                   : *reinterpret_cast<const uint4*>(wrow + c0 + s * 32 + fq * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (s0 + u < steps)   // (uniform)
+          acc = MFMA_16x16x32(*reinterpret_cast<const opx8_t*>(&v[u]), *reinterpret_cast<const opx8_t*>(lds + (s0 + u) * 64 + fq * 16), acc);
+    }
+  }
+  return acc;
 }
 
 // what a row's exponentials over 64 columns at a time come to: (largest score, sum) of a wave's share of the pairs
@@ -758,7 +783,10 @@ __device__ __forceinline__ float2 join_pairs(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x), ref = m == -INFINITY ? 0.f : m;
   return make_float2(m, a.y * __builtin_amdgcn_exp2f(a.x - ref) + b.y * __builtin_amdgcn_exp2f(b.x - ref));
 }
-__device__ __forceinline__ float lse_of(float2 p) { return LN2 * ((p.x == -INFINITY ? 0.f : p.x) + log2f(p.y)); }
+// logsumexp(z / T) - z / T of one score, p the row's pair: the difference is taken next to the exponentials' own arithmetic
+__device__ __forceinline__ float minus_log_q(float2 p, float z, float scale2) {
+  return LN2 * (log2f(p.y) - fmaf(z, scale2, p.x == -INFINITY ? 0.f : -p.x));
+}
 
 // Forward over several pieces of the vocabulary: a piece's n pairs of every live row (rows n_part apart), and what the pieces before
 // it (`more`) came to, in one pair.  One wave per row; bound by the pairs' bytes.  A loss in one piece / several: 131 072 rows (H 128),
@@ -792,16 +820,23 @@ __device__ __forceinline__ void finish_rows(const VocabRows& a, int groups, floa
 // 18 us for 63 MB of pairs and 50 MB of rows; 4096 rows 8 us.
 __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
   __shared__ float red[4];
+  __shared__ __attribute__((aligned(16))) char stage[4][2048];
   const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (r < *a.count) {
     const int mapped = a.row_map[r], row = mapped < 0 ? ~mapped : mapped;
-    float loss = __builtin_nanf(""), z = 0.f;
+    float loss = __builtin_nanf(""), z = 0.f, b = 0.f;
+    const bf16_t *x = a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh, *wrow = a.w;
     if (mapped >= 0) {
       const int64_t v = a.labels[row];
-      z = wave_score(a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh, a.w + v * a.ldw, a.hidden, lane) + (a.bias ? a.bias[v] : 0.f);
+      wrow += v * a.ldw;
+      if (a.bias) b = a.bias[v];
     }
+    const RowPieces first = row_pieces<true>(x, wrow, 0, a.hidden, lane);
     const float2 all = wave_pairs(part + (int64_t)r * n_part, n_part, lane, 64);
-    if (mapped >= 0) loss = lse_of(all) - z;
+    if (mapped >= 0) {
+      z = tile_scores<true>(first, x, wrow, (f32x4_t){b, b, b, b}, a.hidden, lane, stage[threadIdx.x >> 6])[0];
+      loss = minus_log_q(all, z, LOG2E * a.inv_t);
+    }
     if (lane == 0) {
       a.target[row] = z;
       a.lse_out[row] = all;
@@ -817,6 +852,7 @@ template <int WPR>
 __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
   __shared__ float red[4];
   __shared__ float2 pair[4];
+  __shared__ __attribute__((aligned(16))) char stage[4][1024];
   const int tid = threadIdx.x, lane = tid & 63, w = WPR == 4 ? tid >> 6 : 0;
   const int r = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + (tid >> 6);
   if (r < *a.count) {   // (WPR 4: the same for the whole workgroup)
@@ -829,51 +865,25 @@ __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const f
 #pragma unroll
       for (int i = 1; i < 4; ++i) all = join_pairs(all, pair[i]);
     }
-    const float lse = lse_of(all);
     const bf16_t* x = a.x ? a.x + (int64_t)r * a.hidden : a.h + (int64_t)row * a.ldh;
+    const float scale2 = LOG2E * a.inv_t;
+    const int fr = lane & 15, fq = lane >> 4;
     float loss = 0.f;
     if (mapped >= 0)
-      for (int j0 = w * 8; j0 < a.k; j0 += 8 * WPR) {   // eight entries' rows of W in flight
-        const bf16_t* wr[8];
-        float z[8];
-        const int64_t mine_v = lane < 8 && j0 + lane < a.k ? a.t_index[(int64_t)row * a.ld_ti + j0 + lane] : -1;
-        const int mine_at = mine_v >= 0 && mine_v < a.vocab ? (int)mine_v : -1;   // (beyond only where the value is -inf)
+      for (int j0 = w * 16; j0 < a.k; j0 += 16 * WPR) {
+        const int64_t mine = j0 + fr < a.k ? a.t_index[(int64_t)row * a.ld_ti + j0 + fr] : -1;
+        const int v = mine >= 0 && mine < a.vocab ? (int)mine : -1;   // (beyond only where the value is -inf)
+        f32x4_t z;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int v = __builtin_amdgcn_readlane(mine_at, u);
-          wr[u] = a.w + (int64_t)max(v, 0) * a.ldw;
-          z[u] = 0.f;
-        }
-        for (int c = lane * 8; c < a.hidden; c += 512) {
-          uint4 wv[8];
-          const uint4 xv = *reinterpret_cast<const uint4*>(x + c);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) wv[u] = *reinterpret_cast<const uint4*>(wr[u] + c);
-#pragma unroll
-          for (int u = 0; u < 8; ++u) z[u] = dot8(xv, wv[u], z[u]);
-        }
-        // eight sums over 64 lanes: halve the values with the lanes, then lane l holds that of entry (l >> 3)
-#pragma unroll
-        for (int h = 4; h > 0; h >>= 1) {
-          const bool up = lane & (h * 8);
-#pragma unroll
-          for (int u = 0; u < h; ++u) {
-            const float send = up ? z[u] : z[u + h], keep = up ? z[u + h] : z[u];
-            z[u] = keep + __shfl_xor(send, h * 8, 64);
-          }
-        }
-        float sum = z[0];
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        const int u = lane >> 3, j = j0 + u, v = __shfl(mine_at, u, 64);
-        if ((lane & 7) == 0 && j < a.k) {
-          float zj = 0.f;
-          if (v >= 0) {
-            zj = (sum + (a.bias ? a.bias[v] : 0.f)) * a.inv_t;
-            const float pj = a.t_p[(int64_t)row * a.k + j];
-            if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] - zj + lse);
-          }
-          a.target[(int64_t)row * a.k + j] = zj;
+        for (int e = 0; e < 4; ++e) z[e] = a.bias ? a.bias[max(__shfl(v, fq * 4 + e, 64), 0)] : 0.f;
+        z = tile_scores<false>(row_pieces<false>(x, x, 0, a.hidden, lane), x, a.w + (int64_t)max(v, 0) * a.ldw, z, a.hidden, lane, stage[tid >> 6]);
+        // entry 4 fq + fr is this lane's, fr < 4
+        const int j = j0 + fq * 4 + fr, vj = __shfl(v, fq * 4 + (fr & 3), 64);
+        if (fr < 4 && j < a.k) {
+          const float zj = fr == 0 ? z[0] : fr == 1 ? z[1] : fr == 2 ? z[2] : z[3];
+          a.target[(int64_t)row * a.k + j] = vj >= 0 ? zj : 0.f;
+          const float pj = vj >= 0 ? a.t_p[(int64_t)row * a.k + j] : 0.f;
+          if (pj != 0.f) loss += pj * (a.t_logp[(int64_t)row * a.k + j] + minus_log_q(all, zj, scale2));
         }
       }
     loss = wave_sum(loss);
@@ -922,7 +932,7 @@ __device__ __forceinline__ bool teacher_entry(const VocabRows& a, const float4& 
   if (a.fix && table && v >= 0 && fabsf(lc.z * own) <= 1.f)
     atomicAdd(reinterpret_cast<unsigned long long*>(a.fix + (r & (FIX_COPIES - 1)) * a.vocab + v), (unsigned long long)__double2ll_rn((double)(lc.z * own) * FIX));
   if (!first) return false;
-  const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E, -lc.x)) * lc.y;
+  const float q = __builtin_amdgcn_exp2f(fmaf(a.target_in[(int64_t)row * a.k + j], LOG2E * a.inv_t, -lc.x)) * lc.y;
   const float e = lc.z * (q - p) * G_SCALE;
   if (v >= v0 && v < v1) {
     g[(int64_t)r * ldg + (v - v0)] = f32_to_op(e);

@@ -332,6 +332,66 @@ def test_large_scores_and_common_shift():
         _check(h, w, b, lambda h, w, b: losses.linear_cross_entropy(h, w, b, y, reduction="none"), p, live, 1.0, "none", 3)
 
 
+def _saturated(n, vocab, dtype, spread, seed, least):
+    """rows whose largest score is ahead of the next by `least` and more: their softmax is one-hot to fp32's last bit; scores big
+    enough that two orders of the same fp32 sum differ by a part of it that shows"""
+    h, w, b = R.make(16 * n, vocab, 128, dtype, seed, spread=spread)
+    top = (h.double() @ w.double().t() + b.double()).topk(2, 1)
+    keep = (top.values[:, 0] - top.values[:, 1] >= least).nonzero()[:n, 0]
+    assert len(keep) == n
+    return h[keep].contiguous(), w, b, top.indices[keep, 0]
+
+
+def _check_one_hot(h, w, b, top, p, scale, up, grads):
+    """dz = up scale (onehot(top) - p), the one rounding of the operand type on its way into dh and dw (and of the results), fp32 sums:
+    no error of a score is let in"""
+    n, vocab = p.shape
+    u = R.half_step(h.dtype)
+    q = torch.zeros_like(p)
+    q[torch.arange(n), top] = 1.0
+    dz = up * scale * (q - p)
+    # exp2, reciprocals and products of c, q and p; p of values / T up to 13.5, off by three half steps (T, its reciprocal, the product)
+    near = up * scale * 64 * R.F32 * (q + p)
+    hd, wd = h.double(), w.double()
+    for name, got, want, size in zip(("dh", "dw", "db"), grads, (dz @ wd, dz.t() @ hd, dz.sum(0)),
+                                     ((u * dz.abs() + near) @ wd.abs(), (u * dz.abs() + near).t() @ hd.abs(), near.sum(0))):
+        own = u if name != "db" else 0
+        sums = (n if name != "dh" else 4) * R.F32 * {"dh": (dz.abs() + near) @ wd.abs(), "dw": dz.abs().t() @ hd.abs(), "db": (q + p).sum(0) * up * scale}[name]
+        R.assert_within(name, got, want, size + sums + 1.01 * own * want.abs() + (R.TINY[h.dtype] if own else n * 2.0 ** -38 * up * scale))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("n,vocab", [(40, 700), (100, 700), (300, 128100)])
+def test_large_scores_of_rows_that_are_sure(n, vocab, dtype):
+    # scores of some 10 000: a label that is the row's largest score has no gradient, another one that of a one-hot softmax
+    h, w, b, top = _saturated(n, vocab, dtype, 20.0, 61, 120.0)
+    y = torch.where(torch.arange(n).cuda() % 2 == 0, top, (top + 1) % vocab)
+    p = torch.zeros(n, vocab, dtype=torch.float64, device="cuda")
+    p[torch.arange(n), y] = 1.0
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_cross_entropy(*leaves, y, reduction="sum")
+    _check_one_hot(h, w, b, top, p, 1.0, 0.5, torch.autograd.grad(loss, leaves, torch.tensor(0.5).cuda()))
+    # and no loss: exp2, log2 and a product next to the exact difference from the largest score
+    rows = losses.linear_cross_entropy(h, w, b, y, reduction="none")
+    assert rows[::2].abs().max() <= 16 * R.F32 and (rows[1::2] > 100).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("temperature", [1e-3, 1e-5, 1e-6])
+@pytest.mark.parametrize("n,vocab,k", [(40, 700, 5), (100, 700, 5), (100, 700, 90), (300, 128100, 5), (300, 128100, 90), (4500, 500, 5)])
+def test_small_temperatures(n, vocab, k, temperature, dtype):
+    # scores over T of some thousand to some million: q is one-hot, and the teacher's list names its entry in every other row
+    h, w, b, top = _saturated(n, vocab, dtype, 0.5, 62, 100 * temperature)
+    values, index = _teacher(n, vocab, k, 63)
+    values *= temperature
+    index[::2, 1] = top[::2]
+    p, live, _ = R.targets_distill(values, index, vocab, temperature)
+    leaves = [t.clone().requires_grad_() for t in (h, w, b)]
+    loss = losses.linear_distillation(*leaves, values, index, temperature=temperature, reduction="sum")
+    up = 0.5 / temperature
+    _check_one_hot(h, w, b, top, p, temperature, up, torch.autograd.grad(loss, leaves, torch.tensor(up).cuda()))
+
+
 def test_loss_differences():
     # central differences of the loss itself along +-1 directions; hidden values on a grid of 2^-5 that bf16 holds with the
     # step added.  Third derivative of logsumexp along d: a third cumulant of d.w_v, at most 8 M^3, M = max |d.w_v|.
