@@ -698,6 +698,34 @@ def test_teacher_to_student_step():
         R.assert_within(name, got, x + y_, e + f + (u if name != "db" else R.F32) * 1.01 * (x + y_).abs())
 
 
+@pytest.mark.parametrize("held", [F32, BF16])
+def test_decoder_as_a_linear_layer_holds_it(held):
+    """the documented use: weight and bias of one type, the other one cast, gradients back in the layer's own type"""
+    batch, width, hidden_size, vocab = 3, 20, 128, 900
+    torch.manual_seed(7)
+    decoder = torch.nn.Linear(hidden_size, vocab).to("cuda", held)
+    hidden = torch.randn(batch, width, hidden_size, device="cuda", requires_grad=True)
+    mlm_labels = _labels(batch * width, vocab, 8, 0.5).view(batch, width)
+    teacher_scores = 2 * torch.randn(batch, width, vocab, device="cuda")
+    weight, bias = decoder.weight.to(BF16), decoder.bias.float()
+    loss = losses.linear_cross_entropy(hidden.to(BF16), weight, bias, mlm_labels)
+    values, index = losses.topk_logits(teacher_scores, 64)
+    loss = loss + losses.linear_distillation(hidden.to(BF16), weight, bias, values, index, temperature=2.0)
+    loss.backward()
+    h, w, b = hidden.detach().to(BF16).view(-1, hidden_size), decoder.weight.detach().to(BF16), decoder.bias.detach().float()
+    n, y = batch * width, mlm_labels.view(-1)
+    p1, l1 = R.targets_ce(y, vocab, -100)
+    p2, l2, ent = R.targets_distill(values.view(n, 64), index.view(n, 64), vocab, 2.0)
+    a, ea = R.reference(h, w, b, p1, l1, 1.0, torch.full((n,), 1 / int(l1.sum())).cuda())
+    c, ec = R.reference(h, w, b, p2, l2, 2.0, torch.full((n,), 1 / n).cuda(), ent)
+    for name, got, x, y_, e, f, u in (("dh", hidden.grad.view(n, -1), a[1], c[1], ea[1], ec[1], R.half_step(BF16)),
+                                      ("dw", decoder.weight.grad, a[2], c[2], ea[2], ec[2], R.half_step(BF16)),
+                                      ("db", decoder.bias.grad, a[3], c[3], ea[3], ec[3], R.half_step(held))):
+        # (the two gradients, each rounded within its own bound, are added in bf16, and kept in the layer's type)
+        R.assert_within(name, got, x + y_, e + f + 2.02 * u * (x + y_).abs() + 1.01 * u * (e + f))
+    assert hidden.grad.dtype == F32 and decoder.weight.grad.dtype == decoder.bias.grad.dtype == held
+
+
 @pytest.mark.parametrize("n,vocab", [(500, 3000), (500, 31000), (500, 128100), (50, 3000)])
 def test_other_stream(n, vocab):
     h, w, b = R.make(n, vocab, 128, BF16, 60)
