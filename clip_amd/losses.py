@@ -59,7 +59,7 @@ def linear_distillation(hidden, weight, bias, teacher_values, teacher_index, *, 
     student's softmax over the whole vocabulary of (hidden @ weight.T + bias) / temperature; teacher_index [..., k] (int64) holds
     the scores' vocabulary ids (topk_logits gives both).  An entry with a negative id or the value -inf is left out, a row
     without entries contributes nothing.  Differentiable in hidden, weight and bias (not in the teacher).  k <= 1024,
-    1e-6 <= temperature <= 1e6."""
+    1e-6 <= temperature <= 1e6, scores / temperature up to 2^30."""
     return (_ext or load()).linear_distillation(hidden, weight, bias, teacher_values, teacher_index, temperature, reduction)
 
 

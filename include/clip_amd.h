@@ -223,8 +223,9 @@ int clip_linear_ce_grad(const clip_linear* d, const int64_t* dev_labels, int64_t
  *   row_loss[i] = T^2 sum_j p_ij (log p_ij - log q_i[index_ij]).
  * An entry with a negative id or the value -inf is left out; a row with none left contributes nothing (loss 0, no gradient,
  * not counted by the mean).  Ids may repeat within a row.  An id >= vocab, a NaN or a +inf makes the row's loss NaN (and the
- * gradients).  1 <= k <= 1024.  dev_target [n (2 k + 1)] is what the gradient call
- * needs of the lists, which it does not read again.  No counterpart in the reference. */
+ * gradients).  Scores / T are good up to 2^30 (beyond, fp32 has no digits left for their differences: infinite or NaN).  1 <= k <= 1024.
+ * dev_target [n (2 k + 1)] is what the gradient call needs of the lists, which it does not read again.  No counterpart in the
+ * reference. */
 int clip_linear_distill(const clip_linear* d, const float* dev_teacher_values, const int64_t* dev_teacher_index, int32_t k,
                         float temperature, int32_t reduction, float* dev_row_loss, float* dev_lse, float* dev_target,
                         float* dev_loss, void* dev_work, int64_t work_bytes, void* stream);
