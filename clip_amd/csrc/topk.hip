@@ -3,12 +3,13 @@
 // One workgroup per row; a chunk of 64 KB (16 384 fp32 scores or 32 768 of 16 bits) is read at once into registers, 64 per
 // thread.  A threshold that the k largest all reach and few others do is found to 16 bits by bisection on ballots:
 // for k <= 128 the k-th largest of the 256 threads' maxima (177 random scores reach it at k = 128, 74 at k = 64), beyond that
-// the k-th largest of the maxima of 16 bytes, and the k-th largest score itself where a row has not twice k of these.  Each wave notes what reaches it, one comparison per 16 bytes read, in its own part of LDS
-// as 64-bit keys (order-preserving bits of the score above the inverted id: all keys differ, a larger key comes first), and
+// the k-th largest of the maxima of 16 bytes, and the k-th largest score itself where a row has not twice k of these.  Each wave notes what reaches it,
+// one comparison per 16 bytes read, in its own part of LDS as 64-bit keys (order-preserving bits of the score above the inverted id: all keys differ, a larger key comes first), and
 // the few keys noted are sorted by counting, for each, how many are larger.  Where too many reach the threshold (equal
 // scores) the chunk is gone through again, a list being cut back to its k largest whenever it is full.
-// Bound: reading the scores; 8192 x 30 522 with k 64: fp32 200 us (5.0 TB/s), bf16 138 us, fp16 119 us (4.2 TB/s); five rows 8.4 us;
-// k 300 on 4096 rows: fp32 360 us, bf16 290 us (the search's 16 barriers; 540 and 940 us with every score searched).
+// Bound: reading the scores; 8192 x 30 522 with k 64: fp32 178 - 202 us (5.0 - 5.6 TB/s), bf16 114 - 138 us (3.6 - 4.4), fp16 107 -
+// 119 us (4.2 - 4.7); five rows 8.4 - 10.4 us; k 300 on 4096 rows: fp32 360 us, bf16 290 - 300 us, fp16 242 us (the search's 16
+// barriers, then every noted key against every other; 540 and 940 us, fp32 and bf16, with every score searched).
 #include "common.h"
 #include "kernels.h"
 

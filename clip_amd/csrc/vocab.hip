@@ -14,7 +14,8 @@
 // What G's rounding costs: most of a row's gradient sits in few entries (its targets), whose rounding errors do not average
 // out.  dh gets them back in fp32: the residuals of a row's largest entries times their rows of W, added where the partials are
 // joined.  dW of few rows (at most 64) is a product of G's high AND low parts, k twice as long under an output that is the
-// bound; with more rows its errors average out like those of the operands.
+// bound; with more rows its errors average out like those of the operands, but where an entry's gradient comes from a row or two
+// they are a second rounding beside the result's (4096 distilled rows: 2.3e-3 off, 1.7e-3 without G's rounding).
 // Rows that take no part (ignored label, empty teacher list) are dropped first: the live rows are copied side by side, so
 // their products cost nothing and whatever a dropped row holds (NaN included) reaches no gradient.
 // Times below: one MI355X, V 30 522, H 768, bf16, unless said otherwise; the card copies at 4.7 TB/s and multiplies large
@@ -460,7 +461,7 @@ __device__ __forceinline__ void vocab_tile(const VocabGemm& a, const std::condit
   }
 }
 
-// Scores (V_STATS, V_GRAD), a tile per workgroup.  Few rows: bound by W's bytes, one row 10.9 us for 47 MB (4.3 TB/s).  Rings that
+// Scores (V_STATS, V_GRAD), a tile per workgroup.  Few rows: bound by W's bytes, one row 10.9 - 11.8 us for 47 MB (4.0 - 4.3 TB/s).  Rings that
 // leave room for two workgroups on a CU, so that 257 tiles and more are not two rounds (us of a loss, one 4-deep ring a CU / two
 // 3-deep: V 30 522, H 768 18.0 / 17.8; V 33 000 25 / 20; V 40 000, H 1024 30 / 26; 128-row tiles, one 3-deep / two 2-deep: 128 rows of
 // V 30 522 27.5 / 28.6, V 50 257 38 / 32; 4096 rows, H 704 314 / 229).  G with its low part (19 rows) 15 us for 47 MB read and
@@ -536,8 +537,8 @@ __global__ __launch_bounds__(256) void vocab_teacher_kernel(VocabRows a) {
   if (lane == 0) a.state[row] = any_bad ? 2 : (any_in ? 1 : 0);
 }
 
-// Calls of many rows: the live rows before every 16th row, by one workgroup (a thread reads 16 rows' states at a time); 16 384
-// labels in 11 us, latency
+// Calls of many rows (PACK_COUNTS and more): the live rows before every 16th row, by one workgroup (a thread reads 16 rows' states at
+// a time); 131 072 labels in 76 us, latency
 template <bool GRAD>
 __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
   __shared__ int sums[16];
@@ -599,7 +600,7 @@ __global__ __launch_bounds__(1024) void vocab_scan_kernel(VocabRows a) {
 
 // Live rows side by side: x[r] = hidden[row_map[r]], zero rows up to the end of their last tile.  A workgroup per NT / 16 rows,
 // four to a wave; without a scan before it each counts all rows' states itself.  Backward: also what V_GRAD needs of every row,
-// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 24 us (50 MB), 4096 rows 14 us (12.6 MB).
+// zero gradients of the dropped rows, and a zeroed table of target sums.  16 384 rows 25 us (50 MB), 4096 rows 14 us (12.6 MB).
 template <bool GRAD, int NT>
 __global__ __launch_bounds__(NT) void vocab_pack_kernel(VocabRows a) {
   constexpr int NW = NT / 64, ROWS = NT / 16;
@@ -817,7 +818,7 @@ __device__ __forceinline__ void finish_rows(const VocabRows& a, int groups, floa
 }
 
 // Cross entropy, one wave per live row: lse from the tiles' (max, sum) pairs, the label's score, the row's loss.  16 384 rows
-// 18 us for 63 MB of pairs and 50 MB of rows; 4096 rows 8 us.
+// 21 us for 63 MB of pairs and 50 MB of rows; 4096 rows 10 us; one row 4.4, the chain of 24 MFMAs and its LDS passes 0.6 of it.
 __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) char stage[4][2048];
@@ -847,7 +848,7 @@ __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2
 }
 
 // Distillation, WPR waves per live row sharing the teacher's entries: one for short lists, four for long ones.  Bound: the
-// gather of k rows of W per row, which the caches serve: 4096 rows, k 64, H 512: 46 us for 268 MB (5.8 TB/s).
+// gather of k rows of W per row, which the caches serve: 4096 rows, k 64, H 512: 44 us for 268 MB (6.1 TB/s).
 template <int WPR>
 __global__ __launch_bounds__(256) void vocab_distill_kernel(VocabRows a, const float2* __restrict__ part, int n_part) {
   __shared__ float red[4];
@@ -1038,7 +1039,7 @@ __global__ __launch_bounds__(256) void vocab_teacher_hash_kernel(VocabRows a, bf
 }
 
 // dh of the live rows from the fp32 partials (fixed order), and db of the entries v0 .. v1 (a piece of the vocabulary) from its column
-// sums and the targets' table; dW from its partials where its k was split.  Bound: the partials' bytes; 16 384 rows 46 us, 4096 rows 14 us
+// sums and the targets' table; dW from its partials where its k was split.  Bound: the partials' bytes; 16 384 rows 48 us, 4096 rows 15 us
 __global__ __launch_bounds__(256) void vocab_finish_kernel(VocabRows a, VocabPlan p, const float* __restrict__ part,
                                                            const float* __restrict__ colsum, const float* __restrict__ dw_part,
                                                            bf16_t* __restrict__ dw, int64_t ld_dw, int row_blocks, int dw_blocks, int64_t v0, int64_t v1) {

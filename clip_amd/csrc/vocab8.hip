@@ -12,8 +12,9 @@
 // cycles); 256 x 256 tiles because each byte that a CU takes in feeds twice the MFMAs that it does in a 128 x 128 tile (of which
 // two fit: 16 384 rows 4.6 ms instead of 2.7).  bf16, V 30 522, H 768, us (2 n V H, twice that for the pair; 1.29 PF is the rate
 // of a large library product):
-//   4096 rows:   scores 160 - 177 (1.08 - 1.20 PF), G 180 - 198 (0.97 - 1.07 PF; 250 MB leave it), dW + dh 339 - 371 (1.03 - 1.13 PF)
-//   16 384 rows: scores 590 - 635 (1.21 - 1.30 PF), G 649 - 706 (1.09 - 1.18 PF; 1 GB leaves it), dW + dh 1220 - 1294 (1.19 - 1.26 PF)
+//   4096 rows:   scores 160 - 181 (1.06 - 1.20 PF), G 180 - 205 (0.94 - 1.07 PF; 250 MB leave it), dW + dh 339 - 382 (1.01 - 1.13 PF)
+//   16 384 rows: scores 590 - 662 (1.16 - 1.30 PF), G 649 - 732 (1.05 - 1.18 PF; 1 GB leaves it), dW + dh 1220 - 1330 (1.15 - 1.26 PF)
+// (averages on different boards; the first calls after a pause run slower)
 #include "vocab.h"
 
 namespace {
