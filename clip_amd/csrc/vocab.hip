@@ -837,6 +837,7 @@ __global__ __launch_bounds__(256) void vocab_ce_kernel(VocabRows a, const float2
     if (mapped >= 0) {
       z = tile_scores<true>(first, x, wrow, (f32x4_t){b, b, b, b}, a.hidden, lane, stage[threadIdx.x >> 6])[0];
       loss = minus_log_q(all, z, LOG2E * a.inv_t);
+      loss = loss < 0.f ? 0.f : loss;   // (the sum holds the label's own term: what is below zero is exp2's and log2's rounding; NaN stays)
     }
     if (lane == 0) {
       a.target[row] = z;

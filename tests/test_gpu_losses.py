@@ -376,6 +376,16 @@ def test_large_scores_of_rows_that_are_sure(n, vocab, dtype):
     assert rows[::2].abs().max() <= 16 * R.F32 and (rows[1::2] > 100).all()
 
 
+@pytest.mark.parametrize("spread", [0.5, 1.0, 3.0, 20.0])
+@pytest.mark.parametrize("n,vocab", [(60, 2000), (4000, 2000), (4000, 30001)])
+def test_no_negative_losses(n, vocab, spread):
+    # labels that are their rows' largest scores: losses down to fp32's last bits
+    h, w, b = R.make(n, vocab, 128, BF16, 64, spread=spread)
+    y = (h.double() @ w.double().t() + b.double()).argmax(1)
+    rows = losses.linear_cross_entropy(h, w, b, y, reduction="none")
+    assert (rows >= 0).all() and rows.isfinite().all()
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("temperature", [1e-3, 1e-5, 1e-6])
 @pytest.mark.parametrize("n,vocab,k", [(40, 700, 5), (100, 700, 5), (100, 700, 90), (300, 128100, 5), (300, 128100, 90), (4500, 500, 5)])
