@@ -976,6 +976,53 @@ def test_large_tiles_of_rows_far_apart(k):
         R.assert_within(name, got, a, e)
 
 
+@pytest.mark.parametrize("n,vocab,hidden,k", [((1 << 21) - 1, 300, 64, 0), ((1 << 21) - 1, 300, 64, 3), (200001, 300, 8192, 0), (261887, 129, 8192, 0)])
+def test_as_many_rows_as_are_allowed(n, vocab, hidden, k):
+    """fewer than 2^21 rows and (n + 256) hidden < 2^31: loss, dh, dW and db against 64 bits, 2^15 rows at a time"""
+    T, step = 2.0 if k else 1.0, 1 << 15
+    base, w, b = R.make(step, vocab, hidden, BF16, 96, spread=0.02)
+    h = base.repeat(-(-n // step), 1)[:n].contiguous()
+    if k:
+        values, index = (t.repeat(-(-n // step), 1)[:n].contiguous() for t in _teacher(step, vocab, k, 97, 0.3))
+    else:
+        y = _labels(n, vocab, 98, 0.4)
+    leaves = [t.requires_grad_() for t in (h, w, b)]
+    loss = (losses.linear_distillation(*leaves, values, index, temperature=T, reduction="none") if k else
+            losses.linear_cross_entropy(*leaves, y, reduction="none"))
+    dh, dw, db = torch.autograd.grad(loss, leaves, torch.ones(n, device="cuda"))
+    h, w, b = (t.detach() for t in leaves)
+    u, wd = R.half_step(BF16), w.double()
+    want_w, each_w, size_w = (torch.zeros(vocab, hidden, dtype=torch.float64, device="cuda") for _ in range(3))
+    want_b, each_b, size_b = (torch.zeros(vocab, dtype=torch.float64, device="cuda") for _ in range(3))
+    for i in range(0, n, step):
+        at = slice(i, min(i + step, n))
+        if k:
+            p, live, entropy = R.targets_distill(values[at], index[at], vocab, T)
+        else:
+            (p, live), entropy = R.targets_ce(y[at], vocab, -100), None
+        if i < 2 * step or at.stop == n:
+            want, err = R.reference(h[at], w, b, p, live, T, torch.ones(len(p), device="cuda"), entropy)
+            R.assert_within("loss", loss[at], want[0], err[0])
+            R.assert_within("dh", dh[at], want[1], err[1])
+        # dW and db as R.reference has them, the sums' errors over all rows
+        hd = h[at].double()
+        z = (hd @ wd.t() + b.double()) / T
+        lse = torch.logsumexp(z, 1)
+        mag = z.abs().amax(1) + lse.abs()
+        z_err = ((hidden + 2) * R.F32 * (hd.abs() @ wd.abs().t() + b.abs()) / T).amax(1) + 8 * R.F32 * mag
+        q = (z - lse[:, None]).exp() * live[:, None]
+        dz, s = T * (q - p), T * (q + p)
+        dz_err = (2 * z_err + (16 + vocab / 64) * R.F32)[:, None] * s
+        want_w += dz.t() @ hd
+        each_w += (dz_err + u * dz.abs()).t() @ hd.abs()
+        size_w += s.t() @ hd.abs()
+        want_b += dz.sum(0)
+        each_b += dz_err.sum(0)
+        size_b += s.sum(0)
+    R.assert_within("dw", dw, want_w, each_w + n * R.F32 * size_w + 1.01 * u * want_w.abs() + R.TINY[BF16])
+    R.assert_within("db", db, want_b, each_b + (n + 4) * R.F32 * size_b + n * 2.0 ** -38 * T)
+
+
 def test_ignore_index_inside_the_vocabulary():
     n, vocab = 300, 260
     h, w, b = R.make(n, vocab, 128, BF16, 44)
