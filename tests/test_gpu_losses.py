@@ -661,6 +661,21 @@ def test_topk_strides_and_shapes(dtype):
     assert v.shape == i.shape == (0, 4)
 
 
+@pytest.mark.parametrize("k", [5, 200])
+def test_topk_of_the_longest_row(k):
+    # 2^31 - 1 scores: ids up to the last of 32 bits
+    vocab = (1 << 31) - 1
+    x = torch.empty(1, vocab, dtype=F16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(5))
+    x[0, [vocab - 1, 0, vocab - 2]] = torch.tensor([9.0, 9.0, 8.0], dtype=F16, device="cuda")
+    values, index = losses.topk_logits(x, k)
+    parts = [_topk_plain(x[:, i:i + (1 << 24)], k) for i in range(0, vocab, 1 << 24)]
+    v = torch.cat([p[0] for p in parts], 1)
+    i = torch.cat([p[1] + (at << 24) for at, p in enumerate(parts)], 1)
+    want, at = _topk_plain(v, k)          # (parts and their ties are in the order of the ids)
+    assert torch.equal(values, want) and torch.equal(index, torch.gather(i, 1, at))
+    assert index[0, 0] == 0 and index[0, 1] == vocab - 1
+
+
 def test_topk_of_more_rows_than_one_grid():
     n = (1 << 24) + 70001
     x = torch.randint(-3, 3, (n, 3), generator=torch.Generator().manual_seed(5), dtype=torch.int8).cuda().to(BF16)
